@@ -25,7 +25,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libb2g.so"
 
 # b2g_dtype
-F32, F16, BF16, E4M3 = 0, 1, 2, 3
+F32, F16, BF16, E4M3, S8 = 0, 1, 2, 3, 4
 # cudaDataType_t values used by linear_lt's signature
 CUDA_R_32F, CUDA_R_16F, CUDA_R_16BF = 0, 2, 14
 # b2g_epilogue
@@ -77,6 +77,38 @@ class QkvRopeDesc(ctypes.Structure):
     _fields_ = [("pe", ctypes.c_void_p), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
                 ("gelu_out", ctypes.c_void_p), ("gelu_ld", ctypes.c_int64), ("pe_period", ctypes.c_int64),
                 ("a_scale", ctypes.c_void_p), ("b_scale", ctypes.c_void_p), ("pe_compact", ctypes.c_int64)]
+
+
+class QkNormRopeDesc(ctypes.Structure):
+    """Mirror of b2g_qk_norm_rope_desc."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("dtype", ctypes.c_int),
+        ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("out_dtype", ctypes.c_int),
+        ("ldq", ctypes.c_int64), ("hsq", ctypes.c_int64), ("ldk", ctypes.c_int64), ("hsk", ctypes.c_int64),
+        ("ldq_out", ctypes.c_int64), ("hsq_out", ctypes.c_int64), ("ldk_out", ctypes.c_int64),
+        ("hsk_out", ctypes.c_int64),
+        ("tokens", ctypes.c_int64), ("n_head", ctypes.c_int), ("n_kv_head", ctypes.c_int), ("d_head", ctypes.c_int),
+        ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+        ("positions", ctypes.c_void_p), ("ldp", ctypes.c_int64),
+        ("n_axes", ctypes.c_int), ("axis_dim", ctypes.c_int * 4), ("theta", ctypes.c_double),
+        ("interleaved", ctypes.c_int),
+    ]
+
+
+class AttentionPackedDesc(ctypes.Structure):
+    """Mirror of b2g_attention_packed_desc."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("ldq", ctypes.c_int64), ("hsq", ctypes.c_int64), ("ldk", ctypes.c_int64), ("hsk", ctypes.c_int64),
+        ("ldv", ctypes.c_int64), ("hsv", ctypes.c_int64), ("ldo", ctypes.c_int64), ("hso", ctypes.c_int64),
+        ("total_q", ctypes.c_int64), ("total_k", ctypes.c_int64), ("batch", ctypes.c_int64),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p), ("k_lens", ctypes.c_void_p),
+        ("n_head", ctypes.c_int), ("n_kv_head", ctypes.c_int), ("d_head", ctypes.c_int),
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int),
+    ]
 
 
 _lib = None
@@ -146,6 +178,16 @@ _SIGNATURES = {
     "b2g_add_inplace": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p], ctypes.c_int),
     "b2g_nerf_final": ([ctypes.c_void_p] * 5 + [ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                                  ctypes.c_void_p], ctypes.c_int),
+    "b2g_quantize_s8": ([ctypes.c_void_p, ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_void_p, ctypes.c_int64,
+                                                                                 ctypes.c_void_p, ctypes.c_void_p],
+                        ctypes.c_int),
+    "b2g_gemm_s8_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int], ctypes.c_size_t),
+    "b2g_gemm_s8": ([ctypes.POINTER(GemmDesc)] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p],
+                    ctypes.c_int),
+    "b2g_qk_norm_rope": ([ctypes.POINTER(QkNormRopeDesc), ctypes.c_void_p], ctypes.c_int),
+    "b2g_attention_packed_workspace": ([ctypes.POINTER(AttentionPackedDesc)], ctypes.c_size_t),
+    "b2g_attention_packed": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+                             ctypes.c_int),
     "b2g_check_device_error": ([ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "b2g_launch_count": ([], ctypes.c_uint64),
     "b2g_set_gemm_variant": ([ctypes.c_int, ctypes.c_int], ctypes.c_int),
@@ -974,4 +1016,183 @@ def nerf_final(feat_cond: torch.Tensor, feat_uncond: torch.Tensor | None, norm_s
     _require_cuda(feat_cond, norm_scale, conv_w, conv_b, out)
     _check(load().b2g_nerf_final(feat_cond.data_ptr(), _ptr(feat_uncond), norm_scale.data_ptr(), conv_w.data_ptr(),
                                  conv_b.data_ptr(), float(cfg_scale), H, W, out.data_ptr(), _stream(out, stream)))
+    return out
+
+
+# ---------------------------------------------------------------------------- packed batches
+def _on(stream: torch.cuda.Stream | None, *ts: torch.Tensor | None):
+    """The raw stream of a call on the CUDA tensors `ts`, all of the current device."""
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise B2GError("all tensors must be CUDA tensors of the current device")
+    return (stream or torch.cuda.current_stream()).cuda_stream
+
+
+def _empty(shape, dtype: torch.dtype, like: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A new tensor for use on `stream` (memory of torch's allocator belongs to a stream)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def quantize_s8(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-row 8-bit integer quantisation of a 2-D F32/BF16/F16 tensor: (codes int8 [rows, cols],
+    scales F32 [rows]), scales = absmax / 127 and codes = round(x * 127 / absmax), into `out` and
+    `scales` when given.  New codes have rows padded to 16 bytes, as gemm_s8 needs its operands."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.dtype not in _TORCH_TO_B2G:
+        raise B2GError("quantize_s8: 2-D F32/BF16/F16 tensor with unit column stride expected")
+    rows, cols = x.shape
+    if out is None:
+        out = _empty((rows, (cols + 15) // 16 * 16), torch.int8, x, stream)[:, :cols]
+    if scales is None:
+        scales = _empty((rows,), torch.float32, x, stream)
+    if out.dtype != torch.int8 or out.shape != x.shape or (cols > 1 and out.stride(1) != 1):
+        raise B2GError("quantize_s8: out must be int8 [rows, cols] with unit column stride")
+    if scales.dtype != torch.float32 or scales.shape != (rows,) or not scales.is_contiguous():
+        raise B2GError("quantize_s8: scales must be contiguous F32 [rows]")
+    s = _on(stream, x, out, scales)
+    _check(load().b2g_quantize_s8(x.data_ptr(), _TORCH_TO_B2G[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
+                                  out.data_ptr(), out.stride(0) if rows > 1 else cols, scales.data_ptr(), s))
+    return out, scales
+
+
+def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, epilogue: str = "none",
+            gate: torch.Tensor | None = None, x_scale: torch.Tensor | None = None,
+            stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """8-bit integer linear: out = epilogue((x . wq^T) * x_scale[m] * w_scale[n] + bias).
+
+    wq: int8 [N, K] with 16-byte aligned rows (quantize_s8 of the weight), w_scale its scales.
+    x: int8 codes with x_scale, or F32/BF16/F16 activations, quantised per token in the call.  The
+    epilogues are gemm()'s."""
+    if x.dim() != 2 or wq.dim() != 2 or wq.dtype != torch.int8:
+        raise B2GError("gemm_s8: 2-D x and int8 wq expected")
+    M, K = x.shape
+    N = wq.shape[0]
+    if wq.shape[1] != K:
+        raise B2GError(f"gemm_s8: K mismatch {tuple(x.shape)} vs {tuple(wq.shape)}")
+    if K > 1 and (x.stride(1) != 1 or wq.stride(1) != 1):
+        raise B2GError("gemm_s8: x and wq need unit stride along K")
+    codes = x.dtype == torch.int8
+    if not codes and x.dtype not in _TORCH_TO_B2G:
+        raise B2GError("gemm_s8: x must be int8, F32, BF16 or F16")
+    if epilogue not in _EPILOGUES:
+        raise B2GError(f"gemm_s8: unknown epilogue {epilogue!r}")
+    epi = _EPILOGUES[epilogue]
+    if out is None:
+        if epi == EPI_GATED_RESIDUAL:
+            raise B2GError("gemm_s8: gated_residual needs `out` (the residual)")
+        out = _empty((M, N), out_dtype or torch.float32, x, stream)
+    elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1):
+        raise B2GError("gemm_s8: out must be [M, N] with unit column stride")
+    if out.dtype not in _TORCH_TO_B2G or (bias is not None and bias.dtype not in _TORCH_TO_B2G):
+        raise B2GError("gemm_s8: out and bias must be F32, BF16 or F16")
+    for t, n, what in ((w_scale, N, "w_scale"), (x_scale if codes else None, M, "x_scale"),
+                       (gate if epi == EPI_GATED_RESIDUAL else None, N, "gate")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise B2GError(f"gemm_s8: {what} must be contiguous F32 [{n}]")
+    if bias is not None and (bias.numel() != N or not bias.is_contiguous()):
+        raise B2GError(f"gemm_s8: bias must be contiguous [{N}]")
+    s = _on(stream, x, wq, w_scale, bias, out, gate, x_scale)
+    lib = load()
+    a_dtype = S8 if codes else _TORCH_TO_B2G[x.dtype]
+    d = GemmDesc(M, N, K, x.data_ptr(), a_dtype, x.stride(0) if M > 1 else (K + 15) // 16 * 16 if codes else K,
+                 wq.data_ptr(), S8, wq.stride(0) if N > 1 else (K + 15) // 16 * 16,
+                 _ptr(bias), F32 if bias is None else _TORCH_TO_B2G[bias.dtype],
+                 out.data_ptr(), _TORCH_TO_B2G[out.dtype], out.stride(0) if M > 1 else N, epi, _ptr(gate))
+    ws, n = None, 0
+    if not codes:
+        n = lib.b2g_gemm_s8_workspace(M, K, a_dtype)
+        ws = _empty((n,), torch.uint8, x, stream)
+    _check(lib.b2g_gemm_s8(ctypes.byref(d), _ptr(x_scale), w_scale.data_ptr(), _ptr(ws), n, s))
+    return out
+
+
+def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
+    """Token and head stride of a [tokens, heads, d] tensor whose heads are contiguous."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise B2GError(f"{what}: [tokens, heads, d] with unit stride along d expected")
+    return t.stride(0), t.stride(1)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes_dim: list[int],
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 theta: float = 10000.0, interleaved: bool = True, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                 stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMSNorm (with q_norm / k_norm [d], if given) of q [tokens, n_head, d] and k [tokens,
+    n_kv_head, d] and their rotation by positions [tokens, axes] (F32; axis i turns axes_dim[i]
+    values), in one pass.  interleaved: pairs are neighbouring values, else one value of each half of
+    the turned part.  q and k may be views of a fused projection.  Returns (q', k'): q_out and
+    k_out when given (q and k themselves for in place), else new tensors of out_dtype (default: q's)."""
+    (ldq, hsq), (ldk, hsk) = _heads(q, "qk_norm_rope: q"), _heads(k, "qk_norm_rope: k")
+    T, H, D = q.shape
+    if k.shape[0] != T or k.shape[2] != D or k.dtype != q.dtype or q.dtype not in _TORCH_TO_B2G:
+        raise B2GError("qk_norm_rope: q and k must have the same tokens, head width and F32/BF16/F16 type")
+    if positions.dim() != 2 or positions.shape != (T, len(axes_dim)) or positions.dtype != torch.float32 or (
+            positions.shape[1] > 1 and positions.stride(1) != 1):
+        raise B2GError("qk_norm_rope: positions must be F32 [tokens, len(axes_dim)]")
+    if len(axes_dim) > 4:
+        raise B2GError("qk_norm_rope: at most 4 axes")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != D or not w.is_contiguous()):
+            raise B2GError("qk_norm_rope: norm scales must be contiguous F32 [d]")
+    if q_out is None:
+        q_out = _empty(q.shape, out_dtype or (q.dtype if k_out is None else k_out.dtype), q, stream)
+    if k_out is None:
+        k_out = _empty(k.shape, q_out.dtype, k, stream)
+    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype != k_out.dtype or (
+            q_out.dtype not in _TORCH_TO_B2G) or (out_dtype or q_out.dtype) != q_out.dtype:
+        raise B2GError("qk_norm_rope: outputs must have the inputs' shapes and one F32/BF16/F16 type")
+    (ldqo, hsqo), (ldko, hsko) = _heads(q_out, "qk_norm_rope: q_out"), _heads(k_out, "qk_norm_rope: k_out")
+    s = _on(stream, q, k, positions, q_norm, k_norm, q_out, k_out)
+    d = QkNormRopeDesc(q.data_ptr(), k.data_ptr(), _TORCH_TO_B2G[q.dtype], q_out.data_ptr(), k_out.data_ptr(),
+                       _TORCH_TO_B2G[q_out.dtype], ldq, hsq, ldk, hsk, ldqo, hsqo, ldko, hsko, T, H, k.shape[1], D,
+                       _ptr(q_norm), _ptr(k_norm), eps, positions.data_ptr(),
+                       positions.stride(0) if T > 1 else len(axes_dim), len(axes_dim),
+                       (ctypes.c_int * 4)(*axes_dim), theta, 1 if interleaved else 0)
+    _check(load().b2g_qk_norm_rope(ctypes.byref(d), s))
+    return q_out, k_out
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, k_lens: torch.Tensor | None = None, causal: bool = False,
+                     scale: float | None = None, out: torch.Tensor | None = None,
+                     stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Attention within packed sequences of different lengths: q [total_q, n_head, d], k and v
+    [total_k, n_kv_head, d] (BF16 or F16 views, d 64 or 128), sequence b being rows cu_q[b] to cu_q[b+1]
+    of q and cu_k[b] to cu_k[b+1] of k and v (cu_k None: cu_q's), of which k_lens[b] are in use when
+    given.  causal: the last query sees the last key.  scale None: 1 / sqrt(d).  Offsets and lengths are
+    int32 device tensors; a row that sees no key is 0.  Returns [total_q, n_head, d] of q's type (rows
+    of no sequence are left as they were)."""
+    (ldq, hsq), (ldk, hsk), (ldv, hsv) = (_heads(q, "attention_packed: q"), _heads(k, "attention_packed: k"),
+                                          _heads(v, "attention_packed: v"))
+    Tq, H, D = q.shape
+    if k.shape != v.shape or k.shape[2] != D or q.dtype not in (torch.bfloat16, torch.float16) or (
+            k.dtype != q.dtype or v.dtype != q.dtype):
+        raise B2GError("attention_packed: q, k, v must be BF16 or F16 of one head width, k and v of one shape")
+    if cu_k is None:
+        cu_k = cu_q
+    B = cu_q.numel() - 1
+    for t, n in ((cu_q, B + 1), (cu_k, B + 1), (k_lens, B)):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or B < 0 or
+                              not t.is_contiguous()):
+            raise B2GError("attention_packed: cu_q, cu_k [batch + 1] and k_lens [batch] must be contiguous int32")
+    if out is None:
+        out = _empty(q.shape, q.dtype, q, stream)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise B2GError("attention_packed: out must have q's shape and type")
+    ldo, hso = _heads(out, "attention_packed: out")
+    s = _on(stream, q, k, v, cu_q, cu_k, k_lens, out)
+    lib = load()
+    d = AttentionPackedDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[q.dtype], ldq, hsq,
+                            ldk, hsk, ldv, hsv, ldo, hso, Tq, k.shape[0], B, cu_q.data_ptr(), cu_k.data_ptr(),
+                            _ptr(k_lens), H, k.shape[1], D, D ** -0.5 if scale is None else scale, 1 if causal else 0)
+    ref = ctypes.byref(d)
+    n = lib.b2g_attention_packed_workspace(ref)
+    ws = _empty((n,), torch.uint8, q, stream) if n else None
+    _check(lib.b2g_attention_packed(ref, _ptr(ws), n, s))
     return out

@@ -1,0 +1,906 @@
+// attention_packed.cu — attention over packed sequences of different lengths.
+//
+//   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h / group]) v[j, h / group]
+//
+// Sequence b has the query rows [cu_q[b], cu_q[b+1]) and the keys from row cu_k[b] on, as many as
+// k_lens[b] says or up to cu_k[b+1]; each attends within itself.  causal: query i of lq sees the keys
+// j <= i + lk - lq (the last query sees the last key).  A row that sees no key is 0.  A group of
+// n_head / n_kv_head query heads shares a key head.  The offsets are read on the device (a captured
+// graph replays with other lengths), clamped to the buffers' rows: bad offsets cannot make a kernel
+// read or write outside them.
+//
+//   packed_tiles    long queries: two 128-row tiles per CTA on the tensor cores through TMEM
+//   packed_rows     few query rows per key head (single tokens): the keys are read once by
+//                   blocks that share out the key axis; packed_combine joins the shares
+//
+// Statistics (row maximum and sum) and the output sums are fp32.  P is rounded to the operands' 16-bit
+// type as the tensor cores need it; the row sum is taken before that rounding.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+#include "engine.cuh"
+#include "ptx_sm100.cuh"
+
+namespace b2g {
+
+namespace {
+
+struct PkParams {
+  const int* cu_q;
+  const int* cu_k;
+  const int* k_lens;       // [batch] or NULL
+  int batch;
+  int total_q, total_k;    // rows of q and of k, v
+  int hq, hk, group;       // query heads, key heads, hq / hk
+  int causal;
+  float scale_log2;        // scale * log2(e)
+  const void *q, *k, *v;
+  long long ldq, hsq, ldk, hsk, ldv, hsv;  // token and head strides, elements
+  void* out;
+  long long ldo, hso;
+  int* err;
+  // packed_rows
+  int keys_per_share;      // keys that one block takes (times the row tiles of the sequence)
+  int slots;               // capacity of the partial buffers
+  float* part_o;           // [slot][16][D]
+  float2* part_ml;         // [slot][16]: row maximum (log2 units), row sum
+};
+
+// Rows of sequence b, clamped to the buffers.
+struct Seq {
+  int q0, lq, k0, lk;
+};
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+__device__ __forceinline__ Seq load_seq(const PkParams& p, int b) {
+  Seq s;
+  s.q0 = clampi(__ldg(p.cu_q + b), 0, p.total_q);
+  s.lq = clampi(__ldg(p.cu_q + b + 1), s.q0, p.total_q) - s.q0;
+  s.k0 = clampi(__ldg(p.cu_k + b), 0, p.total_k);
+  s.lk = clampi(__ldg(p.cu_k + b + 1), s.k0, p.total_k) - s.k0;
+  if (p.k_lens) s.lk = clampi(__ldg(p.k_lens + b), 0, s.lk);
+  return s;
+}
+
+// The sequence that holds unit `want` when sequence b holds count(b) units, and the number of units
+// before it; -1 if there are not so many.  A whole warp searches, 32 sequences at a time.
+template <typename Count>
+__device__ __forceinline__ int find_seq(int batch, int want, int lane, Count count, int* before) {
+  int base = 0;
+  for (int b0 = 0; b0 < batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < batch ? count(b) : 0;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, base + sum > want);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      *before = base + __shfl_sync(0xffffffffu, sum - n, at);
+      return b0 + at;
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return -1;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
+// ---------------------------------------------------------------------------- long queries
+//
+// A CTA works on two 128-row query tiles that share their keys: two consecutive tiles of one head,
+// or, where two query heads share a key head, the same rows of both (finer steps along the
+// sequence).  Roles as in the engine's other attention kernel: warp 0 loads Q and K, warp 2 V, one
+// thread of warp 1 issues the MMAs, warps 4-7 and 8-11 are the softmax of tiles A and B with one
+// thread per row.  S (fp32) and O live in TMEM, P (16-bit) overwrites S and is the A operand of P.V:
+//   S_A(0), S_B(0), then per key block j: O_A += P_A(j) V_j, S_A(j+1), O_B += P_B(j) V_j, S_B(j+1)
+// so the tensor core works for one tile while the other's softmax runs.  Each tile stops at its own
+// last visible key block.
+//
+// The last key block may reach into the next sequence's rows, whose values may be anything: those
+// scores are replaced by -inf, and those rows of V are zeroed in shared memory before the MMA
+// reads them (0 times a NaN would be a NaN).  Within a sequence, V is expected to be finite: a
+// non-finite row of V reaches the query rows of its tile that do not see it.
+constexpr int kPtThreads = 384;
+constexpr int kPtRegsIdle = 64;      // producers and MMA issuer
+constexpr int kPtRegsSoftmax = 216;  // a 128-key row of scores in registers
+static_assert(4 * 32 * kPtRegsIdle + 8 * 32 * kPtRegsSoftmax <= kPtThreads * 168, "register split");
+constexpr int kPtRows = 128;
+constexpr int kPtKeys = 128;
+constexpr int kPtKStages = 3;
+constexpr int kPtVStages = 2;
+constexpr uint32_t kPtBox = 128 * 128;  // bytes of one 128-row x 128-byte swizzled box
+constexpr float kPtRescaleLog2 = 8.0f;
+
+template <int D>
+struct PtLayout {
+  static constexpr uint32_t kTileBytes = 128 * D * 2;  // Q tile, K block, V block: D / 64 boxes
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kK = kQ + 2 * kTileBytes;
+  static constexpr uint32_t kV = kK + kPtKStages * kTileBytes;
+  static constexpr uint32_t kBars = kV + kPtVStages * kTileBytes;
+  static constexpr uint32_t kSmem = 1024 + kBars + 256;
+};
+
+template <typename T, int D, bool kHeadPairs>
+__global__ void __launch_bounds__(kPtThreads, 1)
+    packed_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV, const PkParams p) {
+  using Ly = PtLayout<D>;
+  constexpr int KS = kPtKStages, VS = kPtVStages;
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem + Ly::kQ;
+  uint8_t* sK = smem + Ly::kK;
+  uint8_t* sV = smem + Ly::kV;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Ly::kBars);
+  uint64_t* q_full = bars;
+  uint64_t* k_full = bars + 1;
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;  // [tile]
+  uint64_t* p_part = s_full + 2;
+  uint64_t* p_full = p_part + 2;
+  uint64_t* pv_done = p_full + 2;
+  uint64_t* v_tail = pv_done + 2;   // the last V block, before its foreign rows are zeroed
+  uint64_t* drain_bar = v_tail + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0 && lane == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_part[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(v_tail, 1);
+    mbar_init(drain_bar, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();  // the set-up above overlapped the previous kernel's tail
+  griddep_launch_dependents();
+
+  // ---- this CTA's sequence and tiles (every warp finds them for itself)
+  constexpr int kSpan = kHeadPairs ? kPtRows : 2 * kPtRows;  // sequence rows per CTA
+  int before = 0;
+  const int unit = static_cast<int>(gridDim.x - 1 - blockIdx.x);  // (the last tiles of a sequence see most keys)
+  const int b = find_seq(p.batch, unit, lane, [&](int i) {
+    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+    return (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kSpan - 1) / kSpan;
+  }, &before);
+  Seq s{0, 0, 0, 0};
+  if (b >= 0) s = load_seq(p, b);
+  int first_row[2], head[2], blocks[2], keys = 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    first_row[t] = (unit - before) * kSpan + (kHeadPairs ? 0 : t * kPtRows);
+    head[t] = kHeadPairs ? 2 * static_cast<int>(blockIdx.y) + t : static_cast<int>(blockIdx.y);
+    int n = first_row[t] < s.lq ? s.lk : 0;
+    if (p.causal) n = clampi(min(first_row[t] + kPtRows, s.lq) + s.lk - s.lq, 0, n);
+    blocks[t] = (n + kPtKeys - 1) / kPtKeys;
+    keys = max(keys, n);
+  }
+  const int nkb = max(blocks[0], blocks[1]);
+  const int kv_head = head[0] / p.group;
+
+  if (warp < 4) {
+    regs_dec<kPtRegsIdle>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- Q and K
+      if (lane == 0 && nkb > 0) {
+        const uint64_t shared_kv = policy_evict_last(), once = policy_evict_first();
+        mbar_arrive_expect_tx(q_full, ((blocks[0] > 0) + (blocks[1] > 0)) * Ly::kTileBytes);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (blocks[t] > 0)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_3d(sQ + t * Ly::kTileBytes + c * kPtBox, &tmQ, q_full, c * 64, s.q0 + first_row[t], head[t], once);
+        int issued = 0;
+        for (int j = 0; j < nkb; ++j) {
+          const int st = j % KS;
+          if (!mbar_wait(&k_empty[st], ((j / KS) & 1) ^ 1u, p.err, kErrWaitProducer)) break;
+          mbar_arrive_expect_tx(&k_full[st], Ly::kTileBytes);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(sK + st * Ly::kTileBytes + c * kPtBox, &tmK, &k_full[st], c * 64, s.k0 + j * kPtKeys, kv_head,
+                        shared_kv);
+          ++issued;
+        }
+        // This thread's copies land before the CTA's shared memory goes away (they have, unless
+        // another role gave up early).
+        mbar_wait_drain(q_full, 0);
+        for (int j = max(0, issued - KS); j < issued; ++j) mbar_wait_drain(&k_full[j % KS], (j / KS) & 1);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------- V
+      const uint64_t shared_kv = policy_evict_last();
+      int issued = 0;
+      for (int j = 0; j < nkb; ++j) {
+        const int st = j % VS;
+        const bool ok = __all_sync(0xffffffffu, lane != 0 || mbar_wait(&v_empty[st], ((j / VS) & 1) ^ 1u, p.err,
+                                                                      kErrWaitProducer));
+        if (!ok) break;
+        const int valid = keys - j * kPtKeys;  // rows of this block that any tile sees
+        uint64_t* bar = valid < kPtKeys ? v_tail : &v_full[st];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, Ly::kTileBytes);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(sV + st * Ly::kTileBytes + c * kPtBox, &tmV, bar, c * 64, s.k0 + j * kPtKeys, kv_head, shared_kv);
+        }
+        if (valid < kPtKeys) {  // the last block: rows past the sequence become zeros
+          if (!__all_sync(0xffffffffu, mbar_wait(v_tail, 0, p.err, kErrWaitProducer))) break;
+          const int words = (kPtKeys - valid) * 8;
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            uint4* z = reinterpret_cast<uint4*>(sV + st * Ly::kTileBytes + c * kPtBox + valid * 128);
+            for (int i = lane; i < words; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[st]);
+        }
+        ++issued;
+      }
+      if (lane == 0)
+        for (int j = max(0, issued - VS); j < issued; ++j) mbar_wait_drain(&v_full[j % VS], (j / VS) & 1);
+    } else if (warp == 1 && lane == 0 && nkb > 0) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_s = idesc_make(kFmt, kPtRows, kPtKeys);
+      constexpr uint32_t idesc_o = idesc_make(kFmt, kPtRows, D) | kIdescBMajorMN;
+      auto issue_s = [&](int t, int j) {
+        const uint32_t q0 = smem_u32(sQ + t * Ly::kTileBytes), k0 = smem_u32(sK + (j % KS) * Ly::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem + t * 256, smem_desc_k_sw128(q0 + c * kPtBox + k * 32),
+                     smem_desc_k_sw128(k0 + c * kPtBox + k * 32), idesc_s, (c | k) != 0 ? 1u : 0u);
+        umma_commit(&s_full[t]);
+      };
+      bool ok = mbar_wait(q_full, 0, p.err, kErrWaitMma) && mbar_wait(&k_full[0], 0, p.err, kErrWaitMma);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (blocks[t] > 0) issue_s(t, 0);
+        umma_commit(&k_empty[0]);
+      }
+      for (int j = 0; j < nkb && ok; ++j) {
+        const int vs = j % VS;
+        const uint32_t v0 = smem_u32(sV + vs * Ly::kTileBytes);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (j >= blocks[t]) continue;
+          // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, 96-127 when all is there.
+          if (!(ok = mbar_wait(&p_part[t], j & 1, p.err, kErrWaitMma))) break;
+          if (!(ok = mbar_wait(&v_full[vs], (j / VS) & 1, p.err, kErrWaitMma))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 6; ++k)
+            umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                        idesc_o, (j | k) != 0 ? 1u : 0u);
+          if (!(ok = mbar_wait(&p_full[t], j & 1, p.err, kErrWaitMma))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 6; k < 8; ++k)
+            umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                        idesc_o, 1u);
+          umma_commit(&pv_done[t]);
+          if (j + 1 < blocks[t]) {
+            if (!(ok = mbar_wait(&k_full[(j + 1) % KS], ((j + 1) / KS) & 1, p.err, kErrWaitMma))) break;
+            // S(j+1) overwrites P(j); issued behind P(j).V_j, which reads P first (issue order).
+            issue_s(t, j + 1);
+          }
+        }
+        if (ok) {
+          umma_commit(&v_empty[vs]);
+          if (j + 1 < nkb) umma_commit(&k_empty[(j + 1) % KS]);
+        }
+      }
+      if (!ok) {
+        umma_commit(drain_bar);  // MMAs already issued retire before TMEM is released
+        mbar_wait_drain(drain_bar, 0);
+      }
+    }
+  } else {
+    regs_inc<kPtRegsSoftmax>();
+    // ------------------------------------------------------------ softmax
+    const int t = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row = (t ? first_row[1] : first_row[0]) + quarter * 32 + lane;
+    const int n = t ? blocks[1] : blocks[0];
+    // Keys this row sees: [0, sees).
+    const int sees = p.causal ? min(s.lk, row + 1 + s.lk - s.lq) : s.lk;
+    const uint32_t sbase = tmem + t * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t obase = sbase + 128;
+    float m_used = -INFINITY, l_sum = 0.f;
+    bool good = true;
+    for (int j = 0; j < n && good; ++j) {
+      good = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, p.err, kErrWaitEpilogue));
+      if (!good) break;
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(sbase + c * 32, r[c]);
+      tmem_wait_ld();
+      const int left = sees - j * kPtKeys;
+      if (__any_sync(0xffffffffu, left < kPtKeys)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i >= left) r[c][i] = 0xFF800000u;  // -inf
+      }
+      float m16[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m16[i] = fmaxf(__uint_as_float(r[0][i]), __uint_as_float(r[0][i + 16]));
+#pragma unroll
+      for (int c = 1; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m16[i] = max3f(m16[i], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 16]));
+      float mx = m16[0];
+#pragma unroll
+      for (int i = 1; i < 15; i += 2) mx = max3f(mx, m16[i], m16[i + 1]);
+      mx = fmaxf(mx, m16[15]) * p.scale_log2;  // scale > 0: the max commutes with it
+      // The maximum in use is raised only when a block exceeds it by 2^8 (O is then rescaled).
+      const bool raise = mx > m_used + kPtRescaleLog2;
+      const float alpha = raise ? fast_exp2(m_used - mx) : 1.f;
+      if (raise) m_used = mx;
+      if (__any_sync(0xffffffffu, raise && j > 0)) {
+        good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (j - 1) & 1, p.err, kErrWaitEpilogue));
+        if (!good) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(obase + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st_32x32b_x32(obase + c * 32, o);
+        }
+      }
+      l_sum *= alpha;
+      const uint64_t ua2 = f2_splat(p.scale_log2), nm2 = f2_splat(m_used == -INFINITY ? 0.f : -m_used);
+      uint64_t ls2[2] = {f2_splat(0.f), f2_splat(0.f)};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 xx = f2_unpack(f2_fma(f2_pack(r[c][i], r[c][i + 1]), ua2, nm2));
+          const float e0 = fast_exp2(xx.x), e1 = fast_exp2(xx.y);
+          ls2[(i >> 1) & 1] = f2_add(ls2[(i >> 1) & 1], f2_pack(__float_as_uint(e0), __float_as_uint(e1)));
+          pk[i >> 1] = pack2<T>(e0, e1);
+        }
+        tmem_st_32x32b_x16(sbase + c * 16, pk);
+        if (c == 2) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_part[t]);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+      const float2 la = f2_unpack(ls2[0]), lb = f2_unpack(ls2[1]);
+      l_sum += (la.x + la.y) + (lb.x + lb.y);
+    }
+    if (good && n > 0) good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (n - 1) & 1, p.err, kErrWaitEpilogue));
+    if (good) {
+      tc_fence_after();
+      const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;  // (a NaN sum stays a NaN)
+      T* dst = static_cast<T*>(p.out) + static_cast<long long>(s.q0 + row) * p.ldo +
+               static_cast<long long>(t ? head[1] : head[0]) * p.hso;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(obase + c * 32, o);
+          tmem_wait_ld();
+        }
+        if (row < s.lq) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = l_sum != 0.f ? pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv)
+                                  : 0u;  // sees nothing (O may not have been written at all)
+            reinterpret_cast<uint4*>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------- few rows
+//
+// The query rows of one key head (lq tokens x group heads) in tiles of 16.  A sequence of `rt`
+// tiles splits its keys into ceil(lk / (keys_per_share * rt)) shares; a work item is (sequence,
+// tile, share, key head), the head running fastest so that neighbouring blocks read whole rows of
+// the cache.  In a block, 4 warps take 16 keys in turn, straight from global memory into the operand
+// registers of m16n8k16 products, without shared memory:
+//   S = Q K^T  lane (g, t) loads 16 bytes of key g at d = 32 c + 8 t: words (0, 1) and (2, 3) are
+//              the B operands of two products; Q is held in the same (permuted) order of d.
+//   O += P V   lane (g, t) loads 16 bytes of keys 2t, 2t+1, 2t+8, 2t+9 at d = 64 c + 8 g; value i of
+//              these pairs up to the B operand of product i, whose column g is d = 64 c + 8 g + i.
+// The warps' sums meet in shared memory; shares of a sequence go to packed_combine.
+constexpr int kPrWarps = 4;
+constexpr int kPrRows = 16;
+
+__device__ __forceinline__ int rows_tiles(const PkParams& p, const Seq& s) {
+  return static_cast<int>((static_cast<long long>(s.lq) * p.group + kPrRows - 1) / kPrRows);
+}
+__device__ __forceinline__ int rows_shares(const PkParams& p, const Seq& s, int rt) {
+  const long long per = static_cast<long long>(p.keys_per_share) * rt;
+  return s.lk > per ? static_cast<int>((s.lk + per - 1) / per) : 1;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kPrWarps, 3) packed_rows_kernel(const PkParams p) {
+  constexpr int KC = D / 32;  // 16-byte pieces of a lane's key
+  constexpr int VC = D / 64;  // 16-byte pieces of a lane's four value rows
+  __shared__ float so[kPrWarps][kPrRows][D + 4];
+  __shared__ float2 sml[kPrWarps][kPrRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  griddep_wait();
+  griddep_launch_dependents();
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    const int unit = item / p.hk, head = item - unit * p.hk;
+    int before = 0;
+    const int b = find_seq(p.batch, unit, lane, [&](int i) {
+      const Seq s = load_seq(p, i);
+      const int rt = rows_tiles(p, s);
+      return rt * rows_shares(p, s, rt);
+    }, &before);
+    if (b < 0) break;
+    const Seq s = load_seq(p, b);
+    const int shares = rows_shares(p, s, rows_tiles(p, s));
+    const int tile = (unit - before) / shares, share = (unit - before) - tile * shares;
+    const int rows = s.lq * p.group, row0 = tile * kPrRows;
+    // This share's 16-key chunks [c0, c1), cut at the last key that any row of the tile sees.
+    const int last_token = min(row0 + kPrRows, rows) - 1;
+    const int tile_sees = p.causal ? clampi(last_token / p.group + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
+    const int chunks = (s.lk + 15) / 16;
+    const int c0 = static_cast<int>(static_cast<long long>(chunks) * share / shares);
+    const int c1 = min(static_cast<int>(static_cast<long long>(chunks) * (share + 1) / shares), (tile_sees + 15) / 16);
+
+    // Q: rows g and g + 8 of the tile (row r is token r / group, head r % group of the group).
+    uint4 q[2][KC];
+    int sees[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = row0 + g + 8 * i;
+      const int token = min(r, rows - 1) / p.group, h = min(r, rows - 1) - token * p.group;
+      sees[i] = p.causal ? min(s.lk, token + 1 + s.lk - s.lq) : s.lk;
+      const T* src = static_cast<const T*>(p.q) + (s.q0 + token) * p.ldq +
+                     (static_cast<long long>(head) * p.group + h) * p.hsq + 8 * t;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) q[i][c] = __ldg(reinterpret_cast<const uint4*>(src + 32 * c));
+    }
+    const T* kbase = static_cast<const T*>(p.k) + s.k0 * p.ldk + head * p.hsk + 8 * t;
+    const T* vbase = static_cast<const T*>(p.v) + s.k0 * p.ldv + head * p.hsv + 8 * g;
+
+    uint4 kr[2][KC], vr[4][VC];
+    auto load_k = [&](int c) {
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const T* src = kbase + min(c * 16 + nt * 8 + g, s.lk - 1) * p.ldk;  // (past the end: masked below)
+#pragma unroll
+        for (int i = 0; i < KC; ++i) kr[nt][i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
+      }
+    };
+    auto load_v = [&](int c) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = c * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+        const T* src = vbase + key * p.ldv;
+#pragma unroll
+        for (int k = 0; k < VC; ++k)
+          vr[i][k] = key < tile_sees ? __ldg(reinterpret_cast<const uint4*>(src + 64 * k)) : make_uint4(0, 0, 0, 0);
+      }
+    };
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    if (c0 + warp < c1) {
+      load_k(c0 + warp);
+      load_v(c0 + warp);
+    }
+    for (int c = c0 + warp; c < c1; c += kPrWarps) {
+      float sc[2][4] = {};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          mma_16816<T>(sc[nt], q[0][i].x, q[1][i].x, q[0][i].y, q[1][i].y, kr[nt][i].x, kr[nt][i].y);
+          mma_16816<T>(sc[nt], q[0][i].z, q[1][i].z, q[0][i].w, q[1][i].w, kr[nt][i].z, kr[nt][i].w);
+        }
+      if (c + kPrWarps < c1) load_k(c + kPrWarps);
+      // Scores in log2 units; sc[nt][2i + e] is row g + 8i, key 16c + 8nt + 2t + e.
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = c * 16 + nt * 8 + 2 * t + (j & 1);
+          sc[nt][j] = key < sees[j >> 1] ? sc[nt][j] * p.scale_log2 : -INFINITY;
+          mx[j >> 1] = fmaxf(mx[j >> 1], sc[nt][j]);
+        }
+      float alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        const float top = fmaxf(m[i], mx[i]);
+        alpha[i] = top == m[i] ? 1.f : fast_exp2(m[i] - top);
+        m[i] = top;
+        l[i] *= alpha[i];
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= alpha[0];
+          o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1];
+          o[i][3] *= alpha[1];
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float shift = m[i] == -INFINITY ? 0.f : m[i];
+          const float e0 = fast_exp2(sc[nt][2 * i] - shift), e1 = fast_exp2(sc[nt][2 * i + 1] - shift);
+          l[i] += e0 + e1;
+          pa[2 * nt + i] = pack2<T>(e0, e1);
+        }
+#pragma unroll
+      for (int k = 0; k < VC; ++k) {
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vr[0][k]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vr[1][k]);
+        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vr[2][k]);
+        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vr[3][k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
+          mma_16816<T>(o[8 * k + i], pa[0], pa[1], pa[2], pa[3], __byte_perm(v0[i >> 1], v1[i >> 1], pick),
+                       __byte_perm(v2[i >> 1], v3[i >> 1], pick));
+        }
+      }
+      if (c + kPrWarps < c1) load_v(c + kPrWarps);
+    }
+    // The warps' statistics and sums, then 8 threads per row.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+      if (t == 0) sml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+    }
+#pragma unroll
+    for (int k = 0; k < VC; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // column 2t + e of product i is d = 64 k + 8 (2t + e) + i
+        so[warp][g][64 * k + 16 * t + i] = o[8 * k + i][0];
+        so[warp][g][64 * k + 16 * t + 8 + i] = o[8 * k + i][1];
+        so[warp][g + 8][64 * k + 16 * t + i] = o[8 * k + i][2];
+        so[warp][g + 8][64 * k + 16 * t + 8 + i] = o[8 * k + i][3];
+      }
+    __syncthreads();
+    const int r = threadIdx.x >> 3, part = threadIdx.x & 7;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kPrWarps; ++w) top = fmaxf(top, sml[w][r].x);
+    float sum = 0.f, acc[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPrWarps; ++w) {
+      const float2 ml = sml[w][r];
+      const float wgt = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      if (ml.x == -INFINITY) continue;
+      sum += wgt * ml.y;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) acc[i] += wgt * so[w][r][part * (D / 8) + i];
+    }
+    if (row0 + r < rows) {
+      if (shares > 1) {
+        if (item < p.slots) {
+          float* dst = p.part_o + (static_cast<long long>(item) * kPrRows + r) * D + part * (D / 8);
+#pragma unroll
+          for (int i = 0; i < D / 8; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          if (part == 0) p.part_ml[static_cast<long long>(item) * kPrRows + r] = make_float2(top, sum);
+        }
+      } else {
+        const int token = (row0 + r) / p.group, h = (row0 + r) - token * p.group;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso +
+                 part * (D / 8);
+#pragma unroll
+        for (int i = 0; i < D / 8; i += 8)
+          *reinterpret_cast<uint4*>(dst + i) =
+              make_uint4(pack2<T>(acc[i] * inv, acc[i + 1] * inv), pack2<T>(acc[i + 2] * inv, acc[i + 3] * inv),
+                         pack2<T>(acc[i + 4] * inv, acc[i + 5] * inv), pack2<T>(acc[i + 6] * inv, acc[i + 7] * inv));
+      }
+    }
+    __syncthreads();  // the shared buffers are reused by the next item
+  }
+}
+
+// Joins the shares of every row tile whose sequence was split: with share i holding (m_i, l_i) and O_i,
+// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  A block takes (tile, key head) items.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) packed_combine_kernel(const PkParams p) {
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  for (int item = blockIdx.x;; item += gridDim.x) {
+    const int unit = item / p.hk, head = item - unit * p.hk;
+    // Units here are row tiles; the slots before this sequence's are counted beside them.
+    int before = 0;
+    const int b = find_seq(p.batch, unit, lane, [&](int i) { return rows_tiles(p, load_seq(p, i)); }, &before);
+    if (b < 0) break;
+    const Seq s = load_seq(p, b);
+    const int rt = rows_tiles(p, s), shares = rows_shares(p, s, rt);
+    if (shares == 1) continue;
+    int slots = 0;
+    for (int i = lane; i < b; i += 32) {
+      const Seq x = load_seq(p, i);
+      const int n = rows_tiles(p, x);
+      slots += n * rows_shares(p, x, n);
+    }
+    slots = __reduce_add_sync(0xffffffffu, slots) + (unit - before) * shares;
+    const int rows = s.lq * p.group, row = (unit - before) * kPrRows + (threadIdx.x >> 3), part = threadIdx.x & 7;
+    if (row >= rows || (slots + shares) * static_cast<long long>(p.hk) > p.slots) continue;
+    const long long first = (static_cast<long long>(slots) * p.hk + head) * kPrRows + (threadIdx.x >> 3);
+    const long long step = static_cast<long long>(p.hk) * kPrRows;
+    float top = -INFINITY;
+    for (int i = 0; i < shares; ++i) top = fmaxf(top, p.part_ml[first + i * step].x);
+    float sum = 0.f, acc[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
+    for (int i = 0; i < shares; ++i) {
+      const float2 ml = p.part_ml[first + i * step];
+      if (ml.x == -INFINITY) continue;
+      const float wgt = fast_exp2(ml.x - top);
+      sum += wgt * ml.y;
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + (first + i * step) * D + part * (D / 8));
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const float4 v = src[k];
+        acc[4 * k] += wgt * v.x;
+        acc[4 * k + 1] += wgt * v.y;
+        acc[4 * k + 2] += wgt * v.z;
+        acc[4 * k + 3] += wgt * v.w;
+      }
+    }
+    const int token = row / p.group, h = row - token * p.group;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso +
+             part * (D / 8);
+#pragma unroll
+    for (int i = 0; i < D / 8; i += 8)
+      *reinterpret_cast<uint4*>(dst + i) =
+          make_uint4(pack2<T>(acc[i] * inv, acc[i + 1] * inv), pack2<T>(acc[i + 2] * inv, acc[i + 3] * inv),
+                     pack2<T>(acc[i + 4] * inv, acc[i + 5] * inv), pack2<T>(acc[i + 6] * inv, acc[i + 7] * inv));
+  }
+}
+
+// ---------------------------------------------------------------------------- host side
+
+// What a call runs, from its sizes alone (the offsets are on the device).
+struct PkPlan {
+  bool rows = false;       // packed_rows (+ packed_combine), else packed_tiles
+  int keys_per_share = 0;
+  int64_t slots = 0;       // shares, an upper bound over all offsets that fit the totals
+  size_t o_bytes = 0, bytes = 0;
+};
+
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+PkPlan plan(const b2g_attention_packed_desc* d, int sms) {
+  PkPlan r;
+  const int64_t group = d->n_head / d->n_kv_head;
+  // Rows per key head: up to 16 on average fit one tile of packed_rows.
+  r.rows = d->total_q * group <= kPrRows * d->batch || d->total_k == 0;
+  if (!r.rows) return r;
+  // Shares that give every SM about 6 blocks' worth (two rounds of its 3), of 256 keys at least.
+  const int64_t want = 6 * static_cast<int64_t>(sms);
+  int64_t per = round_up((d->total_k * d->n_kv_head + want - 1) / want, 64);
+  if (per < 256) per = 256;
+  r.keys_per_share = static_cast<int>(per < (1 << 30) ? per : (1 << 30));
+  // sum over sequences of rt * ceil(lk / (per * rt)) <= total_k / per + sum of rt.
+  const int64_t tiles = d->total_q * group / kPrRows + d->batch;
+  r.slots = (d->total_k / per + tiles) * d->n_kv_head;
+  r.o_bytes = static_cast<size_t>(round_up(r.slots * kPrRows * d->d_head * 4, 256));
+  r.bytes = r.o_bytes + static_cast<size_t>(r.slots) * kPrRows * sizeof(float2);
+  return r;
+}
+
+template <typename T, int D>
+b2g_status launch_rows(const PkParams& p, const PkPlan& pl, int64_t tiles, int sms, cudaStream_t st) {
+  const int64_t most = 3ll * sms;
+  const int64_t blocks = pl.slots < most ? pl.slots : most;
+  b2g_status s = launch_pdl(packed_rows_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrWarps), 0, st,
+                            "packed_rows launch", p);
+  if (s != B2G_OK || p.total_k <= p.keys_per_share) return s;  // (no sequence can have been split)
+  const int64_t items = tiles * p.hk;
+  return launch_pdl(packed_combine_kernel<T, D>, dim3(static_cast<unsigned>(items < 4 * most ? items : 4 * most)),
+                    dim3(128), 0, st, "packed_combine launch", p);
+}
+
+template <typename T, int D, bool kHeadPairs>
+b2g_status launch_tiles(const PkParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                        cudaStream_t st) {
+  constexpr uint32_t smem = PtLayout<D>::kSmem;
+  static_assert(smem <= 227 * 1024, "shared memory budget");
+  auto kern = packed_tiles_kernel<T, D, kHeadPairs>;
+  b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+                            "cudaFuncSetAttribute(packed_tiles)");
+  if (s != B2G_OK) return s;
+  constexpr int kSpan = kHeadPairs ? kPtRows : 2 * kPtRows;
+  const dim3 grid(static_cast<unsigned>(p.total_q / kSpan + p.batch), static_cast<unsigned>(kHeadPairs ? p.hq / 2 : p.hq));
+  return launch_pdl(kern, grid, dim3(kPtThreads), smem, st, "packed_tiles launch", tq, tk, tv, p);
+}
+
+template <typename T, int D>
+b2g_status run_packed(const b2g_attention_packed_desc* d, PkParams p, void* ws, const PkPlan& pl, int sms,
+                      cudaStream_t st) {
+  if (pl.rows) {
+    p.keys_per_share = pl.keys_per_share;
+    p.slots = static_cast<int>(pl.slots);
+    p.part_o = static_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.o_bytes);
+    return launch_rows<T, D>(p, pl, static_cast<int64_t>(p.total_q) * p.group / kPrRows + p.batch, sms, st);
+  }
+  CUtensorMap tq, tk, tv;
+  b2g_status s;
+  const b2g_dtype dt = d->dtype;
+  if ((s = make_operand_map(&tq, p.q, dt, D, p.total_q, p.ldq, p.hq, p.hsq, kPtRows)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tk, p.k, dt, D, p.total_k, p.ldk, p.hk, p.hsk, kPtKeys)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tv, p.v, dt, D, p.total_k, p.ldv, p.hk, p.hsv, kPtKeys)) != B2G_OK) return s;
+  return p.group % 2 == 0 ? launch_tiles<T, D, true>(p, tq, tk, tv, st) : launch_tiles<T, D, false>(p, tq, tk, tv, st);
+}
+
+// A stride of a dimension that has one element says nothing: any valid one.
+int64_t used(int64_t stride, int64_t extent, int64_t fallback) { return extent > 1 ? stride : fallback; }
+
+b2g_status check_packed(const b2g_attention_packed_desc* d) {
+  if (!d) return set_error(B2G_ERR_INVALID, "b2g_attention_packed: null descriptor");
+  if (d->batch < 0 || d->total_q < 0 || d->total_k < 0 || d->n_head < 0 || d->n_kv_head < 0)
+    return set_error(B2G_ERR_INVALID, "b2g_attention_packed: negative size");
+  if (d->dtype != B2G_BF16 && d->dtype != B2G_F16)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: BF16 or F16 operands");
+  if (d->d_head != 64 && d->d_head != 128)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: head dim must be 64 or 128");
+  if (d->n_head > 0 && (d->n_kv_head < 1 || d->n_head % d->n_kv_head != 0))
+    return set_error(B2G_ERR_INVALID, "b2g_attention_packed: n_head must be a multiple of n_kv_head");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale))
+    return set_error(B2G_ERR_INVALID, "b2g_attention_packed: scale must be positive");
+  if (d->batch > 65536 || d->total_q > (1ll << 30) || d->total_k > (1ll << 30) || d->n_head > 65535)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: size");
+  return B2G_OK;
+}
+
+}  // namespace
+
+size_t attention_packed_workspace(const b2g_attention_packed_desc* d) {
+  DeviceInfo* dev = nullptr;
+  if (check_packed(d) != B2G_OK || d->batch == 0 || d->total_q == 0 || d->n_head == 0 || device_info(&dev) != B2G_OK)
+    return 0;
+  return plan(d, dev->num_sms).bytes;
+}
+
+b2g_status attention_packed(const b2g_attention_packed_desc* d, void* workspace, size_t workspace_bytes,
+                            cudaStream_t st) {
+  b2g_status s = check_packed(d);
+  if (s != B2G_OK) return s;
+  if (d->batch == 0 || d->total_q == 0 || d->n_head == 0) return B2G_OK;
+  if (!d->q || !d->out || !d->cu_q || !d->cu_k || (d->total_k > 0 && (!d->k || !d->v)))
+    return set_error(B2G_ERR_INVALID, "b2g_attention_packed: null operand");
+  const int64_t D = d->d_head;
+  PkParams p{};
+  p.ldq = used(d->ldq, d->total_q, d->n_head * D); p.hsq = used(d->hsq, d->n_head, D);
+  p.ldk = used(d->ldk, d->total_k, d->n_kv_head * D); p.hsk = used(d->hsk, d->n_kv_head, D);
+  p.ldv = used(d->ldv, d->total_k, d->n_kv_head * D); p.hsv = used(d->hsv, d->n_kv_head, D);
+  p.ldo = used(d->ldo, d->total_q, d->n_head * D); p.hso = used(d->hso, d->n_head, D);
+  const int64_t strides[8] = {p.ldq, p.hsq, p.ldk, p.hsk, p.ldv, p.hsv, p.ldo, p.hso};
+  for (int64_t x : strides) {
+    if (x < D) return set_error(B2G_ERR_INVALID, "b2g_attention_packed: a token or head stride is below the head dim");
+    if (x % 8 != 0 || x >= (1ll << 38))
+      return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: strides must be multiples of 8 elements");
+  }
+  if ((reinterpret_cast<uintptr_t>(d->q) | reinterpret_cast<uintptr_t>(d->k) | reinterpret_cast<uintptr_t>(d->v) |
+       reinterpret_cast<uintptr_t>(d->out)) & 15u)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: 16-byte aligned operands required");
+  DeviceInfo* dev = nullptr;
+  if ((s = device_info(&dev)) != B2G_OK) return s;
+  p.cu_q = d->cu_q; p.cu_k = d->cu_k; p.k_lens = d->k_lens;
+  p.batch = static_cast<int>(d->batch);
+  p.total_q = static_cast<int>(d->total_q); p.total_k = static_cast<int>(d->total_k);
+  p.hq = d->n_head; p.hk = d->n_kv_head; p.group = d->n_head / d->n_kv_head;
+  p.causal = d->causal ? 1 : 0;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.q = d->q; p.k = d->k; p.v = d->v; p.out = d->out;
+  p.err = dev->err_word;
+  PkPlan pl = plan(d, dev->num_sms);
+  void* ws = workspace;
+  if (pl.bytes > 0) {
+    if (pl.slots > (1ll << 30)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: size");
+    if (!ws && (s = workspace_get(pl.bytes, &ws, kWsAttnSplit)) != B2G_OK) return s;
+    if (workspace && (workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+      return set_error(B2G_ERR_INVALID, "b2g_attention_packed: the workspace is too small or not 256-byte aligned");
+  }
+  if (d->dtype == B2G_F16)
+    return D == 128 ? run_packed<__half, 128>(d, p, ws, pl, dev->num_sms, st)
+                    : run_packed<__half, 64>(d, p, ws, pl, dev->num_sms, st);
+  return D == 128 ? run_packed<__nv_bfloat16, 128>(d, p, ws, pl, dev->num_sms, st)
+                  : run_packed<__nv_bfloat16, 64>(d, p, ws, pl, dev->num_sms, st);
+}
+
+}  // namespace b2g

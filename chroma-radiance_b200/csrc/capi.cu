@@ -209,6 +209,8 @@ b2g_status desc_to_problem(const b2g_gemm_desc* d, const char* who, GemmProblem*
     return set_error(B2G_ERR_UNSUPPORTED, w + ": unknown epilogue");
   if (d->a_dtype == B2G_E4M3 || d->b_dtype == B2G_E4M3 || d->d_dtype == B2G_E4M3)
     return set_error(B2G_ERR_UNSUPPORTED, w + ": E4M3 operands are not implemented");
+  if (d->a_dtype == B2G_S8 || d->b_dtype == B2G_S8 || d->d_dtype == B2G_S8)
+    return set_error(B2G_ERR_UNSUPPORTED, w + ": S8 operands go through b2g_gemm_s8");
   const bool ab16 = d->b_dtype == B2G_BF16 || d->b_dtype == B2G_F16;
   if (!(d->a_dtype == d->b_dtype || (d->a_dtype == B2G_F32 && ab16)))
     return set_error(B2G_ERR_UNSUPPORTED, w + ": unsupported operand dtype combination");
@@ -468,6 +470,29 @@ b2g_status b2g_gemm_fp8(const b2g_gemm_desc* d, const float* a_scale, const floa
   std::string why;
   if (!tc_gemm_supported(p, &why)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_gemm_fp8: " + why);
   return tc_gemm_launch(p, st);
+}
+
+b2g_status b2g_quantize_s8(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
+                           int64_t dst_ld, float* scales, void* stream) {
+  return quantize_rows_s8(src, src_dtype, rows, cols, ld, dst, dst_ld, scales, static_cast<cudaStream_t>(stream));
+}
+
+size_t b2g_gemm_s8_workspace(int64_t M, int64_t K, b2g_dtype a_dtype) { return gemm_s8_workspace(M, K, a_dtype); }
+
+b2g_status b2g_gemm_s8(const b2g_gemm_desc* desc, const float* a_scale, const float* b_scale, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return gemm_s8(desc, a_scale, b_scale, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+b2g_status b2g_qk_norm_rope(const b2g_qk_norm_rope_desc* desc, void* stream) {
+  return qk_norm_rope(desc, static_cast<cudaStream_t>(stream));
+}
+
+size_t b2g_attention_packed_workspace(const b2g_attention_packed_desc* desc) { return attention_packed_workspace(desc); }
+
+b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  return attention_packed(desc, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 b2g_status b2g_gemm_fp8_group(const b2g_gemm_desc* descs, const float* const* a_scales,

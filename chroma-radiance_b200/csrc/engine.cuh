@@ -28,7 +28,7 @@ struct GemmProblem {
                             // stage to nearest TF32 before the MMAs read it (1-CTA kernels)
   float alpha = 1.0f;       // D = epilogue(alpha * A.B^T + bias); internal (attention scores)
   bool allow_split = true;  // false: never split K (split-K needs workspace; b2g_gemm_noalloc)
-  // E4M3 operands: D = (sum_k A.B) * a_scale[m] * b_scale[n] + bias, before the epilogue.
+  // E4M3 and S8 operands: D = (sum_k A.B) * a_scale[m] * b_scale[n] + bias, before the epilogue.
   const float* a_scale = nullptr;
   const float* b_scale = nullptr;
   // Tensor-parallel row-split layer (epilogue kEpiTpReduce): this rank's partial product is
@@ -130,6 +130,21 @@ b2g_status make_operand_map(CUtensorMap* map, const void* base, b2g_dtype dt, in
 // dst[r, c] = E4M3(src[r, c] * 448 / absmax_r), round to nearest even, saturating.
 b2g_status quantize_rows_e4m3(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld,
                               uint8_t* dst, int64_t dst_ld, float* scales, cudaStream_t st);
+
+// 8-bit integer linear layers (s8.cu); see b2g_quantize_s8 and b2g_gemm_s8.
+b2g_status quantize_rows_s8(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
+                            int64_t dst_ld, float* scales, cudaStream_t st);
+size_t gemm_s8_workspace(int64_t M, int64_t K, b2g_dtype a_dtype);
+b2g_status gemm_s8(const b2g_gemm_desc* d, const float* a_scale, const float* b_scale, void* workspace,
+                   size_t workspace_bytes, cudaStream_t st);
+
+// Per-head norm and multi-axis rotation (qk_norm_rope.cu); see b2g_qk_norm_rope.
+b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st);
+
+// Attention over packed sequences (attention_packed.cu); see b2g_attention_packed.
+size_t attention_packed_workspace(const b2g_attention_packed_desc* d);
+b2g_status attention_packed(const b2g_attention_packed_desc* d, void* workspace, size_t workspace_bytes,
+                            cudaStream_t st);
 
 // residual[m, n] += gate[n] * (y[m, n] + bias[n]) after a tensor-parallel all-reduce
 // (elementwise.cu); y BF16 or F32, bias may be NULL.

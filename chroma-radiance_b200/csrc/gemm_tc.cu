@@ -34,6 +34,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include "activations.cuh"
 #include "engine.cuh"
 #include "ptx_sm100.cuh"
 
@@ -53,9 +54,10 @@ constexpr int kThreadsK = KIND == 1 ? kThreads + 32 * kRoundWarps : kThreads;
 constexpr int kEpiThreads = 256;
 constexpr int kEpiWarps = 8;
 // K elements per 128-byte stage row: 64 for bf16/fp16 (KIND 0), 32 for tf32 (KIND 1), 128
-// for E4M3 (KIND 2, kind::f8f6f4).
+// for E4M3 (KIND 2, kind::f8f6f4) and for 8-bit integers (KIND 3, kind::i8, whose accumulators
+// are 32-bit integers: exact, and converted to fp32 once, when the scales are applied).
 template <int KIND>
-constexpr int kKElems = KIND == 1 ? 32 : (KIND == 2 ? 128 : 64);
+constexpr int kKElems = KIND == 1 ? 32 : (KIND >= 2 ? 128 : 64);
 enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2 };
 
 // Output staging: one 4 KB buffer per epilogue warp (32 rows x 32 fp32 or 16-bit columns),
@@ -63,9 +65,9 @@ enum { OUT_F32 = 0, OUT_BF16 = 1, OUT_F16 = 2 };
 constexpr int kOutBufBytes = 4096;
 constexpr int kOutStageBytes = kEpiWarps * kOutBufBytes;  // 32 KB
 constexpr int kBiasBytes = 256 * 4;                       // bias of one tile (<= 256 columns)
-// E4M3 kernels also stage the tile's per-column weight scales (same size as the bias).
+// E4M3 and integer kernels also stage the tile's per-column weight scales (same size as the bias).
 template <int KIND>
-constexpr int kScaleBytes = KIND == 2 ? kBiasBytes : 0;
+constexpr int kScaleBytes = KIND >= 2 ? kBiasBytes : 0;
 
 // A launch computes up to kMaxGroups independent problems that share N, K, dtypes and the
 // epilogue (the txt and img streams of a double block: same layer shapes, their own rows,
@@ -82,8 +84,8 @@ struct TcGroup {
   long long ldd;
   const void* bias;
   const float* gate;
-  const float* a_scale;    // E4M3: per-row scale of A [M]
-  const float* b_scale;    // E4M3: per-column scale of B [N]
+  const float* a_scale;    // E4M3, S8: per-row scale of A [M]
+  const float* b_scale;    // E4M3, S8: per-column scale of B [N]
   long long tp_row0;       // tensor-parallel reduce: first row in the partial/residual buffers
   const float* pe;         // kEpiQkvRope: RoPE table rows of the group's first token [M][64][4]
   const float* qn;         // kEpiQkvRope: RMSNorm scales of q and k heads [128] (NULL: none)
@@ -213,25 +215,6 @@ __device__ __forceinline__ void item_coords(int item, const TcParams& p, int& ti
   tile = p.dp_tiles + (j - split * rest);
   kb0 = static_cast<int>(static_cast<long long>(split) * p.num_k_blocks / p.splits);
   kb1 = static_cast<int>(static_cast<long long>(split + 1) * p.num_k_blocks / p.splits);
-}
-
-// tanh-form GELU, the formula of the reference's gelu_val (kernels.cu:266-269).
-// Evaluated through the identity 0.5 v (1 + tanh(u)) = v * sigmoid(2u) = v / (1 + e^(-2u)),
-// with e^(-2u) = 2^(-2u log2(e)) from the hardware base-2 exponential (ex2.approx, relative
-// error ~2^-22) and a fast division: a few instructions instead of an accurate tanhf, and
-// within a few fp32 ulps of the formula.  The exponent is capped at 2^126 (the quotient is
-// then -0 to fp32 precision, GELU's limit for large negative v).
-__device__ __forceinline__ float gelu_tanh(float v) {
-  const float u = 0.7978845608f * (v + 0.044715f * v * v * v);
-  const float e = fast_exp2(fminf(-2.8853900817779268f * u, 126.0f));
-  return __fdividef(v, 1.0f + e);
-}
-
-// SiLU, the formula of the reference's silu_val (kernels.cu): v / (1 + e^-v), with e^-v from
-// the hardware base-2 exponential (capped at 2^126, where the quotient is -0 to fp32
-// precision) and a fast division.
-__device__ __forceinline__ float silu_fast(float v) {
-  return __fdividef(v, 1.0f + fast_exp2(fminf(-1.4426950408889634f * v, 126.0f)));
 }
 
 // alpha * acc + bias (bias staged in shared memory, zero past N), then GELU or SiLU if asked.
@@ -457,8 +440,14 @@ __device__ __forceinline__ void stage_scale(const TcParams& p, const TcGroup& G,
   }
 }
 
-// acc * a_scale[row] * b_scale[column] for one 32-column chunk (E4M3 operands).
+// acc * a_scale[row] * b_scale[column] for one 32-column chunk (E4M3 operands; 8-bit integer
+// operands, KIND 3, whose 32-bit integer sums become fp32 first).
+template <int KIND>
 __device__ __forceinline__ void scale_chunk(uint32_t (&r)[32], float rs, const float* cs) {
+  if constexpr (KIND == 3) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__int2float_rn(static_cast<int>(r[j])));
+  }
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     const float4 c = *reinterpret_cast<const float4*>(cs + j);
@@ -637,7 +626,7 @@ __device__ __forceinline__ void qkv_rope_item(const TcParams& p, const TcGroup& 
   const int col = n_base + c0 * 32;    // first column of the head (uniform across the warp)
   const int m_warp0 = m - e.lane;
   float rs = 0.f;                      // E4M3: this row's activation scale
-  if constexpr (KIND == 2) rs = m < G.M ? __ldg(G.a_scale + m) : 0.f;
+  if constexpr (KIND >= 2) rs = m < G.M ? __ldg(G.a_scale + m) : 0.f;
   if (p.split && col >= p.split) {
     const float* sbg = p.bias_kind ? e.sbias + c0 * 32 : nullptr;
     uint32_t r[2][32];
@@ -647,7 +636,7 @@ __device__ __forceinline__ void qkv_rope_item(const TcParams& p, const TcGroup& 
       tmem_wait_ld();
       if (i + 1 < 4) tmem_ld_32x32b_x32(tacc + (c0 + i + 1) * 32, r[(i + 1) & 1]);
       if (i == 3) release();
-      if constexpr (KIND == 2) scale_chunk(r[i & 1], rs, e.sscale + (c0 + i) * 32);
+      if constexpr (KIND >= 2) scale_chunk<KIND>(r[i & 1], rs, e.sscale + (c0 + i) * 32);
       float v[32];
       chunk_values<B2G_EPI_GELU>(r[i & 1], sbg ? sbg + i * 32 : nullptr, p.alpha, v);
       if (m_warp0 < G.M && col + i * 32 < p.N)
@@ -668,7 +657,7 @@ __device__ __forceinline__ void qkv_rope_item(const TcParams& p, const TcGroup& 
       float v[32];
       tmem_ld_32x32b_x32(tacc + (c0 + i) * 32, r);
       tmem_wait_ld();
-      if constexpr (KIND == 2) scale_chunk(r, rs, e.sscale + (c0 + i) * 32);
+      if constexpr (KIND >= 2) scale_chunk<KIND>(r, rs, e.sscale + (c0 + i) * 32);
       chunk_values<B2G_EPI_NONE>(r, sb ? sb + i * 32 : nullptr, p.alpha, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) ss += v[j] * v[j];
@@ -690,7 +679,7 @@ __device__ __forceinline__ void qkv_rope_item(const TcParams& p, const TcGroup& 
     tmem_wait_ld();
     if (i + 1 < 4) tmem_ld_32x32b_x32(tacc + (c0 + i + 1) * 32, r[(i + 1) & 1]);
     if (i == 3) release();
-    if constexpr (KIND == 2) scale_chunk(r[i & 1], rs, e.sscale + (c0 + i) * 32);
+    if constexpr (KIND >= 2) scale_chunk<KIND>(r[i & 1], rs, e.sscale + (c0 + i) * 32);
     float v[32];
     chunk_values<B2G_EPI_NONE>(r[i & 1], sb ? sb + i * 32 : nullptr, p.alpha, v);
     if (sec < 2) {
@@ -750,7 +739,7 @@ __device__ __forceinline__ void epilogue_item(const TcParams& p, const TcGroup& 
     return;
   }
   float rs = 0.f;  // E4M3: this row's activation scale
-  if constexpr (KIND == 2) rs = m < G.M ? __ldg(G.a_scale + m) : 0.f;
+  if constexpr (KIND >= 2) rs = m < G.M ? __ldg(G.a_scale + m) : 0.f;
   constexpr int NCH = BN / 64;  // 32-column chunks per warp (half of the tile's columns)
   const int c0 = e.half * NCH;
   const int m_warp0 = m - e.lane;
@@ -770,7 +759,7 @@ __device__ __forceinline__ void epilogue_item(const TcParams& p, const TcGroup& 
     if (i == NCH - 1) release();
     const int c = c0 + i;
     if (!splitk) {
-      if constexpr (KIND == 2) scale_chunk(r[i & 1], rs, e.sscale + c * 32);
+      if constexpr (KIND >= 2) scale_chunk<KIND>(r[i & 1], rs, e.sscale + c * 32);
       emit_chunk<EPI, OUT>(p, G, tmD, e.buf, obuf, bz, m, m_warp0, n_base + c * 32, r[i & 1],
                            sb ? sb + c * 32 : nullptr, e.lane);
     } else {
@@ -809,7 +798,7 @@ __device__ __forceinline__ void epilogue_item(const TcParams& p, const TcGroup& 
         uint32_t rr[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) rr[j] = __float_as_uint(acc[j]);
-        if constexpr (KIND == 2) scale_chunk(rr, rs, e.sscale + c * 32);
+        if constexpr (KIND >= 2) scale_chunk<KIND>(rr, rs, e.sscale + c * 32);
         emit_chunk<EPI, OUT>(p, G, tmD, e.buf, obuf, bz, m, m_warp0, n_base + c * 32, rr,
                              sb ? sb + c * 32 : nullptr, e.lane);
       }
@@ -943,12 +932,13 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
           const uint32_t b0 = smem_u32(sB + stage * B_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            // One MMA consumes 32 bytes of K (16 bf16/fp16, 8 tf32 or 32 E4M3 elements) inside the
+            // One MMA consumes 32 bytes of K (16 bf16/fp16, 8 tf32, 32 E4M3 or S8) inside the
             // 128-byte swizzle row: advance the descriptors by 32 bytes.
             const uint64_t ad = smem_desc_k_sw128(a0 + k * 32), bd = smem_desc_k_sw128(b0 + k * 32);
             const uint32_t accum = (kb != kb0 || k != 0) ? 1u : 0u;
             if constexpr (KIND == 1) umma_tf32(d_tmem, ad, bd, p.idesc, accum);
             else if constexpr (KIND == 2) umma_f8(d_tmem, ad, bd, p.idesc, accum);
+            else if constexpr (KIND == 3) umma_i8(d_tmem, ad, bd, p.idesc, accum);
             else umma_f16(d_tmem, ad, bd, p.idesc, accum);
           }
           umma_commit(&empty_bar[stage]);
@@ -1013,7 +1003,7 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
       const TcGroup& G = p.g[gi];
       if constexpr (EPI == B2G_EPI_GATED_RESIDUAL) prefetch_residual<BN>(p, G, e, bz, mb * kBM + e.row, nb * BN);
       stage_bias<BN>(p, G, sBias, nb * BN);
-      if constexpr (KIND == 2) stage_scale<BN>(p, G, sScale, nb * BN);
+      if constexpr (KIND >= 2) stage_scale<BN>(p, G, sScale, nb * BN);
       const uint32_t acc = local & 1u;
       const uint32_t acc_phase = (local >> 1) & 1u;
       const bool ok = mbar_wait(&tfull_bar[acc], acc_phase, p.err, kErrWaitEpilogue);
@@ -1180,6 +1170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t accum = (kb != kb0 || k != 0) ? 1u : 0u;
             if constexpr (KIND == 1) umma_tf32_pair(d_tmem, ad, bd, idesc, accum);
             else if constexpr (KIND == 2) umma_f8_pair(d_tmem, ad, bd, idesc, accum);
+            else if constexpr (KIND == 3) umma_i8_pair(d_tmem, ad, bd, idesc, accum);
             else umma_f16_pair(d_tmem, ad, bd, idesc, accum);
           }
           umma_commit_pair_bcast(&empty_bar[stage], 0x3);
@@ -1218,7 +1209,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if constexpr (EPI == B2G_EPI_GATED_RESIDUAL)
         prefetch_residual<BN>(p, G, e, bz, mb * 256 + static_cast<int>(rank) * 128 + e.row, nb * BN);
       stage_bias<BN>(p, G, sBias, nb * BN);
-      if constexpr (KIND == 2) stage_scale<BN>(p, G, sScale, nb * BN);
+      if constexpr (KIND >= 2) stage_scale<BN>(p, G, sScale, nb * BN);
       const uint32_t acc = local & 1u;
       const uint32_t acc_phase = (local >> 1) & 1u;
       const bool ok = mbar_wait(&tfull_bar[acc], acc_phase, p.err, kErrWaitEpilogue);
@@ -1298,13 +1289,13 @@ b2g_status make_operand_map(CUtensorMap* map, const void* base, b2g_dtype dt, in
   if (s != B2G_OK) return s;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(batch)};
-  const cuuint64_t esz = dt == B2G_F32 ? 4u : (dt == B2G_E4M3 ? 1u : 2u);
+  const cuuint64_t esz = dt == B2G_F32 ? 4u : (dt == B2G_E4M3 || dt == B2G_S8 ? 1u : 2u);
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * esz, static_cast<cuuint64_t>(bstride) * esz};
   const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esz), box_rows, 1u};  // 128-byte rows
   const cuuint32_t estr[3] = {1u, 1u, 1u};
   const CUtensorMapDataType t = dt == B2G_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : dt == B2G_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                : dt == B2G_E4M3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : dt == B2G_E4M3 || dt == B2G_S8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = g_encode(map, t, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1358,7 +1349,7 @@ b2g_status launch_one(const TcMaps& maps, const TcParams& prm, int grid, cudaStr
   }
 }
 
-// Epilogue and output-type dispatch for 16-bit (KIND 0) and E4M3 (KIND 2) operands.
+// Epilogue and output-type dispatch for 16-bit (KIND 0), E4M3 (KIND 2) and S8 (KIND 3) operands.
 template <bool PAIR, int BN, int STAGES, int KIND>
 b2g_status dispatch_out(const TcMaps& maps, const TcParams& prm, int grid, b2g_epilogue epi, b2g_dtype out,
                         cudaStream_t st) {
@@ -1367,8 +1358,9 @@ b2g_status dispatch_out(const TcMaps& maps, const TcParams& prm, int grid, b2g_e
       return launch_one<PAIR, BN, STAGES, kEpiTpReduce, OUT_F32, 0>(maps, prm, grid, st);
   }
   if (static_cast<int>(epi) == kEpiQkvRope) {
-    if constexpr (BN == 256) return launch_one<PAIR, BN, STAGES, kEpiQkvRope, OUT_BF16, KIND>(maps, prm, grid, st);
-    return set_error(B2G_ERR_UNSUPPORTED, "qkv rope epilogue: 256-column tiles only");
+    if constexpr (BN == 256 && KIND != 3)
+      return launch_one<PAIR, BN, STAGES, kEpiQkvRope, OUT_BF16, KIND>(maps, prm, grid, st);
+    return set_error(B2G_ERR_UNSUPPORTED, "qkv rope epilogue: 256-column tiles, no S8 operands");
   }
   if (epi == B2G_EPI_GATED_RESIDUAL)
     return launch_one<PAIR, BN, STAGES, B2G_EPI_GATED_RESIDUAL, OUT_F32, KIND>(maps, prm, grid, st);
@@ -1377,7 +1369,7 @@ b2g_status dispatch_out(const TcMaps& maps, const TcParams& prm, int grid, b2g_e
     if (out == B2G_BF16) return launch_one<PAIR, BN, STAGES, B2G_EPI_GELU, OUT_BF16, KIND>(maps, prm, grid, st);
     return launch_one<PAIR, BN, STAGES, B2G_EPI_GELU, OUT_F16, KIND>(maps, prm, grid, st);
   }
-  if constexpr (KIND == 0) {
+  if constexpr (KIND == 0 || KIND == 3) {
     if (epi == B2G_EPI_SILU) {
       if (out == B2G_F32) return launch_one<PAIR, BN, STAGES, B2G_EPI_SILU, OUT_F32, KIND>(maps, prm, grid, st);
       if (out == B2G_BF16) return launch_one<PAIR, BN, STAGES, B2G_EPI_SILU, OUT_BF16, KIND>(maps, prm, grid, st);
@@ -1389,8 +1381,9 @@ b2g_status dispatch_out(const TcMaps& maps, const TcParams& prm, int grid, b2g_e
   return launch_one<PAIR, BN, STAGES, B2G_EPI_NONE, OUT_F16, KIND>(maps, prm, grid, st);
 }
 
-// kind: 0 = bf16/fp16 (kind::f16), 1 = tf32, 2 = E4M3 (kind::f8f6f4, STAGES8 ring stages: the
-// column-scale staging area costs one stage's worth of shared memory in the larger variants).
+// kind: 0 = bf16/fp16 (kind::f16), 1 = tf32, 2 = E4M3 (kind::f8f6f4) and 3 = S8 (kind::i8), both with
+// STAGES8 ring stages: the column-scale staging area costs one stage's worth of shared memory in
+// the larger variants.
 template <bool PAIR, int BN, int STAGES, int STAGES8>
 b2g_status dispatch_epi(const TcMaps& maps, const TcParams& prm, int grid, b2g_epilogue epi, b2g_dtype out, int kind,
                         cudaStream_t st) {
@@ -1400,6 +1393,7 @@ b2g_status dispatch_epi(const TcMaps& maps, const TcParams& prm, int grid, b2g_e
     return launch_one<PAIR, BN, STAGES, B2G_EPI_NONE, OUT_F32, 1>(maps, prm, grid, st);
   }
   if (kind == 2) return dispatch_out<PAIR, BN, STAGES8, 2>(maps, prm, grid, epi, out, st);
+  if (kind == 3) return dispatch_out<PAIR, BN, STAGES8, 3>(maps, prm, grid, epi, out, st);
   return dispatch_out<PAIR, BN, STAGES, 0>(maps, prm, grid, epi, out, st);
 }
 
@@ -1414,16 +1408,18 @@ bool tc_gemm_supported(const GemmProblem& p, std::string* why) {
   };
   const bool tf32 = p.a_dtype == B2G_F32 && p.b_dtype == B2G_F32 && p.allow_tf32;
   const bool fp8 = p.a_dtype == B2G_E4M3 && p.b_dtype == B2G_E4M3;
+  const bool s8 = p.a_dtype == B2G_S8 && p.b_dtype == B2G_S8;
   if (!((p.a_dtype == B2G_BF16 && p.b_dtype == B2G_BF16) || (p.a_dtype == B2G_F16 && p.b_dtype == B2G_F16) || tf32 ||
-        fp8))
+        fp8 || s8))
     return no("operand dtypes");
-  if (fp8 && (!p.a_scale || !p.b_scale)) return no("E4M3 operands need row and column scales");
+  if ((fp8 || s8) && (!p.a_scale || !p.b_scale)) return no("8-bit operands need row and column scales");
+  if (s8 && p.allow_split) return no("S8 operands: K is never split");
   if (tf32 && (p.epilogue != B2G_EPI_NONE || p.d_dtype != B2G_F32)) return no("tf32: F32 output, no epilogue");
   if (p.d_dtype != B2G_F32 && p.d_dtype != B2G_BF16 && p.d_dtype != B2G_F16) return no("output dtype");
   if (p.epilogue == B2G_EPI_GATED_RESIDUAL && p.d_dtype != B2G_F32) return no("gated residual needs F32 output");
   if (p.bias && p.bias_dtype != B2G_F32 && p.bias_dtype != B2G_BF16) return no("bias dtype");
   if (!aligned16(p.a) || !aligned16(p.b)) return no("operand base not 16-byte aligned");
-  const int64_t align = tf32 ? 3 : (fp8 ? 15 : 7);  // 16-byte row and batch strides
+  const int64_t align = tf32 ? 3 : (fp8 || s8 ? 15 : 7);  // 16-byte row and batch strides
   if ((p.lda & align) || (p.ldb & align)) return no("operand row stride not a multiple of 16 bytes");
   if (p.batch > 1 && ((p.a_bstride & align) || (p.b_bstride & align))) return no("batch stride not 16-byte aligned");
   if (p.M > (1ll << 31) - 256 || p.N > (1ll << 31) - 256 || p.K > (1ll << 31)) return no("size");
@@ -1461,8 +1457,8 @@ b2g_status tc_gemm_launch_group(const GemmProblem* ps, int count, cudaStream_t s
   const int sms = dev->num_sms;
   const int pairs = sms / 2;
   const bool tf32 = p.a_dtype == B2G_F32;
-  const int kind = tf32 ? 1 : (p.a_dtype == B2G_E4M3 ? 2 : 0);
-  const int kelems = kind == 1 ? 32 : (kind == 2 ? 128 : 64);
+  const int kind = tf32 ? 1 : (p.a_dtype == B2G_E4M3 ? 2 : (p.a_dtype == B2G_S8 ? 3 : 0));
+  const int kelems = kind == 1 ? 32 : (kind >= 2 ? 128 : 64);
   const long long nkb = (p.K + kelems - 1) / kelems;
   // Kernel variant and split-K factor from a cost model in units of one 64-wide k-block of
   // a pair tile: whole waves of work items over the SMs (or SM pairs), times the k-blocks
@@ -1577,8 +1573,10 @@ b2g_status tc_gemm_launch_group(const GemmProblem* ps, int count, cudaStream_t s
   prm.alpha = p.alpha;
   prm.round_tf32 = (kind == 1 && p.round_tf32) ? 1 : 0;
   prm.err = dev->err_word;
-  prm.idesc = idesc_make(kind == 1 ? kFmtTF32 : (kind == 2 ? kFmtE4M3 : (p.a_dtype == B2G_BF16 ? kFmtBF16 : kFmtF16)),
-                         tile_m, bn);
+  prm.idesc = kind == 3 ? idesc_make_s8(tile_m, bn)
+                        : idesc_make(kind == 1 ? kFmtTF32
+                                               : (kind == 2 ? kFmtE4M3 : (p.a_dtype == B2G_BF16 ? kFmtBF16 : kFmtF16)),
+                                     tile_m, bn);
   prm.a_keep = a_bytes <= b_bytes ? 1 : 0;
   if (prm.num_tiles == 0) return B2G_OK;
 

@@ -1,0 +1,376 @@
+// qk_norm_rope.cu — per-head RMSNorm of queries and keys and their rotation by positions of
+// several axes, in one pass.
+//
+//   x'    = x * rsqrt(mean(x^2) + eps) * w            per head of D values (w NULL: x' = x)
+//   pair p turned by a = position[axis] * theta^(-2 j / d_axis), the j-th pair of its axis:
+//           (x0, x1) -> (x0 cos a - x1 sin a, x0 sin a + x1 cos a)
+//
+// The axes (time, height, width, ..) take their d_axis / 2 pairs one after the other; values past
+// the sum of the d_axis are normed and not turned.  A pair is two neighbouring values (as the
+// reference's apply_rope_fused_bf16 has it, rope.cuh:180-221, on the table gen_pe builds, rope.cuh:84)
+// or one value of each half of the turned part.  The reference takes the angles from a table made
+// on the host for one image size; here a token's positions are all there is to it, so tokens of
+// images of any size, of clips and of text can be packed in any order.
+//
+// Bound by memory: q and k are read and written once.  A block works on whole tokens: it computes
+// each token's D / 2 cosines and sines once, in shared memory, for all of the token's heads, while the
+// first heads' values are on their way; 8 values per lane, so D / 8 lanes hold a head and its sum of
+// squares takes log2(D / 8) shuffles.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cmath>
+#include <cstdint>
+#include "engine.cuh"
+#include "ptx_sm100.cuh"
+
+namespace b2g {
+
+namespace {
+
+constexpr int kNrThreads = 256;
+constexpr int kNrMaxPairs = 128;  // D <= 256
+constexpr int kNrMaxTokens = 8;   // tokens a block takes at a time
+
+// Pair layouts: neighbours or halves in groups of 8 values per lane, or any (value by value).
+enum { kPairsNeighbours = 0, kPairsHalves = 1, kPairsAny = 2 };
+
+struct NrArgs {
+  const void* x[2];   // q, k
+  void* y[2];
+  long long ldx[2], hsx[2], ldy[2], hsy[2];  // token and head strides in elements
+  const float* norm[2];
+  float eps;
+  const float* pos;
+  long long ldp;
+  long long tokens;
+  int heads, q_heads;  // q heads, then k heads
+  int D, rot;          // head width, values turned
+  int halves;          // kPairsAny: 1 = pairs (p, p + rot / 2)
+  int block_tokens;    // tokens per block and step
+  // Per pair: turns per unit of position, theta^(-2j/d) / (2 pi), as the sum of two floats.
+  float turn_hi[kNrMaxPairs], turn_lo[kNrMaxPairs];
+  unsigned char axis[kNrMaxPairs];
+};
+
+// cos and sin of 2 pi pos (hi + lo).  The product's whole turns are taken off before anything
+// is rounded away: pos * hi and its rounding error are exact as two floats, so the angle is right to
+// 2^-22 of a turn for positions of any size (a product in fp32 radians is off by 2^-24 of the angle,
+// 0.0005 at a position of 8000).
+__device__ __forceinline__ float2 cos_sin_turns(float pos, float hi, float lo) {
+  const float p = pos * hi;
+  const float rest = fmaf(pos, lo, fmaf(pos, hi, -p));
+  const float r = (p - rintf(p)) + rest;
+  float s, c;
+  sincospif(2.f * r, &s, &c);
+  return make_float2(c, s);
+}
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// N values at p (a multiple of N values' bytes).
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float* v) {
+  constexpr int kWords = static_cast<int>(sizeof(T)) * N / 4;
+  uint32_t w[kWords];
+  if constexpr (kWords == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+  else {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(w)[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = to_f(reinterpret_cast<const T*>(w)[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float* v) {
+  constexpr int kWords = static_cast<int>(sizeof(T)) * N / 4;
+  uint32_t w[kWords];
+#pragma unroll
+  for (int i = 0; i < N; ++i) reinterpret_cast<T*>(w)[i] = from_f<T>(v[i]);
+  if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
+  else {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<uint4*>(w)[i];
+  }
+}
+
+// Eight values of a head: four at e0 and four at e1.
+template <typename T, bool kOnePiece>
+__device__ __forceinline__ void load_lane(const T* row, int e0, int e1, float (&v)[8]) {
+  if constexpr (kOnePiece) load_n<T, 8>(row + e0, v);
+  else {
+    load_n<T, 4>(row + e0, v);
+    load_n<T, 4>(row + e1, v + 4);
+  }
+}
+
+// The cosines and sines of `count` tokens from t0 on, [token][pair].
+__device__ __forceinline__ void fill_table(const NrArgs& a, float2* tab, const float* hi, const float* lo,
+                                           const unsigned char* axis, long long t0, int count, int pairs) {
+  for (int i = threadIdx.x; i < count * pairs; i += kNrThreads) {
+    const int b = i / pairs, p = i - b * pairs;
+    tab[b * kNrMaxPairs + p] = cos_sin_turns(__ldg(a.pos + (t0 + b) * a.ldp + axis[p]), hi[p], lo[p]);
+  }
+}
+
+template <typename TI, typename TO, int G, bool kHalves>
+__global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const __grid_constant__ NrArgs a) {
+  __shared__ float2 tab[2][kNrMaxTokens * kNrMaxPairs];
+  __shared__ float hi[kNrMaxPairs], lo[kNrMaxPairs];
+  __shared__ unsigned char axis[kNrMaxPairs];
+  const int pairs = a.rot / 2;
+  for (int p = threadIdx.x; p < pairs; p += kNrThreads) {
+    hi[p] = a.turn_hi[p];
+    lo[p] = a.turn_lo[p];
+    axis[p] = a.axis[p];
+  }
+  __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int kGroups = kNrThreads / G;
+  const int l = threadIdx.x % G, group = threadIdx.x / G;
+  const bool live = l < a.D / 8;  // (D / 8 is not a power of two for every D)
+  const bool turned = 8 * l < a.rot;
+  const int e0 = !kHalves || !turned ? 8 * l : 4 * l, e1 = !kHalves || !turned ? e0 + 4 : a.rot / 2 + 4 * l;
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  float w[2][8];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[s][i] = live && a.norm[s] ? __ldg(a.norm[s] + (i < 4 ? e0 + i : e1 + i - 4)) : 1.f;
+
+  int buf = 0;
+  for (long long t0 = static_cast<long long>(blockIdx.x) * a.block_tokens; t0 < a.tokens;
+       t0 += static_cast<long long>(gridDim.x) * a.block_tokens, buf ^= 1) {
+    const int count = static_cast<int>(min(static_cast<long long>(a.block_tokens), a.tokens - t0));
+    const int items = count * a.heads;
+    auto read = [&](int item, float (&v)[8]) {
+      const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
+      const TI* row = static_cast<const TI*>(s ? a.x[1] : a.x[0]) + (t0 + b) * (s ? a.ldx[1] : a.ldx[0]) +
+                      (s ? h - a.q_heads : h) * (s ? a.hsx[1] : a.hsx[0]);
+      if (live && item < items) load_lane<TI, !kHalves>(row, e0, e1, v);
+      else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      }
+    };
+    float next[8];
+    read(group, next);
+    fill_table(a, tab[buf], hi, lo, axis, t0, count, pairs);
+    __syncthreads();
+    for (int first = 0; first < items; first += kGroups) {  // (every lane takes part in the shuffles)
+      const int item = first + group;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = next[i];
+      read(item + kGroups, next);
+      const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (!live || item >= items) continue;
+      if (s ? a.norm[1] : a.norm[0]) {
+        const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (s ? w[1][i] : w[0][i]);
+      }
+      if (turned) {
+        const float2* cs = tab[buf] + b * kNrMaxPairs + 4 * l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 t = cs[i];
+          const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1;
+          const float x0 = v[i0], x1 = v[i1];
+          v[i0] = fmaf(x0, t.x, -(x1 * t.y));
+          v[i1] = fmaf(x0, t.y, x1 * t.x);
+        }
+      }
+      TO* row = static_cast<TO*>(s ? a.y[1] : a.y[0]) + (t0 + b) * (s ? a.ldy[1] : a.ldy[0]) +
+                (s ? h - a.q_heads : h) * (s ? a.hsy[1] : a.hsy[0]);
+      if constexpr (!kHalves) store_n<TO, 8>(row + e0, v);
+      else {
+        store_n<TO, 4>(row + e0, v);
+        store_n<TO, 4>(row + e1, v + 4);
+      }
+    }
+  }
+}
+
+// Any even D and rot, any alignment: a warp per head, a lane's pairs p = lane, lane + 32, ..
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(kNrThreads) qk_norm_rope_any_kernel(const __grid_constant__ NrArgs a) {
+  __shared__ float2 tab[2][kNrMaxTokens * kNrMaxPairs];
+  __shared__ float hi[kNrMaxPairs], lo[kNrMaxPairs];
+  __shared__ unsigned char axis[kNrMaxPairs];
+  const int pairs = a.rot / 2;
+  for (int p = threadIdx.x; p < pairs; p += kNrThreads) {
+    hi[p] = a.turn_hi[p];
+    lo[p] = a.turn_lo[p];
+    axis[p] = a.axis[p];
+  }
+  __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int buf = 0;
+  for (long long t0 = static_cast<long long>(blockIdx.x) * a.block_tokens; t0 < a.tokens;
+       t0 += static_cast<long long>(gridDim.x) * a.block_tokens, buf ^= 1) {
+    const int count = static_cast<int>(min(static_cast<long long>(a.block_tokens), a.tokens - t0));
+    fill_table(a, tab[buf], hi, lo, axis, t0, count, pairs);
+    __syncthreads();
+    for (int item = warp; item < count * a.heads; item += kNrThreads / 32) {
+      const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
+      const TI* x = static_cast<const TI*>(s ? a.x[1] : a.x[0]) + (t0 + b) * (s ? a.ldx[1] : a.ldx[0]) +
+                    (s ? h - a.q_heads : h) * (s ? a.hsx[1] : a.hsx[0]);
+      TO* y = static_cast<TO*>(s ? a.y[1] : a.y[0]) + (t0 + b) * (s ? a.ldy[1] : a.ldy[0]) +
+              (s ? h - a.q_heads : h) * (s ? a.hsy[1] : a.hsy[0]);
+      const float* norm = s ? a.norm[1] : a.norm[0];
+      float v[kNrMaxPairs / 32][2];
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < kNrMaxPairs / 32; ++j) {
+        const int p = lane + 32 * j;
+        if (2 * p >= a.D) continue;
+        const bool split = a.halves && p < pairs;
+        v[j][0] = to_f(x[split ? p : 2 * p]);
+        v[j][1] = to_f(x[split ? p + pairs : 2 * p + 1]);
+        ss = fmaf(v[j][0], v[j][0], fmaf(v[j][1], v[j][1], ss));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float inv = norm ? rsqrtf(ss / static_cast<float>(a.D) + a.eps) : 1.f;
+#pragma unroll
+      for (int j = 0; j < kNrMaxPairs / 32; ++j) {
+        const int p = lane + 32 * j;
+        if (2 * p >= a.D) continue;
+        const bool split = a.halves && p < pairs;
+        const int i0 = split ? p : 2 * p, i1 = split ? p + pairs : 2 * p + 1;
+        float x0 = v[j][0], x1 = v[j][1];
+        if (norm) {
+          x0 = x0 * inv * __ldg(norm + i0);
+          x1 = x1 * inv * __ldg(norm + i1);
+        }
+        float y0 = x0, y1 = x1;
+        if (p < pairs) {
+          const float2 t = tab[buf][b * kNrMaxPairs + p];
+          y0 = fmaf(x0, t.x, -(x1 * t.y));
+          y1 = fmaf(x0, t.y, x1 * t.x);
+        }
+        y[i0] = from_f<TO>(y0);
+        y[i1] = from_f<TO>(y1);
+      }
+    }
+  }
+}
+
+template <typename TI, typename TO>
+b2g_status launch_nr(const NrArgs& a, int mode, dim3 grid, cudaStream_t st) {
+  const char* what = "qk_norm_rope launch";
+  const dim3 block(kNrThreads);
+  if (mode == kPairsAny) return launch_pdl(qk_norm_rope_any_kernel<TI, TO>, grid, block, 0, st, what, a);
+  const bool h = mode == kPairsHalves;
+  if (a.D <= 64)
+    return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 8, true>, grid, block, 0, st, what, a)
+             : launch_pdl(qk_norm_rope_kernel<TI, TO, 8, false>, grid, block, 0, st, what, a);
+  if (a.D <= 128)
+    return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 16, true>, grid, block, 0, st, what, a)
+             : launch_pdl(qk_norm_rope_kernel<TI, TO, 16, false>, grid, block, 0, st, what, a);
+  return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 32, true>, grid, block, 0, st, what, a)
+           : launch_pdl(qk_norm_rope_kernel<TI, TO, 32, false>, grid, block, 0, st, what, a);
+}
+
+template <typename TI>
+b2g_status launch_nr_in(const NrArgs& a, int mode, b2g_dtype out, dim3 grid, cudaStream_t st) {
+  if (out == B2G_BF16) return launch_nr<TI, __nv_bfloat16>(a, mode, grid, st);
+  if (out == B2G_F16) return launch_nr<TI, __half>(a, mode, grid, st);
+  return launch_nr<TI, float>(a, mode, grid, st);
+}
+
+bool is_float(b2g_dtype t) { return t == B2G_F32 || t == B2G_F16 || t == B2G_BF16; }
+
+}  // namespace
+
+b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
+  if (!d) return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: null descriptor");
+  if (d->tokens < 0 || d->n_head < 0 || d->n_kv_head < 0 || d->d_head < 0)
+    return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: negative size");
+  if (d->tokens == 0 || d->n_head + d->n_kv_head == 0) return B2G_OK;
+  if (d->d_head < 2 || d->d_head % 2 != 0 || d->d_head > 2 * kNrMaxPairs)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: d_head must be even and at most 256");
+  if (!is_float(d->dtype) || !is_float(d->out_dtype))
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: F32, F16 or BF16 inputs and outputs");
+  if (d->tokens > (1ll << 31) || d->n_head > 65536 || d->n_kv_head > 65536)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: size");
+  if ((d->n_head > 0 && (!d->q || !d->q_out)) || (d->n_kv_head > 0 && (!d->k || !d->k_out)))
+    return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: null operand");
+  if (d->n_axes < 0 || d->n_axes > 4 || (d->n_axes > 0 && (!d->positions || d->ldp < d->n_axes)))
+    return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: 0 to 4 axes with positions [tokens, n_axes]");
+  if (!(d->theta > 0.0) || !std::isfinite(d->theta) || !(d->eps >= 0.f) || !std::isfinite(d->eps))
+    return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: theta must be positive, eps not negative");
+  NrArgs a{};
+  int pairs = 0;
+  for (int i = 0; i < d->n_axes; ++i) {
+    const int w = d->axis_dim[i];
+    if (w < 0 || w % 2 != 0 || 2 * pairs + w > d->d_head)
+      return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: axis widths must be even and fit in the head");
+    for (int j = 0; j < w / 2; ++j, ++pairs) {
+      const double turns = std::pow(d->theta, -2.0 * j / w) / 6.283185307179586476925286766559;
+      a.turn_hi[pairs] = static_cast<float>(turns);
+      a.turn_lo[pairs] = static_cast<float>(turns - static_cast<double>(a.turn_hi[pairs]));
+      a.axis[pairs] = static_cast<unsigned char>(i);
+    }
+  }
+  DeviceInfo* dev = nullptr;
+  b2g_status s = device_info(&dev);
+  if (s != B2G_OK) return s;
+  a.x[0] = d->q; a.x[1] = d->k;
+  a.y[0] = d->q_out; a.y[1] = d->k_out;
+  a.ldx[0] = d->ldq; a.ldx[1] = d->ldk; a.hsx[0] = d->hsq; a.hsx[1] = d->hsk;
+  a.ldy[0] = d->ldq_out; a.ldy[1] = d->ldk_out; a.hsy[0] = d->hsq_out; a.hsy[1] = d->hsk_out;
+  a.norm[0] = d->q_norm; a.norm[1] = d->k_norm;
+  a.eps = d->eps;
+  a.pos = d->positions; a.ldp = d->ldp;
+  a.tokens = d->tokens;
+  a.heads = d->n_head + d->n_kv_head; a.q_heads = d->n_head;
+  a.D = d->d_head; a.rot = 2 * pairs;
+  a.halves = d->interleaved ? 0 : 1;
+  // Groups of 8 values need widths in eighths and rows (heads) that start on a group's boundary:
+  // 8 values for neighbours, 4 for halves.
+  const int n = d->interleaved ? 8 : 4;
+  const int64_t ib = d->dtype == B2G_F32 ? 4 : 2, ob = d->out_dtype == B2G_F32 ? 4 : 2;
+  const int64_t ia = n * ib < 16 ? n * ib : 16, oa = n * ob < 16 ? n * ob : 16;
+  bool vec = a.D % 8 == 0 && a.rot % 8 == 0;
+  for (int i = 0; i < 2; ++i) {
+    if ((i ? d->n_kv_head : d->n_head) == 0) continue;
+    vec = vec && (reinterpret_cast<uintptr_t>(a.x[i]) % ia | (a.ldx[i] * ib) % ia | (a.hsx[i] * ib) % ia) == 0 &&
+          (reinterpret_cast<uintptr_t>(a.y[i]) % oa | (a.ldy[i] * ob) % oa | (a.hsy[i] * ob) % oa) == 0;
+  }
+  const int mode = !vec ? kPairsAny : (d->interleaved ? kPairsNeighbours : kPairsHalves);
+  // Few heads: several tokens per block, so that every group of lanes has a head; no more than
+  // leave every SM a block.
+  const int group = a.D <= 64 ? 8 : (a.D <= 128 ? 16 : 32);
+  const int groups = mode == kPairsAny ? kNrThreads / 32 : kNrThreads / group;
+  int64_t bt = (groups + a.heads - 1) / a.heads;
+  if (bt > d->tokens / dev->num_sms) bt = d->tokens / dev->num_sms;
+  if (bt > kNrMaxTokens) bt = kNrMaxTokens;
+  if (bt < 1) bt = 1;
+  a.block_tokens = static_cast<int>(bt);
+  const int64_t blocks = (d->tokens + bt - 1) / bt, most = 8ll * dev->num_sms;
+  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+  if (d->dtype == B2G_BF16) return launch_nr_in<__nv_bfloat16>(a, mode, d->out_dtype, grid, st);
+  if (d->dtype == B2G_F16) return launch_nr_in<__half>(a, mode, d->out_dtype, grid, st);
+  return launch_nr_in<float>(a, mode, d->out_dtype, grid, st);
+}
+
+}  // namespace b2g

@@ -42,7 +42,8 @@ typedef enum {
   B2G_F32 = 0,
   B2G_F16 = 1,
   B2G_BF16 = 2,
-  B2G_E4M3 = 3
+  B2G_E4M3 = 3,
+  B2G_S8 = 4
 } b2g_dtype;
 
 typedef enum {
@@ -467,6 +468,78 @@ b2g_status b2g_add_inplace(float* x, const float* y, int64_t n, void* stream);
 b2g_status b2g_nerf_final(const float* feat_cond, const float* feat_uncond, const float* norm_scale,
                           const float* conv_w, const float* conv_b, float cfg_scale, int H, int W, float* out,
                           void* stream);
+
+/* ---- Packed batches (no reference counterpart; its sequences have one length and its INT8 path,
+ * cublas_ops.cuh:294-791, runs in cuBLASLt) ---- */
+
+/* 8-bit integer quantisation of the rows of a matrix: scales[r] = absmax_r / 127 (1 for an
+ * all-zero row) and dst[r, c] = round(src[r, c] * 127 / absmax_r), ties to even.  For a weight [N, K]
+ * that is one scale per output channel (once, at load), for activations one per token.  A row
+ * with an infinity or a NaN gets the scale NaN and zero codes.  src F32, BF16 or F16; any sizes, row
+ * strides and alignment (16-byte source rows and 8-byte destination rows are faster). */
+b2g_status b2g_quantize_s8(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
+                           int64_t dst_ld, float* scales, void* stream);
+
+/* D = epilogue((A . W^T) * a_scale[m] * b_scale[n] + bias) with W = desc->b S8 [N, K] and b_scale its
+ * channels' scales; the sums are exact 32-bit integers.  desc->a is S8 with its tokens' scales
+ * a_scale, or F32 / BF16 / F16 activations, which are quantised per token first as
+ * b2g_quantize_s8 does (a_scale ignored).  The epilogues, bias and output types of b2g_gemm.
+ * 1 <= K <= 131071; S8 operands need 16-byte aligned bases and row strides (K itself may be any).
+ * workspace: 256-byte aligned device memory of b2g_gemm_s8_workspace bytes for the codes of float
+ * activations, in use until the call's work on `stream` is done; NULL: the library's own (then
+ * calls on different streams must not overlap).  S8 activations need none. */
+size_t b2g_gemm_s8_workspace(int64_t M, int64_t K, b2g_dtype a_dtype);
+b2g_status b2g_gemm_s8(const b2g_gemm_desc* desc, const float* a_scale, const float* b_scale, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* RMSNorm of each query and key head and its rotation by positions of several axes, in one pass:
+ *   x' = x * rsqrt(mean(x^2) + eps) * norm          (norm NULL: x' = x)
+ *   pair (x0, x1) -> (x0 cos a - x1 sin a, x0 sin a + x1 cos a),
+ *   a = positions[token, axis] * theta^(-2 j / axis_dim[axis]) for the j-th pair of an axis.
+ * The axes take axis_dim / 2 pairs each, one after the other; values past their sum R are not turned.
+ * interleaved: pair p is values (2p, 2p + 1) (as the reference's RoPE, rope.cuh:180-221), else
+ * values (p, p + R / 2).  Token i's head h is at q + i * ldq + h * hsq, and so on.  Outputs may be
+ * the inputs (same pointer, type and strides); they must not overlap otherwise.  Angles are right to
+ * 2^-22 of a turn at any position.  d_head even, at most 256; n_head or n_kv_head may be 0. */
+typedef struct {
+  const void* q; const void* k; b2g_dtype dtype;              /* F32, BF16 or F16 */
+  void* q_out; void* k_out; b2g_dtype out_dtype;
+  int64_t ldq, hsq, ldk, hsk, ldq_out, hsq_out, ldk_out, hsk_out;  /* token, head strides (elements) */
+  int64_t tokens;
+  int n_head, n_kv_head, d_head;
+  const float* q_norm; const float* k_norm;                   /* [d_head] or NULL */
+  float eps;
+  const float* positions; int64_t ldp;                        /* [tokens, n_axes], row stride ldp */
+  int n_axes;                                                 /* 0 to 4 */
+  int axis_dim[4];                                            /* even, sum at most d_head */
+  double theta;
+  int interleaved;
+} b2g_qk_norm_rope_desc;
+b2g_status b2g_qk_norm_rope(const b2g_qk_norm_rope_desc* desc, void* stream);
+
+/* Attention over packed sequences of different lengths, each within itself:
+ *   out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, g]) v[j, g],   g = h / (n_head / n_kv_head)
+ * Sequence b has the query rows [cu_q[b], cu_q[b+1]) and the keys at rows cu_k[b] on: k_lens[b] of them
+ * (a cache with room left), or with k_lens NULL all up to cu_k[b+1].  causal: query i of lq sees the
+ * keys j <= i + lk - lq.  A row that sees no key is 0; rows of no sequence are not written.  Rows of
+ * k and v outside the sequences may hold anything; inside one, v must be finite for rows that do not
+ * see it not to be touched by it.  The offsets are device memory, read when the kernels run; they are
+ * clamped to the buffers.  BF16 or F16, output of the same type; d_head 64 or 128; 16-byte aligned
+ * bases, strides multiples of 8 elements.  workspace: as for b2g_gemm_s8. */
+typedef struct {
+  const void* q; const void* k; const void* v; void* out; b2g_dtype dtype;
+  int64_t ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso;             /* token, head strides (elements) */
+  int64_t total_q, total_k;                                   /* rows of q and out, of k and v */
+  int64_t batch;
+  const int32_t* cu_q; const int32_t* cu_k;                   /* [batch + 1] */
+  const int32_t* k_lens;                                      /* [batch] or NULL */
+  int n_head, n_kv_head, d_head;
+  float scale;
+  int causal;
+} b2g_attention_packed_desc;
+size_t b2g_attention_packed_workspace(const b2g_attention_packed_desc* desc);
+b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /* Reads and clears the device-side error word that the tensor-core kernels set when a
  * pipeline wait exceeds its time limit (they then drain and return instead of hanging).
