@@ -1020,21 +1020,35 @@ def nerf_final(feat_cond: torch.Tensor, feat_uncond: torch.Tensor | None, norm_s
 
 
 # ---------------------------------------------------------------------------- packed batches
-def _on(stream: torch.cuda.Stream | None, *ts: torch.Tensor | None):
+#
+# These wrappers stand in front of kernels of a few microseconds, so they ask torch for as little as
+# they can: one pass over the arguments, the raw stream handle, one workspace.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _on(stream: torch.cuda.Stream | None, *ts: torch.Tensor) -> int:
     """The raw stream of a call on the CUDA tensors `ts`, all of the current device."""
     dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and t.get_device() != dev:
+        if t.get_device() != dev:
             raise B2GError("all tensors must be CUDA tensors of the current device")
-    return (stream or torch.cuda.current_stream()).cuda_stream
+    return _raw_stream(dev) if stream is None else stream.cuda_stream
 
 
 def _empty(shape, dtype: torch.dtype, like: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
     """A new tensor for use on `stream` (memory of torch's allocator belongs to a stream)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _vector(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
+    """The address of a contiguous vector of n values."""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise B2GError(f"{what} must be contiguous {dtype} [{n}]")
+    return t.data_ptr()
 
 
 def quantize_s8(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.Tensor | None = None,
@@ -1051,11 +1065,10 @@ def quantize_s8(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.
         scales = _empty((rows,), torch.float32, x, stream)
     if out.dtype != torch.int8 or out.shape != x.shape or (cols > 1 and out.stride(1) != 1):
         raise B2GError("quantize_s8: out must be int8 [rows, cols] with unit column stride")
-    if scales.dtype != torch.float32 or scales.shape != (rows,) or not scales.is_contiguous():
-        raise B2GError("quantize_s8: scales must be contiguous F32 [rows]")
+    sp = _vector(scales, torch.float32, rows, "quantize_s8: scales")
     s = _on(stream, x, out, scales)
     _check(load().b2g_quantize_s8(x.data_ptr(), _TORCH_TO_B2G[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
-                                  out.data_ptr(), out.stride(0) if rows > 1 else cols, scales.data_ptr(), s))
+                                  out.data_ptr(), out.stride(0) if rows > 1 else cols, sp, s))
     return out, scales
 
 
@@ -1068,54 +1081,59 @@ def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torc
     wq: int8 [N, K] with 16-byte aligned rows (quantize_s8 of the weight), w_scale its scales.
     x: int8 codes with x_scale, or F32/BF16/F16 activations, quantised per token in the call.  The
     epilogues are gemm()'s."""
-    if x.dim() != 2 or wq.dim() != 2 or wq.dtype != torch.int8:
+    if x.dim() != 2 or wq.dim() != 2 or wq.dtype is not torch.int8:
         raise B2GError("gemm_s8: 2-D x and int8 wq expected")
-    M, K = x.shape
-    N = wq.shape[0]
-    if wq.shape[1] != K:
+    (M, K), (N, KW), (ldx, ux), (ldw, uw) = x.shape, wq.shape, x.stride(), wq.stride()
+    if K != KW:
         raise B2GError(f"gemm_s8: K mismatch {tuple(x.shape)} vs {tuple(wq.shape)}")
-    if K > 1 and (x.stride(1) != 1 or wq.stride(1) != 1):
+    if K > 1 and (ux != 1 or uw != 1):
         raise B2GError("gemm_s8: x and wq need unit stride along K")
-    codes = x.dtype == torch.int8
-    if not codes and x.dtype not in _TORCH_TO_B2G:
+    codes = x.dtype is torch.int8
+    a_dtype = S8 if codes else _TORCH_TO_B2G.get(x.dtype)
+    epi = _EPILOGUES.get(epilogue)
+    if a_dtype is None:
         raise B2GError("gemm_s8: x must be int8, F32, BF16 or F16")
-    if epilogue not in _EPILOGUES:
+    if epi is None:
         raise B2GError(f"gemm_s8: unknown epilogue {epilogue!r}")
-    epi = _EPILOGUES[epilogue]
     if out is None:
         if epi == EPI_GATED_RESIDUAL:
             raise B2GError("gemm_s8: gated_residual needs `out` (the residual)")
         out = _empty((M, N), out_dtype or torch.float32, x, stream)
     elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1):
         raise B2GError("gemm_s8: out must be [M, N] with unit column stride")
-    if out.dtype not in _TORCH_TO_B2G or (bias is not None and bias.dtype not in _TORCH_TO_B2G):
-        raise B2GError("gemm_s8: out and bias must be F32, BF16 or F16")
-    for t, n, what in ((w_scale, N, "w_scale"), (x_scale if codes else None, M, "x_scale"),
-                       (gate if epi == EPI_GATED_RESIDUAL else None, N, "gate")):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
-            raise B2GError(f"gemm_s8: {what} must be contiguous F32 [{n}]")
-    if bias is not None and (bias.numel() != N or not bias.is_contiguous()):
-        raise B2GError(f"gemm_s8: bias must be contiguous [{N}]")
-    s = _on(stream, x, wq, w_scale, bias, out, gate, x_scale)
-    lib = load()
-    a_dtype = S8 if codes else _TORCH_TO_B2G[x.dtype]
-    d = GemmDesc(M, N, K, x.data_ptr(), a_dtype, x.stride(0) if M > 1 else (K + 15) // 16 * 16 if codes else K,
-                 wq.data_ptr(), S8, wq.stride(0) if N > 1 else (K + 15) // 16 * 16,
-                 _ptr(bias), F32 if bias is None else _TORCH_TO_B2G[bias.dtype],
-                 out.data_ptr(), _TORCH_TO_B2G[out.dtype], out.stride(0) if M > 1 else N, epi, _ptr(gate))
-    ws, n = None, 0
+    o_dtype = _TORCH_TO_B2G.get(out.dtype)
+    if o_dtype is None:
+        raise B2GError("gemm_s8: out must be F32, BF16 or F16")
+    ts, pad = [x, wq, w_scale, out], (K + 15) // 16 * 16
+    d = GemmDesc(M, N, K, x.data_ptr(), a_dtype, ldx if M > 1 else pad if codes else K, wq.data_ptr(), S8,
+                 ldw if N > 1 else pad, None, F32, out.data_ptr(), o_dtype, out.stride(0) if M > 1 else N, epi, None)
+    w_ptr = _vector(w_scale, torch.float32, N, "gemm_s8: w_scale")
+    if bias is not None:
+        if bias.dtype not in (torch.float32, torch.bfloat16):
+            raise B2GError("gemm_s8: bias must be F32 or BF16")
+        d.bias, d.bias_dtype = _vector(bias, bias.dtype, N, "gemm_s8: bias"), _TORCH_TO_B2G[bias.dtype]
+        ts.append(bias)
+    if epi == EPI_GATED_RESIDUAL and gate is not None:
+        d.gate = _vector(gate, torch.float32, N, "gemm_s8: gate")
+        ts.append(gate)
+    x_ptr, ws_ptr, n = None, None, 0
     if not codes:
-        n = lib.b2g_gemm_s8_workspace(M, K, a_dtype)
-        ws = _empty((n,), torch.uint8, x, stream)
-    _check(lib.b2g_gemm_s8(ctypes.byref(d), _ptr(x_scale), w_scale.data_ptr(), _ptr(ws), n, s))
+        n = M * pad + 4 * M + 512  # b2g_gemm_s8_workspace and some
+        ws = _empty((n,), torch.int8, x, stream)
+        ws_ptr = ws.data_ptr()
+    elif x_scale is not None:
+        x_ptr = _vector(x_scale, torch.float32, M, "gemm_s8: x_scale")
+        ts.append(x_scale)
+    _check(load().b2g_gemm_s8(ctypes.byref(d), x_ptr, w_ptr, ws_ptr, n, _on(stream, *ts)))
     return out
 
 
 def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
     """Token and head stride of a [tokens, heads, d] tensor whose heads are contiguous."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+    st = t.stride()
+    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
         raise B2GError(f"{what}: [tokens, heads, d] with unit stride along d expected")
-    return t.stride(0), t.stride(1)
+    return st[0], st[1]
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes_dim: list[int],
@@ -1129,32 +1147,36 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes
     the turned part.  q and k may be views of a fused projection.  Returns (q', k'): q_out and
     k_out when given (q and k themselves for in place), else new tensors of out_dtype (default: q's)."""
     (ldq, hsq), (ldk, hsk) = _heads(q, "qk_norm_rope: q"), _heads(k, "qk_norm_rope: k")
-    T, H, D = q.shape
-    if k.shape[0] != T or k.shape[2] != D or k.dtype != q.dtype or q.dtype not in _TORCH_TO_B2G:
+    (T, H, D), (TK, HK, DK), n_axes = q.shape, k.shape, len(axes_dim)
+    dt = _TORCH_TO_B2G.get(q.dtype)
+    if TK != T or DK != D or k.dtype is not q.dtype or dt is None:
         raise B2GError("qk_norm_rope: q and k must have the same tokens, head width and F32/BF16/F16 type")
-    if positions.dim() != 2 or positions.shape != (T, len(axes_dim)) or positions.dtype != torch.float32 or (
-            positions.shape[1] > 1 and positions.stride(1) != 1):
+    if positions.shape != (T, n_axes) or positions.dtype is not torch.float32 or (
+            n_axes > 1 and positions.stride(1) != 1):
         raise B2GError("qk_norm_rope: positions must be F32 [tokens, len(axes_dim)]")
-    if len(axes_dim) > 4:
+    if n_axes > 4:
         raise B2GError("qk_norm_rope: at most 4 axes")
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != D or not w.is_contiguous()):
-            raise B2GError("qk_norm_rope: norm scales must be contiguous F32 [d]")
     if q_out is None:
-        q_out = _empty(q.shape, out_dtype or (q.dtype if k_out is None else k_out.dtype), q, stream)
+        q_out = _empty((T, H, D), out_dtype or (q.dtype if k_out is None else k_out.dtype), q, stream)
     if k_out is None:
-        k_out = _empty(k.shape, q_out.dtype, k, stream)
-    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype != k_out.dtype or (
-            q_out.dtype not in _TORCH_TO_B2G) or (out_dtype or q_out.dtype) != q_out.dtype:
+        k_out = _empty((T, HK, D), q_out.dtype, k, stream)
+    odt = _TORCH_TO_B2G.get(q_out.dtype)
+    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype is not k_out.dtype or odt is None or (
+            out_dtype is not None and out_dtype is not q_out.dtype):
         raise B2GError("qk_norm_rope: outputs must have the inputs' shapes and one F32/BF16/F16 type")
     (ldqo, hsqo), (ldko, hsko) = _heads(q_out, "qk_norm_rope: q_out"), _heads(k_out, "qk_norm_rope: k_out")
-    s = _on(stream, q, k, positions, q_norm, k_norm, q_out, k_out)
-    d = QkNormRopeDesc(q.data_ptr(), k.data_ptr(), _TORCH_TO_B2G[q.dtype], q_out.data_ptr(), k_out.data_ptr(),
-                       _TORCH_TO_B2G[q_out.dtype], ldq, hsq, ldk, hsk, ldqo, hsqo, ldko, hsko, T, H, k.shape[1], D,
-                       _ptr(q_norm), _ptr(k_norm), eps, positions.data_ptr(),
-                       positions.stride(0) if T > 1 else len(axes_dim), len(axes_dim),
-                       (ctypes.c_int * 4)(*axes_dim), theta, 1 if interleaved else 0)
-    _check(load().b2g_qk_norm_rope(ctypes.byref(d), s))
+    ts, qn, kn = [q, k, positions, q_out, k_out], None, None
+    if q_norm is not None:
+        qn = _vector(q_norm, torch.float32, D, "qk_norm_rope: q_norm")
+        ts.append(q_norm)
+    if k_norm is not None:
+        kn = _vector(k_norm, torch.float32, D, "qk_norm_rope: k_norm")
+        ts.append(k_norm)
+    d = QkNormRopeDesc(q.data_ptr(), k.data_ptr(), dt, q_out.data_ptr(), k_out.data_ptr(), odt, ldq, hsq, ldk, hsk,
+                       ldqo, hsqo, ldko, hsko, T, H, HK, D, qn, kn, eps, positions.data_ptr(),
+                       positions.stride(0) if T > 1 else n_axes, n_axes, tuple(axes_dim), theta,
+                       1 if interleaved else 0)
+    _check(load().b2g_qk_norm_rope(ctypes.byref(d), _on(stream, *ts)))
     return q_out, k_out
 
 
@@ -1170,29 +1192,33 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     of no sequence are left as they were)."""
     (ldq, hsq), (ldk, hsk), (ldv, hsv) = (_heads(q, "attention_packed: q"), _heads(k, "attention_packed: k"),
                                           _heads(v, "attention_packed: v"))
-    Tq, H, D = q.shape
-    if k.shape != v.shape or k.shape[2] != D or q.dtype not in (torch.bfloat16, torch.float16) or (
-            k.dtype != q.dtype or v.dtype != q.dtype):
+    (TQ, H, D), (TK, HK, DK), dtype = q.shape, k.shape, q.dtype
+    if v.shape != k.shape or DK != D or k.dtype is not dtype or v.dtype is not dtype or (
+            dtype is not torch.bfloat16 and dtype is not torch.float16):
         raise B2GError("attention_packed: q, k, v must be BF16 or F16 of one head width, k and v of one shape")
     if cu_k is None:
         cu_k = cu_q
     B = cu_q.numel() - 1
-    for t, n in ((cu_q, B + 1), (cu_k, B + 1), (k_lens, B)):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or B < 0 or
-                              not t.is_contiguous()):
-            raise B2GError("attention_packed: cu_q, cu_k [batch + 1] and k_lens [batch] must be contiguous int32")
+    if B < 0:
+        raise B2GError("attention_packed: cu_q must hold batch + 1 offsets")
+    cq = _vector(cu_q, torch.int32, B + 1, "attention_packed: cu_q")
+    ck = _vector(cu_k, torch.int32, B + 1, "attention_packed: cu_k")
     if out is None:
-        out = _empty(q.shape, q.dtype, q, stream)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = _empty((TQ, H, D), dtype, q, stream)
+    elif out.shape != q.shape or out.dtype is not dtype:
         raise B2GError("attention_packed: out must have q's shape and type")
     ldo, hso = _heads(out, "attention_packed: out")
-    s = _on(stream, q, k, v, cu_q, cu_k, k_lens, out)
-    lib = load()
-    d = AttentionPackedDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[q.dtype], ldq, hsq,
-                            ldk, hsk, ldv, hsv, ldo, hso, Tq, k.shape[0], B, cu_q.data_ptr(), cu_k.data_ptr(),
-                            _ptr(k_lens), H, k.shape[1], D, D ** -0.5 if scale is None else scale, 1 if causal else 0)
+    ts, kl = [q, k, v, cu_q, cu_k, out], None
+    if k_lens is not None:
+        kl = _vector(k_lens, torch.int32, B, "attention_packed: k_lens")
+        ts.append(k_lens)
+    lib, s = load(), _on(stream, *ts)
+    d = AttentionPackedDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[dtype], ldq, hsq,
+                            ldk, hsk, ldv, hsv, ldo, hso, TQ, TK, B, cq, ck, kl, H, HK, D,
+                            D ** -0.5 if scale is None else scale, 1 if causal else 0)
     ref = ctypes.byref(d)
-    n = lib.b2g_attention_packed_workspace(ref)
-    ws = _empty((n,), torch.uint8, q, stream) if n else None
-    _check(lib.b2g_attention_packed(ref, _ptr(ws), n, s))
+    n, ws = lib.b2g_attention_packed_workspace(ref), None
+    if n:
+        ws = _empty((n,), torch.int8, q, stream)
+    _check(lib.b2g_attention_packed(ref, None if ws is None else ws.data_ptr(), n, s))
     return out

@@ -42,8 +42,7 @@ struct PkParams {
   long long ldo, hso;
   int* err;
   // packed_rows
-  int keys_per_share;      // keys that one block takes (times the row tiles of the sequence)
-  int slots;               // capacity of the partial buffers
+  int shares;              // most shares that the work is cut into
   float* part_o;           // [slot][16][D]
   float2* part_ml;         // [slot][16]: row maximum (log2 units), row sum
 };
@@ -64,17 +63,18 @@ __device__ __forceinline__ Seq load_seq(const PkParams& p, int b) {
 }
 
 // The sequence that holds unit `want` when sequence b holds count(b) units, and the number of units
-// before it; -1 if there are not so many.  A whole warp searches, 32 sequences at a time.
-template <typename Count>
-__device__ __forceinline__ int find_seq(int batch, int want, int lane, Count count, int* before) {
-  int base = 0;
-  for (int b0 = 0; b0 < batch; b0 += 32) {
+// before it; -1 if there are not so many.  A whole warp searches, 32 sequences at a time, from
+// sequence `first` on, before which there are *before units.
+template <typename I, typename Count>
+__device__ __forceinline__ int find_seq(int batch, I want, int lane, Count count, I* before, int first = 0) {
+  I base = *before;
+  for (int b0 = first; b0 < batch; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < batch ? count(b) : 0;
-    int sum = n;
+    const I n = b < batch ? count(b) : 0;
+    I sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      const I up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
     const uint32_t past = __ballot_sync(0xffffffffu, base + sum > want);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
   // ---- this CTA's sequence and tiles (every warp finds them for itself)
   constexpr int kSpan = kHeadPairs ? kPtRows : 2 * kPtRows;  // sequence rows per CTA
-  int before = 0;
+  int before = 0;  // (units of the sequences before)
   const int unit = static_cast<int>(gridDim.x - 1 - blockIdx.x);  // (the last tiles of a sequence see most keys)
   const int b = find_seq(p.batch, unit, lane, [&](int i) {
     const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
@@ -462,25 +462,60 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
 // ---------------------------------------------------------------------------- few rows
 //
-// The query rows of one key head (lq tokens x group heads) in tiles of 16.  A sequence of `rt`
-// tiles splits its keys into ceil(lk / (keys_per_share * rt)) shares; a work item is (sequence,
-// tile, share, key head), the head running fastest so that neighbouring blocks read whole rows of
-// the cache.  In a block, 4 warps take 16 keys in turn, straight from global memory into the operand
-// registers of m16n8k16 products, without shared memory:
-//   S = Q K^T  lane (g, t) loads 16 bytes of key g at d = 32 c + 8 t: words (0, 1) and (2, 3) are
+// The query rows of one key head (lq tokens x group heads) in tiles of 16.  The tiles of all sequences
+// lie end to end on a line, each as long as its 16-key chunks and kPrTileCost more, and the line is
+// cut into equal shares; a block takes a share for one key head (the heads of a share are
+// neighbouring blocks, which read whole rows of the cache together).  So blocks have equal work
+// whatever the lengths; a tile that lies in several shares is joined by packed_combine.  In a block,
+// 4 warps take 16 keys in turn and multiply them by m16n8k16 products:
+//   S = Q K^T  lane (g, t) holds 16 bytes of key g at d = 32 c + 8 t: words (0, 1) and (2, 3) are
 //              the B operands of two products; Q is held in the same (permuted) order of d.
-//   O += P V   lane (g, t) loads 16 bytes of keys 2t, 2t+1, 2t+8, 2t+9 at d = 64 c + 8 g; value i of
+//   O += P V   lane (g, t) holds 16 bytes of keys 2t, 2t+1, 2t+8, 2t+9 at d = 64 c + 8 g; value i of
 //              these pairs up to the B operand of product i, whose column g is d = 64 c + 8 g + i.
-// The warps' sums meet in shared memory; shares of a sequence go to packed_combine.
+// Bound by memory, so what counts is bytes in flight: every lane copies exactly the 16-byte pieces
+// that it will use into its own slots of shared memory (cp.async, kPrStages chunks ahead; nothing
+// is shared between lanes, so there is nothing to wait for but a lane's own copies).  Loaded into
+// registers one chunk ahead instead, the same loop ran at 2.8 TB/s.  The warps' sums meet in
+// shared memory.
 constexpr int kPrWarps = 4;
 constexpr int kPrRows = 16;
+constexpr int kPrKeys = 16;  // keys of a chunk
+template <int D>
+constexpr int kPrPieces = D / 8;  // 16-byte pieces of K and V that a lane has of a chunk
+template <int D>
+constexpr int kPrStages = D == 128 ? 3 : 6;  // 24 KB per warp
+template <int D>
+constexpr uint32_t kPrSmem = kPrWarps * kPrStages<D> * kPrPieces<D> * 512u;
+constexpr int kPrBlocksPerSm = 2;
+
+constexpr int kPrTileCost = 6;   // what a tile costs beside its chunks, in chunks
+constexpr int kPrMinShare = 16;  // a share is at least so long
 
 __device__ __forceinline__ int rows_tiles(const PkParams& p, const Seq& s) {
   return static_cast<int>((static_cast<long long>(s.lq) * p.group + kPrRows - 1) / kPrRows);
 }
-__device__ __forceinline__ int rows_shares(const PkParams& p, const Seq& s, int rt) {
-  const long long per = static_cast<long long>(p.keys_per_share) * rt;
-  return s.lk > per ? static_cast<int>((s.lk + per - 1) / per) : 1;
+__device__ __forceinline__ int tile_length(const Seq& s) { return (s.lk + kPrKeys - 1) / kPrKeys + kPrTileCost; }
+__device__ __forceinline__ long long seq_length(const PkParams& p, int b) {
+  const Seq s = load_seq(p, b);
+  return static_cast<long long>(rows_tiles(p, s)) * tile_length(s);
+}
+// The line's length and the number of shares.  Share i is [total * i / shares, total * (i + 1) / shares).
+struct Line {
+  long long total;
+  int shares;
+};
+__device__ __forceinline__ Line the_line(const PkParams& p, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < p.batch; b += 32) sum += seq_length(p, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const long long most = (sum + kPrMinShare - 1) / kPrMinShare;
+  return {sum, static_cast<int>(min(static_cast<long long>(p.shares), most))};
+}
+// A partial result's slot: of share i and one key head, the part of a tile that begins in the share
+// (1) or before it (0).
+__device__ __forceinline__ int part_slot(const PkParams& p, int share, int begins, int head) {
+  return (2 * share + begins) * p.hk + head;
 }
 
 template <typename T>
@@ -498,96 +533,128 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 bytes, global to shared memory, or zeros where !live (src is not read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kPrWarps, 3) packed_rows_kernel(const PkParams p) {
+__global__ void __launch_bounds__(32 * kPrWarps, kPrBlocksPerSm) packed_rows_kernel(const PkParams p) {
   constexpr int KC = D / 32;  // 16-byte pieces of a lane's key
-  constexpr int VC = D / 64;  // 16-byte pieces of a lane's four value rows
-  __shared__ float so[kPrWarps][kPrRows][D + 4];
+  constexpr int VC = D / 64;  // 16-byte pieces of each of a lane's four value rows
+  constexpr int NS = kPrStages<D>;
+  constexpr uint32_t kStage = kPrPieces<D> * 512u;
+  extern __shared__ __align__(16) uint8_t smem_rows[];
   __shared__ float2 sml[kPrWarps][kPrRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem_rows) + warp * NS * kStage + lane * 16;
+  // The warps' sums [kPrRows][D + 4], each over its own ring.
+  auto so = [&](int w) { return reinterpret_cast<float*>(smem_rows + w * NS * kStage); };
+  static_assert(kPrRows * (D + 4) * 4 <= NS * kStage, "sums fit a ring");
   griddep_wait();
   griddep_launch_dependents();
-  for (int item = blockIdx.x;; item += gridDim.x) {
-    const int unit = item / p.hk, head = item - unit * p.hk;
-    int before = 0;
-    const int b = find_seq(p.batch, unit, lane, [&](int i) {
-      const Seq s = load_seq(p, i);
-      const int rt = rows_tiles(p, s);
-      return rt * rows_shares(p, s, rt);
-    }, &before);
+  const Line line = the_line(p, lane);
+  for (int block = blockIdx.x; block < line.shares * p.hk; block += gridDim.x) {
+   const int share = block / p.hk, head = block - share * p.hk;
+   const long long end = line.total * (share + 1) / line.shares;
+   long long before = 0;
+   int b = 0;
+   for (long long at = line.total * share / line.shares; at < end;) {
+    b = find_seq(p.batch, at, lane, [&](int i) { return seq_length(p, i); }, &before, b);
     if (b < 0) break;
     const Seq s = load_seq(p, b);
-    const int shares = rows_shares(p, s, rows_tiles(p, s));
-    const int tile = (unit - before) / shares, share = (unit - before) - tile * shares;
+    const int length = tile_length(s), tile = static_cast<int>((at - before) / length);
+    const long long tile_at = before + static_cast<long long>(tile) * length;
+    const int from = static_cast<int>(at - tile_at);
+    const int to = static_cast<int>(min(static_cast<long long>(length), end - tile_at));
+    at = tile_at + to;
     const int rows = s.lq * p.group, row0 = tile * kPrRows;
-    // This share's 16-key chunks [c0, c1), cut at the last key that any row of the tile sees.
+    // The chunks [c0, c1) of this part, cut at the last key that any row of the tile sees.
     const int last_token = min(row0 + kPrRows, rows) - 1;
     const int tile_sees = p.causal ? clampi(last_token / p.group + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
-    const int chunks = (s.lk + 15) / 16;
-    const int c0 = static_cast<int>(static_cast<long long>(chunks) * share / shares);
-    const int c1 = min(static_cast<int>(static_cast<long long>(chunks) * (share + 1) / shares), (tile_sees + 15) / 16);
+    const int c0 = max(0, from - kPrTileCost);
+    const int c1 = min(max(0, to - kPrTileCost), (tile_sees + kPrKeys - 1) / kPrKeys);
+    const T* kbase = static_cast<const T*>(p.k) + s.k0 * p.ldk + head * p.hsk + 8 * t;
+    const T* vbase = static_cast<const T*>(p.v) + s.k0 * p.ldv + head * p.hsv + 8 * g;
+    // Copies chunk c into stage st: keys that no row of the tile sees are zeros.
+    auto fetch = [&](int c, int st) {
+      const uint32_t dst = ring + st * kStage;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int key = c * kPrKeys + nt * 8 + g;
+        const bool live = key < tile_sees;
+        const T* src = live ? kbase + key * p.ldk : kbase;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) copy16(dst + (nt * KC + i) * 512, src + 32 * i, live);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = c * kPrKeys + 2 * t + (i & 1) + 8 * (i >> 1);
+        const bool live = key < tile_sees;
+        const T* src = live ? vbase + key * p.ldv : vbase;
+#pragma unroll
+        for (int k = 0; k < VC; ++k) copy16(dst + (2 * KC + i * VC + k) * 512, src + 64 * k, live);
+      }
+    };
+    int ahead = c0 + warp;
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i, ahead += kPrWarps) {
+      if (ahead < c1) fetch(ahead, i);
+      copy_commit();
+    }
 
     // Q: rows g and g + 8 of the tile (row r is token r / group, head r % group of the group).
     uint4 q[2][KC];
     int sees[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = row0 + g + 8 * i;
-      const int token = min(r, rows - 1) / p.group, h = min(r, rows - 1) - token * p.group;
+      const int r = min(row0 + g + 8 * i, rows - 1);
+      const int token = r / p.group, h = r - token * p.group;
       sees[i] = p.causal ? min(s.lk, token + 1 + s.lk - s.lq) : s.lk;
       const T* src = static_cast<const T*>(p.q) + (s.q0 + token) * p.ldq +
                      (static_cast<long long>(head) * p.group + h) * p.hsq + 8 * t;
 #pragma unroll
       for (int c = 0; c < KC; ++c) q[i][c] = __ldg(reinterpret_cast<const uint4*>(src + 32 * c));
     }
-    const T* kbase = static_cast<const T*>(p.k) + s.k0 * p.ldk + head * p.hsk + 8 * t;
-    const T* vbase = static_cast<const T*>(p.v) + s.k0 * p.ldv + head * p.hsv + 8 * g;
-
-    uint4 kr[2][KC], vr[4][VC];
-    auto load_k = [&](int c) {
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const T* src = kbase + min(c * 16 + nt * 8 + g, s.lk - 1) * p.ldk;  // (past the end: masked below)
-#pragma unroll
-        for (int i = 0; i < KC; ++i) kr[nt][i] = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
-      }
-    };
-    auto load_v = [&](int c) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = c * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
-        const T* src = vbase + key * p.ldv;
-#pragma unroll
-        for (int k = 0; k < VC; ++k)
-          vr[i][k] = key < tile_sees ? __ldg(reinterpret_cast<const uint4*>(src + 64 * k)) : make_uint4(0, 0, 0, 0);
-      }
-    };
 
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    if (c0 + warp < c1) {
-      load_k(c0 + warp);
-      load_v(c0 + warp);
-    }
+    int st = 0;
     for (int c = c0 + warp; c < c1; c += kPrWarps) {
+      copy_wait<NS - 2>();
+      if (ahead < c1) fetch(ahead, st == 0 ? NS - 1 : st - 1);  // (the stage used up in the last round)
+      copy_commit();
+      ahead += kPrWarps;
+      const uint32_t src = ring + st * kStage;
+      st = st + 1 == NS ? 0 : st + 1;
       float sc[2][4] = {};
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
+      for (int i = 0; i < KC; ++i)
 #pragma unroll
-        for (int i = 0; i < KC; ++i) {
-          mma_16816<T>(sc[nt], q[0][i].x, q[1][i].x, q[0][i].y, q[1][i].y, kr[nt][i].x, kr[nt][i].y);
-          mma_16816<T>(sc[nt], q[0][i].z, q[1][i].z, q[0][i].w, q[1][i].w, kr[nt][i].z, kr[nt][i].w);
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint4 kr = lds16(src + (nt * KC + i) * 512);
+          mma_16816<T>(sc[nt], q[0][i].x, q[1][i].x, q[0][i].y, q[1][i].y, kr.x, kr.y);
+          mma_16816<T>(sc[nt], q[0][i].z, q[1][i].z, q[0][i].w, q[1][i].w, kr.z, kr.w);
         }
-      if (c + kPrWarps < c1) load_k(c + kPrWarps);
       // Scores in log2 units; sc[nt][2i + e] is row g + 8i, key 16c + 8nt + 2t + e.
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int key = c * 16 + nt * 8 + 2 * t + (j & 1);
+          const int key = c * kPrKeys + nt * 8 + 2 * t + (j & 1);
           sc[nt][j] = key < sees[j >> 1] ? sc[nt][j] * p.scale_log2 : -INFINITY;
           mx[j >> 1] = fmaxf(mx[j >> 1], sc[nt][j]);
         }
@@ -622,10 +689,11 @@ __global__ void __launch_bounds__(32 * kPrWarps, 3) packed_rows_kernel(const PkP
         }
 #pragma unroll
       for (int k = 0; k < VC; ++k) {
-        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vr[0][k]);
-        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vr[1][k]);
-        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vr[2][k]);
-        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vr[3][k]);
+        uint4 vr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[i] = lds16(src + (2 * KC + i * VC + k) * 512);
+        const uint32_t v0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, v1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+        const uint32_t v2[4] = {vr[2].x, vr[2].y, vr[2].z, vr[2].w}, v3[4] = {vr[3].x, vr[3].y, vr[3].z, vr[3].w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
@@ -633,122 +701,133 @@ __global__ void __launch_bounds__(32 * kPrWarps, 3) packed_rows_kernel(const PkP
                        __byte_perm(v2[i >> 1], v3[i >> 1], pick));
         }
       }
-      if (c + kPrWarps < c1) load_v(c + kPrWarps);
     }
-    // The warps' statistics and sums, then 8 threads per row.
+    copy_wait<0>();
+    // The warps' statistics and sums.
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
       if (t == 0) sml[warp][g + 8 * i] = make_float2(m[i], l[i]);
     }
+    __syncwarp();  // (the ring's slots belong to lanes, the sums do not)
 #pragma unroll
     for (int k = 0; k < VC; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // column 2t + e of product i is d = 64 k + 8 (2t + e) + i
-        so[warp][g][64 * k + 16 * t + i] = o[8 * k + i][0];
-        so[warp][g][64 * k + 16 * t + 8 + i] = o[8 * k + i][1];
-        so[warp][g + 8][64 * k + 16 * t + i] = o[8 * k + i][2];
-        so[warp][g + 8][64 * k + 16 * t + 8 + i] = o[8 * k + i][3];
-      }
-    __syncthreads();
-    const int r = threadIdx.x >> 3, part = threadIdx.x & 7;
-    float top = -INFINITY;
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int w = 0; w < kPrWarps; ++w) top = fmaxf(top, sml[w][r].x);
-    float sum = 0.f, acc[D / 8];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kPrWarps; ++w) {
-      const float2 ml = sml[w][r];
-      const float wgt = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-      if (ml.x == -INFINITY) continue;
-      sum += wgt * ml.y;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) acc[i] += wgt * so[w][r][part * (D / 8) + i];
-    }
-    if (row0 + r < rows) {
-      if (shares > 1) {
-        if (item < p.slots) {
-          float* dst = p.part_o + (static_cast<long long>(item) * kPrRows + r) * D + part * (D / 8);
-#pragma unroll
-          for (int i = 0; i < D / 8; i += 4)
-            *reinterpret_cast<float4*>(dst + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-          if (part == 0) p.part_ml[static_cast<long long>(item) * kPrRows + r] = make_float2(top, sum);
+        for (int i = 0; i < 8; i += 4) {  // column 2t + e of product i is d = 64 k + 8 (2t + e) + i
+          float* dst = so(warp) + g * (D + 4) + 64 * k + 16 * t + 8 * e + i;
+          const float(*x)[4] = o + 8 * k + i;
+          *reinterpret_cast<float4*>(dst) = make_float4(x[0][e], x[1][e], x[2][e], x[3][e]);
+          *reinterpret_cast<float4*>(dst + 8 * (D + 4)) = make_float4(x[0][2 + e], x[1][2 + e], x[2][2 + e], x[3][2 + e]);
         }
+    __syncthreads();
+    // Groups of 4 values of the tile's rows.
+    const int live_rows = min(kPrRows, rows - row0);
+    for (int at = threadIdx.x; at < live_rows * (D / 4); at += 32 * kPrWarps) {
+      const int r = at / (D / 4), d = (at - r * (D / 4)) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kPrWarps; ++w) top = fmaxf(top, sml[w][r].x);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kPrWarps; ++w) {
+        const float2 ml = sml[w][r];
+        const float4 x = *reinterpret_cast<const float4*>(so(w) + r * (D + 4) + d);
+        // (a warp without a key has the sums 0; a NaN maximum does not occur, a NaN sum stays one)
+        const float wgt = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
+        sum += wgt * ml.y;
+        acc.x += wgt * x.x;
+        acc.y += wgt * x.y;
+        acc.z += wgt * x.z;
+        acc.w += wgt * x.w;
+      }
+      if (to - from < length) {
+        const long long slot = static_cast<long long>(part_slot(p, share, from == 0, head)) * kPrRows + r;
+        *reinterpret_cast<float4*>(p.part_o + slot * D + d) = acc;
+        if (d == 0) p.part_ml[slot] = make_float2(top, sum);
       } else {
         const int token = (row0 + r) / p.group, h = (row0 + r) - token * p.group;
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso +
-                 part * (D / 8);
-#pragma unroll
-        for (int i = 0; i < D / 8; i += 8)
-          *reinterpret_cast<uint4*>(dst + i) =
-              make_uint4(pack2<T>(acc[i] * inv, acc[i + 1] * inv), pack2<T>(acc[i + 2] * inv, acc[i + 3] * inv),
-                         pack2<T>(acc[i + 4] * inv, acc[i + 5] * inv), pack2<T>(acc[i + 6] * inv, acc[i + 7] * inv));
+        T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
       }
     }
-    __syncthreads();  // the shared buffers are reused by the next item
+    __syncthreads();  // the shared buffers are used again for the next tile
+   }
   }
 }
 
-// Joins the shares of every row tile whose sequence was split: with share i holding (m_i, l_i) and O_i,
-// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  A block takes (tile, key head) items.
+// Joins the parts of every tile that lies in several shares: with part i holding (m_i, l_i) and O_i,
+// out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  A block looks at the cut between two shares, for
+// one key head, and takes the tile there if it is the tile's first cut; a thread joins 4 values of a
+// row, kPcAhead parts' loads at a time.  All but the parts is read before the wait for packed_rows:
+// that kernel lets this one start after its own wait, when everything before it is complete.
+constexpr int kPcAhead = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(128) packed_combine_kernel(const PkParams p) {
-  griddep_wait();
   const int lane = threadIdx.x & 31;
-  for (int item = blockIdx.x;; item += gridDim.x) {
-    const int unit = item / p.hk, head = item - unit * p.hk;
-    // Units here are row tiles; the slots before this sequence's are counted beside them.
-    int before = 0;
-    const int b = find_seq(p.batch, unit, lane, [&](int i) { return rows_tiles(p, load_seq(p, i)); }, &before);
+  const Line line = the_line(p, lane);
+  bool waited = false;
+  for (int block = blockIdx.x; block < (line.shares - 1) * p.hk; block += gridDim.x) {
+    const int cut = block / p.hk + 1, head = block - (cut - 1) * p.hk;
+    const long long at = line.total * cut / line.shares;
+    long long before = 0;
+    const int b = find_seq(p.batch, at, lane, [&](int i) { return seq_length(p, i); }, &before);
     if (b < 0) break;
     const Seq s = load_seq(p, b);
-    const int rt = rows_tiles(p, s), shares = rows_shares(p, s, rt);
-    if (shares == 1) continue;
-    int slots = 0;
-    for (int i = lane; i < b; i += 32) {
-      const Seq x = load_seq(p, i);
-      const int n = rows_tiles(p, x);
-      slots += n * rows_shares(p, x, n);
-    }
-    slots = __reduce_add_sync(0xffffffffu, slots) + (unit - before) * shares;
-    const int rows = s.lq * p.group, row = (unit - before) * kPrRows + (threadIdx.x >> 3), part = threadIdx.x & 7;
-    if (row >= rows || (slots + shares) * static_cast<long long>(p.hk) > p.slots) continue;
-    const long long first = (static_cast<long long>(slots) * p.hk + head) * kPrRows + (threadIdx.x >> 3);
-    const long long step = static_cast<long long>(p.hk) * kPrRows;
-    float top = -INFINITY;
-    for (int i = 0; i < shares; ++i) top = fmaxf(top, p.part_ml[first + i * step].x);
-    float sum = 0.f, acc[D / 8];
+    const int length = tile_length(s), tile = static_cast<int>((at - before) / length);
+    const long long tile_at = before + static_cast<long long>(tile) * length;
+    // (a share may be longer than the tile: then the cut before this one is outside it)
+    if (tile_at == at || line.total * (cut - 1) / line.shares > tile_at) continue;
+    int parts = 2;  // the part before the cut and those after it
+    while (cut + parts - 1 < line.shares && line.total * (cut + parts - 1) / line.shares < tile_at + length) ++parts;
+    const int rows = s.lq * p.group, row0 = tile * kPrRows, live_rows = min(kPrRows, rows - row0);
+    const long long first = static_cast<long long>(part_slot(p, cut - 1, 1, head)) * kPrRows;
+    const long long second = static_cast<long long>(part_slot(p, cut, 0, head)) * kPrRows;
+    const long long step = 2ll * p.hk * kPrRows;
+    if (!waited) griddep_wait();
+    waited = true;
+    for (int at4 = threadIdx.x; at4 < live_rows * (D / 4); at4 += 128) {
+      const int r = at4 / (D / 4), d = (at4 - r * (D / 4)) * 4;
+      float top = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i0 = 0; i0 < parts; i0 += kPcAhead) {
+        float2 ml[kPcAhead];
+        float4 x[kPcAhead];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) acc[i] = 0.f;
-    for (int i = 0; i < shares; ++i) {
-      const float2 ml = p.part_ml[first + i * step];
-      if (ml.x == -INFINITY) continue;
-      const float wgt = fast_exp2(ml.x - top);
-      sum += wgt * ml.y;
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + (first + i * step) * D + part * (D / 8));
+        for (int i = 0; i < kPcAhead; ++i) {
+          const bool in = i0 + i < parts;
+          const long long slot = (i0 + i == 0 ? first : second + (i0 + i - 1) * step) + r;
+          ml[i] = in ? __ldcg(p.part_ml + slot) : make_float2(-INFINITY, 0.f);
+          x[i] = in ? __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float next = top;
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const float4 v = src[k];
-        acc[4 * k] += wgt * v.x;
-        acc[4 * k + 1] += wgt * v.y;
-        acc[4 * k + 2] += wgt * v.z;
-        acc[4 * k + 3] += wgt * v.w;
+        for (int i = 0; i < kPcAhead; ++i) next = fmaxf(next, ml[i].x);
+        const float alpha = top == next ? 1.f : fast_exp2(top - next);
+        top = next;
+        sum *= alpha;
+        acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
+#pragma unroll
+        for (int i = 0; i < kPcAhead; ++i) {
+          const float wgt = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : 1.f) : fast_exp2(ml[i].x - top);
+          sum += wgt * ml[i].y;
+          acc.x += wgt * x[i].x;
+          acc.y += wgt * x[i].y;
+          acc.z += wgt * x[i].z;
+          acc.w += wgt * x[i].w;
+        }
       }
+      const int token = (row0 + r) / p.group, h = (row0 + r) - token * p.group;
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
     }
-    const int token = row / p.group, h = row - token * p.group;
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso +
-             part * (D / 8);
-#pragma unroll
-    for (int i = 0; i < D / 8; i += 8)
-      *reinterpret_cast<uint4*>(dst + i) =
-          make_uint4(pack2<T>(acc[i] * inv, acc[i + 1] * inv), pack2<T>(acc[i + 2] * inv, acc[i + 3] * inv),
-                     pack2<T>(acc[i + 4] * inv, acc[i + 5] * inv), pack2<T>(acc[i + 6] * inv, acc[i + 7] * inv));
   }
+  if (!waited) griddep_wait();  // (this kernel's end stands for packed_rows' end too)
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -756,8 +835,7 @@ __global__ void __launch_bounds__(128) packed_combine_kernel(const PkParams p) {
 // What a call runs, from its sizes alone (the offsets are on the device).
 struct PkPlan {
   bool rows = false;       // packed_rows (+ packed_combine), else packed_tiles
-  int keys_per_share = 0;
-  int64_t slots = 0;       // shares, an upper bound over all offsets that fit the totals
+  int shares = 0;
   size_t o_bytes = 0, bytes = 0;
 };
 
@@ -769,28 +847,34 @@ PkPlan plan(const b2g_attention_packed_desc* d, int sms) {
   // Rows per key head: up to 16 on average fit one tile of packed_rows.
   r.rows = d->total_q * group <= kPrRows * d->batch || d->total_k == 0;
   if (!r.rows) return r;
-  // Shares that give every SM about 6 blocks' worth (two rounds of its 3), of 256 keys at least.
-  const int64_t want = 6 * static_cast<int64_t>(sms);
-  int64_t per = round_up((d->total_k * d->n_kv_head + want - 1) / want, 64);
-  if (per < 256) per = 256;
-  r.keys_per_share = static_cast<int>(per < (1 << 30) ? per : (1 << 30));
-  // sum over sequences of rt * ceil(lk / (per * rt)) <= total_k / per + sum of rt.
+  // A block per share and key head, as many as run at the same time; no more shares than the
+  // longest line possible has pieces of kPrMinShare.
   const int64_t tiles = d->total_q * group / kPrRows + d->batch;
-  r.slots = (d->total_k / per + tiles) * d->n_kv_head;
-  r.o_bytes = static_cast<size_t>(round_up(r.slots * kPrRows * d->d_head * 4, 256));
-  r.bytes = r.o_bytes + static_cast<size_t>(r.slots) * kPrRows * sizeof(float2);
+  const int64_t blocks = static_cast<int64_t>(kPrBlocksPerSm) * sms;
+  int64_t shares = blocks / d->n_kv_head;
+  const int64_t per_tile = (d->total_k + kPrKeys - 1) / kPrKeys + kPrTileCost;
+  const int64_t line = tiles <= (1ll << 31) / per_tile ? tiles * per_tile : (1ll << 31);
+  if (shares > (line + kPrMinShare - 1) / kPrMinShare) shares = (line + kPrMinShare - 1) / kPrMinShare;
+  if (shares < 1) shares = 1;
+  r.shares = static_cast<int>(shares);
+  if (shares == 1) return r;
+  const int64_t slots = 2 * shares * d->n_kv_head;
+  r.o_bytes = static_cast<size_t>(round_up(slots * kPrRows * d->d_head * 4, 256));
+  r.bytes = r.o_bytes + static_cast<size_t>(slots) * kPrRows * sizeof(float2);
   return r;
 }
 
 template <typename T, int D>
-b2g_status launch_rows(const PkParams& p, const PkPlan& pl, int64_t tiles, int sms, cudaStream_t st) {
-  const int64_t most = 3ll * sms;
-  const int64_t blocks = pl.slots < most ? pl.slots : most;
-  b2g_status s = launch_pdl(packed_rows_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(32 * kPrWarps), 0, st,
-                            "packed_rows launch", p);
-  if (s != B2G_OK || p.total_k <= p.keys_per_share) return s;  // (no sequence can have been split)
-  const int64_t items = tiles * p.hk;
-  return launch_pdl(packed_combine_kernel<T, D>, dim3(static_cast<unsigned>(items < 4 * most ? items : 4 * most)),
+b2g_status launch_rows(const PkParams& p, int sms, cudaStream_t st) {
+  const int64_t most = static_cast<int64_t>(kPrBlocksPerSm) * sms, blocks = static_cast<int64_t>(p.shares) * p.hk;
+  auto kern = packed_rows_kernel<T, D>;
+  b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPrSmem<D>),
+                            "cudaFuncSetAttribute(packed_rows)");
+  if (s != B2G_OK) return s;
+  s = launch_pdl(kern, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(32 * kPrWarps), kPrSmem<D>, st,
+                 "packed_rows launch", p);
+  if (s != B2G_OK || p.shares == 1) return s;
+  return launch_pdl(packed_combine_kernel<T, D>, dim3(static_cast<unsigned>(blocks - p.hk < most ? blocks - p.hk : most)),
                     dim3(128), 0, st, "packed_combine launch", p);
 }
 
@@ -812,11 +896,10 @@ template <typename T, int D>
 b2g_status run_packed(const b2g_attention_packed_desc* d, PkParams p, void* ws, const PkPlan& pl, int sms,
                       cudaStream_t st) {
   if (pl.rows) {
-    p.keys_per_share = pl.keys_per_share;
-    p.slots = static_cast<int>(pl.slots);
+    p.shares = pl.shares;
     p.part_o = static_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.o_bytes);
-    return launch_rows<T, D>(p, pl, static_cast<int64_t>(p.total_q) * p.group / kPrRows + p.batch, sms, st);
+    return launch_rows<T, D>(p, sms, st);
   }
   CUtensorMap tq, tk, tv;
   b2g_status s;
@@ -891,7 +974,6 @@ b2g_status attention_packed(const b2g_attention_packed_desc* d, void* workspace,
   PkPlan pl = plan(d, dev->num_sms);
   void* ws = workspace;
   if (pl.bytes > 0) {
-    if (pl.slots > (1ll << 30)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_packed: size");
     if (!ws && (s = workspace_get(pl.bytes, &ws, kWsAttnSplit)) != B2G_OK) return s;
     if (workspace && (workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
       return set_error(B2G_ERR_INVALID, "b2g_attention_packed: the workspace is too small or not 256-byte aligned");

@@ -30,6 +30,7 @@ namespace {
 constexpr int kNrThreads = 256;
 constexpr int kNrMaxPairs = 128;  // D <= 256
 constexpr int kNrMaxTokens = 8;   // tokens a block takes at a time
+constexpr int kNrAhead = 4;       // heads whose loads a lane has in flight
 
 // Pair layouts: neighbours or halves in groups of 8 values per lane, or any (value by value).
 enum { kPairsNeighbours = 0, kPairsHalves = 1, kPairsAny = 2 };
@@ -114,94 +115,113 @@ __device__ __forceinline__ void load_lane(const T* row, int e0, int e1, float (&
 }
 
 // The cosines and sines of `count` tokens from t0 on, [token][pair].
-__device__ __forceinline__ void fill_table(const NrArgs& a, float2* tab, const float* hi, const float* lo,
-                                           const unsigned char* axis, long long t0, int count, int pairs) {
+__device__ __forceinline__ void fill_table(const NrArgs& a, float2* tab, long long t0, int count, int pairs) {
   for (int i = threadIdx.x; i < count * pairs; i += kNrThreads) {
     const int b = i / pairs, p = i - b * pairs;
-    tab[b * kNrMaxPairs + p] = cos_sin_turns(__ldg(a.pos + (t0 + b) * a.ldp + axis[p]), hi[p], lo[p]);
+    tab[b * kNrMaxPairs + p] = cos_sin_turns(__ldg(a.pos + (t0 + b) * a.ldp + a.axis[p]), a.turn_hi[p], a.turn_lo[p]);
   }
 }
 
+// One of a block's heads: token b of its step and head h of q, then k.  Moves on by a number of heads.
+struct Item {
+  int b, h;
+  __device__ __forceinline__ void advance(int n, int heads) {
+    h += n;
+    while (h >= heads) {
+      h -= heads;
+      ++b;
+    }
+  }
+};
+
 template <typename TI, typename TO, int G, bool kHalves>
 __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const __grid_constant__ NrArgs a) {
-  __shared__ float2 tab[2][kNrMaxTokens * kNrMaxPairs];
-  __shared__ float hi[kNrMaxPairs], lo[kNrMaxPairs];
-  __shared__ unsigned char axis[kNrMaxPairs];
-  const int pairs = a.rot / 2;
-  for (int p = threadIdx.x; p < pairs; p += kNrThreads) {
-    hi[p] = a.turn_hi[p];
-    lo[p] = a.turn_lo[p];
-    axis[p] = a.axis[p];
-  }
-  __syncthreads();
-  griddep_wait();
-  griddep_launch_dependents();
+  __shared__ __align__(16) float2 tab[2][kNrMaxTokens * kNrMaxPairs];
   constexpr int kGroups = kNrThreads / G;
-  const int l = threadIdx.x % G, group = threadIdx.x / G;
+  const int pairs = a.rot / 2;
+  const int l = threadIdx.x % G;
   const bool live = l < a.D / 8;  // (D / 8 is not a power of two for every D)
   const bool turned = 8 * l < a.rot;
   const int e0 = !kHalves || !turned ? 8 * l : 4 * l, e1 = !kHalves || !turned ? e0 + 4 : a.rot / 2 + 4 * l;
   const float inv_d = 1.f / static_cast<float>(a.D);
+  Item start{0, 0};
+  start.advance(threadIdx.x / G, a.heads);
+  griddep_wait();
+  griddep_launch_dependents();
   float w[2][8];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+  for (int s = 0; s < 2; ++s) {
+    if (live && a.norm[s]) load_lane<float, false>(a.norm[s], e0, e1, w[s]);
+    else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[s][i] = live && a.norm[s] ? __ldg(a.norm[s] + (i < 4 ? e0 + i : e1 + i - 4)) : 1.f;
+      for (int i = 0; i < 8; ++i) w[s][i] = 1.f;
+    }
+  }
 
   int buf = 0;
   for (long long t0 = static_cast<long long>(blockIdx.x) * a.block_tokens; t0 < a.tokens;
        t0 += static_cast<long long>(gridDim.x) * a.block_tokens, buf ^= 1) {
     const int count = static_cast<int>(min(static_cast<long long>(a.block_tokens), a.tokens - t0));
     const int items = count * a.heads;
-    auto read = [&](int item, float (&v)[8]) {
-      const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
-      const TI* row = static_cast<const TI*>(s ? a.x[1] : a.x[0]) + (t0 + b) * (s ? a.ldx[1] : a.ldx[0]) +
-                      (s ? h - a.q_heads : h) * (s ? a.hsx[1] : a.hsx[0]);
-      if (live && item < items) load_lane<TI, !kHalves>(row, e0, e1, v);
-      else {
+    Item in = start, out = start;
+    for (int first = 0; first < items; first += kGroups * kNrAhead) {
+      float v[kNrAhead][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
-    };
-    float next[8];
-    read(group, next);
-    fill_table(a, tab[buf], hi, lo, axis, t0, count, pairs);
-    __syncthreads();
-    for (int first = 0; first < items; first += kGroups) {  // (every lane takes part in the shuffles)
-      const int item = first + group;
-      float v[8];
+      for (int u = 0; u < kNrAhead; ++u) {
+        if (first + u * kGroups >= items) break;
+        const bool k = in.h >= a.q_heads;
+        const TI* row = static_cast<const TI*>(k ? a.x[1] : a.x[0]) + (t0 + in.b) * (k ? a.ldx[1] : a.ldx[0]) +
+                        (k ? in.h - a.q_heads : in.h) * (k ? a.hsx[1] : a.hsx[0]);
+        if (live && in.b < count) load_lane<TI, !kHalves>(row, e0, e1, v[u]);
+        else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = next[i];
-      read(item + kGroups, next);
-      const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (!live || item >= items) continue;
-      if (s ? a.norm[1] : a.norm[0]) {
-        const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (s ? w[1][i] : w[0][i]);
-      }
-      if (turned) {
-        const float2* cs = tab[buf] + b * kNrMaxPairs + 4 * l;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 t = cs[i];
-          const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1;
-          const float x0 = v[i0], x1 = v[i1];
-          v[i0] = fmaf(x0, t.x, -(x1 * t.y));
-          v[i1] = fmaf(x0, t.y, x1 * t.x);
+          for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
         }
+        in.advance(kGroups, a.heads);
       }
-      TO* row = static_cast<TO*>(s ? a.y[1] : a.y[0]) + (t0 + b) * (s ? a.ldy[1] : a.ldy[0]) +
-                (s ? h - a.q_heads : h) * (s ? a.hsy[1] : a.hsy[0]);
-      if constexpr (!kHalves) store_n<TO, 8>(row + e0, v);
-      else {
-        store_n<TO, 4>(row + e0, v);
-        store_n<TO, 4>(row + e1, v + 4);
+      if (first == 0) {  // (the loads above are on their way)
+        fill_table(a, tab[buf], t0, count, pairs);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < kNrAhead; ++u) {  // (every lane takes part in the shuffles)
+        if (first + u * kGroups >= items) break;
+        const bool k = out.h >= a.q_heads;
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = fmaf(v[u][i], v[u][i], ss);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (live && out.b < count) {
+          if (k ? a.norm[1] : a.norm[0]) {
+            const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * inv * (k ? w[1][i] : w[0][i]);
+          }
+          if (turned) {
+            const float4* cs = reinterpret_cast<const float4*>(tab[buf] + out.b * kNrMaxPairs + 4 * l);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float4 t = cs[i >> 1];  // cos, sin of pairs 4 l + i and the next
+              const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1, step = kHalves ? 1 : 2;
+              float x0 = v[u][i0], x1 = v[u][i1];
+              v[u][i0] = fmaf(x0, t.x, -(x1 * t.y));
+              v[u][i1] = fmaf(x0, t.y, x1 * t.x);
+              x0 = v[u][i0 + step];
+              x1 = v[u][i1 + step];
+              v[u][i0 + step] = fmaf(x0, t.z, -(x1 * t.w));
+              v[u][i1 + step] = fmaf(x0, t.w, x1 * t.z);
+            }
+          }
+          TO* row = static_cast<TO*>(k ? a.y[1] : a.y[0]) + (t0 + out.b) * (k ? a.ldy[1] : a.ldy[0]) +
+                    (k ? out.h - a.q_heads : out.h) * (k ? a.hsy[1] : a.hsy[0]);
+          if constexpr (!kHalves) store_n<TO, 8>(row + e0, v[u]);
+          else {
+            store_n<TO, 4>(row + e0, v[u]);
+            store_n<TO, 4>(row + e1, v[u] + 4);
+          }
+        }
+        out.advance(kGroups, a.heads);
       }
     }
   }
@@ -211,15 +231,7 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const __grid_c
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_any_kernel(const __grid_constant__ NrArgs a) {
   __shared__ float2 tab[2][kNrMaxTokens * kNrMaxPairs];
-  __shared__ float hi[kNrMaxPairs], lo[kNrMaxPairs];
-  __shared__ unsigned char axis[kNrMaxPairs];
   const int pairs = a.rot / 2;
-  for (int p = threadIdx.x; p < pairs; p += kNrThreads) {
-    hi[p] = a.turn_hi[p];
-    lo[p] = a.turn_lo[p];
-    axis[p] = a.axis[p];
-  }
-  __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_any_kernel(const __gr
   for (long long t0 = static_cast<long long>(blockIdx.x) * a.block_tokens; t0 < a.tokens;
        t0 += static_cast<long long>(gridDim.x) * a.block_tokens, buf ^= 1) {
     const int count = static_cast<int>(min(static_cast<long long>(a.block_tokens), a.tokens - t0));
-    fill_table(a, tab[buf], hi, lo, axis, t0, count, pairs);
+    fill_table(a, tab[buf], t0, count, pairs);
     __syncthreads();
     for (int item = warp; item < count * a.heads; item += kNrThreads / 32) {
       const int b = item / a.heads, h = item - b * a.heads, s = h >= a.q_heads;
@@ -324,8 +336,10 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
     const int w = d->axis_dim[i];
     if (w < 0 || w % 2 != 0 || 2 * pairs + w > d->d_head)
       return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: axis widths must be even and fit in the head");
-    for (int j = 0; j < w / 2; ++j, ++pairs) {
-      const double turns = std::pow(d->theta, -2.0 * j / w) / 6.283185307179586476925286766559;
+    // (a product per pair instead of a power: 64 roundings of 2^-53 at most)
+    const double ratio = w ? std::pow(d->theta, -2.0 / w) : 1.0;
+    double turns = 1.0 / 6.283185307179586476925286766559;
+    for (int j = 0; j < w / 2; ++j, ++pairs, turns *= ratio) {
       a.turn_hi[pairs] = static_cast<float>(turns);
       a.turn_lo[pairs] = static_cast<float>(turns - static_cast<double>(a.turn_hi[pairs]));
       a.axis[pairs] = static_cast<unsigned char>(i);
@@ -350,24 +364,25 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
   const int n = d->interleaved ? 8 : 4;
   const int64_t ib = d->dtype == B2G_F32 ? 4 : 2, ob = d->out_dtype == B2G_F32 ? 4 : 2;
   const int64_t ia = n * ib < 16 ? n * ib : 16, oa = n * ob < 16 ? n * ob : 16;
-  bool vec = a.D % 8 == 0 && a.rot % 8 == 0;
+  bool vec = a.D % 8 == 0 && a.rot % 8 == 0 &&
+             ((reinterpret_cast<uintptr_t>(a.norm[0]) | reinterpret_cast<uintptr_t>(a.norm[1])) & 15u) == 0;
   for (int i = 0; i < 2; ++i) {
     if ((i ? d->n_kv_head : d->n_head) == 0) continue;
     vec = vec && (reinterpret_cast<uintptr_t>(a.x[i]) % ia | (a.ldx[i] * ib) % ia | (a.hsx[i] * ib) % ia) == 0 &&
           (reinterpret_cast<uintptr_t>(a.y[i]) % oa | (a.ldy[i] * ob) % oa | (a.hsy[i] * ob) % oa) == 0;
   }
   const int mode = !vec ? kPairsAny : (d->interleaved ? kPairsNeighbours : kPairsHalves);
-  // Few heads: several tokens per block, so that every group of lanes has a head; no more than
-  // leave every SM a block.
+  // As many tokens per block as give every group of lanes kNrAhead heads, but a block for every SM.
   const int group = a.D <= 64 ? 8 : (a.D <= 128 ? 16 : 32);
-  const int groups = mode == kPairsAny ? kNrThreads / 32 : kNrThreads / group;
-  int64_t bt = (groups + a.heads - 1) / a.heads;
+  const int groups = mode == kPairsAny ? kNrThreads / 32 : kNrThreads / group * kNrAhead;
+  int64_t bt = groups / a.heads;
   if (bt > d->tokens / dev->num_sms) bt = d->tokens / dev->num_sms;
   if (bt > kNrMaxTokens) bt = kNrMaxTokens;
   if (bt < 1) bt = 1;
   a.block_tokens = static_cast<int>(bt);
-  const int64_t blocks = (d->tokens + bt - 1) / bt, most = 8ll * dev->num_sms;
-  const dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most));
+  // One step per block while that is a few waves, else blocks that stay and step.
+  const int64_t blocks = (d->tokens + bt - 1) / bt, most = 16ll * dev->num_sms;
+  const dim3 grid(static_cast<unsigned>(blocks <= most ? blocks : most));
   if (d->dtype == B2G_BF16) return launch_nr_in<__nv_bfloat16>(a, mode, d->out_dtype, grid, st);
   if (d->dtype == B2G_F16) return launch_nr_in<__half>(a, mode, d->out_dtype, grid, st);
   return launch_nr_in<float>(a, mode, d->out_dtype, grid, st);
