@@ -12,10 +12,13 @@
 // on the host for one image size; here a token's positions are all there is to it, so tokens of
 // images of any size, of clips and of text can be packed in any order.
 //
-// Bound by memory: q and k are read and written once.  A block works on whole tokens: it computes
-// each token's D / 2 cosines and sines once, in shared memory, for all of the token's heads, while the
-// first heads' values are on their way; 8 values per lane, so D / 8 lanes hold a head and its sum of
-// squares takes log2(D / 8) shuffles.
+// Bound by memory: q and k are read and written once.  A head is 8 values in each of D / 8 lanes, so
+// its sum of squares takes log2(D / 8) shuffles, and a lane turns the same 4 pairs of every head of a
+// token: it computes their cosines and sines once per token and keeps them in registers.  Warps
+// work alone, on kNrAhead steps' heads at a time: the loads of the next ones are on their way meanwhile,
+// and the four chains of sums, shuffles and roots run side by side.  (One step at a time through
+// copies in shared memory, the chain's latency bound the kernel: 190 us for 29120 tokens of 24 + 8 heads;
+// blocks that share a table of a token's angles, behind a barrier: 150 us, and 21 us for 1536 tokens.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
@@ -29,8 +32,8 @@ namespace {
 
 constexpr int kNrThreads = 256;
 constexpr int kNrMaxPairs = 128;  // D <= 256
-constexpr int kNrMaxTokens = 8;   // tokens a block takes at a time
-constexpr int kNrAhead = 4;       // heads whose loads a lane has in flight
+constexpr int kNrMaxTokens = 8;   // tokens a block of the any-layout kernel takes at a time
+constexpr int kNrAhead = 4;       // steps (of 32 / G heads) that a warp takes at a time
 
 // Pair layouts: neighbours or halves in groups of 8 values per lane, or any (value by value).
 enum { kPairsNeighbours = 0, kPairsHalves = 1, kPairsAny = 2 };
@@ -47,9 +50,10 @@ struct NrArgs {
   int heads, q_heads;  // q heads, then k heads
   int D, rot;          // head width, values turned
   int halves;          // kPairsAny: 1 = pairs (p, p + rot / 2)
-  int block_tokens;    // tokens per block and step
+  int block_tokens;    // kPairsAny: tokens per block and step
+  int parts_log2;      // otherwise: a token's heads are shared out among 2^parts_log2 warps
   // Per pair: turns per unit of position, theta^(-2j/d) / (2 pi), as the sum of two floats.
-  float turn_hi[kNrMaxPairs], turn_lo[kNrMaxPairs];
+  float2 turn[kNrMaxPairs];
   unsigned char axis[kNrMaxPairs];
 };
 
@@ -57,9 +61,9 @@ struct NrArgs {
 // is rounded away: pos * hi and its rounding error are exact as two floats, so the angle is right to
 // 2^-22 of a turn for positions of any size (a product in fp32 radians is off by 2^-24 of the angle,
 // 0.0005 at a position of 8000).
-__device__ __forceinline__ float2 cos_sin_turns(float pos, float hi, float lo) {
-  const float p = pos * hi;
-  const float rest = fmaf(pos, lo, fmaf(pos, hi, -p));
+__device__ __forceinline__ float2 cos_sin_turns(float pos, float2 turn) {
+  const float p = pos * turn.x;
+  const float rest = fmaf(pos, turn.y, fmaf(pos, turn.x, -p));
   const float r = (p - rintf(p)) + rest;
   float s, c;
   sincospif(2.f * r, &s, &c);
@@ -104,126 +108,164 @@ __device__ __forceinline__ void store_n(T* p, const float* v) {
   }
 }
 
-// Eight values of a head: four at e0 and four at e1.
-template <typename T, bool kOnePiece>
-__device__ __forceinline__ void load_lane(const T* row, int e0, int e1, float (&v)[8]) {
-  if constexpr (kOnePiece) load_n<T, 8>(row + e0, v);
-  else {
-    load_n<T, 4>(row + e0, v);
-    load_n<T, 4>(row + e1, v + 4);
-  }
-}
-
 // The cosines and sines of `count` tokens from t0 on, [token][pair].
 __device__ __forceinline__ void fill_table(const NrArgs& a, float2* tab, long long t0, int count, int pairs) {
   for (int i = threadIdx.x; i < count * pairs; i += kNrThreads) {
     const int b = i / pairs, p = i - b * pairs;
-    tab[b * kNrMaxPairs + p] = cos_sin_turns(__ldg(a.pos + (t0 + b) * a.ldp + a.axis[p]), a.turn_hi[p], a.turn_lo[p]);
+    tab[b * kNrMaxPairs + p] = cos_sin_turns(__ldg(a.pos + (t0 + b) * a.ldp + a.axis[p]), a.turn[p]);
   }
 }
 
-// One of a block's heads: token b of its step and head h of q, then k.  Moves on by a number of heads.
-struct Item {
-  int b, h;
-  __device__ __forceinline__ void advance(int n, int heads) {
-    h += n;
-    while (h >= heads) {
-      h -= heads;
-      ++b;
+// The raw bits of a lane's 8 values: four at `at`, four at `at + apart` (kHalves), or all at `at`.
+template <typename T, bool kHalves>
+struct Raw {
+  static constexpr int kWords = 2 * static_cast<int>(sizeof(T));
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* at, int apart) {
+    if constexpr (kWords == 4 && kHalves) {
+      *reinterpret_cast<uint2*>(w) = __ldcs(reinterpret_cast<const uint2*>(at));
+      *reinterpret_cast<uint2*>(w + 2) = __ldcs(reinterpret_cast<const uint2*>(at + apart));
+    } else if constexpr (kWords == 4) {
+      *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(at));
+    } else {
+      *reinterpret_cast<uint4*>(w) = __ldcs(reinterpret_cast<const uint4*>(at));
+      *reinterpret_cast<uint4*>(w + 4) = __ldcs(reinterpret_cast<const uint4*>(at + (kHalves ? apart : 4)));
     }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    const T* t = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f(t[i]);
   }
 };
 
+// A warp's place in its work.  A token's query heads, then its key heads, are taken kNrAhead steps of
+// 32 / G heads at a time (so that such a group has one set of scales and strides); the warp takes the
+// groups [first, end) of a token, then those of the token `stride` further on.
+struct Place {
+  int token, group;
+};
+
 template <typename TI, typename TO, int G, bool kHalves>
-__global__ void __launch_bounds__(kNrThreads) qk_norm_rope_kernel(const __grid_constant__ NrArgs a) {
-  __shared__ __align__(16) float2 tab[2][kNrMaxTokens * kNrMaxPairs];
-  constexpr int kGroups = kNrThreads / G;
-  const int pairs = a.rot / 2;
-  const int l = threadIdx.x % G;
+__global__ void __launch_bounds__(kNrThreads, 2) qk_norm_rope_kernel(const __grid_constant__ NrArgs a) {
+  constexpr int kHeads = 32 / G, U = kNrAhead;
+  __shared__ float2 turns[kNrMaxPairs];
+  __shared__ unsigned char axes[kNrMaxPairs];
+  for (int p = threadIdx.x; p < a.rot / 2; p += kNrThreads) {
+    turns[p] = a.turn[p];
+    axes[p] = a.axis[p];
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % G, sub = lane / G;
   const bool live = l < a.D / 8;  // (D / 8 is not a power of two for every D)
   const bool turned = 8 * l < a.rot;
-  const int e0 = !kHalves || !turned ? 8 * l : 4 * l, e1 = !kHalves || !turned ? e0 + 4 : a.rot / 2 + 4 * l;
+  const int e0 = !kHalves || !turned ? 8 * l : 4 * l, apart = !kHalves || !turned ? 4 : a.rot / 2;
   const float inv_d = 1.f / static_cast<float>(a.D);
-  Item start{0, 0};
-  start.advance(threadIdx.x / G, a.heads);
+  const int hq = live ? a.q_heads - sub : 0, hk = live ? a.heads - a.q_heads - sub : 0;  // (this lane's, counted from sub)
+  const int unit = blockIdx.x * (kNrThreads / 32) + warp, parts = 1 << a.parts_log2, part = unit & (parts - 1);
+  const int q_groups = (a.q_heads + kHeads * U - 1) / (kHeads * U);
+  const int groups = q_groups + (a.heads - a.q_heads + kHeads * U - 1) / (kHeads * U);
+  const int first = groups * part / parts, end = groups * (part + 1) / parts;
+  const int stride = static_cast<int>(gridDim.x * (kNrThreads / 32)) >> a.parts_log2;  // (parts divide 8)
+  const int tokens = static_cast<int>(a.tokens);
+  if (first == end) return;
+  auto next = [&](Place at) {
+    if (++at.group == end) {
+      at.group = first;
+      at.token += stride;
+    }
+    return at;
+  };
   griddep_wait();
   griddep_launch_dependents();
-  float w[2][8];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (live && a.norm[s]) load_lane<float, false>(a.norm[s], e0, e1, w[s]);
-    else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[s][i] = 1.f;
-    }
-  }
 
-  int buf = 0;
-  for (long long t0 = static_cast<long long>(blockIdx.x) * a.block_tokens; t0 < a.tokens;
-       t0 += static_cast<long long>(gridDim.x) * a.block_tokens, buf ^= 1) {
-    const int count = static_cast<int>(min(static_cast<long long>(a.block_tokens), a.tokens - t0));
-    const int items = count * a.heads;
-    Item in = start, out = start;
-    for (int first = 0; first < items; first += kGroups * kNrAhead) {
-      float v[kNrAhead][8];
+  Raw<TI, kHalves> raw[U];
+  auto load = [&](Place at) {
+    const bool k = at.group >= q_groups;
+    const int h0 = (k ? at.group - q_groups : at.group) * (kHeads * U), n = at.token < tokens ? (k ? hk : hq) - h0 : 0;
+    const long long hs = k ? a.hsx[1] : a.hsx[0];
+    const TI* from = static_cast<const TI*>(k ? a.x[1] : a.x[0]) + at.token * (k ? a.ldx[1] : a.ldx[0]) + (h0 + sub) * hs + e0;
 #pragma unroll
-      for (int u = 0; u < kNrAhead; ++u) {
-        if (first + u * kGroups >= items) break;
-        const bool k = in.h >= a.q_heads;
-        const TI* row = static_cast<const TI*>(k ? a.x[1] : a.x[0]) + (t0 + in.b) * (k ? a.ldx[1] : a.ldx[0]) +
-                        (k ? in.h - a.q_heads : in.h) * (k ? a.hsx[1] : a.hsx[0]);
-        if (live && in.b < count) load_lane<TI, !kHalves>(row, e0, e1, v[u]);
-        else {
+    for (int u = 0; u < U; ++u) {
+      if (u * kHeads < n) raw[u].load(from + u * (kHeads * hs), apart);
+      else raw[u].zero();
+    }
+  };
+  Place at{unit >> a.parts_log2, first};
+  load(at);
+  float w[8];  // the scales of the kind of head at hand
+  float2 cs[4];
+  const float* norm = nullptr;
+  int seen = -1;  // the token of cs
+  while (at.token < tokens) {
+    const bool k = at.group >= q_groups;
+    float v[U][8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        }
-        in.advance(kGroups, a.heads);
-      }
-      if (first == 0) {  // (the loads above are on their way)
-        fill_table(a, tab[buf], t0, count, pairs);
-        __syncthreads();
-      }
+    for (int u = 0; u < U; ++u) raw[u].values(v[u]);
+    const Place then = next(at);
+    load(then);
+    if (at.token != seen) {
+      seen = at.token;
+      if (turned) {
 #pragma unroll
-      for (int u = 0; u < kNrAhead; ++u) {  // (every lane takes part in the shuffles)
-        if (first + u * kGroups >= items) break;
-        const bool k = out.h >= a.q_heads;
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(v[u][i], v[u][i], ss);
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (live && out.b < count) {
-          if (k ? a.norm[1] : a.norm[0]) {
-            const float inv = rsqrtf(fmaf(ss, inv_d, a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * inv * (k ? w[1][i] : w[0][i]);
-          }
-          if (turned) {
-            const float4* cs = reinterpret_cast<const float4*>(tab[buf] + out.b * kNrMaxPairs + 4 * l);
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              const float4 t = cs[i >> 1];  // cos, sin of pairs 4 l + i and the next
-              const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1, step = kHalves ? 1 : 2;
-              float x0 = v[u][i0], x1 = v[u][i1];
-              v[u][i0] = fmaf(x0, t.x, -(x1 * t.y));
-              v[u][i1] = fmaf(x0, t.y, x1 * t.x);
-              x0 = v[u][i0 + step];
-              x1 = v[u][i1 + step];
-              v[u][i0 + step] = fmaf(x0, t.z, -(x1 * t.w));
-              v[u][i1 + step] = fmaf(x0, t.w, x1 * t.z);
-            }
-          }
-          TO* row = static_cast<TO*>(k ? a.y[1] : a.y[0]) + (t0 + out.b) * (k ? a.ldy[1] : a.ldy[0]) +
-                    (k ? out.h - a.q_heads : out.h) * (k ? a.hsy[1] : a.hsy[0]);
-          if constexpr (!kHalves) store_n<TO, 8>(row + e0, v[u]);
-          else {
-            store_n<TO, 4>(row + e0, v[u]);
-            store_n<TO, 4>(row + e1, v[u] + 4);
-          }
-        }
-        out.advance(kGroups, a.heads);
+        for (int i = 0; i < 4; ++i)
+          cs[i] = cos_sin_turns(__ldg(a.pos + at.token * a.ldp + axes[4 * l + i]), turns[4 * l + i]);
       }
     }
+    if (at.group == first || at.group == q_groups) {
+      norm = k ? a.norm[1] : a.norm[0];
+      if (norm && live) {
+        load_n<float, 4>(norm + e0, w);
+        load_n<float, 4>(norm + e0 + apart, w + 4);
+      }
+    }
+    if (norm) {
+      float ss[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ss[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss[u] = fmaf(v[u][i], v[u][i], ss[u]);
+      }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float inv = rsqrtf(fmaf(ss[u], inv_d, a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * inv * w[i];
+      }
+    }
+    if (turned) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1;
+          const float x0 = v[u][i0], x1 = v[u][i1];
+          v[u][i0] = fmaf(x0, cs[i].x, -(x1 * cs[i].y));
+          v[u][i1] = fmaf(x0, cs[i].y, x1 * cs[i].x);
+        }
+    }
+    const int h0 = (k ? at.group - q_groups : at.group) * (kHeads * U), n = (k ? hk : hq) - h0;
+    const long long hs = k ? a.hsy[1] : a.hsy[0];
+    TO* to = static_cast<TO*>(k ? a.y[1] : a.y[0]) + at.token * (k ? a.ldy[1] : a.ldy[0]) + (h0 + sub) * hs + e0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (u * kHeads >= n) break;
+      if constexpr (!kHalves) store_n<TO, 8>(to + u * (kHeads * hs), v[u]);
+      else {
+        store_n<TO, 4>(to + u * (kHeads * hs), v[u]);
+        store_n<TO, 4>(to + u * (kHeads * hs) + apart, v[u] + 4);
+      }
+    }
+    at = then;
   }
 }
 
@@ -322,7 +364,7 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
     return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: d_head must be even and at most 256");
   if (!is_float(d->dtype) || !is_float(d->out_dtype))
     return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: F32, F16 or BF16 inputs and outputs");
-  if (d->tokens > (1ll << 31) || d->n_head > 65536 || d->n_kv_head > 65536)
+  if (d->tokens > (1ll << 30) || d->n_head > 65536 || d->n_kv_head > 65536)
     return set_error(B2G_ERR_UNSUPPORTED, "b2g_qk_norm_rope: size");
   if ((d->n_head > 0 && (!d->q || !d->q_out)) || (d->n_kv_head > 0 && (!d->k || !d->k_out)))
     return set_error(B2G_ERR_INVALID, "b2g_qk_norm_rope: null operand");
@@ -340,8 +382,8 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
     const double ratio = w ? std::pow(d->theta, -2.0 / w) : 1.0;
     double turns = 1.0 / 6.283185307179586476925286766559;
     for (int j = 0; j < w / 2; ++j, ++pairs, turns *= ratio) {
-      a.turn_hi[pairs] = static_cast<float>(turns);
-      a.turn_lo[pairs] = static_cast<float>(turns - static_cast<double>(a.turn_hi[pairs]));
+      a.turn[pairs].x = static_cast<float>(turns);
+      a.turn[pairs].y = static_cast<float>(turns - static_cast<double>(a.turn[pairs].x));
       a.axis[pairs] = static_cast<unsigned char>(i);
     }
   }
@@ -372,17 +414,26 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
           (reinterpret_cast<uintptr_t>(a.y[i]) % oa | (a.ldy[i] * ob) % oa | (a.hsy[i] * ob) % oa) == 0;
   }
   const int mode = !vec ? kPairsAny : (d->interleaved ? kPairsNeighbours : kPairsHalves);
-  // As many tokens per block as give every group of lanes kNrAhead heads, but a block for every SM.
-  const int group = a.D <= 64 ? 8 : (a.D <= 128 ? 16 : 32);
-  const int groups = mode == kPairsAny ? kNrThreads / 32 : kNrThreads / group * kNrAhead;
-  int64_t bt = groups / a.heads;
-  if (bt > d->tokens / dev->num_sms) bt = d->tokens / dev->num_sms;
-  if (bt > kNrMaxTokens) bt = kNrMaxTokens;
-  if (bt < 1) bt = 1;
-  a.block_tokens = static_cast<int>(bt);
-  // One step per block while that is a few waves, else blocks that stay and step.
-  const int64_t blocks = (d->tokens + bt - 1) / bt, most = 16ll * dev->num_sms;
-  const dim3 grid(static_cast<unsigned>(blocks <= most ? blocks : most));
+  int64_t blocks;
+  if (mode == kPairsAny) {
+    // As many tokens per block as give every warp a head, but a block for every SM.
+    int64_t bt = kNrThreads / 32 / a.heads;
+    if (bt > d->tokens / dev->num_sms) bt = d->tokens / dev->num_sms;
+    if (bt < 1) bt = 1;
+    a.block_tokens = static_cast<int>(bt);
+    const int64_t most = 16ll * dev->num_sms;
+    blocks = (d->tokens + bt - 1) / bt < most ? (d->tokens + bt - 1) / bt : most;
+  } else {
+    // A token's heads go to several warps (which all compute its angles) while that still brings
+    // more warps to work, at 16 warps per SM.
+    const int64_t most = 2ll * dev->num_sms, warps = most * (kNrThreads / 32);
+    while (a.parts_log2 < 3 && (d->tokens << (a.parts_log2 + 1)) <= warps) ++a.parts_log2;
+    const int64_t need = ((d->tokens << a.parts_log2) + kNrThreads / 32 - 1) / (kNrThreads / 32);
+    // As many tokens for every warp: the rounds that `most` blocks need, shared out evenly.
+    const int64_t rounds = (need + most - 1) / most;
+    blocks = (need + rounds - 1) / rounds;
+  }
+  const dim3 grid(static_cast<unsigned>(blocks));
   if (d->dtype == B2G_BF16) return launch_nr_in<__nv_bfloat16>(a, mode, d->out_dtype, grid, st);
   if (d->dtype == B2G_F16) return launch_nr_in<__half>(a, mode, d->out_dtype, grid, st);
   return launch_nr_in<float>(a, mode, d->out_dtype, grid, st);
