@@ -88,6 +88,13 @@ __device__ __forceinline__ int find_seq(int batch, I want, int lane, Count count
   return -1;
 }
 
+// A shared-memory int read afresh at every use, so that it occupies no register in between.
+__device__ __forceinline__ int ld_shared_int(const int* p) {
+  int v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+  return v;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
@@ -101,46 +108,89 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // ---------------------------------------------------------------------------- long queries
 //
-// A CTA works on two 128-row query tiles that share their keys: two consecutive tiles of one head,
-// or, where two query heads share a key head, the same rows of both (finer steps along the
-// sequence).  Roles as in the engine's other attention kernel: warp 0 loads Q and K, warp 2 V, one
-// thread of warp 1 issues the MMAs, warps 4-7 and 8-11 are the softmax of tiles A and B with one
-// thread per row.  S (fp32) and O live in TMEM, P (16-bit) overwrites S and is the A operand of P.V:
-//   S_A(0), S_B(0), then per key block j: O_A += P_A(j) V_j, S_A(j+1), O_B += P_B(j) V_j, S_B(j+1)
-// so the tensor core works for one tile while the other's softmax runs.  Each tile stops at its own
-// last visible key block.
+// A persistent CTA per SM works on two 128-row query tiles at a time, in one of three ways:
+//   kTilesOfHead   consecutive tiles of one head, which share the keys' shared-memory stages
+//   kHeadsOfGroup  the same rows of two query heads that share a key head: shared stages, finer steps
+//   kHeadsApart    the same rows of two heads with their own keys: twice the key traffic, but no idle
+//                  second tile where sequences are short
+// Roles: warp 3 finds the work items and hands them round in a ring, warp 0 loads Q and K, warp 2 V, one
+// thread of warp 1 issues the MMAs, warps 4-7 and 8-11 are the softmax of tiles A and B with one thread
+// per row.  S (fp32) and O live in TMEM, P (16-bit)
+// overwrites S and is the A operand of P.V.  Per key block j, for A then B:
+//   O += P(j) V_j, S(j+1)
+// so the tensor core works for one tile while the other's softmax runs.  The roles run through the
+// work items without stopping: S of the next item's first block is issued behind the last P.V, Q, K and V
+// are loaded ahead as their stages come free, and only the tile's own softmax warps pause to write O.
+// (With a CTA per item, its start and end cost 8 us beside 2.3 us per key block.)
+//
+// Items: sequences by falling key count (up to kPtSorted of them; else as they come), tiles from the
+// last, which see most keys; dealt to the CTAs back and forth, so that the sums of long and short
+// ones stay even.
 //
 // The last key block may reach into the next sequence's rows, whose values may be anything: those
 // scores are replaced by -inf, and those rows of V are zeroed in shared memory before the MMA
 // reads them (0 times a NaN would be a NaN).  Within a sequence, V is expected to be finite: a
 // non-finite row of V reaches the query rows of its tile that do not see it.
 constexpr int kPtThreads = 384;
-constexpr int kPtRegsIdle = 64;      // producers and MMA issuer
-constexpr int kPtRegsSoftmax = 216;  // a 128-key row of scores in registers
+constexpr int kPtRegsIdle = 88;      // producers and MMA issuer
+constexpr int kPtRegsSoftmax = 208;  // a 128-key row of scores in registers
 static_assert(4 * 32 * kPtRegsIdle + 8 * 32 * kPtRegsSoftmax <= kPtThreads * 168, "register split");
 constexpr int kPtRows = 128;
 constexpr int kPtKeys = 128;
-constexpr int kPtKStages = 3;
-constexpr int kPtVStages = 2;
 constexpr uint32_t kPtBox = 128 * 128;  // bytes of one 128-row x 128-byte swizzled box
 constexpr float kPtRescaleLog2 = 8.0f;
+constexpr int kPtSorted = 512;
+constexpr int kPtItems = 4;      // items in the ring
+constexpr int kPtReaders = 11;   // Q/K, V, MMA, 8 softmax warps
+enum { kTilesOfHead = 0, kHeadsOfGroup = 1, kHeadsApart = 2 };
 
 template <int D>
 struct PtLayout {
+  static constexpr int KS = D == 128 ? 3 : 6, VS = D == 128 ? 2 : 4;
   static constexpr uint32_t kTileBytes = 128 * D * 2;  // Q tile, K block, V block: D / 64 boxes
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kK = kQ + 2 * kTileBytes;
-  static constexpr uint32_t kV = kK + kPtKStages * kTileBytes;
-  static constexpr uint32_t kBars = kV + kPtVStages * kTileBytes;
-  static constexpr uint32_t kSmem = 1024 + kBars + 256;
+  static constexpr uint32_t kV = kK + KS * kTileBytes;
+  static constexpr uint32_t kBars = kV + VS * kTileBytes;
+  static constexpr uint32_t kOrder = kBars + 384;      // sequences in working order, uint16 [kPtSorted]
+  static constexpr uint32_t kItems = kOrder + 2 * kPtSorted;
+  static constexpr uint32_t kSmem = 1024 + kItems + 32 * kPtItems;
 };
 
-template <typename T, int D, bool kHeadPairs>
+// One work item: rows [row0, row0 + 128) of tile A and B (B's 128 further on in kTilesOfHead).
+struct PtItem {
+  int q0, lq, k0, lk;
+  int row0, head;  // of tile A; head -1: no more items
+  int blocks[2];   // key blocks of each tile (0: nothing to see, or no rows)
+};
+static_assert(sizeof(PtItem) == 32, "two 16-byte words");
+
+// A place in a ring of n stages: the stage and the parity of its use.
+template <int n>
+struct Turn {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == n) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+  __device__ __forceinline__ void back() {
+    if (stage-- == 0) {
+      stage = n - 1;
+      parity ^= 1u;
+    }
+  }
+};
+
+template <typename T, int D, int kMode>
 __global__ void __launch_bounds__(kPtThreads, 1)
     packed_tiles_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const PkParams p) {
   using Ly = PtLayout<D>;
-  constexpr int KS = kPtKStages, VS = kPtVStages;
+  constexpr int KS = Ly::KS, VS = Ly::VS;
+  constexpr bool kApart = kMode == kHeadsApart;
   constexpr uint32_t kFmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -148,22 +198,43 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint8_t* sK = smem + Ly::kK;
   uint8_t* sV = smem + Ly::kV;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Ly::kBars);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;
+  uint64_t* q_full = bars;          // [tile] Q landed
+  uint64_t* q_empty = bars + 2;     // [tile] the item's last S is computed
+  uint64_t* s_full = bars + 4;      // [tile] S computed
+  uint64_t* p_part = bars + 6;      // [tile] P of keys 0-95 written (4 softmax warps)
+  uint64_t* p_full = bars + 8;      // [tile] all of P written
+  uint64_t* pv_done = bars + 10;    // [tile] P.V added
+  uint64_t* o_empty = bars + 12;    // [tile] O read (4 softmax warps)
+  uint64_t* v_tail = bars + 14;     // an item's last V block, before its foreign rows are zeroed
+  uint64_t* drain_bar = bars + 15;
+  uint64_t* k_full = bars + 16;
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + VS;
-  uint64_t* s_full = v_empty + VS;  // [tile]
-  uint64_t* p_part = s_full + 2;
-  uint64_t* p_full = p_part + 2;
-  uint64_t* pv_done = p_full + 2;
-  uint64_t* v_tail = pv_done + 2;   // the last V block, before its foreign rows are zeroed
-  uint64_t* drain_bar = v_tail + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* item_full = v_empty + VS;
+  uint64_t* item_empty = item_full + kPtItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + kPtItems);
+  static_assert(8 * (16 + 2 * (KS + VS + kPtItems)) + 4 <= 384, "barriers");
+  PtItem* items = reinterpret_cast<PtItem*>(smem + Ly::kItems);
+  uint16_t* order = reinterpret_cast<uint16_t*>(smem + Ly::kOrder);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0 && lane == 0) {
-    mbar_init(q_full, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_part[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+      mbar_init(&o_empty[t], 4);
+    }
+    mbar_init(v_tail, 1);
+    mbar_init(drain_bar, 1);
+    for (int i = 0; i < kPtItems; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], kPtReaders);
+    }
     for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -172,14 +243,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_part[t], 4);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&pv_done[t], 1);
-    }
-    mbar_init(v_tail, 1);
-    mbar_init(drain_bar, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -189,104 +252,220 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  griddep_wait();  // the set-up above overlapped the previous kernel's tail
+  griddep_launch_dependents();
+  const bool sorted = p.batch <= kPtSorted;
+  if (sorted) {
+    // Rank of each sequence by its keys (the counts pass through Q's space, still unused).
+    int* count = reinterpret_cast<int*>(sQ);
+    for (int b = threadIdx.x; b < p.batch; b += kPtThreads) count[b] = load_seq(p, b).lk;
+    __syncthreads();
+    for (int b = threadIdx.x; b < p.batch; b += kPtThreads) {
+      int rank = 0;
+      for (int i = 0; i < p.batch; ++i) rank += count[i] > count[b] || (count[i] == count[b] && i < b);
+      order[rank] = static_cast<uint16_t>(b);
+    }
+    fence_proxy_async_smem();  // (Q arrives there by the async proxy)
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  griddep_wait();  // the set-up above overlapped the previous kernel's tail
-  griddep_launch_dependents();
 
-  // ---- this CTA's sequence and tiles (every warp finds them for itself)
-  constexpr int kSpan = kHeadPairs ? kPtRows : 2 * kPtRows;  // sequence rows per CTA
-  int before = 0;  // (units of the sequences before)
-  const int unit = static_cast<int>(gridDim.x - 1 - blockIdx.x);  // (the last tiles of a sequence see most keys)
-  const int b = find_seq(p.batch, unit, lane, [&](int i) {
-    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
-    return (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kSpan - 1) / kSpan;
-  }, &before);
-  Seq s{0, 0, 0, 0};
-  if (b >= 0) s = load_seq(p, b);
-  int first_row[2], head[2], blocks[2], keys = 0;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    first_row[t] = (unit - before) * kSpan + (kHeadPairs ? 0 : t * kPtRows);
-    head[t] = kHeadPairs ? 2 * static_cast<int>(blockIdx.y) + t : static_cast<int>(blockIdx.y);
-    int n = first_row[t] < s.lq ? s.lk : 0;
-    if (p.causal) n = clampi(min(first_row[t] + kPtRows, s.lq) + s.lk - s.lq, 0, n);
-    blocks[t] = (n + kPtKeys - 1) / kPtKeys;
-    keys = max(keys, n);
-  }
-  const int nkb = max(blocks[0], blocks[1]);
-  const int kv_head = head[0] / p.group;
+  constexpr int kSpan = kMode == kTilesOfHead ? 2 * kPtRows : kPtRows;  // sequence rows per item
+  // Keys that either tile sees: V rows from there on are zeroed.
+  auto keys_seen = [&](const PtItem& w) {
+    const int last = w.row0 + (kMode == kTilesOfHead && w.blocks[1] > 0 ? 2 : 1) * kPtRows;
+    return p.causal ? clampi(min(last, w.lq) + w.lk - w.lq, 0, w.lk) : w.lk;
+  };
 
   if (warp < 4) {
     regs_dec<kPtRegsIdle>();
-    if (warp == 0) {
-      // ---------------------------------------------------------- Q and K
-      if (lane == 0 && nkb > 0) {
-        const uint64_t shared_kv = policy_evict_last(), once = policy_evict_first();
-        mbar_arrive_expect_tx(q_full, ((blocks[0] > 0) + (blocks[1] > 0)) * Ly::kTileBytes);
+    if (warp == 3) {
+      // ---------------------------------------------------------- work items
+      const int head_units = kMode == kTilesOfHead ? p.hq : (p.hq + 1) / 2;
+      const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
+      int units_before = 0, i = 0;
+      Turn<kPtItems> at;
+      for (int round = 0; i >= 0; ++round, at.next()) {
+        const long long index = static_cast<long long>(round) * grid + (round & 1 ? grid - 1 - cta : cta);
+        const int unit = static_cast<int>(index / head_units);
+        const int head_unit = static_cast<int>(index - static_cast<long long>(unit) * head_units);
+        auto seq_of = [&](int j) { return sorted ? static_cast<int>(order[j]) : j; };
+        i = find_seq(p.batch, unit, lane, [&](int j) {
+          const int b = seq_of(j), lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
+          return (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kSpan - 1) / kSpan;
+        }, &units_before, i);
+        PtItem w{};
+        w.head = -1;
+        if (i >= 0) {
+          const Seq s = load_seq(p, seq_of(i));
+          w.q0 = s.q0;
+          w.lq = s.lq;
+          w.k0 = s.k0;
+          w.lk = s.lk;
+          w.row0 = ((s.lq + kSpan - 1) / kSpan - 1 - (unit - units_before)) * kSpan;
+          w.head = kMode == kTilesOfHead ? head_unit : 2 * head_unit;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (blocks[t] > 0)
+          for (int t = 0; t < 2; ++t) {
+            const int row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0);
+            int n = row < s.lq && (!kApart || w.head + t < p.hq) ? s.lk : 0;
+            if (p.causal) n = clampi(min(row + kPtRows, s.lq) + s.lk - s.lq, 0, n);
+            w.blocks[t] = (n + kPtKeys - 1) / kPtKeys;
+          }
+        }
+        bool ok = true;
+        if (lane == 0) {
+          ok = mbar_wait(&item_empty[at.stage], at.parity ^ 1u, p.err, kErrWaitProducer);
+          if (ok) {
+            items[at.stage] = w;
+            mbar_arrive(&item_full[at.stage]);
+          }
+        }
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      }
+    } else if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- Q and K
+      const uint64_t shared_kv = policy_evict_last(), once = policy_evict_first();
+      Turn<kPtItems> at;
+      Turn<KS> k_at;
+      uint32_t q_parity[2] = {0, 0};
+      int k_used = 0;
+      bool ok = true, q_used[2] = {false, false};
+      for (; ok; at.next()) {
+        if (!(ok = mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitProducer))) break;
+        const PtItem w = items[at.stage];
+        mbar_arrive(&item_empty[at.stage]);
+        if (w.head < 0) break;
+        const int nkb = max(w.blocks[0], w.blocks[1]);
+        const int kv_head = w.head / p.group, kv_head_b = kApart ? (w.head + 1) / p.group : kv_head;
+        for (int j = 0; j < nkb && ok; ++j) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (ok && j == 0 && w.blocks[t] > 0) {  // this tile's Q
+              ok = mbar_wait(&q_empty[t], q_parity[t] ^ 1u, p.err, kErrWaitProducer);
+              if (!ok) break;
+              q_parity[t] ^= 1u;
+              q_used[t] = true;
+              mbar_arrive_expect_tx(&q_full[t], Ly::kTileBytes);
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_3d(sQ + t * Ly::kTileBytes + c * kPtBox, &tmQ, &q_full[t], c * 64,
+                            w.q0 + w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0),
+                            w.head + (kMode == kTilesOfHead ? 0 : t), once);
+            }
+            if (kApart ? j >= w.blocks[t] : t != 0) continue;
+            ok = mbar_wait(&k_empty[k_at.stage], k_at.parity ^ 1u, p.err, kErrWaitProducer);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&k_full[k_at.stage], Ly::kTileBytes);
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-              tma_load_3d(sQ + t * Ly::kTileBytes + c * kPtBox, &tmQ, q_full, c * 64, s.q0 + first_row[t], head[t], once);
-        int issued = 0;
-        for (int j = 0; j < nkb; ++j) {
-          const int st = j % KS;
-          if (!mbar_wait(&k_empty[st], ((j / KS) & 1) ^ 1u, p.err, kErrWaitProducer)) break;
-          mbar_arrive_expect_tx(&k_full[st], Ly::kTileBytes);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_3d(sK + st * Ly::kTileBytes + c * kPtBox, &tmK, &k_full[st], c * 64, s.k0 + j * kPtKeys, kv_head,
-                        shared_kv);
-          ++issued;
+              tma_load_3d(sK + k_at.stage * Ly::kTileBytes + c * kPtBox, &tmK, &k_full[k_at.stage], c * 64,
+                          w.k0 + j * kPtKeys, t ? kv_head_b : kv_head, shared_kv);
+            k_at.next();
+            ++k_used;
+          }
         }
-        // This thread's copies land before the CTA's shared memory goes away (they have, unless
-        // another role gave up early).
-        mbar_wait_drain(q_full, 0);
-        for (int j = max(0, issued - KS); j < issued; ++j) mbar_wait_drain(&k_full[j % KS], (j / KS) & 1);
+      }
+      // This thread's copies land before the CTA's shared memory goes away (they have, unless
+      // another role gave up early).
+      for (int t = 0; t < 2; ++t)
+        if (q_used[t]) mbar_wait_drain(&q_full[t], q_parity[t] ^ 1u);
+      for (int i = min(k_used, KS); i > 0; --i) {
+        k_at.back();
+        mbar_wait_drain(&k_full[k_at.stage], k_at.parity);
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------- V
       const uint64_t shared_kv = policy_evict_last();
-      int issued = 0;
-      for (int j = 0; j < nkb; ++j) {
-        const int st = j % VS;
-        const bool ok = __all_sync(0xffffffffu, lane != 0 || mbar_wait(&v_empty[st], ((j / VS) & 1) ^ 1u, p.err,
-                                                                      kErrWaitProducer));
+      Turn<kPtItems> at;
+      Turn<VS> v_at;
+      uint32_t tail_parity = 0;
+      int v_used = 0;
+      bool ok = true;
+      for (; ok; at.next()) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitProducer));
         if (!ok) break;
-        const int valid = keys - j * kPtKeys;  // rows of this block that any tile sees
-        uint64_t* bar = valid < kPtKeys ? v_tail : &v_full[st];
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar, Ly::kTileBytes);
+        const PtItem w = items[at.stage];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[at.stage]);
+        if (w.head < 0) break;
+        const int nkb = max(w.blocks[0], w.blocks[1]), seen = keys_seen(w);
+        const int kv_head = w.head / p.group, kv_head_b = kApart ? (w.head + 1) / p.group : kv_head;
+        for (int j = 0; j < nkb && ok; ++j) {
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_3d(sV + st * Ly::kTileBytes + c * kPtBox, &tmV, bar, c * 64, s.k0 + j * kPtKeys, kv_head, shared_kv);
-        }
-        if (valid < kPtKeys) {  // the last block: rows past the sequence become zeros
-          if (!__all_sync(0xffffffffu, mbar_wait(v_tail, 0, p.err, kErrWaitProducer))) break;
-          const int words = (kPtKeys - valid) * 8;
+          for (int t = 0; t < (kApart ? 2 : 1); ++t) {
+            if (!ok || (kApart && j >= w.blocks[t])) continue;
+            ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[v_at.stage], v_at.parity ^ 1u, p.err, kErrWaitProducer));
+            if (!ok) break;
+            const int valid = seen - j * kPtKeys;  // rows of this block that are seen
+            uint8_t* dst = sV + v_at.stage * Ly::kTileBytes;
+            uint64_t* bar = valid < kPtKeys ? v_tail : &v_full[v_at.stage];
+            if (lane == 0) {
+              mbar_arrive_expect_tx(bar, Ly::kTileBytes);
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            uint4* z = reinterpret_cast<uint4*>(sV + st * Ly::kTileBytes + c * kPtBox + valid * 128);
-            for (int i = lane; i < words; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < D / 64; ++c)
+                tma_load_3d(dst + c * kPtBox, &tmV, bar, c * 64, w.k0 + j * kPtKeys, t ? kv_head_b : kv_head, shared_kv);
+            }
+            if (valid < kPtKeys) {  // the last block: rows past the sequence become zeros
+              ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tail_parity, p.err, kErrWaitProducer));
+              if (!ok) break;
+              tail_parity ^= 1u;
+              const int words = (kPtKeys - valid) * 8;
+#pragma unroll
+              for (int c = 0; c < D / 64; ++c) {
+                uint4* z = reinterpret_cast<uint4*>(dst + c * kPtBox + valid * 128);
+                for (int i = lane; i < words; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&v_full[v_at.stage]);
+            }
+            v_at.next();
+            ++v_used;
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[st]);
         }
-        ++issued;
       }
-      if (lane == 0)
-        for (int j = max(0, issued - VS); j < issued; ++j) mbar_wait_drain(&v_full[j % VS], (j / VS) & 1);
-    } else if (warp == 1 && lane == 0 && nkb > 0) {
+      if (lane == 0) {
+        if (!ok) mbar_wait_drain(v_tail, tail_parity);
+        for (int i = min(v_used, VS); i > 0; --i) {
+          v_at.back();
+          mbar_wait_drain(&v_full[v_at.stage], v_at.parity);
+        }
+      }
+    } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_s = idesc_make(kFmt, kPtRows, kPtKeys);
       constexpr uint32_t idesc_o = idesc_make(kFmt, kPtRows, D) | kIdescBMajorMN;
-      auto issue_s = [&](int t, int j) {
-        const uint32_t q0 = smem_u32(sQ + t * Ly::kTileBytes), k0 = smem_u32(sK + (j % KS) * Ly::kTileBytes);
+      Turn<kPtItems> at;
+      Turn<KS> k_at;
+      Turn<VS> v_at;
+      // Parities of the tiles' barriers: q_full, P (one use per block), o_empty.
+      uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0}, o_parity[2] = {0, 0};
+      bool ok = true;
+      // The next item with a key block; none: blocks 0, 0.
+      auto next_blocks = [&](int (&blocks)[2]) {
+        for (;;) {
+          blocks[0] = blocks[1] = 0;
+          if (!(ok = mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
+          const bool end = ld_shared_int(&items[at.stage].head) < 0;
+          blocks[0] = ld_shared_int(&items[at.stage].blocks[0]);
+          blocks[1] = ld_shared_int(&items[at.stage].blocks[1]);
+          if (end) return;  // (not handed back: asked again, it says the same)
+          mbar_arrive(&item_empty[at.stage]);
+          at.next();
+          if ((blocks[0] | blocks[1]) != 0) return;
+        }
+      };
+      // S of the key block at k_at, of tile t; first: of its item (Q), last: Q is free afterwards.
+      auto issue_s = [&](int t, bool first, bool last) {
+        if (first) {
+          if (!(ok = mbar_wait(&q_full[t], q_parity[t], p.err, kErrWaitMma))) return;
+          q_parity[t] ^= 1u;
+        }
+        if (!(ok = mbar_wait(&k_full[k_at.stage], k_at.parity, p.err, kErrWaitMma))) return;
+        tc_fence_after();
+        const uint32_t q0 = smem_u32(sQ + t * Ly::kTileBytes), k0 = smem_u32(sK + k_at.stage * Ly::kTileBytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -294,44 +473,74 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             umma_f16(tmem + t * 256, smem_desc_k_sw128(q0 + c * kPtBox + k * 32),
                      smem_desc_k_sw128(k0 + c * kPtBox + k * 32), idesc_s, (c | k) != 0 ? 1u : 0u);
         umma_commit(&s_full[t]);
+        if (last) umma_commit(&q_empty[t]);
+        if constexpr (kApart) {
+          umma_commit(&k_empty[k_at.stage]);
+          k_at.next();
+        }
       };
-      bool ok = mbar_wait(q_full, 0, p.err, kErrWaitMma) && mbar_wait(&k_full[0], 0, p.err, kErrWaitMma);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (blocks[t] > 0) issue_s(t, 0);
-        umma_commit(&k_empty[0]);
+      int cur[2], then[2];
+      next_blocks(cur);
+      for (int t = 0; t < 2; ++t)
+        if (ok && cur[t] > 0) issue_s(t, true, cur[t] == 1);
+      if (!kApart && ok && (cur[0] | cur[1]) != 0) {
+        umma_commit(&k_empty[k_at.stage]);
+        k_at.next();
       }
-      for (int j = 0; j < nkb && ok; ++j) {
-        const int vs = j % VS;
-        const uint32_t v0 = smem_u32(sV + vs * Ly::kTileBytes);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= blocks[t]) continue;
-          // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, 96-127 when all is there.
-          if (!(ok = mbar_wait(&p_part[t], j & 1, p.err, kErrWaitMma))) break;
-          if (!(ok = mbar_wait(&v_full[vs], (j / VS) & 1, p.err, kErrWaitMma))) break;
-          tc_fence_after();
+      while (ok && (cur[0] | cur[1]) != 0) {
+        const int nkb = max(cur[0], cur[1]);
+        for (int j = 0; j < nkb && ok; ++j) {
+          if (j + 1 == nkb) next_blocks(then);
+          bool more = false;  // some tile's next S was issued
 #pragma unroll
-          for (int k = 0; k < 6; ++k)
-            umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                        idesc_o, (j | k) != 0 ? 1u : 0u);
-          if (!(ok = mbar_wait(&p_full[t], j & 1, p.err, kErrWaitMma))) break;
-          tc_fence_after();
+          for (int t = 0; t < 2; ++t) {
+            if (!ok) break;
+            if (j < cur[t]) {
+              const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
+              if (j == 0) {  // O is overwritten: the last item's has been read
+                if (!(ok = mbar_wait(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
+                o_parity[t] ^= 1u;
+              }
+              // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
+              if (!(ok = mbar_wait(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
+              if (!(ok = mbar_wait(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
+              tc_fence_after();
 #pragma unroll
-          for (int k = 6; k < 8; ++k)
-            umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                        idesc_o, 1u);
-          umma_commit(&pv_done[t]);
-          if (j + 1 < blocks[t]) {
-            if (!(ok = mbar_wait(&k_full[(j + 1) % KS], ((j + 1) / KS) & 1, p.err, kErrWaitMma))) break;
-            // S(j+1) overwrites P(j); issued behind P(j).V_j, which reads P first (issue order).
-            issue_s(t, j + 1);
+              for (int k = 0; k < 6; ++k)
+                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                            idesc_o, (j | k) != 0 ? 1u : 0u);
+              if (!(ok = mbar_wait(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 6; k < 8; ++k)
+                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                            idesc_o, 1u);
+              umma_commit(&pv_done[t]);
+              p_parity[t] ^= 1u;
+              if constexpr (kApart) {
+                umma_commit(&v_empty[v_at.stage]);
+                v_at.next();
+              }
+            }
+            // The tile's next S, of this item or the next: over P, which the P.V issued before it
+            // reads first (issue order).
+            const bool same = j + 1 < cur[t], other = j + 1 == nkb && then[t] > 0;
+            if (same || other) {
+              issue_s(t, other, same ? j + 2 == cur[t] : then[t] == 1);
+              more = true;
+            }
+          }
+          if (!kApart && ok) {
+            umma_commit(&v_empty[v_at.stage]);
+            v_at.next();
+            if (more) {
+              umma_commit(&k_empty[k_at.stage]);
+              k_at.next();
+            }
           }
         }
-        if (ok) {
-          umma_commit(&v_empty[vs]);
-          if (j + 1 < nkb) umma_commit(&k_empty[(j + 1) % KS]);
-        }
+        cur[0] = then[0];
+        cur[1] = then[1];
       }
       if (!ok) {
         umma_commit(drain_bar);  // MMAs already issued retire before TMEM is released
@@ -343,111 +552,134 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     // ------------------------------------------------------------ softmax
     const int t = (warp - 4) >> 2;
     const int quarter = warp & 3;
-    const int row = (t ? first_row[1] : first_row[0]) + quarter * 32 + lane;
-    const int n = t ? blocks[1] : blocks[0];
-    // Keys this row sees: [0, sees).
-    const int sees = p.causal ? min(s.lk, row + 1 + s.lk - s.lq) : s.lk;
     const uint32_t sbase = tmem + t * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t obase = sbase + 128;
-    float m_used = -INFINITY, l_sum = 0.f;
+    uint32_t s_parity = 0;  // of s_full and pv_done: one use per block
+    Turn<kPtItems> at;
     bool good = true;
-    for (int j = 0; j < n && good; ++j) {
-      good = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, p.err, kErrWaitEpilogue));
-      if (!good) break;
-      tc_fence_after();
-      uint32_t r[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(sbase + c * 32, r[c]);
-      tmem_wait_ld();
-      const int left = sees - j * kPtKeys;
-      if (__any_sync(0xffffffffu, left < kPtKeys)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i >= left) r[c][i] = 0xFF800000u;  // -inf
+    for (;; at.next()) {
+      good = __all_sync(0xffffffffu, mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitEpilogue));
+      if (!good || ld_shared_int(&items[at.stage].head) < 0) break;
+      const int n = ld_shared_int(&items[at.stage].blocks[t]);
+      int left;  // keys that this row sees, from the block at hand on
+      {
+        const int lq = ld_shared_int(&items[at.stage].lq), lk = ld_shared_int(&items[at.stage].lk);
+        const int row = ld_shared_int(&items[at.stage].row0) + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32 + lane;
+        left = p.causal ? min(lk, row + 1 + lk - lq) : lk;
       }
-      float m16[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) m16[i] = fmaxf(__uint_as_float(r[0][i]), __uint_as_float(r[0][i + 16]));
-#pragma unroll
-      for (int c = 1; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m16[i] = max3f(m16[i], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 16]));
-      float mx = m16[0];
-#pragma unroll
-      for (int i = 1; i < 15; i += 2) mx = max3f(mx, m16[i], m16[i + 1]);
-      mx = fmaxf(mx, m16[15]) * p.scale_log2;  // scale > 0: the max commutes with it
-      // The maximum in use is raised only when a block exceeds it by 2^8 (O is then rescaled).
-      const bool raise = mx > m_used + kPtRescaleLog2;
-      const float alpha = raise ? fast_exp2(m_used - mx) : 1.f;
-      if (raise) m_used = mx;
-      if (__any_sync(0xffffffffu, raise && j > 0)) {
-        good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (j - 1) & 1, p.err, kErrWaitEpilogue));
+      float m_used = -INFINITY, l_sum = 0.f;
+      for (int j = 0; j < n; ++j, s_parity ^= 1u, left -= kPtKeys) {
+        good = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_parity, p.err, kErrWaitEpilogue));
         if (!good) break;
         tc_fence_after();
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(sbase + c * 32, r[c]);
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, left < kPtKeys)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= left) r[c][i] = 0xFF800000u;  // -inf
+        }
+        float m16[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m16[i] = fmaxf(__uint_as_float(r[0][i]), __uint_as_float(r[0][i + 16]));
+#pragma unroll
+        for (int c = 1; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) m16[i] = max3f(m16[i], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 16]));
+        float mx = m16[0];
+#pragma unroll
+        for (int i = 1; i < 15; i += 2) mx = max3f(mx, m16[i], m16[i + 1]);
+        mx = fmaxf(mx, m16[15]) * p.scale_log2;  // scale > 0: the max commutes with it
+        // The maximum in use is raised only when a block exceeds it by 2^8 (O is then rescaled).
+        const bool raise = mx > m_used + kPtRescaleLog2;
+        const float alpha = raise ? fast_exp2(m_used - mx) : 1.f;
+        if (raise) m_used = mx;
+        if (__any_sync(0xffffffffu, raise && j > 0)) {
+          good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
+          if (!good) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(obase + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x32(obase + c * 32, o);
+          }
+        }
+        l_sum *= alpha;
+        const uint64_t ua2 = f2_splat(p.scale_log2), nm2 = f2_splat(m_used == -INFINITY ? 0.f : -m_used);
+        uint64_t ls2[2] = {f2_splat(0.f), f2_splat(0.f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 xx = f2_unpack(f2_fma(f2_pack(r[c][i], r[c][i + 1]), ua2, nm2));
+            const float x0 = fast_exp2(xx.x), x1 = fast_exp2(xx.y);
+            ls2[(i >> 1) & 1] = f2_add(ls2[(i >> 1) & 1], f2_pack(__float_as_uint(x0), __float_as_uint(x1)));
+            pk[i >> 1] = pack2<T>(x0, x1);
+          }
+          tmem_st_32x32b_x16(sbase + c * 16, pk);
+          if (c == 2) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_part[t]);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        const float2 la = f2_unpack(ls2[0]), lb = f2_unpack(ls2[1]);
+        l_sum += (la.x + la.y) + (lb.x + lb.y);
+      }
+      if (!good) break;
+      if (n > 0) {
+        good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
+        if (!good) break;
+        tc_fence_after();
+      }
+      const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;  // (a NaN sum stays a NaN)
+      const PtItem w = items[at.stage];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[at.stage]);
+      const int row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32 + lane;
+      const int head = w.head + (kMode == kTilesOfHead ? 0 : t);
+      T* dst = static_cast<T*>(p.out) + static_cast<long long>(w.q0 + row) * p.ldo + static_cast<long long>(head) * p.hso;
+      const bool write = row < w.lq && (!kApart || head < p.hq);
+      if (n > 0) {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(obase + c * 32, o);
           tmem_wait_ld();
+          if (c == D / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_empty[t]);
+          }
+          if (write) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32b_x32(obase + c * 32, o);
-        }
-      }
-      l_sum *= alpha;
-      const uint64_t ua2 = f2_splat(p.scale_log2), nm2 = f2_splat(m_used == -INFINITY ? 0.f : -m_used);
-      uint64_t ls2[2] = {f2_splat(0.f), f2_splat(0.f)};
+            for (int i = 0; i < 4; ++i) {
+              uint32_t x[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 xx = f2_unpack(f2_fma(f2_pack(r[c][i], r[c][i + 1]), ua2, nm2));
-          const float e0 = fast_exp2(xx.x), e1 = fast_exp2(xx.y);
-          ls2[(i >> 1) & 1] = f2_add(ls2[(i >> 1) & 1], f2_pack(__float_as_uint(e0), __float_as_uint(e1)));
-          pk[i >> 1] = pack2<T>(e0, e1);
-        }
-        tmem_st_32x32b_x16(sbase + c * 16, pk);
-        if (c == 2) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_part[t]);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
-      const float2 la = f2_unpack(ls2[0]), lb = f2_unpack(ls2[1]);
-      l_sum += (la.x + la.y) + (lb.x + lb.y);
-    }
-    if (good && n > 0) good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], (n - 1) & 1, p.err, kErrWaitEpilogue));
-    if (good) {
-      tc_fence_after();
-      const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;  // (a NaN sum stays a NaN)
-      T* dst = static_cast<T*>(p.out) + static_cast<long long>(s.q0 + row) * p.ldo +
-               static_cast<long long>(t ? head[1] : head[0]) * p.hso;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_ld_32x32b_x32(obase + c * 32, o);
-          tmem_wait_ld();
-        }
-        if (row < s.lq) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = l_sum != 0.f ? pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv)
-                                  : 0u;  // sees nothing (O may not have been written at all)
-            reinterpret_cast<uint4*>(dst + c * 32)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 4; ++k)
+                x[k] = l_sum != 0.f ? pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv)
+                                    : 0u;  // sees nothing
+              reinterpret_cast<uint4*>(dst + c * 32)[i] = make_uint4(x[0], x[1], x[2], x[3]);
+            }
           }
         }
+      } else if (write) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
       }
     }
   }
@@ -832,6 +1064,9 @@ __global__ void __launch_bounds__(128) packed_combine_kernel(const PkParams p) {
 
 // ---------------------------------------------------------------------------- host side
 
+// Average query rows per sequence up to which two heads beat two tiles of one head.
+constexpr int64_t kPtApartRows = 256;
+
 // What a call runs, from its sizes alone (the offsets are on the device).
 struct PkPlan {
   bool rows = false;       // packed_rows (+ packed_combine), else packed_tiles
@@ -878,18 +1113,19 @@ b2g_status launch_rows(const PkParams& p, int sms, cudaStream_t st) {
                     dim3(128), 0, st, "packed_combine launch", p);
 }
 
-template <typename T, int D, bool kHeadPairs>
-b2g_status launch_tiles(const PkParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+template <typename T, int D, int kMode>
+b2g_status launch_tiles(const PkParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, int sms,
                         cudaStream_t st) {
   constexpr uint32_t smem = PtLayout<D>::kSmem;
   static_assert(smem <= 227 * 1024, "shared memory budget");
-  auto kern = packed_tiles_kernel<T, D, kHeadPairs>;
+  auto kern = packed_tiles_kernel<T, D, kMode>;
   b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                             "cudaFuncSetAttribute(packed_tiles)");
   if (s != B2G_OK) return s;
-  constexpr int kSpan = kHeadPairs ? kPtRows : 2 * kPtRows;
-  const dim3 grid(static_cast<unsigned>(p.total_q / kSpan + p.batch), static_cast<unsigned>(kHeadPairs ? p.hq / 2 : p.hq));
-  return launch_pdl(kern, grid, dim3(kPtThreads), smem, st, "packed_tiles launch", tq, tk, tv, p);
+  constexpr int kSpan = kMode == kTilesOfHead ? 2 * kPtRows : kPtRows;
+  const int64_t items = (static_cast<int64_t>(p.total_q) / kSpan + p.batch) * (kMode == kTilesOfHead ? p.hq : (p.hq + 1) / 2);
+  return launch_pdl(kern, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kPtThreads), smem, st,
+                    "packed_tiles launch", tq, tk, tv, p);
 }
 
 template <typename T, int D>
@@ -907,7 +1143,10 @@ b2g_status run_packed(const b2g_attention_packed_desc* d, PkParams p, void* ws, 
   if ((s = make_operand_map(&tq, p.q, dt, D, p.total_q, p.ldq, p.hq, p.hsq, kPtRows)) != B2G_OK) return s;
   if ((s = make_operand_map(&tk, p.k, dt, D, p.total_k, p.ldk, p.hk, p.hsk, kPtKeys)) != B2G_OK) return s;
   if ((s = make_operand_map(&tv, p.v, dt, D, p.total_k, p.ldv, p.hk, p.hsv, kPtKeys)) != B2G_OK) return s;
-  return p.group % 2 == 0 ? launch_tiles<T, D, true>(p, tq, tk, tv, st) : launch_tiles<T, D, false>(p, tq, tk, tv, st);
+  if (p.group % 2 == 0) return launch_tiles<T, D, kHeadsOfGroup>(p, tq, tk, tv, sms, st);
+  if (p.total_q <= kPtApartRows * static_cast<int64_t>(p.batch))
+    return launch_tiles<T, D, kHeadsApart>(p, tq, tk, tv, sms, st);
+  return launch_tiles<T, D, kTilesOfHead>(p, tq, tk, tv, sms, st);
 }
 
 // A stride of a dimension that has one element says nothing: any valid one.
