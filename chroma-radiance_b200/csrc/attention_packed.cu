@@ -146,12 +146,13 @@ enum { kTilesOfHead = 0, kHeadsOfGroup = 1, kHeadsApart = 2 };
 
 template <int D>
 struct PtLayout {
-  static constexpr int KS = D == 128 ? 3 : 6, VS = D == 128 ? 2 : 4;
+  static constexpr int KS = D == 128 ? 2 : 6, VS = D == 128 ? 2 : 4;
   static constexpr uint32_t kTileBytes = 128 * D * 2;  // Q tile, K block, V block: D / 64 boxes
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kK = kQ + 2 * kTileBytes;
   static constexpr uint32_t kV = kK + KS * kTileBytes;
-  static constexpr uint32_t kBars = kV + VS * kTileBytes;
+  static constexpr uint32_t kOut = kV + VS * kTileBytes;   // 32 rows x 64 columns of output per softmax warp
+  static constexpr uint32_t kBars = kOut + 8 * 4096;
   static constexpr uint32_t kOrder = kBars + 384;      // sequences in working order, uint16 [kPtSorted]
   static constexpr uint32_t kItems = kOrder + 2 * kPtSorted;
   static constexpr uint32_t kSmem = 1024 + kItems + 32 * kPtItems;
@@ -205,16 +206,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* p_full = bars + 8;      // [tile] all of P written
   uint64_t* pv_done = bars + 10;    // [tile] P.V added
   uint64_t* o_empty = bars + 12;    // [tile] O read (4 softmax warps)
-  uint64_t* v_tail = bars + 14;     // an item's last V block, before its foreign rows are zeroed
-  uint64_t* drain_bar = bars + 15;
-  uint64_t* k_full = bars + 16;
+  uint64_t* drain_bar = bars + 14;
+  uint64_t* k_full = bars + 15;
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;
   uint64_t* v_empty = v_full + VS;
-  uint64_t* item_full = v_empty + VS;
+  uint64_t* v_land = v_empty + VS;  // V blocks whose rows past the keys in sight are still to be zeroed
+  uint64_t* item_full = v_land + VS;
   uint64_t* item_empty = item_full + kPtItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + kPtItems);
-  static_assert(8 * (16 + 2 * (KS + VS + kPtItems)) + 4 <= 384, "barriers");
+  static_assert(8 * (15 + 2 * KS + 3 * VS + 2 * kPtItems) + 4 <= 384, "barriers");
   PtItem* items = reinterpret_cast<PtItem*>(smem + Ly::kItems);
   uint16_t* order = reinterpret_cast<uint16_t*>(smem + Ly::kOrder);
 
@@ -229,7 +230,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&pv_done[t], 1);
       mbar_init(&o_empty[t], 4);
     }
-    mbar_init(v_tail, 1);
     mbar_init(drain_bar, 1);
     for (int i = 0; i < kPtItems; ++i) {
       mbar_init(&item_full[i], 1);
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int i = 0; i < VS; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_land[i], 1);
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     return p.causal ? clampi(min(last, w.lq) + w.lk - w.lq, 0, w.lk) : w.lk;
   };
 
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return mbar_wait_short(bar, parity, p.err, code); };
   if (warp < 4) {
     regs_dec<kPtRegsIdle>();
     if (warp == 3) {
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         bool ok = true;
         if (lane == 0) {
-          ok = mbar_wait(&item_empty[at.stage], at.parity ^ 1u, p.err, kErrWaitProducer);
+          ok = mbar_wait_short(&item_empty[at.stage], at.parity ^ 1u, p.err, kErrWaitProducer);
           if (ok) {
             items[at.stage] = w;
             mbar_arrive(&item_full[at.stage]);
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       int k_used = 0;
       bool ok = true, q_used[2] = {false, false};
       for (; ok; at.next()) {
-        if (!(ok = mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitProducer))) break;
+        if (!(ok = mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitProducer))) break;
         const PtItem w = items[at.stage];
         mbar_arrive(&item_empty[at.stage]);
         if (w.head < 0) break;
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (ok && j == 0 && w.blocks[t] > 0) {  // this tile's Q
-              ok = mbar_wait(&q_empty[t], q_parity[t] ^ 1u, p.err, kErrWaitProducer);
+              ok = mbar_wait_short(&q_empty[t], q_parity[t] ^ 1u, p.err, kErrWaitProducer);
               if (!ok) break;
               q_parity[t] ^= 1u;
               q_used[t] = true;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                             w.head + (kMode == kTilesOfHead ? 0 : t), once);
             }
             if (kApart ? j >= w.blocks[t] : t != 0) continue;
-            ok = mbar_wait(&k_empty[k_at.stage], k_at.parity ^ 1u, p.err, kErrWaitProducer);
+            ok = mbar_wait_short(&k_empty[k_at.stage], k_at.parity ^ 1u, p.err, kErrWaitProducer);
             if (!ok) break;
             mbar_arrive_expect_tx(&k_full[k_at.stage], Ly::kTileBytes);
 #pragma unroll
@@ -377,60 +379,90 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
     } else if (warp == 2) {
       // ---------------------------------------------------------- V
+      // A block that reaches past the keys in sight lands on v_land; its rows from there on (of a
+      // block of few keys) are zeroed before it is
+      // passed to the MMAs.  Loads go
+      // out ahead of that while stages are free.
       const uint64_t shared_kv = policy_evict_last();
       Turn<kPtItems> at;
-      Turn<VS> v_at;
-      uint32_t tail_parity = 0;
-      int v_used = 0;
+      Turn<VS> v_at, tail_at;
+      PtItem w{};
+      int seen = 0;
+      auto nkb = [](const PtItem& i) { return max(i.blocks[0], i.blocks[1]); };
+      int key = 0, t = 0;              // the next load: this block of the item, and head
+      bool have = false, more = true;  // there is a next load; there may be more items
+      int used = 0;
+      uint32_t tails = 0;              // a byte per stage: rows to keep of an unfinished tail (0: none)
+      uint32_t land_parity = 0;        // bit per stage
+      auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(smem_u32(bar), parity)); };
       bool ok = true;
-      for (; ok; at.next()) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitProducer));
-        if (!ok) break;
-        const PtItem w = items[at.stage];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&item_empty[at.stage]);
-        if (w.head < 0) break;
-        const int nkb = max(w.blocks[0], w.blocks[1]), seen = keys_seen(w);
-        const int kv_head = w.head / p.group, kv_head_b = kApart ? (w.head + 1) / p.group : kv_head;
-        for (int j = 0; j < nkb && ok; ++j) {
-#pragma unroll
-          for (int t = 0; t < (kApart ? 2 : 1); ++t) {
-            if (!ok || (kApart && j >= w.blocks[t])) continue;
-            ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[v_at.stage], v_at.parity ^ 1u, p.err, kErrWaitProducer));
-            if (!ok) break;
-            const int valid = seen - j * kPtKeys;  // rows of this block that are seen
-            uint8_t* dst = sV + v_at.stage * Ly::kTileBytes;
-            uint64_t* bar = valid < kPtKeys ? v_tail : &v_full[v_at.stage];
-            if (lane == 0) {
-              mbar_arrive_expect_tx(bar, Ly::kTileBytes);
-#pragma unroll
-              for (int c = 0; c < D / 64; ++c)
-                tma_load_3d(dst + c * kPtBox, &tmV, bar, c * 64, w.k0 + j * kPtKeys, t ? kv_head_b : kv_head, shared_kv);
-            }
-            if (valid < kPtKeys) {  // the last block: rows past the sequence become zeros
-              ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tail_parity, p.err, kErrWaitProducer));
-              if (!ok) break;
-              tail_parity ^= 1u;
-              const int words = (kPtKeys - valid) * 8;
-#pragma unroll
-              for (int c = 0; c < D / 64; ++c) {
-                uint4* z = reinterpret_cast<uint4*>(dst + c * kPtBox + valid * 128);
-                for (int i = lane; i < words; i += 32) z[i] = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&v_full[v_at.stage]);
-            }
-            v_at.next();
-            ++v_used;
-          }
+#pragma unroll 1
+      while (ok) {
+        if (!have && more && (tails == 0 || ready(&item_full[at.stage], at.parity))) {
+          ok = __all_sync(0xffffffffu, wait(&item_full[at.stage], at.parity, kErrWaitProducer));
+          if (!ok) break;
+          w = items[at.stage];
+          __syncwarp();
+          more = w.head >= 0;
+          if (more && lane == 0) mbar_arrive(&item_empty[at.stage]);
+          at.next();
+          key = 0;
+          t = kApart && w.blocks[0] == 0 ? 1 : 0;
+          seen = keys_seen(w);
+          have = more && nkb(w) > 0;
+          continue;
         }
+        if (have && (tails == 0 || ready(&v_empty[v_at.stage], v_at.parity ^ 1u))) {
+          const int st = v_at.stage;
+          ok = __all_sync(0xffffffffu, wait(&v_empty[st], v_at.parity ^ 1u, kErrWaitProducer));
+          if (!ok) break;
+          const int valid = seen - key;  // rows of this block that are seen
+          if (lane == 0) {
+            uint64_t* bar = valid < kPtKeys ? &v_land[st] : &v_full[st];
+            mbar_arrive_expect_tx(bar, Ly::kTileBytes);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_3d(sV + st * Ly::kTileBytes + c * kPtBox, &tmV, bar, c * 64, w.k0 + key, (w.head + t) / p.group,
+                          shared_kv);
+          }
+          if (valid < kPtKeys) tails |= static_cast<uint32_t>(valid) << (8 * st);
+          v_at.next();
+          ++used;
+          if (kApart && t == 0 && key < w.blocks[1] * kPtKeys) t = 1;
+          else {
+            key += kPtKeys;
+            t = kApart && key >= w.blocks[0] * kPtKeys ? 1 : 0;
+            have = key < nkb(w) * kPtKeys;
+          }
+          continue;
+        }
+        if (tails == 0) break;  // nothing left to do
+        const uint32_t valid = (tails >> (8 * tail_at.stage)) & 0xFFu;
+        if (valid) {  // the oldest tail
+          const int st = tail_at.stage;
+          ok = __all_sync(0xffffffffu, wait(&v_land[st], (land_parity >> st) & 1u, kErrWaitProducer));
+          if (!ok) break;
+          land_parity ^= 1u << st;
+          const int zeros = kPtKeys - static_cast<int>(valid);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            uint4* z = reinterpret_cast<uint4*>(sV + st * Ly::kTileBytes + c * kPtBox + valid * 128);
+            for (int i = lane; i < zeros * 8; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[st]);
+          tails &= ~(0xFFu << (8 * st));
+        }
+        tail_at.next();
       }
       if (lane == 0) {
-        if (!ok) mbar_wait_drain(v_tail, tail_parity);
-        for (int i = min(v_used, VS); i > 0; --i) {
+        // Loads of an abandoned run land before the shared memory goes away.
+#pragma unroll 1
+        for (int i = min(used, VS); i > 0; --i) {
           v_at.back();
-          mbar_wait_drain(&v_full[v_at.stage], v_at.parity);
+          if ((tails >> (8 * v_at.stage)) & 0xFFu) mbar_wait_drain(&v_land[v_at.stage], (land_parity >> v_at.stage) & 1u);
+          else mbar_wait_drain(&v_full[v_at.stage], v_at.parity);
         }
       }
     } else if (warp == 1 && lane == 0) {
@@ -447,7 +479,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       auto next_blocks = [&](int (&blocks)[2]) {
         for (;;) {
           blocks[0] = blocks[1] = 0;
-          if (!(ok = mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
+          if (!(ok = mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
           const bool end = ld_shared_int(&items[at.stage].head) < 0;
           blocks[0] = ld_shared_int(&items[at.stage].blocks[0]);
           blocks[1] = ld_shared_int(&items[at.stage].blocks[1]);
@@ -460,10 +492,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // S of the key block at k_at, of tile t; first: of its item (Q), last: Q is free afterwards.
       auto issue_s = [&](int t, bool first, bool last) {
         if (first) {
-          if (!(ok = mbar_wait(&q_full[t], q_parity[t], p.err, kErrWaitMma))) return;
+          if (!(ok = mbar_wait_short(&q_full[t], q_parity[t], p.err, kErrWaitMma))) return;
           q_parity[t] ^= 1u;
         }
-        if (!(ok = mbar_wait(&k_full[k_at.stage], k_at.parity, p.err, kErrWaitMma))) return;
+        if (!(ok = mbar_wait_short(&k_full[k_at.stage], k_at.parity, p.err, kErrWaitMma))) return;
         tc_fence_after();
         const uint32_t q0 = smem_u32(sQ + t * Ly::kTileBytes), k0 = smem_u32(sK + k_at.stage * Ly::kTileBytes);
 #pragma unroll
@@ -498,18 +530,18 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (j < cur[t]) {
               const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
               if (j == 0) {  // O is overwritten: the last item's has been read
-                if (!(ok = mbar_wait(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
+                if (!(ok = mbar_wait_short(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
                 o_parity[t] ^= 1u;
               }
               // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
-              if (!(ok = mbar_wait(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
-              if (!(ok = mbar_wait(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
+              if (!(ok = mbar_wait_short(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
+              if (!(ok = mbar_wait_short(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
               tc_fence_after();
 #pragma unroll
               for (int k = 0; k < 6; ++k)
                 umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
                             idesc_o, (j | k) != 0 ? 1u : 0u);
-              if (!(ok = mbar_wait(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
+              if (!(ok = mbar_wait_short(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
               tc_fence_after();
 #pragma unroll
               for (int k = 6; k < 8; ++k)
@@ -558,18 +590,39 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     Turn<kPtItems> at;
     bool good = true;
     for (;; at.next()) {
-      good = __all_sync(0xffffffffu, mbar_wait(&item_full[at.stage], at.parity, p.err, kErrWaitEpilogue));
+      good = __all_sync(0xffffffffu, mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitEpilogue));
       if (!good || ld_shared_int(&items[at.stage].head) < 0) break;
       const int n = ld_shared_int(&items[at.stage].blocks[t]);
       int left;  // keys that this row sees, from the block at hand on
+      bool idle;
       {
         const int lq = ld_shared_int(&items[at.stage].lq), lk = ld_shared_int(&items[at.stage].lk);
         const int row = ld_shared_int(&items[at.stage].row0) + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32 + lane;
         left = p.causal ? min(lk, row + 1 + lk - lq) : lk;
+        idle = row - lane >= lq;
+      }
+      if (idle) {
+        // None of the warp's rows is in the sequence: what its P and O hold matters to no other row.
+#pragma unroll 1
+        for (int j = 0; j < n; ++j, s_parity ^= 1u) {
+          good = __all_sync(0xffffffffu, mbar_wait_short(&s_full[t], s_parity, p.err, kErrWaitEpilogue));
+          if (!good) break;
+          if (lane == 0) {
+            mbar_arrive(&p_part[t]);
+            mbar_arrive(&p_full[t]);
+          }
+        }
+        if (!good) break;
+        if (lane == 0) {
+          if (n > 0) mbar_arrive(&o_empty[t]);
+          mbar_arrive(&item_empty[at.stage]);
+        }
+        __syncwarp();
+        continue;
       }
       float m_used = -INFINITY, l_sum = 0.f;
       for (int j = 0; j < n; ++j, s_parity ^= 1u, left -= kPtKeys) {
-        good = __all_sync(0xffffffffu, mbar_wait(&s_full[t], s_parity, p.err, kErrWaitEpilogue));
+        good = __all_sync(0xffffffffu, mbar_wait_short(&s_full[t], s_parity, p.err, kErrWaitEpilogue));
         if (!good) break;
         tc_fence_after();
         uint32_t r[4][32];
@@ -599,7 +652,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const float alpha = raise ? fast_exp2(m_used - mx) : 1.f;
         if (raise) m_used = mx;
         if (__any_sync(0xffffffffu, raise && j > 0)) {
-          good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
+          good = __all_sync(0xffffffffu, mbar_wait_short(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
           if (!good) break;
           tc_fence_after();
 #pragma unroll
@@ -642,44 +695,57 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       if (!good) break;
       if (n > 0) {
-        good = __all_sync(0xffffffffu, mbar_wait(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
+        good = __all_sync(0xffffffffu, mbar_wait_short(&pv_done[t], s_parity ^ 1u, p.err, kErrWaitEpilogue));
         if (!good) break;
         tc_fence_after();
       }
-      const float inv = l_sum != 0.f ? 1.f / l_sum : 0.f;  // (a NaN sum stays a NaN)
+      const float inv = l_sum != 0.f ? __fdividef(1.f, l_sum) : 0.f;  // (a NaN sum stays a NaN)
       const PtItem w = items[at.stage];
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[at.stage]);
-      const int row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32 + lane;
+      const int warp_row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32;
       const int head = w.head + (kMode == kTilesOfHead ? 0 : t);
-      T* dst = static_cast<T*>(p.out) + static_cast<long long>(w.q0 + row) * p.ldo + static_cast<long long>(head) * p.hso;
-      const bool write = row < w.lq && (!kApart || head < p.hq);
-      if (n > 0) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
+      const int rows = !kApart || head < p.hq ? w.lq - warp_row : 0;  // of this warp's 32
+      // 64 columns at a time through this warp's staging space: a row per lane in, four rows of
+      // 128 bytes per instruction out (16-byte pieces swizzled by the row).  A row that sees nothing
+      // has P = 0 and so O = 0; without any key O was not written, and counts as 0.
+      uint8_t* stage = smem + Ly::kOut + (warp - 4) * 4096;
+      const int out_row = lane >> 3, piece = lane & 7;
+      T* dst = static_cast<T*>(p.out) + static_cast<long long>(w.q0 + warp_row + out_row) * p.ldo +
+               static_cast<long long>(head) * p.hso + piece * 8;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
           tmem_ld_32x32b_x32(obase + c * 32, o);
           tmem_wait_ld();
-          if (c == D / 32 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[t]);
-          }
-          if (write) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t x[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                x[k] = l_sum != 0.f ? pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv)
-                                    : 0u;  // sees nothing
-              reinterpret_cast<uint4*>(dst + c * 32)[i] = make_uint4(x[0], x[1], x[2], x[3]);
-            }
-          }
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-      } else if (write) {
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            x[k] = pack2<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4)) =
+              make_uint4(x[0], x[1], x[2], x[3]);
+        }
+        if (c & 1) {
+          __syncwarp();
+          T* to = dst + (c >> 1) * 64;
+#pragma unroll 1
+          for (int row = out_row; row < 32; row += 4, to += 4 * p.ldo)
+            if (row < rows)
+              *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(stage + row * 128 + ((piece ^ (row & 7)) << 4));
+          __syncwarp();
+        }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[t]);
       }
     }
   }
@@ -1064,7 +1130,10 @@ __global__ void __launch_bounds__(128) packed_combine_kernel(const PkParams p) {
 
 // ---------------------------------------------------------------------------- host side
 
-// Average query rows per sequence up to which two heads beat two tiles of one head.
+// Average queries per sequence up to which packed_rows takes a call.
+constexpr int64_t kPrQueries = 16;
+// Average queries per sequence up to which two heads beat two tiles of one head (24 heads of 128, 64 x 128
+// tokens: 51 and 53 us; 32 x 256: the same; 16 x 512: 92 and 89 us; 96 short prompts 237 and 301 us).
 constexpr int64_t kPtApartRows = 256;
 
 // What a call runs, from its sizes alone (the offsets are on the device).
@@ -1079,8 +1148,10 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 PkPlan plan(const b2g_attention_packed_desc* d, int sms) {
   PkPlan r;
   const int64_t group = d->n_head / d->n_kv_head;
-  // Rows per key head: up to 16 on average fit one tile of packed_rows.
-  r.rows = d->total_q * group <= kPrRows * d->batch || d->total_k == 0;
+  // Up to kPrQueries queries per sequence on average.  Measured on 64 sequences of their own 8 / 16 / 30
+  // tokens, 32 and 8 heads: packed_rows 24 / 35 / 66 us, packed_tiles 39 us; with 24 and 24 heads of
+  // 64 values, 128 sequences of 24: 66 and 54 us.  Long keys favour packed_rows, which shares them out.
+  r.rows = d->total_q <= kPrQueries * d->batch || d->total_k == 0;
   if (!r.rows) return r;
   // A block per share and key head, as many as run at the same time; no more shares than the
   // longest line possible has pieces of kPrMinShare.

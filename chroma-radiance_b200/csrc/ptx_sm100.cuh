@@ -76,6 +76,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Whether the phase has completed, at once (try_wait may suspend the thread for microseconds).
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Waits for the phase with the given parity to complete.  Gives up after kWaitLimitNs,
 // or early when another CTA has already recorded an error; then records `code` in the
 // device error word and returns false so the caller can drain and exit.
@@ -93,6 +106,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
       }
     }
   }
+}
+
+// The same wait in few instructions, for kernels whose roles have many of them (other CTAs' errors
+// are not looked for; the low half of the timer wraps after 4.3 s, past the limit).
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity, int* err, int code) {
+  const uint32_t addr = smem_u32(bar);
+  if (mbar_try_wait(addr, parity)) return true;
+  uint32_t t0, now;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
+#pragma unroll 1
+  do {
+    if (mbar_try_wait(addr, parity)) return true;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
+  } while (now - t0 < static_cast<uint32_t>(kWaitLimitNs));
+  atomicOr(err, code);
+  return false;
 }
 
 // Bounded wait used only on the abort path: never records anything, just stops.
