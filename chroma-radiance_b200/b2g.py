@@ -1118,9 +1118,10 @@ def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torc
         ts.append(gate)
     x_ptr, ws_ptr, n = None, None, 0
     if not codes:
-        n = M * pad + 4 * M + 512  # b2g_gemm_s8_workspace and some
-        ws = _empty((n,), torch.int8, x, stream)
-        ws_ptr = ws.data_ptr()
+        if M > 1 or K > 16384:  # (one token up to there needs none)
+            n = M * pad + 4 * M + 512  # b2g_gemm_s8_workspace and some
+            ws = _empty((n,), torch.int8, x, stream)
+            ws_ptr = ws.data_ptr()
     elif x_scale is not None:
         x_ptr = _vector(x_scale, torch.float32, M, "gemm_s8: x_scale")
         ts.append(x_scale)
