@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -111,6 +112,20 @@ class AttentionPackedDesc(ctypes.Structure):
     ]
 
 
+def _packer(cls):
+    """A function of a descriptor's fields in order (addresses of nothing: 0) that returns its bytes, in a
+    third of the time that filling the ctypes structure takes."""
+    codes = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
+    fields = "".join(codes[t] if t in codes else f"{t._length_}{codes[t._type_]}" for _, t in cls._fields_)
+    packed = struct.Struct("@" + fields + "0q")  # C's alignment, the end's as well
+    assert packed.size == ctypes.sizeof(cls)
+    return packed.pack
+
+
+_pack_gemm = _packer(GemmDesc)
+_pack_qk_norm_rope = _packer(QkNormRopeDesc)
+_pack_attention_packed = _packer(AttentionPackedDesc)
+
 _lib = None
 
 # Exported symbols of libb2g.so with their ctypes signatures (status-returning unless noted).
@@ -182,11 +197,11 @@ _SIGNATURES = {
                                                                                  ctypes.c_void_p, ctypes.c_void_p],
                         ctypes.c_int),
     "b2g_gemm_s8_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int], ctypes.c_size_t),
-    "b2g_gemm_s8": ([ctypes.POINTER(GemmDesc)] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p],
+    "b2g_gemm_s8": ([ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.c_void_p],
                     ctypes.c_int),
-    "b2g_qk_norm_rope": ([ctypes.POINTER(QkNormRopeDesc), ctypes.c_void_p], ctypes.c_int),
-    "b2g_attention_packed_workspace": ([ctypes.POINTER(AttentionPackedDesc)], ctypes.c_size_t),
-    "b2g_attention_packed": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    "b2g_qk_norm_rope": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "b2g_attention_packed_workspace": ([ctypes.c_void_p], ctypes.c_size_t),
+    "b2g_attention_packed": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
                              ctypes.c_int),
     "b2g_check_device_error": ([ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "b2g_launch_count": ([], ctypes.c_uint64),
@@ -1044,6 +1059,14 @@ def _empty(shape, dtype: torch.dtype, like: torch.Tensor, stream: torch.cuda.Str
         return like.new_empty(shape, dtype=dtype)
 
 
+def _empty_like(t: torch.Tensor, dtype: torch.dtype, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A new contiguous tensor of t's shape for use on `stream`."""
+    if stream is None:
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _vector(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
     """The address of a contiguous vector of n values."""
     if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
@@ -1104,18 +1127,20 @@ def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torc
     o_dtype = _TORCH_TO_B2G.get(out.dtype)
     if o_dtype is None:
         raise B2GError("gemm_s8: out must be F32, BF16 or F16")
-    ts, pad = [x, wq, w_scale, out], (K + 15) // 16 * 16
-    d = GemmDesc(M, N, K, x.data_ptr(), a_dtype, ldx if M > 1 else pad if codes else K, wq.data_ptr(), S8,
-                 ldw if N > 1 else pad, None, F32, out.data_ptr(), o_dtype, out.stride(0) if M > 1 else N, epi, None)
+    ts, pad, b_ptr, b_dtype, g_ptr = [x, wq, w_scale, out], (K + 15) // 16 * 16, 0, F32, 0
     w_ptr = _vector(w_scale, torch.float32, N, "gemm_s8: w_scale")
     if bias is not None:
-        if bias.dtype not in (torch.float32, torch.bfloat16):
+        b_dtype = _TORCH_TO_B2G.get(bias.dtype)
+        if b_dtype is None or b_dtype == F16:
             raise B2GError("gemm_s8: bias must be F32 or BF16")
-        d.bias, d.bias_dtype = _vector(bias, bias.dtype, N, "gemm_s8: bias"), _TORCH_TO_B2G[bias.dtype]
+        b_ptr = _vector(bias, bias.dtype, N, "gemm_s8: bias")
         ts.append(bias)
     if epi == EPI_GATED_RESIDUAL and gate is not None:
-        d.gate = _vector(gate, torch.float32, N, "gemm_s8: gate")
+        g_ptr = _vector(gate, torch.float32, N, "gemm_s8: gate")
         ts.append(gate)
+    d = _pack_gemm(M, N, K, x.data_ptr(), a_dtype, ldx if M > 1 else pad if codes else K, wq.data_ptr(), S8,
+                   ldw if N > 1 else pad, b_ptr, b_dtype, out.data_ptr(), o_dtype, out.stride(0) if M > 1 else N, epi,
+                   g_ptr)
     x_ptr, ws_ptr, n = None, None, 0
     if not codes:
         if M > 1 or K > 16384:  # (one token up to there needs none)
@@ -1125,7 +1150,7 @@ def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torc
     elif x_scale is not None:
         x_ptr = _vector(x_scale, torch.float32, M, "gemm_s8: x_scale")
         ts.append(x_scale)
-    _check(load().b2g_gemm_s8(ctypes.byref(d), x_ptr, w_ptr, ws_ptr, n, _on(stream, *ts)))
+    _check(load().b2g_gemm_s8(d, x_ptr, w_ptr, ws_ptr, n, _on(stream, *ts)))
     return out
 
 
@@ -1158,26 +1183,26 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes
     if n_axes > 4:
         raise B2GError("qk_norm_rope: at most 4 axes")
     if q_out is None:
-        q_out = _empty((T, H, D), out_dtype or (q.dtype if k_out is None else k_out.dtype), q, stream)
+        q_out = _empty_like(q, out_dtype or (q.dtype if k_out is None else k_out.dtype), stream)
     if k_out is None:
-        k_out = _empty((T, HK, D), q_out.dtype, k, stream)
+        k_out = _empty_like(k, q_out.dtype, stream)
     odt = _TORCH_TO_B2G.get(q_out.dtype)
     if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype is not k_out.dtype or odt is None or (
             out_dtype is not None and out_dtype is not q_out.dtype):
         raise B2GError("qk_norm_rope: outputs must have the inputs' shapes and one F32/BF16/F16 type")
     (ldqo, hsqo), (ldko, hsko) = _heads(q_out, "qk_norm_rope: q_out"), _heads(k_out, "qk_norm_rope: k_out")
-    ts, qn, kn = [q, k, positions, q_out, k_out], None, None
+    ts, qn, kn = [q, k, positions, q_out, k_out], 0, 0
     if q_norm is not None:
         qn = _vector(q_norm, torch.float32, D, "qk_norm_rope: q_norm")
         ts.append(q_norm)
     if k_norm is not None:
         kn = _vector(k_norm, torch.float32, D, "qk_norm_rope: k_norm")
         ts.append(k_norm)
-    d = QkNormRopeDesc(q.data_ptr(), k.data_ptr(), dt, q_out.data_ptr(), k_out.data_ptr(), odt, ldq, hsq, ldk, hsk,
-                       ldqo, hsqo, ldko, hsko, T, H, HK, D, qn, kn, eps, positions.data_ptr(),
-                       positions.stride(0) if T > 1 else n_axes, n_axes, tuple(axes_dim), theta,
-                       1 if interleaved else 0)
-    _check(load().b2g_qk_norm_rope(ctypes.byref(d), _on(stream, *ts)))
+    dims = (*axes_dim, 0, 0, 0, 0)
+    d = _pack_qk_norm_rope(q.data_ptr(), k.data_ptr(), dt, q_out.data_ptr(), k_out.data_ptr(), odt, ldq, hsq, ldk, hsk,
+                           ldqo, hsqo, ldko, hsko, T, H, HK, D, qn, kn, eps, positions.data_ptr(),
+                           positions.stride(0) if T > 1 else n_axes, n_axes, *dims[:4], theta, 1 if interleaved else 0)
+    _check(load().b2g_qk_norm_rope(d, _on(stream, *ts)))
     return q_out, k_out
 
 
@@ -1205,21 +1230,20 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     cq = _vector(cu_q, torch.int32, B + 1, "attention_packed: cu_q")
     ck = _vector(cu_k, torch.int32, B + 1, "attention_packed: cu_k")
     if out is None:
-        out = _empty((TQ, H, D), dtype, q, stream)
+        out = _empty_like(q, dtype, stream)
     elif out.shape != q.shape or out.dtype is not dtype:
         raise B2GError("attention_packed: out must have q's shape and type")
     ldo, hso = _heads(out, "attention_packed: out")
-    ts, kl = [q, k, v, cu_q, cu_k, out], None
+    ts, kl = [q, k, v, cu_q, cu_k, out], 0
     if k_lens is not None:
         kl = _vector(k_lens, torch.int32, B, "attention_packed: k_lens")
         ts.append(k_lens)
     lib, s = load(), _on(stream, *ts)
-    d = AttentionPackedDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[dtype], ldq, hsq,
-                            ldk, hsk, ldv, hsv, ldo, hso, TQ, TK, B, cq, ck, kl, H, HK, D,
-                            D ** -0.5 if scale is None else scale, 1 if causal else 0)
-    ref = ctypes.byref(d)
-    n, ws = lib.b2g_attention_packed_workspace(ref), None
+    d = _pack_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[dtype], ldq, hsq,
+                               ldk, hsk, ldv, hsv, ldo, hso, TQ, TK, B, cq, ck, kl, H, HK, D,
+                               D ** -0.5 if scale is None else scale, 1 if causal else 0)
+    n, ws = lib.b2g_attention_packed_workspace(d), None
     if n:
         ws = _empty((n,), torch.int8, q, stream)
-    _check(lib.b2g_attention_packed(ref, None if ws is None else ws.data_ptr(), n, s))
+    _check(lib.b2g_attention_packed(d, None if ws is None else ws.data_ptr(), n, s))
     return out
