@@ -19,6 +19,8 @@
 // and the four chains of sums, shuffles and roots run side by side.  (One step at a time through
 // copies in shared memory, the chain's latency bound the kernel: 190 us for 29120 tokens of 24 + 8 heads;
 // blocks that share a table of a token's angles, behind a barrier: 150 us, and 21 us for 1536 tokens.)
+// As it is: 111 us at 29120 tokens, F32 to bf16 (the copy rate), 11.5 us at 1536 of 24 + 24 heads in bf16 (half of
+// it the chain of one round: positions, angles, load, sum, store), 2.5 us at 64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
