@@ -1059,14 +1059,6 @@ def _empty(shape, dtype: torch.dtype, like: torch.Tensor, stream: torch.cuda.Str
         return like.new_empty(shape, dtype=dtype)
 
 
-def _empty_like(t: torch.Tensor, dtype: torch.dtype, stream: torch.cuda.Stream | None) -> torch.Tensor:
-    """A new contiguous tensor of t's shape for use on `stream`."""
-    if stream is None:
-        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
-    with torch.cuda.stream(stream):
-        return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
-
-
 def _vector(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> int:
     """The address of a contiguous vector of n values."""
     if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
@@ -1162,6 +1154,23 @@ def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
     return st[0], st[1]
 
 
+def _heads_like(t: torch.Tensor, out: torch.Tensor | None, dtype: torch.dtype, stream: torch.cuda.Stream | None,
+                what: str) -> tuple[torch.Tensor, int, int]:
+    """An output of t's [tokens, heads, d] and of `dtype` for use on `stream`, new if `out` is None, and its
+    token and head strides."""
+    if out is None:
+        if stream is None:
+            out = torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+        else:
+            with torch.cuda.stream(stream):
+                out = torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+        _, h, d = t.shape
+        return out, h * d, d
+    if out.shape != t.shape or out.dtype is not dtype:
+        raise B2GError(f"{what} must be {dtype} {list(t.shape)}")
+    return out, *_heads(out, what)
+
+
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes_dim: list[int],
                  q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
                  theta: float = 10000.0, interleaved: bool = True, q_out: torch.Tensor | None = None,
@@ -1182,15 +1191,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes
         raise B2GError("qk_norm_rope: positions must be F32 [tokens, len(axes_dim)]")
     if n_axes > 4:
         raise B2GError("qk_norm_rope: at most 4 axes")
-    if q_out is None:
-        q_out = _empty_like(q, out_dtype or (q.dtype if k_out is None else k_out.dtype), stream)
-    if k_out is None:
-        k_out = _empty_like(k, q_out.dtype, stream)
-    odt = _TORCH_TO_B2G.get(q_out.dtype)
-    if q_out.shape != q.shape or k_out.shape != k.shape or q_out.dtype is not k_out.dtype or odt is None or (
-            out_dtype is not None and out_dtype is not q_out.dtype):
-        raise B2GError("qk_norm_rope: outputs must have the inputs' shapes and one F32/BF16/F16 type")
-    (ldqo, hsqo), (ldko, hsko) = _heads(q_out, "qk_norm_rope: q_out"), _heads(k_out, "qk_norm_rope: k_out")
+    if out_dtype is None:
+        out_dtype = (k_out if q_out is None and k_out is not None else q if q_out is None else q_out).dtype
+    odt = _TORCH_TO_B2G.get(out_dtype)
+    if odt is None:
+        raise B2GError("qk_norm_rope: outputs must be F32, BF16 or F16")
+    q_out, ldqo, hsqo = _heads_like(q, q_out, out_dtype, stream, "qk_norm_rope: q_out")
+    k_out, ldko, hsko = _heads_like(k, k_out, out_dtype, stream, "qk_norm_rope: k_out")
     ts, qn, kn = [q, k, positions, q_out, k_out], 0, 0
     if q_norm is not None:
         qn = _vector(q_norm, torch.float32, D, "qk_norm_rope: q_norm")
@@ -1229,11 +1236,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         raise B2GError("attention_packed: cu_q must hold batch + 1 offsets")
     cq = _vector(cu_q, torch.int32, B + 1, "attention_packed: cu_q")
     ck = _vector(cu_k, torch.int32, B + 1, "attention_packed: cu_k")
-    if out is None:
-        out = _empty_like(q, dtype, stream)
-    elif out.shape != q.shape or out.dtype is not dtype:
-        raise B2GError("attention_packed: out must have q's shape and type")
-    ldo, hso = _heads(out, "attention_packed: out")
+    out, ldo, hso = _heads_like(q, out, dtype, stream, "attention_packed: out")
     ts, kl = [q, k, v, cu_q, cu_k, out], 0
     if k_lens is not None:
         kl = _vector(k_lens, torch.int32, B, "attention_packed: k_lens")
