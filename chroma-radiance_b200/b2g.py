@@ -17,13 +17,15 @@ CPU fallback: without the library or a B200 every call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
-import struct
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libb2g.so"
+CALLS_PATH = LIB_PATH.with_name("b2g_calls.so")
 
 # b2g_dtype
 F32, F16, BF16, E4M3, S8 = 0, 1, 2, 3, 4
@@ -112,20 +114,6 @@ class AttentionPackedDesc(ctypes.Structure):
     ]
 
 
-def _packer(cls):
-    """A function of a descriptor's fields in order (addresses of nothing: 0) that returns its bytes, in a
-    third of the time that filling the ctypes structure takes."""
-    codes = {ctypes.c_void_p: "P", ctypes.c_int: "i", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_double: "d"}
-    fields = "".join(codes[t] if t in codes else f"{t._length_}{codes[t._type_]}" for _, t in cls._fields_)
-    packed = struct.Struct("@" + fields + "0q")  # C's alignment, the end's as well
-    assert packed.size == ctypes.sizeof(cls)
-    return packed.pack
-
-
-_pack_gemm = _packer(GemmDesc)
-_pack_qk_norm_rope = _packer(QkNormRopeDesc)
-_pack_attention_packed = _packer(AttentionPackedDesc)
-
 _lib = None
 
 # Exported symbols of libb2g.so with their ctypes signatures (status-returning unless noted).
@@ -197,11 +185,11 @@ _SIGNATURES = {
                                                                                  ctypes.c_void_p, ctypes.c_void_p],
                         ctypes.c_int),
     "b2g_gemm_s8_workspace": ([ctypes.c_int64, ctypes.c_int64, ctypes.c_int], ctypes.c_size_t),
-    "b2g_gemm_s8": ([ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.c_void_p],
+    "b2g_gemm_s8": ([ctypes.POINTER(GemmDesc)] + [ctypes.c_void_p] * 3 + [ctypes.c_size_t, ctypes.c_void_p],
                     ctypes.c_int),
-    "b2g_qk_norm_rope": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
-    "b2g_attention_packed_workspace": ([ctypes.c_void_p], ctypes.c_size_t),
-    "b2g_attention_packed": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    "b2g_qk_norm_rope": ([ctypes.POINTER(QkNormRopeDesc), ctypes.c_void_p], ctypes.c_int),
+    "b2g_attention_packed_workspace": ([ctypes.POINTER(AttentionPackedDesc)], ctypes.c_size_t),
+    "b2g_attention_packed": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
                              ctypes.c_int),
     "b2g_check_device_error": ([ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "b2g_launch_count": ([], ctypes.c_uint64),
@@ -1038,17 +1026,26 @@ def nerf_final(feat_cond: torch.Tensor, feat_uncond: torch.Tensor | None, norm_s
 #
 # These wrappers stand in front of kernels of a few microseconds, so they ask torch for as little as
 # they can: one pass over the arguments, the raw stream handle, one workspace.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_calls = None
 
 
-def _on(stream: torch.cuda.Stream | None, *ts: torch.Tensor) -> int:
-    """The raw stream of a call on the CUDA tensors `ts`, all of the current device."""
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t.get_device() != dev:
-            raise B2GError("all tensors must be CUDA tensors of the current device")
-    return _raw_stream(dev) if stream is None else stream.cuda_stream
+def _call(name: str, stream: torch.cuda.Stream | None, *args):
+    """The function `name` of csrc/calls.cpp (checks, outputs, workspace, launch) on `stream`, or on torch's
+    current stream.  Raises B2GError if its library is absent."""
+    global _calls
+    if _calls is None:
+        if not CALLS_PATH.exists():
+            raise B2GError(f"{CALLS_PATH} is missing: build it with `python chroma-radiance_b200/build.py`")
+        lib = load()
+        loader = importlib.machinery.ExtensionFileLoader("b2g_calls", str(CALLS_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("b2g_calls", loader))
+        module.bind(lambda symbol: ctypes.cast(getattr(lib, symbol), ctypes.c_void_p).value, B2GError)
+        _calls = module
+    f = getattr(_calls, name)
+    if stream is None:
+        return f(*args)
+    with torch.cuda.stream(stream):
+        return f(*args)
 
 
 def _empty(shape, dtype: torch.dtype, like: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
@@ -1081,7 +1078,10 @@ def quantize_s8(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.
     if out.dtype != torch.int8 or out.shape != x.shape or (cols > 1 and out.stride(1) != 1):
         raise B2GError("quantize_s8: out must be int8 [rows, cols] with unit column stride")
     sp = _vector(scales, torch.float32, rows, "quantize_s8: scales")
-    s = _on(stream, x, out, scales)
+    dev = torch.cuda.current_device()
+    if any(t.get_device() != dev for t in (x, out, scales)):
+        raise B2GError("all tensors must be CUDA tensors of the current device")
+    s = (stream or torch.cuda.current_stream()).cuda_stream
     _check(load().b2g_quantize_s8(x.data_ptr(), _TORCH_TO_B2G[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
                                   out.data_ptr(), out.stride(0) if rows > 1 else cols, sp, s))
     return out, scales
@@ -1096,79 +1096,7 @@ def gemm_s8(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: torc
     wq: int8 [N, K] with 16-byte aligned rows (quantize_s8 of the weight), w_scale its scales.
     x: int8 codes with x_scale, or F32/BF16/F16 activations, quantised per token in the call.  The
     epilogues are gemm()'s."""
-    if x.dim() != 2 or wq.dim() != 2 or wq.dtype is not torch.int8:
-        raise B2GError("gemm_s8: 2-D x and int8 wq expected")
-    (M, K), (N, KW), (ldx, ux), (ldw, uw) = x.shape, wq.shape, x.stride(), wq.stride()
-    if K != KW:
-        raise B2GError(f"gemm_s8: K mismatch {tuple(x.shape)} vs {tuple(wq.shape)}")
-    if K > 1 and (ux != 1 or uw != 1):
-        raise B2GError("gemm_s8: x and wq need unit stride along K")
-    codes = x.dtype is torch.int8
-    a_dtype = S8 if codes else _TORCH_TO_B2G.get(x.dtype)
-    epi = _EPILOGUES.get(epilogue)
-    if a_dtype is None:
-        raise B2GError("gemm_s8: x must be int8, F32, BF16 or F16")
-    if epi is None:
-        raise B2GError(f"gemm_s8: unknown epilogue {epilogue!r}")
-    if out is None:
-        if epi == EPI_GATED_RESIDUAL:
-            raise B2GError("gemm_s8: gated_residual needs `out` (the residual)")
-        out = _empty((M, N), out_dtype or torch.float32, x, stream)
-    elif out.shape != (M, N) or (N > 1 and out.stride(1) != 1):
-        raise B2GError("gemm_s8: out must be [M, N] with unit column stride")
-    o_dtype = _TORCH_TO_B2G.get(out.dtype)
-    if o_dtype is None:
-        raise B2GError("gemm_s8: out must be F32, BF16 or F16")
-    ts, pad, b_ptr, b_dtype, g_ptr = [x, wq, w_scale, out], (K + 15) // 16 * 16, 0, F32, 0
-    w_ptr = _vector(w_scale, torch.float32, N, "gemm_s8: w_scale")
-    if bias is not None:
-        b_dtype = _TORCH_TO_B2G.get(bias.dtype)
-        if b_dtype is None or b_dtype == F16:
-            raise B2GError("gemm_s8: bias must be F32 or BF16")
-        b_ptr = _vector(bias, bias.dtype, N, "gemm_s8: bias")
-        ts.append(bias)
-    if epi == EPI_GATED_RESIDUAL and gate is not None:
-        g_ptr = _vector(gate, torch.float32, N, "gemm_s8: gate")
-        ts.append(gate)
-    d = _pack_gemm(M, N, K, x.data_ptr(), a_dtype, ldx if M > 1 else pad if codes else K, wq.data_ptr(), S8,
-                   ldw if N > 1 else pad, b_ptr, b_dtype, out.data_ptr(), o_dtype, out.stride(0) if M > 1 else N, epi,
-                   g_ptr)
-    x_ptr, ws_ptr, n = None, None, 0
-    if not codes:
-        if M > 1 or K > 16384:  # (one token up to there needs none)
-            n = M * pad + 4 * M + 512  # b2g_gemm_s8_workspace and some
-            ws = _empty((n,), torch.int8, x, stream)
-            ws_ptr = ws.data_ptr()
-    elif x_scale is not None:
-        x_ptr = _vector(x_scale, torch.float32, M, "gemm_s8: x_scale")
-        ts.append(x_scale)
-    _check(load().b2g_gemm_s8(d, x_ptr, w_ptr, ws_ptr, n, _on(stream, *ts)))
-    return out
-
-
-def _heads(t: torch.Tensor, what: str) -> tuple[int, int]:
-    """Token and head stride of a [tokens, heads, d] tensor whose heads are contiguous."""
-    st = t.stride()
-    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
-        raise B2GError(f"{what}: [tokens, heads, d] with unit stride along d expected")
-    return st[0], st[1]
-
-
-def _heads_like(t: torch.Tensor, out: torch.Tensor | None, dtype: torch.dtype, stream: torch.cuda.Stream | None,
-                what: str) -> tuple[torch.Tensor, int, int]:
-    """An output of t's [tokens, heads, d] and of `dtype` for use on `stream`, new if `out` is None, and its
-    token and head strides."""
-    if out is None:
-        if stream is None:
-            out = torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
-        else:
-            with torch.cuda.stream(stream):
-                out = torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
-        _, h, d = t.shape
-        return out, h * d, d
-    if out.shape != t.shape or out.dtype is not dtype:
-        raise B2GError(f"{what} must be {dtype} {list(t.shape)}")
-    return out, *_heads(out, what)
+    return _call("gemm_s8", stream, x, wq, w_scale, bias, out, out_dtype, epilogue, gate, x_scale)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes_dim: list[int],
@@ -1181,36 +1109,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes
     values), in one pass.  interleaved: pairs are neighbouring values, else one value of each half of
     the turned part.  q and k may be views of a fused projection.  Returns (q', k'): q_out and
     k_out when given (q and k themselves for in place), else new tensors of out_dtype (default: q's)."""
-    (ldq, hsq), (ldk, hsk) = _heads(q, "qk_norm_rope: q"), _heads(k, "qk_norm_rope: k")
-    (T, H, D), (TK, HK, DK), n_axes = q.shape, k.shape, len(axes_dim)
-    dt = _TORCH_TO_B2G.get(q.dtype)
-    if TK != T or DK != D or k.dtype is not q.dtype or dt is None:
-        raise B2GError("qk_norm_rope: q and k must have the same tokens, head width and F32/BF16/F16 type")
-    if positions.shape != (T, n_axes) or positions.dtype is not torch.float32 or (
-            n_axes > 1 and positions.stride(1) != 1):
-        raise B2GError("qk_norm_rope: positions must be F32 [tokens, len(axes_dim)]")
-    if n_axes > 4:
-        raise B2GError("qk_norm_rope: at most 4 axes")
-    if out_dtype is None:
-        out_dtype = (k_out if q_out is None and k_out is not None else q if q_out is None else q_out).dtype
-    odt = _TORCH_TO_B2G.get(out_dtype)
-    if odt is None:
-        raise B2GError("qk_norm_rope: outputs must be F32, BF16 or F16")
-    q_out, ldqo, hsqo = _heads_like(q, q_out, out_dtype, stream, "qk_norm_rope: q_out")
-    k_out, ldko, hsko = _heads_like(k, k_out, out_dtype, stream, "qk_norm_rope: k_out")
-    ts, qn, kn = [q, k, positions, q_out, k_out], 0, 0
-    if q_norm is not None:
-        qn = _vector(q_norm, torch.float32, D, "qk_norm_rope: q_norm")
-        ts.append(q_norm)
-    if k_norm is not None:
-        kn = _vector(k_norm, torch.float32, D, "qk_norm_rope: k_norm")
-        ts.append(k_norm)
-    dims = (*axes_dim, 0, 0, 0, 0)
-    d = _pack_qk_norm_rope(q.data_ptr(), k.data_ptr(), dt, q_out.data_ptr(), k_out.data_ptr(), odt, ldq, hsq, ldk, hsk,
-                           ldqo, hsqo, ldko, hsko, T, H, HK, D, qn, kn, eps, positions.data_ptr(),
-                           positions.stride(0) if T > 1 else n_axes, n_axes, *dims[:4], theta, 1 if interleaved else 0)
-    _check(load().b2g_qk_norm_rope(d, _on(stream, *ts)))
-    return q_out, k_out
+    return _call("qk_norm_rope", stream, q, k, positions, axes_dim, q_norm, k_norm, eps, theta, interleaved, q_out, k_out,
+                 out_dtype)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -1223,30 +1123,4 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     given.  causal: the last query sees the last key.  scale None: 1 / sqrt(d).  Offsets and lengths are
     int32 device tensors; a row that sees no key is 0.  Returns [total_q, n_head, d] of q's type (rows
     of no sequence are left as they were)."""
-    (ldq, hsq), (ldk, hsk), (ldv, hsv) = (_heads(q, "attention_packed: q"), _heads(k, "attention_packed: k"),
-                                          _heads(v, "attention_packed: v"))
-    (TQ, H, D), (TK, HK, DK), dtype = q.shape, k.shape, q.dtype
-    if v.shape != k.shape or DK != D or k.dtype is not dtype or v.dtype is not dtype or (
-            dtype is not torch.bfloat16 and dtype is not torch.float16):
-        raise B2GError("attention_packed: q, k, v must be BF16 or F16 of one head width, k and v of one shape")
-    if cu_k is None:
-        cu_k = cu_q
-    B = cu_q.numel() - 1
-    if B < 0:
-        raise B2GError("attention_packed: cu_q must hold batch + 1 offsets")
-    cq = _vector(cu_q, torch.int32, B + 1, "attention_packed: cu_q")
-    ck = _vector(cu_k, torch.int32, B + 1, "attention_packed: cu_k")
-    out, ldo, hso = _heads_like(q, out, dtype, stream, "attention_packed: out")
-    ts, kl = [q, k, v, cu_q, cu_k, out], 0
-    if k_lens is not None:
-        kl = _vector(k_lens, torch.int32, B, "attention_packed: k_lens")
-        ts.append(k_lens)
-    lib, s = load(), _on(stream, *ts)
-    d = _pack_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _TORCH_TO_B2G[dtype], ldq, hsq,
-                               ldk, hsk, ldv, hsv, ldo, hso, TQ, TK, B, cq, ck, kl, H, HK, D,
-                               D ** -0.5 if scale is None else scale, 1 if causal else 0)
-    n, ws = lib.b2g_attention_packed_workspace(d), None
-    if n:
-        ws = _empty((n,), torch.int8, q, stream)
-    _check(lib.b2g_attention_packed(d, None if ws is None else ws.data_ptr(), n, s))
-    return out
+    return _call("attention_packed", stream, q, k, v, cu_q, cu_k, k_lens, causal, scale, out)

@@ -1,4 +1,5 @@
-"""Builds libb2g.so (the engine) in-tree with nvcc for sm_100a.
+"""Builds libb2g.so (the engine) in-tree with nvcc for sm_100a, and b2g_calls.so (the Python side of the
+packed operators, csrc/calls.cpp) with the host compiler against torch.
 
     python chroma-radiance_b200/build.py [--force]
 
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,6 +23,7 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "lib" / "libb2g.so"
+CALLS = PKG / "lib" / "b2g_calls.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -56,6 +59,25 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_calls(force: bool = False) -> Path:
+    src = CSRC / "calls.cpp"
+    if not force and not _stale(CALLS, [src, REPO / "include" / "b2g.h"]):
+        return CALLS
+    import torch  # (its headers and libraries; the interpreter's are beside them)
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [REPO / "include", root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           *(f"-I{i}" for i in includes), str(src), "-o", str(CALLS), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compiling calls.cpp failed:\n{r.stdout}\n{r.stderr}")
+    return CALLS
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     BUILD.mkdir(parents=True, exist_ok=True)
     LIB.parent.mkdir(parents=True, exist_ok=True)
@@ -88,6 +110,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_calls(force)
     return LIB
 
 
