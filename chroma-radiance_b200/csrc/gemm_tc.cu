@@ -445,8 +445,16 @@ __device__ __forceinline__ void stage_scale(const TcParams& p, const TcGroup& G,
 template <int KIND>
 __device__ __forceinline__ void scale_chunk(uint32_t (&r)[32], float rs, const float* cs) {
   if constexpr (KIND == 3) {
+    // The channel's scale first: a token's may be near either end of the type's range.
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__int2float_rn(static_cast<int>(r[j])));
+    for (int j = 0; j < 32; j += 4) {
+      const float4 c = *reinterpret_cast<const float4*>(cs + j);
+      r[j] = __float_as_uint(__int2float_rn(static_cast<int>(r[j])) * c.x * rs);
+      r[j + 1] = __float_as_uint(__int2float_rn(static_cast<int>(r[j + 1])) * c.y * rs);
+      r[j + 2] = __float_as_uint(__int2float_rn(static_cast<int>(r[j + 2])) * c.z * rs);
+      r[j + 3] = __float_as_uint(__int2float_rn(static_cast<int>(r[j + 3])) * c.w * rs);
+    }
+    return;
   }
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {

@@ -2,7 +2,7 @@
 //
 //   s[m] = max_k |x[m, k]| / 127          (1 for an all-zero row)
 //   q[m, k] = round(x[m, k] * 127 / max)  (ties to even, |q| <= 127)
-//   y[m, n] = act((sum_k q[m, k] w[n, k]) * s[m] * t[n] + bias[n])
+//   y[m, n] = act((sum_k q[m, k] w[n, k]) * t[n] * s[m] + bias[n])
 //
 // The sums are exact 32-bit integers (K <= 131071, so |sum| < 2^31 even for codes of -128 that a
 // caller may give).  Products of many tokens run on tcgen05.mma kind::i8
@@ -265,7 +265,8 @@ __device__ __forceinline__ Channel load_channel(const S8Out& o, int n) {
 }
 // Writes D[m, n] from the exact integer sum.
 __device__ __forceinline__ void put_s8(const S8Out& o, const Channel& c, long long m, int n, int sum, float xs) {
-  float y = fmaf(__int2float_rn(sum) * xs, c.ws, c.bias);
+  // (the channel's scale first: a token's may be near either end of the type's range)
+  float y = fmaf(__int2float_rn(sum) * c.ws, xs, c.bias);
   if (o.epi == B2G_EPI_GELU) y = gelu_tanh(y);
   if (o.epi == B2G_EPI_SILU) y = silu_fast(y);
   const long long at = m * o.ldd + n;
