@@ -6,7 +6,7 @@
 //
 // The sums are exact 32-bit integers (K <= 131071, so |sum| < 2^31 even for codes of -128 that a
 // caller may give).  Products of many tokens run on tcgen05.mma kind::i8
-// (gemm_tc.cu, KIND 3); those of up to 128 here, see s8_one_kernel and s8_split_kernel.  The reference's
+// (gemm_tc.cu, KIND 3); the others here, see s8_one_kernel and s8_split_kernel.  The reference's
 // quantised path has the same form per channel (cublas_ops.cuh:294-352, quantize_activations
 // kernels.cu:1988-2125), with the product in cuBLASLt.
 #include <cuda_bf16.h>
@@ -425,11 +425,11 @@ __global__ void __launch_bounds__(32 * kOneWarps, kOneBlocks<T, NV>) s8_one_kern
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// ---------------------------------------------------------------------------- up to 128 tokens
+// ---------------------------------------------------------------------------- up to 128 tokens, or few channels
 //
 // With few tokens the tiles of gemm_tc.cu are few (N / 128), and each streams its 128 weight rows
 // through one SM at the 90 bytes per ns that an SM takes in: its time grows with K alone.  Here the weights are
-// the MMA's M side (128 rows) and all tokens its N side (16 to 128), and a cluster of up to 8 CTAs shares out the K
+// the MMA's M side (128 rows) and the tokens its N side (16 to 128), and a cluster of up to 8 CTAs shares out the K
 // axis of a tile: every SM streams, the tokens are read once per 128 weight rows, and the exact integer sums of
 // the cluster meet through distributed shared memory, each CTA finishing its share of the tokens.  No
 // workspace, no second launch, and the order of the sums does not matter.  After a quantising launch of the same call
@@ -438,6 +438,8 @@ __global__ void __launch_bounds__(32 * kOneWarps, kOneBlocks<T, NV>) s8_one_kern
 // M = K / 48.  us with the quantiser, here against gemm_tc.cu's tiles, [N, K] and tokens:
 //   [5120, 5120] 16: 12.2, 19.1; 64: 15.6, 19.3; 96: 19.1, 19.5; 128: 22, 18.7    [1024, 1024] 64: 13.9, 9.2
 //   [21504, 3072] 16: 15.6, 22.4; 64: 20.3, 22.2; 128: 26.5, 22.5    [3072, 12288] 16: 17.7, 37.7; 128: 28.2, 38.6
+// More tokens, in blocks of up to 128, where few channels leave a cluster of 3 or more to each block and tile
+// (codes given): [512, 10944] 148: 10.8, 26.8; 600: 18.5, 27.1    [1024, 10944] 600: 22.3, 27.9    [256, 15360] 1000: 17, 36
 //   warp 0 TMA, warp 1 MMA (kind::i8, sums in TMEM), warps 2-5 epilogue (a weight row per thread).
 constexpr int kSplitThreads = 192;
 constexpr uint32_t kSplitW = 128 * 128;  // bytes of a stage's weights: 128 rows x 128 of K
@@ -445,7 +447,7 @@ constexpr int kSplitMaxStages = 8;
 
 struct SplitArgs {
   int M, N, nkb;     // nkb: blocks of 128 of K
-  int tokens;        // M, up to a multiple of 16
+  int tokens;        // per block of tokens: a multiple of 16, at most 128
   int stages;
   uint32_t tmem_cols;
   int early;         // the weights do not depend on the launch before this one
@@ -473,7 +475,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   const uint32_t x_bytes = static_cast<uint32_t>(a.tokens) * 128u, stage_bytes = kSplitW + x_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
-  const int n0 = static_cast<int>(blockIdx.x / S) * 128;
+  const int n0 = static_cast<int>(blockIdx.x / S) * 128, m0 = static_cast<int>(blockIdx.y) * a.tokens;
+  const int m_end = min(a.M, m0 + a.tokens);
   const int kb0 = static_cast<int>(static_cast<long long>(a.nkb) * rank / S);
   const int kb1 = static_cast<int>(static_cast<long long>(a.nkb) * (rank + 1) / S);
   if (warp == 0 && lane == 0) {
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         tma_load_3d(smem + st * stage_bytes, &tmW, &full[st], kb * 128, n0, 0, once);
       };
       auto load_x = [&](int kb, int st) {
-        tma_load_3d(smem + st * stage_bytes + kSplitW, &tmX, &full[st], kb * 128, 0, 0, keep);
+        tma_load_3d(smem + st * stage_bytes + kSplitW, &tmX, &full[st], kb * 128, m0, 0, keep);
       };
       int issued = 0;
       for (; issued < a.stages && kb0 + issued < kb1; ++issued) load_w(kb0 + issued, issued);
@@ -576,14 +579,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   };
   if (S == 1) {
     if (warp >= 2 && ok) {
-      for (int c = 0; c < a.M; c += 16) {
+      for (int c = 0; m0 + c < m_end; c += 16) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(lane_tmem + c, r);
         tmem_wait_ld();
         int sum[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[i] = static_cast<int>(r[i]);
-        put(sum, c, min(16, a.M - c));
+        put(sum, m0 + c, min(16, m_end - m0 - c));
       }
     }
   } else {
@@ -599,7 +602,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncwarp();
     cluster_sync_all();  // every CTA's sums are in its shared memory
     if (warp >= 2 && ok) {
-      const int c0 = a.M * rank / S, c1 = a.M * (rank + 1) / S;
+      const int live = m_end - m0, c0 = live * rank / S, c1 = live * (rank + 1) / S;
       const uint32_t mine = smem_u32(part) + row * 4;
       for (int c = c0; c < c1; c += 16) {
         int sum[16];
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum[i] += v[i];
         }
-        put(sum, c, count);
+        put(sum, m0 + c, count);
       }
     }
     __syncwarp();
@@ -630,7 +633,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 }
 
 // Most tokens that take s8_split_kernel.
-constexpr int64_t kSplitMaxM = 128;
+constexpr int64_t kSplitTokens = 128;  // per block of tokens
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
@@ -677,12 +680,13 @@ b2g_status launch_split(const GemmProblem& p, bool early, const DeviceInfo* dev,
   SplitArgs a{};
   a.M = static_cast<int>(p.M); a.N = static_cast<int>(p.N);
   a.nkb = static_cast<int>((p.K + 127) / 128);
-  a.tokens = static_cast<int>(round_up(p.M, 16));
+  const int64_t blocks = (p.M + kSplitTokens - 1) / kSplitTokens;
+  a.tokens = static_cast<int>(round_up((p.M + blocks - 1) / blocks, 16));
   a.tmem_cols = 32;
   while (a.tmem_cols < static_cast<uint32_t>(a.tokens)) a.tmem_cols *= 2;
   const int64_t tiles = (p.N + 127) / 128;
   // As many CTAs per tile as find an SM, each of 4 blocks of K or more.
-  int64_t S = dev->num_sms / tiles;
+  int64_t S = dev->num_sms / (tiles * blocks);
   if (S > a.nkb / 4) S = a.nkb / 4;
   if (S > 8) S = 8;
   if (S < 1) S = 1;
@@ -704,7 +708,7 @@ b2g_status launch_split(const GemmProblem& p, bool early, const DeviceInfo* dev,
                       "cudaFuncSetAttribute(s8_split)")) != B2G_OK)
     return s;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * S));
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * S), static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kSplitThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -737,7 +741,12 @@ b2g_status run_quantize(const void* src, b2g_dtype src_dtype, int64_t rows, int6
   return launch_quantize_s8<float>(a, st);
 }
 
-static bool takes_split(int64_t M, int64_t K) { return M <= kSplitMaxM && 48 * M <= K; }
+// Tokens and channels that s8_split_kernel takes.
+static bool takes_split(const GemmProblem& p, int num_sms) {
+  const int64_t blocks = (p.M + kSplitTokens - 1) / kSplitTokens;
+  if (blocks > 1 && 3 * blocks * ((p.N + 127) / 128) > num_sms) return false;
+  return 48 * ((p.M + blocks - 1) / blocks) <= p.K;
+}
 
 constexpr int64_t kS8MaxK = 131071;  // 128 * 128 * K < 2^31
 
@@ -799,7 +808,7 @@ b2g_status gemm_s8(const b2g_gemm_desc* d, const float* a_scale, const float* b_
   }
   if (!tc_gemm_supported(p, &why)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_gemm_s8: " + why);
   if (p.N > 0x7fffffff - 256) return set_error(B2G_ERR_UNSUPPORTED, "b2g_gemm_s8: too many channels");
-  if (d->a_dtype == B2G_S8) return takes_split(p.M, p.K) ? launch_split(p, false, dev, st) : tc_gemm_launch(p, st);
+  if (d->a_dtype == B2G_S8) return takes_split(p, dev->num_sms) ? launch_split(p, false, dev, st) : tc_gemm_launch(p, st);
   if (takes_one_launch(p.M, p.K)) {
     p.a = d->a;
     p.lda = d->lda;
@@ -817,7 +826,7 @@ b2g_status gemm_s8(const b2g_gemm_desc* d, const float* a_scale, const float* b_
   p.a = q;
   p.a_scale = scales;
   if ((s = run_quantize(d->a, d->a_dtype, p.M, p.K, d->lda, q, p.lda, scales, st)) != B2G_OK) return s;
-  return takes_split(p.M, p.K) ? launch_split(p, true, dev, st) : tc_gemm_launch(p, st);
+  return takes_split(p, dev->num_sms) ? launch_split(p, true, dev, st) : tc_gemm_launch(p, st);
 }
 
 }  // namespace b2g

@@ -47,6 +47,30 @@ def test_shared_k(engine, m, n, k, given):
     check_gemm(engine, x, xs, wq, ws, randn((n,), 3, 0.1, torch.bfloat16), torch.bfloat16, "none")
 
 
+@pytest.mark.parametrize("m,n,k", [(129, 300, 3200), (200, 512, 10000), (257, 100, 4200), (400, 700, 6500), (1000, 130, 6001)])
+@pytest.mark.parametrize("given", ["codes", "bf16"])
+def test_shared_k_blocks_of_tokens(engine, m, n, k, given):
+    wq, ws = weight(n, k, m + n + k)
+    x, xs = randn((m, k), k, 1.0, torch.bfloat16), None
+    if given == "codes":
+        x, xs = engine.quantize_s8(x)
+    check_gemm(engine, x, xs, wq, ws, randn((n,), 3, 0.1), torch.float16, "silu")
+
+
+@pytest.mark.parametrize("m,n,k", [(130, 261, 304), (700, 1003, 160), (1500, 2307, 64)])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_of_odd_width(engine, m, n, k, out_dtype):
+    """Output rows without the alignment of wide stores, whole and as a view that leaves its neighbours alone."""
+    wq, ws = weight(n, k, m)
+    x = randn((m, k), 9, 1.0, torch.bfloat16)
+    check_gemm(engine, x, None, wq, ws, randn((n,), 3, 0.1), out_dtype, "gelu")
+    buf = torch.full((m, n + 11), 7.0, dtype=out_dtype, device=DEV)
+    engine.gemm_s8(x, wq, ws, out=buf[:, 5:5 + n])
+    torch.cuda.synchronize()
+    assert torch.equal(buf[:, 5:5 + n], engine.gemm_s8(x, wq, ws, out_dtype=out_dtype))
+    assert bool((buf[:, :5] == 7).all()) and bool((buf[:, 5 + n:] == 7).all())
+
+
 @pytest.mark.parametrize("m,k", [(3, 700), (40, 2600)])
 @pytest.mark.parametrize("epilogue", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -73,6 +97,22 @@ def test_gated_residual(engine, m, k):
     assert_within(out, want, g.abs() * 8 * e * prod.abs() + 2 * e * want.abs())
     with pytest.raises(engine.B2GError, match="needs a gate"):
         engine.gemm_s8(x, wq, ws, out=out, epilogue="gated_residual")
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 301, 600), (300, 130, 5000)])
+def test_gated_residual_of_many_tokens(engine, m, n, k):
+    """Rows of odd width; K shared out over blocks of tokens."""
+    wq, ws = weight(n, k, 8)
+    x, xs = engine.quantize_s8(randn((m, k), 9, 1.0, torch.bfloat16))
+    gate, res = randn((n,), 10), randn((m, n), 12)
+    out = res.clone()
+    engine.gemm_s8(x, wq, ws, out=out, epilogue="gated_residual", gate=gate, x_scale=xs)
+    torch.cuda.synchronize()
+    g = gate.to(F64)
+    prod = (x.to(F64) @ wq.to(F64).T) * xs.to(F64)[:, None] * ws.to(F64)
+    want = res.to(F64) + g * prod
+    e = 2.0 ** -24
+    assert_within(out, want, g.abs() * 8 * e * prod.abs() + 2 * e * want.abs())
 
 
 @pytest.mark.parametrize("m,k", [(4, 900), (20, 1100), (130, 1100)])
