@@ -40,6 +40,8 @@ constexpr int kNrAhead = 4;       // steps (of 32 / G heads) that a warp takes a
 // Pair layouts: neighbours or halves in groups of 8 values per lane, or any (value by value).
 enum { kPairsNeighbours = 0, kPairsHalves = 1, kPairsAny = 2 };
 
+constexpr int kNrFewHeads = 8, kNrFewTokens = 1024;  // qk_norm_rope_few_kernel's heads at most, tokens at least
+
 struct NrArgs {
   const void* x[2];   // q, k
   void* y[2];
@@ -271,6 +273,119 @@ __global__ void __launch_bounds__(kNrThreads, 2) qk_norm_rope_kernel(const __gri
   }
 }
 
+// Few heads, many tokens: G lanes work on a token, so that a warp takes 32 / G neighbouring tokens at a time and
+// the heads of each (query heads, then key heads) kNrAhead after one another.  A warp per token computes
+// its angles in every group of lanes, which with few heads is most of the work.  us here and with a warp
+// per token, tokens of q + k heads: 300 of 2 + 1: 2.8, 2.3; 1536 of 2 + 1: 2.9, 4.1; of 4 + 2: 4.1, 4.1; of 8 + 2: 6.1, 4.8;
+// 29120 of 2 + 1: 16.8, 38.2; of 4 + 2: 17.6, 39.3; of 8 + 2: 42.9, 43.9; of 12 + 12 (width 96): 89.0, 76.1.
+template <typename TI, typename TO, int G, bool kHalves>
+__global__ void __launch_bounds__(kNrThreads, 2) qk_norm_rope_few_kernel(const __grid_constant__ NrArgs a) {
+  constexpr int kTokens = 32 / G, U = kNrAhead;
+  __shared__ float2 turns[kNrMaxPairs];
+  __shared__ unsigned char axes[kNrMaxPairs];
+  for (int p = threadIdx.x; p < a.rot / 2; p += kNrThreads) {
+    turns[p] = a.turn[p];
+    axes[p] = a.axis[p];
+  }
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % G, sub = lane / G;
+  const bool live = l < a.D / 8;  // (D / 8 is not a power of two for every D)
+  const bool turned = 8 * l < a.rot;
+  const int e0 = !kHalves || !turned ? 8 * l : 4 * l, apart = !kHalves || !turned ? 4 : a.rot / 2;
+  const float inv_d = 1.f / static_cast<float>(a.D);
+  const int stride = static_cast<int>(gridDim.x * (kNrThreads / 32)) * kTokens, tokens = static_cast<int>(a.tokens);
+  int base = static_cast<int>(blockIdx.x * (kNrThreads / 32) + warp) * kTokens;
+  griddep_wait();
+  griddep_launch_dependents();
+  // The scales of query and key heads (1 where there are none, and the norm is left out).
+  float w[2][8];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[k][i] = 1.f;
+    if (a.norm[k] && live) {
+      load_n<float, 4>(a.norm[k] + e0, w[k]);
+      load_n<float, 4>(a.norm[k] + e0 + apart, w[k] + 4);
+    }
+  }
+  Raw<TI, kHalves> raw[U];
+  float pos[4];
+  auto load = [&](int t, int h0) {
+    const bool ok = live && t < tokens;
+    if (h0 == 0 && turned && ok) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pos[i] = __ldg(a.pos + t * a.ldp + axes[4 * l + i]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u;
+      const bool k = h >= a.q_heads;
+      const TI* from = static_cast<const TI*>(k ? a.x[1] : a.x[0]) + t * (k ? a.ldx[1] : a.ldx[0]) +
+                       (k ? h - a.q_heads : h) * (k ? a.hsx[1] : a.hsx[0]) + e0;
+      if (ok && h < a.heads) raw[u].load(from, apart);
+      else raw[u].zero();
+    }
+  };
+  int h0 = 0;
+  load(base + sub, h0);
+  float2 cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = make_float2(1.f, 0.f);
+  while (base < tokens) {
+    const int t = base + sub, at = h0;
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].values(v[u]);
+    if (at == 0 && turned) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cs[i] = cos_sin_turns(pos[i], turns[4 * l + i]);
+    }
+    h0 += U;
+    if (h0 >= a.heads) {
+      h0 = 0;
+      base += stride;
+    }
+    load(base + sub, h0);
+    float ss[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ss[u] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss[u] = fmaf(v[u][i], v[u][i], ss[u]);
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], o);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = at + u;
+      if (h >= a.heads) break;
+      const bool k = h >= a.q_heads;
+      const float inv = (k ? a.norm[1] : a.norm[0]) ? rsqrtf(fmaf(ss[u], inv_d, a.eps)) : 1.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * inv * (k ? w[1][i] : w[0][i]);
+      if (turned) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int i0 = kHalves ? i : 2 * i, i1 = kHalves ? i + 4 : 2 * i + 1;
+          const float x0 = v[u][i0], x1 = v[u][i1];
+          v[u][i0] = fmaf(x0, cs[i].x, -(x1 * cs[i].y));
+          v[u][i1] = fmaf(x0, cs[i].y, x1 * cs[i].x);
+        }
+      }
+      if (!live || t >= tokens) continue;
+      TO* to = static_cast<TO*>(k ? a.y[1] : a.y[0]) + t * (k ? a.ldy[1] : a.ldy[0]) +
+               (k ? h - a.q_heads : h) * (k ? a.hsy[1] : a.hsy[0]) + e0;
+      if constexpr (!kHalves) store_n<TO, 8>(to, v[u]);
+      else {
+        store_n<TO, 4>(to, v[u]);
+        store_n<TO, 4>(to + apart, v[u] + 4);
+      }
+    }
+  }
+}
+
 // Any even D and rot, any alignment: a warp per head, a lane's pairs p = lane, lane + 32, ..
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_any_kernel(const __grid_constant__ NrArgs a) {
@@ -330,27 +445,32 @@ __global__ void __launch_bounds__(kNrThreads) qk_norm_rope_any_kernel(const __gr
   }
 }
 
-template <typename TI, typename TO>
-b2g_status launch_nr(const NrArgs& a, int mode, dim3 grid, cudaStream_t st) {
+template <typename TI, typename TO, int G>
+b2g_status launch_nr_vec(const NrArgs& a, bool halves, bool few, dim3 grid, cudaStream_t st) {
   const char* what = "qk_norm_rope launch";
   const dim3 block(kNrThreads);
-  if (mode == kPairsAny) return launch_pdl(qk_norm_rope_any_kernel<TI, TO>, grid, block, 0, st, what, a);
+  if (few)
+    return halves ? launch_pdl(qk_norm_rope_few_kernel<TI, TO, G, true>, grid, block, 0, st, what, a)
+                  : launch_pdl(qk_norm_rope_few_kernel<TI, TO, G, false>, grid, block, 0, st, what, a);
+  return halves ? launch_pdl(qk_norm_rope_kernel<TI, TO, G, true>, grid, block, 0, st, what, a)
+                : launch_pdl(qk_norm_rope_kernel<TI, TO, G, false>, grid, block, 0, st, what, a);
+}
+
+template <typename TI, typename TO>
+b2g_status launch_nr(const NrArgs& a, int mode, bool few, dim3 grid, cudaStream_t st) {
+  if (mode == kPairsAny)
+    return launch_pdl(qk_norm_rope_any_kernel<TI, TO>, grid, dim3(kNrThreads), 0, st, "qk_norm_rope launch", a);
   const bool h = mode == kPairsHalves;
-  if (a.D <= 64)
-    return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 8, true>, grid, block, 0, st, what, a)
-             : launch_pdl(qk_norm_rope_kernel<TI, TO, 8, false>, grid, block, 0, st, what, a);
-  if (a.D <= 128)
-    return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 16, true>, grid, block, 0, st, what, a)
-             : launch_pdl(qk_norm_rope_kernel<TI, TO, 16, false>, grid, block, 0, st, what, a);
-  return h ? launch_pdl(qk_norm_rope_kernel<TI, TO, 32, true>, grid, block, 0, st, what, a)
-           : launch_pdl(qk_norm_rope_kernel<TI, TO, 32, false>, grid, block, 0, st, what, a);
+  if (a.D <= 64) return launch_nr_vec<TI, TO, 8>(a, h, few, grid, st);
+  if (a.D <= 128) return launch_nr_vec<TI, TO, 16>(a, h, few, grid, st);
+  return launch_nr_vec<TI, TO, 32>(a, h, few, grid, st);
 }
 
 template <typename TI>
-b2g_status launch_nr_in(const NrArgs& a, int mode, b2g_dtype out, dim3 grid, cudaStream_t st) {
-  if (out == B2G_BF16) return launch_nr<TI, __nv_bfloat16>(a, mode, grid, st);
-  if (out == B2G_F16) return launch_nr<TI, __half>(a, mode, grid, st);
-  return launch_nr<TI, float>(a, mode, grid, st);
+b2g_status launch_nr_in(const NrArgs& a, int mode, bool few, b2g_dtype out, dim3 grid, cudaStream_t st) {
+  if (out == B2G_BF16) return launch_nr<TI, __nv_bfloat16>(a, mode, few, grid, st);
+  if (out == B2G_F16) return launch_nr<TI, __half>(a, mode, few, grid, st);
+  return launch_nr<TI, float>(a, mode, few, grid, st);
 }
 
 bool is_float(b2g_dtype t) { return t == B2G_F32 || t == B2G_F16 || t == B2G_BF16; }
@@ -416,6 +536,7 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
           (reinterpret_cast<uintptr_t>(a.y[i]) % oa | (a.ldy[i] * ob) % oa | (a.hsy[i] * ob) % oa) == 0;
   }
   const int mode = !vec ? kPairsAny : (d->interleaved ? kPairsNeighbours : kPairsHalves);
+  const bool few = mode != kPairsAny && a.heads <= kNrFewHeads && d->tokens >= kNrFewTokens;
   int64_t blocks;
   if (mode == kPairsAny) {
     // As many tokens per block as give every warp a head, but a block for every SM.
@@ -429,16 +550,18 @@ b2g_status qk_norm_rope(const b2g_qk_norm_rope_desc* d, cudaStream_t st) {
     // A token's heads go to several warps (which all compute its angles) while that still brings
     // more warps to work, at 16 warps per SM.
     const int64_t most = 2ll * dev->num_sms, warps = most * (kNrThreads / 32);
-    while (a.parts_log2 < 3 && (d->tokens << (a.parts_log2 + 1)) <= warps) ++a.parts_log2;
-    const int64_t need = ((d->tokens << a.parts_log2) + kNrThreads / 32 - 1) / (kNrThreads / 32);
+    const int64_t per_warp = !few ? 1 : a.D <= 64 ? 4 : a.D <= 128 ? 2 : 1;
+    while (!few && a.parts_log2 < 3 && (d->tokens << (a.parts_log2 + 1)) <= warps) ++a.parts_log2;
+    const int64_t units = ((d->tokens << a.parts_log2) + per_warp - 1) / per_warp;
+    const int64_t need = (units + kNrThreads / 32 - 1) / (kNrThreads / 32);
     // As many tokens for every warp: the rounds that `most` blocks need, shared out evenly.
     const int64_t rounds = (need + most - 1) / most;
     blocks = (need + rounds - 1) / rounds;
   }
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (d->dtype == B2G_BF16) return launch_nr_in<__nv_bfloat16>(a, mode, d->out_dtype, grid, st);
-  if (d->dtype == B2G_F16) return launch_nr_in<__half>(a, mode, d->out_dtype, grid, st);
-  return launch_nr_in<float>(a, mode, d->out_dtype, grid, st);
+  if (d->dtype == B2G_BF16) return launch_nr_in<__nv_bfloat16>(a, mode, few, d->out_dtype, grid, st);
+  if (d->dtype == B2G_F16) return launch_nr_in<__half>(a, mode, few, d->out_dtype, grid, st);
+  return launch_nr_in<float>(a, mode, few, d->out_dtype, grid, st);
 }
 
 }  // namespace b2g
