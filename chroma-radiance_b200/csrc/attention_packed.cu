@@ -34,6 +34,7 @@ struct PkParams {
   int batch;
   int total_q, total_k;    // rows of q and of k, v
   int hq, hk, group;       // query heads, key heads, hq / hk
+  int item_heads;          // kHeadsApart: heads per work item, 1 or 2
   int causal;
   float scale_log2;        // scale * log2(e)
   const void *q, *k, *v;
@@ -112,7 +113,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 //   kTilesOfHead   consecutive tiles of one head, which share the keys' shared-memory stages
 //   kHeadsOfGroup  the same rows of two query heads that share a key head: shared stages, finer steps
 //   kHeadsApart    the same rows of two heads with their own keys: twice the key traffic, but no idle
-//                  second tile where sequences are short
+//                  second tile where sequences are short; or of one head, where there are few tiles
 // Roles: warp 3 finds the work items and hands them round in a ring, warp 0 loads Q and K, warp 2 V, one
 // thread of warp 1 issues the MMAs, warps 4-7 and 8-11 are the softmax of tiles A and B with one thread
 // per row.  S (fp32) and O live in TMEM, P (16-bit) overwrites S and is the A operand of P.V.  Per key
@@ -291,7 +292,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     regs_dec<kPtRegsIdle>();
     if (warp == 3) {
       // ---------------------------------------------------------- work items
-      const int head_units = kMode == kTilesOfHead ? p.hq : (p.hq + 1) / 2;
+      const int item_heads = kApart ? p.item_heads : kMode == kTilesOfHead ? 1 : 2;
+      const int head_units = (p.hq + item_heads - 1) / item_heads;
       const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
       int units_before = 0, i = 0;
       Turn<kPtItems> at;
@@ -313,11 +315,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           w.k0 = s.k0;
           w.lk = s.lk;
           w.row0 = ((s.lq + kSpan - 1) / kSpan - 1 - (unit - units_before)) * kSpan;
-          w.head = kMode == kTilesOfHead ? head_unit : 2 * head_unit;
+          w.head = item_heads * head_unit;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0);
-            int n = row < s.lq && (!kApart || w.head + t < p.hq) ? s.lk : 0;
+            int n = row < s.lq && (!kApart || (t < item_heads && w.head + t < p.hq)) ? s.lk : 0;
             if (p.causal) n = clampi(min(row + kPtRows, s.lq) + s.lk - s.lq, 0, n);
             w.blocks[t] = (n + kPtKeys - 1) / kPtKeys;
           }
@@ -709,7 +711,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (lane == 0) mbar_arrive(&item_empty[at.stage]);
       const int warp_row = w.row0 + (kMode == kTilesOfHead ? t * kPtRows : 0) + quarter * 32;
       const int head = w.head + (kMode == kTilesOfHead ? 0 : t);
-      const int rows = !kApart || head < p.hq ? w.lq - warp_row : 0;  // of this warp's 32
+      const int rows = !kApart || (t < p.item_heads && head < p.hq) ? w.lq - warp_row : 0;  // of this warp's 32
       // 64 columns at a time through this warp's staging space: a row per lane in, four rows of
       // 128 bytes per instruction out (16-byte pieces swizzled by the row).  A row that sees nothing
       // has P = 0 and so O = 0; without any key O was not written, and counts as 0.
@@ -1199,7 +1201,7 @@ b2g_status launch_tiles(const PkParams& p, const CUtensorMap& tq, const CUtensor
                             "cudaFuncSetAttribute(packed_tiles)");
   if (s != B2G_OK) return s;
   constexpr int kSpan = kMode == kTilesOfHead ? 2 * kPtRows : kPtRows;
-  const int64_t items = (static_cast<int64_t>(p.total_q) / kSpan + p.batch) * (kMode == kTilesOfHead ? p.hq : (p.hq + 1) / 2);
+  const int64_t items = (static_cast<int64_t>(p.total_q) / kSpan + p.batch) * (kMode == kTilesOfHead ? p.hq : (p.hq + p.item_heads - 1) / p.item_heads);
   return launch_pdl(kern, dim3(static_cast<unsigned>(items < sms ? items : sms)), dim3(kPtThreads), smem, st,
                     "packed_tiles launch", tq, tk, tv, p);
 }
@@ -1219,6 +1221,13 @@ b2g_status run_packed(const b2g_attention_packed_desc* d, PkParams p, void* ws, 
   if ((s = make_operand_map(&tq, p.q, dt, D, p.total_q, p.ldq, p.hq, p.hsq, kPtRows)) != B2G_OK) return s;
   if ((s = make_operand_map(&tk, p.k, dt, D, p.total_k, p.ldk, p.hk, p.hsk, kPtKeys)) != B2G_OK) return s;
   if ((s = make_operand_map(&tv, p.v, dt, D, p.total_k, p.ldv, p.hk, p.hsv, kPtKeys)) != B2G_OK) return s;
+  p.item_heads = 2;
+  // Where every tile finds an SM of its own, two tiles in turn only slow each other: 8 heads of 128, 2048 tokens: 37.6
+  // and 42.2 us; 2 heads, 612 causal: 14.9 and 17.7; 18 heads, 1024 (half as many tiles more than SMs): 26.1 in pairs.
+  if ((static_cast<int64_t>(p.total_q) / kPtRows + p.batch) * p.hq <= sms) {
+    p.item_heads = 1;
+    return launch_tiles<T, D, kHeadsApart>(p, tq, tk, tv, sms, st);
+  }
   if (p.group % 2 == 0) return launch_tiles<T, D, kHeadsOfGroup>(p, tq, tk, tv, sms, st);
   if (p.total_q <= kPtApartRows * static_cast<int64_t>(p.batch))
     return launch_tiles<T, D, kHeadsApart>(p, tq, tk, tv, sms, st);
