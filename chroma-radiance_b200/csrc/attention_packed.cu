@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
+#include <climits>
 #include <cstdint>
 #include <type_traits>
 #include "engine.cuh"
@@ -481,15 +482,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // Parities of the tiles' barriers: q_full, P (one use per block), o_empty.
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0}, o_parity[2] = {0, 0};
       bool ok = true;
-      // The next item with a key block; none: blocks 0, 0.
-      auto next_blocks = [&](int (&blocks)[2]) {
-        for (;;) {
-          blocks[0] = blocks[1] = 0;
+      // The next item with a key block, among the next `most` items; none: blocks 0, 0.
+      bool end = false;
+      auto next_blocks = [&](int (&blocks)[2], int most) {
+        blocks[0] = blocks[1] = 0;
+        for (int i = 0; i < most; ++i) {
           if (!(ok = mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
-          const bool end = ld_shared_int(&items[at.stage].head) < 0;
+          end = ld_shared_int(&items[at.stage].head) < 0;
+          if (end) return;
           blocks[0] = ld_shared_int(&items[at.stage].blocks[0]);
           blocks[1] = ld_shared_int(&items[at.stage].blocks[1]);
-          if (end) return;  // (not handed back: asked again, it says the same)
           mbar_arrive(&item_empty[at.stage]);
           at.next();
           if ((blocks[0] | blocks[1]) != 0) return;
@@ -518,67 +520,72 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       };
       int cur[2], then[2];
-      next_blocks(cur);
-      for (int t = 0; t < 2; ++t)
-        if (ok && cur[t] > 0) issue_s(t, true, cur[t] == 1);
-      if (!kApart && ok && (cur[0] | cur[1]) != 0) {
-        umma_commit(&k_empty[k_at.stage]);
-        k_at.next();
-      }
-      while (ok && (cur[0] | cur[1]) != 0) {
-        const int nkb = max(cur[0], cur[1]);
-        for (int j = 0; j < nkb && ok; ++j) {
-          if (j + 1 == nkb) next_blocks(then);
-          bool more = false;  // some tile's next S was issued
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok) break;
-            if (j < cur[t]) {
-              const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
-              if (j == 0) {  // O is overwritten: the last item's has been read
-                if (!(ok = mbar_wait_short(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
-                o_parity[t] ^= 1u;
-              }
-              // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
-              if (!(ok = mbar_wait_short(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
-              if (!(ok = mbar_wait_short(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
-              tc_fence_after();
-#pragma unroll
-              for (int k = 0; k < 6; ++k)
-                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                            idesc_o, (j | k) != 0 ? 1u : 0u);
-              if (!(ok = mbar_wait_short(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
-              tc_fence_after();
-#pragma unroll
-              for (int k = 6; k < 8; ++k)
-                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                            idesc_o, 1u);
-              umma_commit(&pv_done[t]);
-              p_parity[t] ^= 1u;
-              if constexpr (kApart) {
-                umma_commit(&v_empty[v_at.stage]);
-                v_at.next();
-              }
-            }
-            // The tile's next S, of this item or the next: over P, which the P.V issued before it
-            // reads first (issue order).
-            const bool same = j + 1 < cur[t], other = j + 1 == nkb && then[t] > 0;
-            if (same || other) {
-              issue_s(t, other, same ? j + 2 == cur[t] : then[t] == 1);
-              more = true;
-            }
-          }
-          if (!kApart && ok) {
-            umma_commit(&v_empty[v_at.stage]);
-            v_at.next();
-            if (more) {
-              umma_commit(&k_empty[k_at.stage]);
-              k_at.next();
-            }
-          }
+#pragma unroll 1
+      while (ok && !end) {
+        next_blocks(cur, INT_MAX);
+        for (int t = 0; t < 2; ++t)
+          if (ok && cur[t] > 0) issue_s(t, true, cur[t] == 1);
+        if (!kApart && ok && (cur[0] | cur[1]) != 0) {
+          umma_commit(&k_empty[k_at.stage]);
+          k_at.next();
         }
-        cur[0] = then[0];
-        cur[1] = then[1];
+        while (ok && (cur[0] | cur[1]) != 0) {
+          const int nkb = max(cur[0], cur[1]);
+          for (int j = 0; j < nkb && ok; ++j) {
+            // (Not past the ring: an item further on comes only when this one's softmax has handed it back,
+            // which waits for the P.V below.  Behind so many empty items the next S starts anew.)
+            if (j + 1 == nkb) next_blocks(then, kPtItems - 1);
+            bool more = false;  // some tile's next S was issued
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok) break;
+              if (j < cur[t]) {
+                const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
+                if (j == 0) {  // O is overwritten: the last item's has been read
+                  if (!(ok = mbar_wait_short(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
+                  o_parity[t] ^= 1u;
+                }
+                // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
+                if (!(ok = mbar_wait_short(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
+                if (!(ok = mbar_wait_short(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 6; ++k)
+                  umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                              idesc_o, (j | k) != 0 ? 1u : 0u);
+                if (!(ok = mbar_wait_short(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 6; k < 8; ++k)
+                  umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                              idesc_o, 1u);
+                umma_commit(&pv_done[t]);
+                p_parity[t] ^= 1u;
+                if constexpr (kApart) {
+                  umma_commit(&v_empty[v_at.stage]);
+                  v_at.next();
+                }
+              }
+              // The tile's next S, of this item or the next: over P, which the P.V issued before it
+              // reads first (issue order).
+              const bool same = j + 1 < cur[t], other = j + 1 == nkb && then[t] > 0;
+              if (same || other) {
+                issue_s(t, other, same ? j + 2 == cur[t] : then[t] == 1);
+                more = true;
+              }
+            }
+            if (!kApart && ok) {
+              umma_commit(&v_empty[v_at.stage]);
+              v_at.next();
+              if (more) {
+                umma_commit(&k_empty[k_at.stage]);
+                k_at.next();
+              }
+            }
+          }
+          cur[0] = then[0];
+          cur[1] = then[1];
+        }
       }
       if (!ok) {
         umma_commit(drain_bar);  // MMAs already issued retire before TMEM is released
