@@ -18,7 +18,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
-#include <climits>
 #include <cstdint>
 #include <type_traits>
 #include "engine.cuh"
@@ -128,8 +127,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // Bound by the chain of a tile: S, softmax (128 exponentials a row on 16 units a clock and SM), P.V; with
 // two tiles in turn the tensor core is busy some 60 % of the time at d = 128, 35 % at d = 64, whose
 // products take half as long beside the same softmax.  d = 128, 24 heads, sequences of 4608: 1050 TFLOP/s; 7
-// images of 300 to 4608: 702 us.  Short sequences pay for whole 128 x 128 blocks, of which a
-// sequence of 1 to 509 tokens sees half: 96 of them, 64 heads of 64: 239 us; 40 causal prompts of 1 to 2047: 206 us.
+// images of 300 to 4608: 700 us.  Short sequences pay for whole 128 x 128 blocks, of which a
+// sequence of 1 to 509 tokens sees half: 96 of them, 64 heads of 64: 228 us; 40 causal prompts of 1 to 2047: 206 us.
+//
+// Items that see no key (causal rows before the first key, empty caches) are written as zeros by warp 3 and stay
+// out of the ring: the MMA thread looks one item ahead, and so many in a row that the ring ends before the next one
+// with keys would leave it waiting for a place that its own tile holds.
 //
 // Items: sequences by falling key count (up to kPtSorted of them; else as they come), tiles from the
 // last, which see most keys; dealt to the CTAs back and forth, so that the sums of long and short
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
       int units_before = 0, i = 0;
       Turn<kPtItems> at;
-      for (int round = 0; i >= 0; ++round, at.next()) {
+      for (int round = 0; i >= 0; ++round) {
         const long long index = static_cast<long long>(round) * grid + (round & 1 ? grid - 1 - cta : cta);
         const int unit = static_cast<int>(index / head_units);
         const int head_unit = static_cast<int>(index - static_cast<long long>(unit) * head_units);
@@ -324,6 +327,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (p.causal) n = clampi(min(row + kPtRows, s.lq) + s.lk - s.lq, 0, n);
             w.blocks[t] = (n + kPtKeys - 1) / kPtKeys;
           }
+          if ((w.blocks[0] | w.blocks[1]) == 0) {
+            // Rows that see no key are 0, written here: no other role has to find its way past such items.
+            const int rows = min(s.lq - w.row0, kSpan), heads = min(item_heads, p.hq - w.head);
+            T* to = static_cast<T*>(p.out) + static_cast<long long>(s.q0 + w.row0) * p.ldo +
+                    static_cast<long long>(w.head) * p.hso;
+            for (int h = 0; h < heads; ++h, to += p.hso)
+              for (int x = lane; x < rows * (D / 8); x += 32)
+                *reinterpret_cast<uint4*>(to + static_cast<long long>(x / (D / 8)) * p.ldo + x % (D / 8) * 8) =
+                    make_uint4(0, 0, 0, 0);
+            continue;
+          }
         }
         bool ok = true;
         if (lane == 0) {
@@ -334,6 +348,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
         }
         if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        at.next();
       }
     } else if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- Q and K
@@ -416,7 +431,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           key = 0;
           t = kApart && w.blocks[0] == 0 ? 1 : 0;
           seen = keys_seen(w);
-          have = more && nkb(w) > 0;
+          have = more;
           continue;
         }
         if (have && (tails == 0 || ready(&v_empty[v_at.stage], v_at.parity ^ 1u))) {
@@ -482,20 +497,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // Parities of the tiles' barriers: q_full, P (one use per block), o_empty.
       uint32_t q_parity[2] = {0, 0}, p_parity[2] = {0, 0}, o_parity[2] = {0, 0};
       bool ok = true;
-      // The next item with a key block, among the next `most` items; none: blocks 0, 0.
-      bool end = false;
-      auto next_blocks = [&](int (&blocks)[2], int most) {
+      // The next item's blocks; no more items: blocks 0, 0.
+      auto next_blocks = [&](int (&blocks)[2]) {
         blocks[0] = blocks[1] = 0;
-        for (int i = 0; i < most; ++i) {
-          if (!(ok = mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
-          end = ld_shared_int(&items[at.stage].head) < 0;
-          if (end) return;
-          blocks[0] = ld_shared_int(&items[at.stage].blocks[0]);
-          blocks[1] = ld_shared_int(&items[at.stage].blocks[1]);
-          mbar_arrive(&item_empty[at.stage]);
-          at.next();
-          if ((blocks[0] | blocks[1]) != 0) return;
-        }
+        if (!(ok = mbar_wait_short(&item_full[at.stage], at.parity, p.err, kErrWaitMma))) return;
+        if (ld_shared_int(&items[at.stage].head) < 0) return;  // (not handed back: asked again, it says the same)
+        blocks[0] = ld_shared_int(&items[at.stage].blocks[0]);
+        blocks[1] = ld_shared_int(&items[at.stage].blocks[1]);
+        mbar_arrive(&item_empty[at.stage]);
+        at.next();
       };
       // S of the key block at k_at, of tile t; first: of its item (Q), last: Q is free afterwards.
       auto issue_s = [&](int t, bool first, bool last) {
@@ -520,72 +530,67 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       };
       int cur[2], then[2];
-#pragma unroll 1
-      while (ok && !end) {
-        next_blocks(cur, INT_MAX);
-        for (int t = 0; t < 2; ++t)
-          if (ok && cur[t] > 0) issue_s(t, true, cur[t] == 1);
-        if (!kApart && ok && (cur[0] | cur[1]) != 0) {
-          umma_commit(&k_empty[k_at.stage]);
-          k_at.next();
-        }
-        while (ok && (cur[0] | cur[1]) != 0) {
-          const int nkb = max(cur[0], cur[1]);
-          for (int j = 0; j < nkb && ok; ++j) {
-            // (Not past the ring: an item further on comes only when this one's softmax has handed it back,
-            // which waits for the P.V below.  Behind so many empty items the next S starts anew.)
-            if (j + 1 == nkb) next_blocks(then, kPtItems - 1);
-            bool more = false;  // some tile's next S was issued
+      next_blocks(cur);
+      for (int t = 0; t < 2; ++t)
+        if (ok && cur[t] > 0) issue_s(t, true, cur[t] == 1);
+      if (!kApart && ok && (cur[0] | cur[1]) != 0) {
+        umma_commit(&k_empty[k_at.stage]);
+        k_at.next();
+      }
+      while (ok && (cur[0] | cur[1]) != 0) {
+        const int nkb = max(cur[0], cur[1]);
+        for (int j = 0; j < nkb && ok; ++j) {
+          if (j + 1 == nkb) next_blocks(then);
+          bool more = false;  // some tile's next S was issued
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!ok) break;
-              if (j < cur[t]) {
-                const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
-                if (j == 0) {  // O is overwritten: the last item's has been read
-                  if (!(ok = mbar_wait_short(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
-                  o_parity[t] ^= 1u;
-                }
-                // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
-                if (!(ok = mbar_wait_short(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
-                if (!(ok = mbar_wait_short(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < 6; ++k)
-                  umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                              idesc_o, (j | k) != 0 ? 1u : 0u);
-                if (!(ok = mbar_wait_short(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int k = 6; k < 8; ++k)
-                  umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
-                              idesc_o, 1u);
-                umma_commit(&pv_done[t]);
-                p_parity[t] ^= 1u;
-                if constexpr (kApart) {
-                  umma_commit(&v_empty[v_at.stage]);
-                  v_at.next();
-                }
+          for (int t = 0; t < 2; ++t) {
+            if (!ok) break;
+            if (j < cur[t]) {
+              const uint32_t v0 = smem_u32(sV + v_at.stage * Ly::kTileBytes);
+              if (j == 0) {  // O is overwritten: the last item's has been read
+                if (!(ok = mbar_wait_short(&o_empty[t], o_parity[t] ^ 1u, p.err, kErrWaitMma))) break;
+                o_parity[t] ^= 1u;
               }
-              // The tile's next S, of this item or the next: over P, which the P.V issued before it
-              // reads first (issue order).
-              const bool same = j + 1 < cur[t], other = j + 1 == nkb && then[t] > 0;
-              if (same || other) {
-                issue_s(t, other, same ? j + 2 == cur[t] : then[t] == 1);
-                more = true;
+              // 16 keys per MMA: keys 0-95 as soon as the softmax has written them, then 96-127.
+              if (!(ok = mbar_wait_short(&p_part[t], p_parity[t], p.err, kErrWaitMma))) break;
+              if (!(ok = mbar_wait_short(&v_full[v_at.stage], v_at.parity, p.err, kErrWaitMma))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < 6; ++k)
+                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                            idesc_o, (j | k) != 0 ? 1u : 0u);
+              if (!(ok = mbar_wait_short(&p_full[t], p_parity[t], p.err, kErrWaitMma))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 6; k < 8; ++k)
+                umma_f16_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * k, smem_desc_mn_sw128(v0 + k * 2048, kPtBox),
+                            idesc_o, 1u);
+              umma_commit(&pv_done[t]);
+              p_parity[t] ^= 1u;
+              if constexpr (kApart) {
+                umma_commit(&v_empty[v_at.stage]);
+                v_at.next();
               }
             }
-            if (!kApart && ok) {
-              umma_commit(&v_empty[v_at.stage]);
-              v_at.next();
-              if (more) {
-                umma_commit(&k_empty[k_at.stage]);
-                k_at.next();
-              }
+            // The tile's next S, of this item or the next: over P, which the P.V issued before it
+            // reads first (issue order).
+            const bool same = j + 1 < cur[t], other = j + 1 == nkb && then[t] > 0;
+            if (same || other) {
+              issue_s(t, other, same ? j + 2 == cur[t] : then[t] == 1);
+              more = true;
             }
           }
-          cur[0] = then[0];
-          cur[1] = then[1];
+          if (!kApart && ok) {
+            umma_commit(&v_empty[v_at.stage]);
+            v_at.next();
+            if (more) {
+              umma_commit(&k_empty[k_at.stage]);
+              k_at.next();
+            }
+          }
         }
+        cur[0] = then[0];
+        cur[1] = then[1];
       }
       if (!ok) {
         umma_commit(drain_bar);  // MMAs already issued retire before TMEM is released

@@ -34,3 +34,20 @@ def test_other_keys(engine, lq, lk, causal, hq, hk, d):
 def test_one_long_sequence_of_few_heads(engine, heads, causal):
     n = 3001
     check_attention(engine, *qkv(n, n, heads, 1, 128, torch.bfloat16, heads), [n], [n], causal)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(24, 24, 128), (23, 23, 64), (32, 8, 128)])
+@pytest.mark.parametrize("lq,lk", [([2000, 300, 1500, 400, 900], [0, 500, 0, 800, 10]), ([3000, 3000, 20], [100, 0, 3000]),
+                                   ([200] * 8 + [30], [0] * 8 + [70]), ([400] * 6, [0] * 6)])
+def test_many_rows_without_keys(engine, hq, hk, d, lq, lk):
+    check_attention(engine, *qkv(sum(lq), sum(lk), hq, hk, d, torch.bfloat16, hq), lq, lk, True)
+
+
+@pytest.mark.parametrize("hq,hk,d,scale", [(3, 3, 64, 1), (4, 2, 128, 1), (2, 1, 64, 6)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_sequences_than_are_sorted(engine, hq, hk, d, scale, causal):
+    """Thousands of sequences, taken as they come; empty ones among them."""
+    g = torch.Generator().manual_seed(hq)
+    lq = (torch.randint(0, 60, (2500,), generator=g) * scale).tolist()
+    lk = (torch.randint(0, 60, (2500,), generator=g) * torch.randint(0, 2, (2500,), generator=g)).tolist()
+    check_attention(engine, *qkv(sum(lq), sum(lk), hq, hk, d, torch.bfloat16, hq), lq, lk, causal)
