@@ -773,7 +773,7 @@ static bool takes_one_launch(int64_t M, int64_t K) { return M <= 8 && pow2_ceil(
 
 // Workspace of float activations: codes [M, round_up(K, 16)], then M scales.
 size_t gemm_s8_workspace(int64_t M, int64_t K, b2g_dtype a_dtype) {
-  if (a_dtype == B2G_S8 || M <= 0 || K <= 0) return 0;
+  if (a_dtype == B2G_S8 || M <= 0 || K <= 0 || M > 0x7fffffff || K > kS8MaxK) return 0;
   return static_cast<size_t>(round_up(M * round_up(K, 16), 256) + 4 * M);
 }
 
