@@ -27,6 +27,7 @@ struct GemmProblem {
   bool round_tf32 = false;  // TF32 operands still plain fp32: the kernel rounds each shared-memory
                             // stage to nearest TF32 before the MMAs read it (1-CTA kernels)
   float alpha = 1.0f;       // D = epilogue(alpha * A.B^T + bias); internal (attention scores)
+  bool b_early = false;     // S8: B is ready before the launch that makes A is done (see gemm_tc.cu)
   bool allow_split = true;  // false: never split K (split-K needs workspace; b2g_gemm_noalloc)
   // E4M3 and S8 operands: D = (sum_k A.B) * a_scale[m] * b_scale[n] + bias, before the epilogue.
   const float* a_scale = nullptr;

@@ -108,6 +108,7 @@ struct TcParams {
   int bias_kind;           // 0 none, 1 f32, 2 bf16
   int* err;
   uint32_t idesc;
+  int b_early;             // S8: only A depends on the launch before this one, which waited for all others
   int a_keep;              // 1: keep A in L2 (evict_last), stream B (evict_first); 0: reverse
   int splits;              // split-K factor S of the split tiles (1 = none)
   int dp_tiles;            // tiles [0, dp_tiles) run whole; tiles [dp_tiles, num_tiles) split S ways
@@ -904,8 +905,12 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  griddep_wait();  // the set-up above overlapped the previous kernel's tail
-  griddep_launch_dependents();
+  bool b_early = false;  // the producer loads B of the first stages, then waits
+  if constexpr (KIND == 3) b_early = p.b_early && warp == 0;
+  if (!b_early) {
+    griddep_wait();  // the set-up above overlapped the previous kernel's tail
+    griddep_launch_dependents();
+  }
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -917,6 +922,24 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
       int stage = 0;
       uint32_t phase = 0, issued = 0;
       bool ok = true;
+      // S8 after its own quantiser: the weights of the first stages set out while that still runs (us with and without:
+      // 2000 x 1024 x 1024 13.5, 16.6; 200 x 7296 x 2240 16.6, 18.2; 344 x 5120 x 5120 21.7, 22.3).
+      int ahead = 0;  // stages whose B is on its way
+      if constexpr (KIND == 3) {
+        if (b_early) {
+          int tile, split, kb0, kb1, gi, bz, mb, nb;
+          if (static_cast<int>(blockIdx.x) < p.num_items) {
+            item_coords(blockIdx.x, p, tile, split, kb0, kb1);
+            tile_coords(tile, p, gi, bz, mb, nb);
+            for (; ahead < STAGES && kb0 + ahead < kb1; ++ahead) {
+              mbar_arrive_expect_tx(&full_bar[ahead], A_BYTES + B_BYTES);
+              tma_load_3d(sB + ahead * B_BYTES, &maps.b[gi], &full_bar[ahead], (kb0 + ahead) * kKElems<KIND>, nb * BN, bz, pb);
+            }
+          }
+          griddep_wait();
+          griddep_launch_dependents();
+        }
+      }
       for (int item = blockIdx.x; item < p.num_items && ok; item += gridDim.x) {
         int tile, split, kb0, kb1, gi, bz, mb, nb;
         item_coords(item, p, tile, split, kb0, kb1);
@@ -928,9 +951,11 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full_bar[stage], A_BYTES + B_BYTES);
+          const bool whole = KIND != 3 || ahead == 0;
+          if (whole) mbar_arrive_expect_tx(&full_bar[stage], A_BYTES + B_BYTES);
+          else --ahead;
           tma_load_3d(sA + stage * A_BYTES, tmA, &full_bar[stage], kb * kKElems<KIND>, mb * kBM, bz, pa);
-          tma_load_3d(sB + stage * B_BYTES, tmB, &full_bar[stage], kb * kKElems<KIND>, nb * BN, bz, pb);
+          if (whole) tma_load_3d(sB + stage * B_BYTES, tmB, &full_bar[stage], kb * kKElems<KIND>, nb * BN, bz, pb);
           ++issued;
           if (++stage == STAGES) {
             stage = 0;
@@ -1135,8 +1160,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync_all();  // barrier inits and the TMEM allocation are visible pair-wide
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  griddep_wait();  // the set-up above overlapped the previous kernel's tail
-  griddep_launch_dependents();
+  bool b_early = false;  // the producer loads B of the first stages, then waits
+  if constexpr (KIND == 3) b_early = p.b_early && warp == 0;
+  if (!b_early) {
+    griddep_wait();  // the set-up above overlapped the previous kernel's tail
+    griddep_launch_dependents();
+  }
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -1148,6 +1177,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0, issued = 0;
       bool ok = true;
+      int ahead = 0;  // stages whose B is on its way
+      if constexpr (KIND == 3) {
+        if (b_early) {
+          int tile, split, kb0, kb1, gi, bz, mb, nb;
+          if (cluster < p.num_items) {
+            item_coords(cluster, p, tile, split, kb0, kb1);
+            tile_coords(tile, p, gi, bz, mb, nb);
+            for (; ahead < STAGES && kb0 + ahead < kb1; ++ahead) {
+              if (rank == 0) mbar_arrive_expect_tx(&full_bar[ahead], 2 * (A_BYTES + B_BYTES));
+              tma_load_3d_pair(sB + ahead * B_BYTES, &maps.b[gi], map_to_cta(smem_u32(&full_bar[ahead]), 0),
+                               (kb0 + ahead) * kKElems<KIND>, nb * BN + static_cast<int>(rank) * 128, bz, pb);
+            }
+          }
+          griddep_wait();
+          griddep_launch_dependents();
+        }
+      }
       for (int item = cluster; item < p.num_items && ok; item += nclusters) {
         int tile, split, kb0, kb1, gi, bz, mb, nb;
         item_coords(item, p, tile, split, kb0, kb1);
@@ -1161,10 +1207,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (A_BYTES + B_BYTES));
+          const bool whole = KIND != 3 || ahead == 0;
+          if (whole) {
+            if (rank == 0) mbar_arrive_expect_tx(&full_bar[stage], 2 * (A_BYTES + B_BYTES));
+          } else --ahead;
           const uint32_t leader_full = map_to_cta(smem_u32(&full_bar[stage]), 0);
           tma_load_3d_pair(sA + stage * A_BYTES, tmA, leader_full, kb * kKElems<KIND>, arow, bz, pa);
-          tma_load_3d_pair(sB + stage * B_BYTES, tmB, leader_full, kb * kKElems<KIND>, brow, bz, pb);
+          if (whole) tma_load_3d_pair(sB + stage * B_BYTES, tmB, leader_full, kb * kKElems<KIND>, brow, bz, pb);
           ++issued;
           if (++stage == STAGES) {
             stage = 0;
@@ -1617,6 +1666,7 @@ b2g_status tc_gemm_launch_group(const GemmProblem* ps, int count, cudaStream_t s
                                                : (kind == 2 ? kFmtE4M3 : (p.a_dtype == B2G_BF16 ? kFmtBF16 : kFmtF16)),
                                      tile_m, bn);
   prm.a_keep = a_bytes <= b_bytes ? 1 : 0;
+  prm.b_early = p.b_early ? 1 : 0;
   if (prm.num_tiles == 0) return B2G_OK;
 
   if (splits > 1) {

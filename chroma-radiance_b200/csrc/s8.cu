@@ -826,6 +826,7 @@ b2g_status gemm_s8(const b2g_gemm_desc* d, const float* a_scale, const float* b_
   p.a = q;
   p.a_scale = scales;
   if ((s = run_quantize(d->a, d->a_dtype, p.M, p.K, d->lda, q, p.lda, scales, st)) != B2G_OK) return s;
+  p.b_early = true;
   return takes_split(p, dev->num_sms) ? launch_split(p, true, dev, st) : tc_gemm_launch(p, st);
 }
 
