@@ -933,7 +933,8 @@ __global__ void __launch_bounds__(kThreadsK<KIND>, 1)
             tile_coords(tile, p, gi, bz, mb, nb);
             for (; ahead < STAGES && kb0 + ahead < kb1; ++ahead) {
               mbar_arrive_expect_tx(&full_bar[ahead], A_BYTES + B_BYTES);
-              tma_load_3d(sB + ahead * B_BYTES, &maps.b[gi], &full_bar[ahead], (kb0 + ahead) * kKElems<KIND>, nb * BN, bz, pb);
+              tma_load_3d(sB + ahead * B_BYTES, &maps.b[gi], &full_bar[ahead], (kb0 + ahead) * kKElems<KIND>, nb * BN, bz,
+                          pb);
             }
           }
           griddep_wait();
