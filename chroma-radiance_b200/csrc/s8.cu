@@ -755,8 +755,8 @@ constexpr int64_t kS8MaxK = 131071;  // 128 * 128 * K < 2^31
 b2g_status quantize_rows_s8(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
                             int64_t dst_ld, float* scales, cudaStream_t st) {
   if (rows < 0 || cols < 0) return set_error(B2G_ERR_INVALID, "b2g_quantize_s8: negative size");
-  if (rows == 0 || cols == 0) return B2G_OK;
-  if (!src || !dst || !scales) return set_error(B2G_ERR_INVALID, "b2g_quantize_s8: null pointer");
+  if (rows == 0) return B2G_OK;
+  if ((cols > 0 && (!src || !dst)) || !scales) return set_error(B2G_ERR_INVALID, "b2g_quantize_s8: null pointer");
   if (ld < cols || dst_ld < cols) return set_error(B2G_ERR_INVALID, "b2g_quantize_s8: ld < cols");
   if (rows > 0x7fffffff || cols > 0x7ffffff0)
     return set_error(B2G_ERR_UNSUPPORTED, "b2g_quantize_s8: too many rows or columns");

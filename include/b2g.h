@@ -472,8 +472,8 @@ b2g_status b2g_nerf_final(const float* feat_cond, const float* feat_uncond, cons
 /* ---- Packed batches (no reference counterpart; its sequences have one length and its INT8 path,
  * cublas_ops.cuh:294-791, runs in cuBLASLt) ---- */
 
-/* 8-bit integer quantisation of the rows of a matrix: scales[r] = absmax_r / 127 (1 for an
- * all-zero row) and dst[r, c] = round(src[r, c] * 127 / absmax_r), ties to even.  For a weight [N, K]
+/* 8-bit integer quantisation of the rows of a matrix: scales[r] = absmax_r / 127 (1 for a row
+ * of zeros or of no value) and dst[r, c] = round(src[r, c] * 127 / absmax_r), ties to even.  For a weight [N, K]
  * that is one scale per output channel (once, at load), for activations one per token.  A row
  * with an infinity or a NaN gets the scale NaN and zero codes.  src F32, BF16 or F16; any sizes, row
  * strides and alignment (16-byte source rows and 8-byte destination rows are faster). */
