@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(256) quantize_rows_s8_kernel(const QuantArgs a
   }
 }
 
-// Rows of more than 16384 values: read twice (the second time from L2).
+// Rows of more than 16384 values: read twice (the second time from L2).  Columns are counted in 64 bits: a step past the
+// longest row's end would not fit 32.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_long_rows_s8_kernel(const QuantArgs a) {
   __shared__ uint32_t red[8];
@@ -213,17 +214,17 @@ __global__ void __launch_bounds__(256) quantize_long_rows_s8_kernel(const QuantA
   const long long row = blockIdx.x;
   const T* s = static_cast<const T*>(a.src) + row * a.ld;
   uint32_t m = 0;
-  for (int c = static_cast<int>(threadIdx.x) * 8; c < a.cols; c += 2048) {
-    const Raw8<T> v[1] = {load8<T>(s + c, a.cols - c, a.src_vec && c + 8 <= a.cols)};
+  for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+    const Raw8<T> v[1] = {load8<T>(s + c, static_cast<int>(a.cols - c), a.src_vec && c + 8 <= a.cols)};
     m = max(m, top8<T, 1>(v));
   }
   m = row_max<8>(m, red);
   const RowCodes rc = row_codes(m);
   if (threadIdx.x == 0) a.scales[row] = row_scale(m);
   int8_t* d = a.dst + row * a.dst_ld;
-  for (int c = static_cast<int>(threadIdx.x) * 8; c < a.cols; c += 2048) {
-    const Raw8<T> v = load8<T>(s + c, a.cols - c, a.src_vec && c + 8 <= a.cols);
-    store8<T>(d, c, a.cols, a.dst_vec && c + 8 <= a.cols, v, rc);
+  for (int64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+    const Raw8<T> v = load8<T>(s + c, static_cast<int>(a.cols - c), a.src_vec && c + 8 <= a.cols);
+    store8<T>(d, static_cast<int>(c), a.cols, a.dst_vec && c + 8 <= a.cols, v, rc);
   }
 }
 
