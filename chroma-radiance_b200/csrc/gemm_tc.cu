@@ -218,8 +218,9 @@ __device__ __forceinline__ void item_coords(int item, const TcParams& p, int& ti
   kb1 = static_cast<int>(static_cast<long long>(split + 1) * p.num_k_blocks / p.splits);
 }
 
-// alpha * acc + bias (bias staged in shared memory, zero past N), then GELU or SiLU if asked.
-template <int EPI>
+// alpha * acc + bias (bias staged in shared memory, zero past N), then GELU or SiLU if asked (kFar: of sums of any
+// size, see activations.cuh).
+template <int EPI, bool kFar = false>
 __device__ __forceinline__ void chunk_values(const uint32_t (&r)[32], const float* sb, float alpha, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
@@ -239,11 +240,11 @@ __device__ __forceinline__ void chunk_values(const uint32_t (&r)[32], const floa
   }
   if constexpr (EPI == B2G_EPI_GELU) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = gelu_tanh(v[j]);
+    for (int j = 0; j < 32; ++j) v[j] = gelu_tanh<kFar>(v[j]);
   }
   if constexpr (EPI == B2G_EPI_SILU) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = silu_fast(v[j]);
+    for (int j = 0; j < 32; ++j) v[j] = silu_fast<kFar>(v[j]);
   }
 }
 
@@ -329,12 +330,12 @@ template <bool REDUCE, int OUT>
 __device__ __forceinline__ void stage_store_values(const CUtensorMap* tmD, uint8_t* stage, int& obuf, int bz,
                                                    int m_warp0, int n0, const float (&v)[32], int lane);
 
-template <int EPI, int OUT>
+template <int EPI, int OUT, bool kFar>
 __device__ __forceinline__ void stage_store_chunk(const CUtensorMap* tmD, uint8_t* stage, int& obuf, int bz,
                                                   int m_warp0, int n0, const uint32_t (&r)[32], const float* sb,
                                                   float alpha, int lane, const float* gate, int N) {
   float v[32];
-  chunk_values<EPI>(r, sb, alpha, v);
+  chunk_values<EPI, kFar>(r, sb, alpha, v);
   if constexpr (EPI == B2G_EPI_GATED_RESIDUAL) {
     const float* gp = gate + n0;
     if (n0 + 32 <= N && (reinterpret_cast<uintptr_t>(gp) & 15u) == 0) {
@@ -403,7 +404,7 @@ template <int EPI, int OUT>
 __device__ __forceinline__ void store_rows(const TcParams& p, const TcGroup& G, uint8_t* stage, int m_warp0, int n0,
                                            const uint32_t (&r)[32], const float* sb, int lane) {
   float v[32];
-  chunk_values<EPI>(r, sb, p.alpha, v);
+  chunk_values<EPI, true>(r, sb, p.alpha, v);
   float* buf = reinterpret_cast<float*>(stage);
   __syncwarp();  // the last chunk has been read
 #pragma unroll
@@ -432,7 +433,7 @@ __device__ __forceinline__ void emit_chunk(const TcParams& p, const TcGroup& G, 
                                            const float* sb, int lane) {
   if (p.tma_store) {
     if (m_warp0 < G.M && n0 < p.N)
-      stage_store_chunk<EPI, OUT>(tmD, buf, obuf, bz, m_warp0, n0, r, sb, p.alpha, lane, G.gate, p.N);
+      stage_store_chunk<EPI, OUT, KIND == 3>(tmD, buf, obuf, bz, m_warp0, n0, r, sb, p.alpha, lane, G.gate, p.N);
   } else if constexpr (KIND == 3) {
     if (m_warp0 < G.M && n0 < p.N) store_rows<EPI, OUT>(p, G, buf, m_warp0, n0, r, sb, lane);
   } else if (m < G.M && n0 < p.N) {

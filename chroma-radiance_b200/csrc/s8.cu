@@ -268,8 +268,8 @@ __device__ __forceinline__ Channel load_channel(const S8Out& o, int n) {
 __device__ __forceinline__ void put_s8(const S8Out& o, const Channel& c, long long m, int n, int sum, float xs) {
   // (the channel's scale first: a token's may be near either end of the type's range)
   float y = fmaf(__int2float_rn(sum) * c.ws, xs, c.bias);
-  if (o.epi == B2G_EPI_GELU) y = gelu_tanh(y);
-  if (o.epi == B2G_EPI_SILU) y = silu_fast(y);
+  if (o.epi == B2G_EPI_GELU) y = gelu_tanh<true>(y);
+  if (o.epi == B2G_EPI_SILU) y = silu_fast<true>(y);
   const long long at = m * o.ldd + n;
   if (o.epi == B2G_EPI_GATED_RESIDUAL) static_cast<float*>(o.d)[at] += c.gate * y;
   else if (o.out == B2G_F32) static_cast<float*>(o.d)[at] = y;
