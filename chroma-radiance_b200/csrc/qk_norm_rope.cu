@@ -62,9 +62,11 @@ struct NrArgs {
 };
 
 // cos and sin of 2 pi pos (hi + lo).  The product's whole turns are taken off before anything
-// is rounded away: pos * hi and its rounding error are exact as two floats, so the angle is right to
-// 2^-22 of a turn for positions of any size (a product in fp32 radians is off by 2^-24 of the angle,
-// 0.0005 at a position of 8000).
+// is rounded away: pos * hi and its rounding error are exact as two floats.  hi + lo holds the frequency, of a radian at
+// most, to 2^-45 of itself (128 products in doubles and their ratio's rounding), so that the angle is right to 2^-22 of a
+// turn for |pos| up to 2^24; the error grows with the angle from there on (largest in a sample against rationals: 2^-24.6 of
+// a turn up to 2^24, 2^-23.4 up to 2^26, 2^-20.1 up to 2^30).  A product in fp32 radians is off by 2^-24 of the angle,
+// 0.0005 at a position of 8000.
 __device__ __forceinline__ float2 cos_sin_turns(float pos, float2 turn) {
   const float p = pos * turn.x;
   const float rest = fmaf(pos, turn.y, fmaf(pos, turn.x, -p));

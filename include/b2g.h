@@ -500,7 +500,9 @@ b2g_status b2g_gemm_s8(const b2g_gemm_desc* desc, const float* a_scale, const fl
  * interleaved: pair p is values (2p, 2p + 1) (as the reference's RoPE, rope.cuh:180-221), else
  * values (p, p + R / 2).  Token i's head h is at q + i * ldq + h * hsq, and so on.  Outputs may be
  * the inputs (same pointer, type and strides); they must not overlap otherwise.  Angles are right to
- * 2^-22 of a turn at any position.  d_head even, at most 256; n_head or n_kv_head may be 0. */
+ * 2^-22 of a turn for positions of up to 2^24 in size (whole numbers past that are not all F32) and theta from 1 on;
+ * further out the error grows with the angle.
+ * d_head even, at most 256; n_head or n_kv_head may be 0. */
 typedef struct {
   const void* q; const void* k; b2g_dtype dtype;              /* F32, BF16 or F16 */
   void* q_out; void* k_out; b2g_dtype out_dtype;
