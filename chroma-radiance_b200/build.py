@@ -59,11 +59,19 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
-def build_calls(force: bool = False) -> Path:
+def build_calls(force: bool = False) -> Path | None:
+    """None, with a message, where there is no torch or no Python.h: the C library needs neither."""
     src = CSRC / "calls.cpp"
     if not force and not _stale(CALLS, [src, REPO / "include" / "b2g.h"]):
         return CALLS
-    import torch  # (its headers and libraries; the interpreter's are beside them)
+    try:
+        import torch  # (its headers and libraries; the interpreter's are beside them)
+    except ImportError:
+        torch = None
+    if torch is None or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        print(f"{CALLS.name} is not built: no {'torch' if torch is None else 'Python.h'} here.  {LIB.name} is complete; only the "
+              "Python functions of the packed operators need the other.", file=sys.stderr)
+        return None
 
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
