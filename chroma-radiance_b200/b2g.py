@@ -20,12 +20,14 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sysconfig
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libb2g.so"
-CALLS_PATH = LIB_PATH.with_name("b2g_calls.so")
+# (compiled against torch's C++ classes and the interpreter's API: another version's file is not this one's)
+CALLS_PATH = LIB_PATH.with_name(f"b2g_calls.torch-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
 
 # b2g_dtype
 F32, F16, BF16, E4M3, S8 = 0, 1, 2, 3, 4

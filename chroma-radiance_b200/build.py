@@ -1,4 +1,4 @@
-"""Builds libb2g.so (the engine) in-tree with nvcc for sm_100a, and b2g_calls.so (the Python side of the
+"""Builds libb2g.so (the engine) in-tree with nvcc for sm_100a, and b2g_calls.*.so (the Python side of the
 packed operators, csrc/calls.cpp) with the host compiler against torch.
 
     python chroma-radiance_b200/build.py [--force]
@@ -23,7 +23,6 @@ REPO = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "lib" / "libb2g.so"
-CALLS = PKG / "lib" / "b2g_calls.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -60,30 +59,36 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 
 def build_calls(force: bool = False) -> Path | None:
-    """None, with a message, where there is no torch or no Python.h: the C library needs neither."""
-    src = CSRC / "calls.cpp"
-    if not force and not _stale(CALLS, [src, REPO / "include" / "b2g.h"]):
-        return CALLS
+    """The library for the torch and the interpreter at hand (their versions are in its name).  None, with a
+    message, where there is no torch with CUDA or no Python.h: the C library needs neither."""
     try:
         import torch  # (its headers and libraries; the interpreter's are beside them)
+        found = torch.version.cuda is not None
     except ImportError:
-        torch = None
-    if torch is None or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
-        print(f"{CALLS.name} is not built: no {'torch' if torch is None else 'Python.h'} here.  {LIB.name} is complete; only the "
+        found = False
+    if not found or not (Path(sysconfig.get_paths()["include"]) / "Python.h").exists():
+        print(f"b2g_calls is not built: no {'Python.h' if found else 'torch with CUDA'} here.  {LIB.name} is complete; only the "
               "Python functions of the packed operators need the other.", file=sys.stderr)
         return None
+    if str(PKG) not in sys.path:
+        sys.path.insert(0, str(PKG))
+    import b2g  # (which loads it)
 
+    src, calls = CSRC / "calls.cpp", b2g.CALLS_PATH
+    if not force and not _stale(calls, [src, REPO / "include" / "b2g.h"]):
+        return calls
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
     includes = [REPO / "include", root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
                 sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           *(f"-I{i}" for i in includes), str(src), "-o", str(CALLS), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{i}" for i in includes), str(src), "-o", str(calls), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compiling calls.cpp failed:\n{r.stdout}\n{r.stderr}")
-    return CALLS
+    return calls
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

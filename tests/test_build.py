@@ -46,3 +46,21 @@ def test_both_libraries_are_built(recorded):
     build, commands = recorded
     build.build(force=True)
     assert any(str(build.LIB) in c for c in commands) and any(x.endswith("calls.cpp") for c in commands for x in c)
+
+
+def test_the_python_side_belongs_to_one_torch_and_interpreter(recorded, monkeypatch, tmp_path):
+    """Their versions are in its name, and a file of another name does not pass for it, however new."""
+    import torch
+
+    import b2g
+
+    build, commands = recorded
+    assert torch.__version__ in b2g.CALLS_PATH.name and sysconfig.get_config_var("SOABI") in b2g.CALLS_PATH.name
+    other = tmp_path / b2g.CALLS_PATH.name.replace(torch.__version__, "0.0.1")
+    monkeypatch.setattr(b2g, "CALLS_PATH", other)
+    assert build.build_calls() == other
+    assert [c for c in commands if str(other) in c and any(x.endswith("calls.cpp") for x in c)]
+    assert f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}" in commands[0]
+    with pytest.raises(b2g.B2GError, match="is missing: build it"):
+        monkeypatch.setattr(b2g, "_calls", None)
+        b2g.gemm_s8(torch.zeros(1, 16), torch.zeros(1, 16, dtype=torch.int8), torch.ones(1))
