@@ -128,15 +128,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // two tiles in turn the tensor core is busy some 60 % of the time at d = 128, 35 % at d = 64, whose
 // products take half as long beside the same softmax.  d = 128, 24 heads, sequences of 4608: 1050 TFLOP/s; 7
 // images of 300 to 4608: 700 us.  Short sequences pay for whole 128 x 128 blocks, of which a
-// sequence of 1 to 509 tokens sees half: 96 of them, 64 heads of 64: 228 us; 40 causal prompts of 1 to 2047: 206 us.
+// sequence of 1 to 509 tokens sees half, and for what a tile costs once (at d = 64 1.35 us an SM, beside 0.81 us per key
+// block: 96 sequences of 128 and of 256 tokens take 90 and 247 us): 96 of them, 64 heads of 64: 228 us; 40 causal prompts
+// of 1 to 2047: 206 us.
 //
 // Items that see no key (causal rows before the first key, empty caches) are written as zeros by warp 3 and stay
 // out of the ring: the MMA thread looks one item ahead, and so many in a row that the ring ends before the next one
 // with keys would leave it waiting for a place that its own tile holds.
 //
 // Items: sequences by falling key count (up to kPtSorted of them; else as they come), tiles from the
-// last, which see most keys; dealt to the CTAs back and forth, so that the sums of long and short
-// ones stay even.
+// last, which see most keys; dealt to the CTAs back and forth.  That evens out many short sequences without a mask (96 short
+// prompts: the busiest CTA has 140 tile blocks, the mean is 139), a few long ones less (7 images: 604, 562).  Causal tiles
+// fall from many blocks to one within each sequence, so that the order is not by size (40 causal prompts: 148, 120).
 //
 // The last key block may reach into the next sequence's rows, whose values may be anything: those
 // scores are replaced by -inf, and those rows of V are zeroed in shared memory before the MMA

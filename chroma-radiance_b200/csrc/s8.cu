@@ -22,10 +22,11 @@ namespace {
 
 // ---------------------------------------------------------------------------- quantisation
 //
-// Bound by memory: each value is read once and kept in registers between the row's maximum and its
+// Each value is read once and kept in registers between the row's maximum and its
 // codes.  kWarps warps share a row of up to 32 * kWarps * 8 * NV values (a block is 8 warps, so rows of up to
-// 1024 go 8 to a block; a warp for rows of 3072 took 21.6 us where a block takes 14.7); longer rows are
-// read twice.  4608 x 3072 of bf16: 14.7 us, of f32: 15.2 us (4.6 TB/s); 128 x 5120 of bf16: 3.1 us, most of it
+// 1024 go 8 to a block; a warp for rows of 3072 took 21.6 us where a block takes 14.5); longer rows are
+// read twice.  4608 x 3072 of bf16: 14.5 us (2.9 TB/s), of f32: 15.3 us (4.6 TB/s): not the bytes count but a block's chain
+// of load, barrier and store, with no next row on its way.  128 x 5120 of bf16: 3.0 us, most of it
 // one round trip to memory, one through the block and the launch.
 
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -281,9 +282,11 @@ __device__ __forceinline__ void put_s8(const S8Out& o, const Channel& c, long lo
 //
 // Float activations of up to 8 tokens and kOneMax values in all: one launch that quantises and
 // multiplies.  The weight [N, K] is read once and nothing else matters (one token at N = K = 5120:
-// 26 MB, 6.9 us, 3.8 TB/s; N = 16 takes 4.2 us, a latency chain of token, maximum, codes, products), so the
+// 26 MB, 8.4 us from HBM, 3.1 TB/s, 6.9 us with the weight in L2; N = 16 takes 4.2 us, a latency chain of token, maximum, codes,
+// products), so the
 // tokens are quantised by every block for itself, while its weights are on their way: a launch of its own before
-// this one costs 3 to 4 us.  8 tokens of 2048: 9.6 us; past kOneMax quantising everywhere costs more than it saves.  A block takes 16 weight rows at a time; its 8 warps take the
+// this one costs 3 to 4 us.  8 tokens of 2048: 9.6 us; past kOneMax quantising everywhere costs more than it saves.
+// A block takes 16 weight rows at a time; its 8 warps take the
 // 64-byte chunks of K in turn, so that together they read 512 consecutive bytes of each row.  Lane (g, t)
 // of a warp has 16 bytes of rows g and g + 8 and of token g at offset 16 t of the chunk: words (0, 1) and
 // (2, 3) of these are the operands of two m16n8k32 products, whose K order is permuted in the same way

@@ -13,6 +13,12 @@ every row carries its own positions.  The block is that of the reference's singl
     q, k     = qk_norm_rope(q, k, positions)                 in place
     cat[attn] = attention_packed(q, k, v, offsets)           into the concat buffer
     x       += gate * gemm_s8(cat, W2)                       quantised per token in the call
+
+q, k and v leave their projection in bf16, the type that the attention takes, so that the rotation can write over its inputs
+and qkv is held once; q and k are thus rounded before the norm and again after the rotation, where the epilogue of the
+bf16 block's projection rounds them once, at the end.  In F32 they would be written and read as 4 bytes a value: for
+1536 rows 38 MB more of traffic.  The rounding is at most 2^-8 of a value; the operands' 8 bits leave an rms of 1.3 % (two
+roundings with a step of 4 sigma / 127).
 """
 from __future__ import annotations
 

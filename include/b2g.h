@@ -475,7 +475,8 @@ b2g_status b2g_nerf_final(const float* feat_cond, const float* feat_uncond, cons
 /* 8-bit integer quantisation of the rows of a matrix: scales[r] = absmax_r / 127 (1 for a row
  * of zeros or of no value) and dst[r, c] = round(src[r, c] * 127 / absmax_r), ties to even.  For a weight [N, K]
  * that is one scale per output channel (once, at load), for activations one per token.  A row
- * with an infinity or a NaN gets the scale NaN and zero codes.  src F32, BF16 or F16; any sizes, row
+ * with an infinity or a NaN gets the scale NaN and zero codes.  F32 values whose quotient is within 2^-16
+ * of a half may get the code on its other side.  src F32, BF16 or F16; any sizes, row
  * strides and alignment (16-byte source rows and 8-byte destination rows are faster). */
 b2g_status b2g_quantize_s8(const void* src, b2g_dtype src_dtype, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
                            int64_t dst_ld, float* scales, void* stream);
