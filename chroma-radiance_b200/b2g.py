@@ -116,6 +116,23 @@ class AttentionPackedDesc(ctypes.Structure):
     ]
 
 
+class LoraDesc(ctypes.Structure):
+    """Mirror of b2g_lora_desc."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("dtype", ctypes.c_int),
+        ("ldx", ctypes.c_int64), ("lda", ctypes.c_int64), ("a_stride", ctypes.c_int64), ("ldb", ctypes.c_int64),
+        ("b_stride", ctypes.c_int64),
+        ("t", ctypes.c_void_p), ("ldt", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("out", ctypes.c_void_p), ("y_dtype", ctypes.c_int),
+        ("ldy", ctypes.c_int64), ("ldo", ctypes.c_int64),
+        ("rows", ctypes.c_int64), ("K", ctypes.c_int64), ("N", ctypes.c_int64), ("R", ctypes.c_int64),
+        ("adapters", ctypes.c_int64), ("batch", ctypes.c_int64),
+        ("cu", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("epilogue", ctypes.c_int),
+    ]
+
+
 _lib = None
 
 # Exported symbols of libb2g.so with their ctypes signatures (status-returning unless noted).
@@ -193,6 +210,14 @@ _SIGNATURES = {
     "b2g_attention_packed_workspace": ([ctypes.POINTER(AttentionPackedDesc)], ctypes.c_size_t),
     "b2g_attention_packed": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
                              ctypes.c_int),
+    "b2g_block_means": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+                        ctypes.c_int),
+    "b2g_select_blocks": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p] + [ctypes.c_int64] * 4 +
+                          [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p], ctypes.c_int),
+    "b2g_attention_blocks": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                              ctypes.c_void_p], ctypes.c_int),
+    "b2g_lora_down": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
+    "b2g_lora_up": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
     "b2g_check_device_error": ([ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "b2g_launch_count": ([], ctypes.c_uint64),
     "b2g_set_gemm_variant": ([ctypes.c_int, ctypes.c_int], ctypes.c_int),
@@ -1126,3 +1151,61 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     int32 device tensors; a row that sees no key is 0.  Returns [total_q, n_head, d] of q's type (rows
     of no sequence are left as they were)."""
     return _call("attention_packed", stream, q, k, v, cu_q, cu_k, k_lens, causal, scale, out)
+
+
+def block_means(k: torch.Tensor, cu_k: torch.Tensor, k_lens: torch.Tensor | None = None, since: torch.Tensor | None = None,
+                out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The means of the keys' blocks of 128, F32 [blocks, n_kv_head, d], for select_blocks: k [total_k, n_kv_head, d]
+    (BF16 or F16, d 64 or 128), sequence b at rows cu_k[b] to cu_k[b+1], of which k_lens[b] are in use when given.  A
+    sequence has a row for every block that it has room for; blocks without a key, and rows past the last block, are 0.
+    With since (int32 [batch]) and out, the means kept so far: only the blocks that hold a key from since[b] on are
+    written anew, as a step that added those keys needs it."""
+    return _call("block_means", stream, k, cu_k, k_lens, since, out)
+
+
+def select_blocks(q: torch.Tensor, means: torch.Tensor, cu_q: torch.Tensor, top: int, cu_k: torch.Tensor | None = None,
+                  k_lens: torch.Tensor | None = None, first: int = 0, last: int = 0, causal: bool = False,
+                  max_k: int | None = None, out: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The key blocks that each tile of 128 queries of a sequence is to see, per key head: int32 [tiles, n_kv_head,
+    words], bit j % 32 of word j / 32 for block j.  Always the `first` first and `last` last blocks in the tile's sight
+    and those that some of its queries see in part; of the others the `top` with the largest product of the summed
+    queries (all heads of the key head's group) and the block's mean (block_means), in 64 bits, of equal ones the first.
+    max_k: keys of the longest sequence, or more (None: what `means` has rows for); it sets the number of words, at
+    most 256 of them.  New results have total_q / 128 + batch tiles; rows past the last tile are 0."""
+    return _call("select_blocks", stream, q, means, cu_q, top, cu_k, k_lens, first, last, causal, max_k, out)
+
+
+def attention_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, chosen: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, k_lens: torch.Tensor | None = None, causal: bool = False,
+                     scale: float | None = None, out: torch.Tensor | None = None,
+                     stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """attention_packed over the keys of chosen blocks: chosen as select_blocks gives it (or set by hand), the other
+    arguments as there.  Blocks out of a tile's sight are not looked at; a row that sees no key is 0."""
+    return _call("attention_blocks", stream, q, k, v, chosen, cu_q, cu_k, k_lens, causal, scale, out)
+
+
+def lora_down(x: torch.Tensor, a: torch.Tensor, cu: torch.Tensor, ids: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The first half of lora: t = x . a[r]^T, F32 [rows, R], for several lora_up calls on one x."""
+    return _call("lora_down", stream, x, a, cu, ids, out)
+
+
+def lora_up(t: torch.Tensor, b: torch.Tensor, y: torch.Tensor, cu: torch.Tensor, ids: torch.Tensor | None = None,
+            scale: torch.Tensor | None = None, epilogue: str = "none", gate: torch.Tensor | None = None,
+            out: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The second half of lora: out = epilogue(y + scale[r] * t . b[r]^T)."""
+    return _call("lora_up", stream, t, b, y, cu, ids, scale, epilogue, gate, out)
+
+
+def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, y: torch.Tensor, cu: torch.Tensor,
+         ids: torch.Tensor | None = None, scale: torch.Tensor | None = None, epilogue: str = "none",
+         gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+         stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Low-rank adapters of a packed batch's requests beside a projection that they share: with y the projection's
+    result, out = epilogue(y + scale[r] * (x . a[r]^T) . b[r]^T) for the rows cu[i] to cu[i+1] of request i, r = ids[i]
+    (None: i); "gated_residual": y + gate * (..).  x [rows, K], a [adapters, R, K] and b [adapters, N, R] are BF16 or F16, y and
+    out F32 or of that type; scale F32 [adapters] or None.  A request with an id outside the adapters has none: out =
+    epilogue(y).  R is a multiple of 8 up to 128 (lower ranks padded with zeros), K a multiple of 8.  out None: a new
+    tensor; y itself: in place.  Rows of no request are left as they were."""
+    return _call("lora", stream, x, a, b, y, cu, ids, scale, epilogue, gate, out)

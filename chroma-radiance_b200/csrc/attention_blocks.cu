@@ -1,0 +1,747 @@
+// attention_blocks.cu — attention over packed sequences, of which every tile of queries sees some key
+// blocks only, and what chooses the blocks.
+//
+// The keys of a sequence lie in blocks of 128, its queries in tiles of 128 (a single query is a tile of one).
+//
+//   block_means       m[j, g] = mean over the keys of block j of k[., g]
+//   select_blocks     s[j] = (sum of the tile's queries, all heads of key head g's group) . m[j, g];
+//                     bit j is set for the first and the last few blocks in sight, for blocks that some query of the
+//                     tile sees in part, and for the `top` largest s[j] of the others (of equals the lowest j)
+//   attention_blocks  out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, g]) v[j, g] over the keys of the set blocks
+//
+// Offsets are read on the device and clamped to the buffers, as in attention_packed.cu.
+//
+//   packed_tiles (attention_packed.cuh)  long queries: tensor cores through TMEM, K and V by chosen block
+//   chosen_rows                          few query rows per key head: a cluster shares out the chosen blocks
+#include "attention_packed.cuh"
+
+namespace b2g {
+
+namespace {
+
+// ---------------------------------------------------------------------------- means of blocks
+//
+// Bound by memory: k is read once.  A warp reads 512 bytes of a key's row (8 values a lane) for 32 of the block's
+// keys, kMnAhead loads at a time; the four warps' sums meet in shared memory in a fixed order.
+constexpr int kMnWarps = 4;
+constexpr int kMnAhead = 8;
+constexpr int kMnCols = 256;  // values of a row that a block takes
+
+struct MnParams {
+  PkParams p;            // k, cu_k, k_lens
+  const int* since;      // [batch] or NULL: all blocks
+  float* means;          // [blocks, hk, D]
+  int blocks, D;
+};
+
+__device__ __forceinline__ int key_blocks(const PkParams& p, int b) {  // with room left for more keys
+  const int lo = clampi(__ldg(p.cu_k + b), 0, p.total_k);
+  return (clampi(__ldg(p.cu_k + b + 1), lo, p.total_k) - lo + kPtKeys - 1) / kPtKeys;
+}
+// Blocks before sequence b's first (the whole warp).
+__device__ __forceinline__ int blocks_before(const PkParams& p, int b, int lane) {
+  int sum = 0;
+  for (int i = lane; i < b; i += 32) sum += key_blocks(p, i);
+  return __reduce_add_sync(0xffffffffu, sum);
+}
+
+template <typename T>
+__device__ __forceinline__ void add8(float (&sum)[8], uint4 v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f;
+    if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    sum[2 * i] += f.x;
+    sum[2 * i + 1] += f.y;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kMnWarps) block_means_kernel(const MnParams a) {
+  __shared__ float4 sums[kMnWarps][2][32];
+  const PkParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.y * kMnCols + lane * 8, cols = p.hk * a.D;
+  griddep_wait();
+  griddep_launch_dependents();
+  int b, j, stop, base;
+  const int step = a.since ? static_cast<int>(gridDim.z) : 1;
+  if (a.since) {  // sequence blockIdx.x, its blocks from the one of key since[b] on
+    b = blockIdx.x;
+    base = blocks_before(p, b, lane);
+    const Seq s = load_seq(p, b);
+    j = clampi(__ldg(a.since + b), 0, s.lk) / kPtKeys + static_cast<int>(blockIdx.z);
+    stop = (s.lk + kPtKeys - 1) / kPtKeys;
+  } else {        // row blockIdx.x of the means
+    base = 0;
+    b = find_seq(p.batch, static_cast<int>(blockIdx.x), lane, [&](int i) { return key_blocks(p, i); }, &base);
+    j = static_cast<int>(blockIdx.x) - base;
+    stop = j + 1;
+  }
+  const Seq s = b >= 0 ? load_seq(p, b) : Seq{};
+  const T* k = static_cast<const T*>(p.k) + (col < cols ? (col / a.D) * p.hsk + col % a.D : 0);
+  for (; j < stop && base + j < a.blocks; j += step) {
+    const int key0 = j * kPtKeys, n = b >= 0 ? clampi(s.lk - key0, 0, kPtKeys) : 0;
+    float sum[8] = {};
+    if (col < cols)
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += kMnAhead) {
+        uint4 v[kMnAhead];
+#pragma unroll
+        for (int i = 0; i < kMnAhead; ++i) {
+          const int r = warp * 32 + r0 + i;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r < n) v[i] = __ldg(reinterpret_cast<const uint4*>(k + static_cast<long long>(s.k0 + key0 + r) * p.ldk));
+        }
+#pragma unroll
+        for (int i = 0; i < kMnAhead; ++i) add8<T>(sum, v[i]);
+      }
+    sums[warp][0][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    sums[warp][1][lane] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+    __syncthreads();
+    if (warp < 2) {  // values 4 warp to 4 warp + 3 of each lane's 8
+      const float4 x = sums[0][warp][lane], y = sums[1][warp][lane], z = sums[2][warp][lane], w = sums[3][warp][lane];
+      const float count = static_cast<float>(max(n, 1));
+      if (col < cols)
+        *reinterpret_cast<float4*>(a.means + static_cast<long long>(base + j) * cols + col + 4 * warp) =
+            make_float4(((x.x + y.x) + (z.x + w.x)) / count, ((x.y + y.y) + (z.y + w.y)) / count,
+                        ((x.z + y.z) + (z.z + w.z)) / count, ((x.w + y.w) + (z.w + w.w)) / count);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------- choice of blocks
+//
+// Scores are sums of 64 bits: a choice compares neighbours, and any rounding of theirs in 32 bits would decide
+// the choice where two are close; in 64 bits the order of a sum moves one in some 10^12.
+constexpr int kSlThreads = 256;
+constexpr int kSlCounted = 256;  // up to so many blocks a block's rank is counted, else the threshold is searched
+constexpr int kSlMostWords = 256;
+
+struct SlParams {
+  PkParams p;           // q, cu_q, cu_k, k_lens, causal
+  const float* means;   // [blocks, hk, D]
+  int blocks, D;
+  int top, first, last;
+  uint32_t* chosen;     // [tiles, hk, words]
+  int tiles, words;
+};
+
+// Order of scores as that of whole numbers: NaN as -inf, -0 as 0; 0 is below every score.
+__device__ __forceinline__ unsigned long long score_order(double s) {
+  if (isnan(s)) s = -INFINITY;
+  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(s + 0.0));
+  return u >> 63 ? ~u : u | (1ull << 63);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParams a) {
+  constexpr int kPieces = D / 8, kGroups = kSlThreads / kPieces;  // 16-byte pieces of a row, rows at a time
+  extern __shared__ unsigned long long order[];  // [32 words] the blocks' scores
+  __shared__ double part[kGroups][D];
+  __shared__ int counts[2];
+  const PkParams& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / p.hk, g = blockIdx.x - tile * p.hk;
+  griddep_wait();
+  griddep_launch_dependents();
+  uint32_t* out = a.chosen + (static_cast<long long>(tile) * p.hk + g) * a.words;
+  int before = 0;
+  const int b = find_seq(p.batch, tile, lane, [&](int i) {
+    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+    return (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+  }, &before);
+  if (b < 0) {
+    for (int i = threadIdx.x; i < a.words; i += kSlThreads) out[i] = 0;
+    return;
+  }
+  const Seq s = load_seq(p, b);
+  const int base = blocks_before(p, b, lane);
+  const int row0 = (tile - before) * kPtRows, rows = min(kPtRows, s.lq - row0);
+  const int sees_first = p.causal ? clampi(row0 + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
+  const int sees_last = p.causal ? clampi(row0 + rows + s.lk - s.lq, 0, s.lk) : s.lk;
+  const int nb = min((sees_last + kPtKeys - 1) / kPtKeys, 32 * a.words);
+  auto sure = [&](int j) {
+    return j < a.first || j >= nb - a.last || min((j + 1) * kPtKeys, sees_last) > sees_first;
+  };
+
+  // The tile's queries, summed.
+  {
+    const int piece = threadIdx.x % kPieces, from = threadIdx.x / kPieces;
+    double sum[8] = {};
+    const T* q = static_cast<const T*>(p.q) + static_cast<long long>(s.q0 + row0) * p.ldq +
+                 static_cast<long long>(g) * p.group * p.hsq + piece * 8;
+    for (int i = from; i < rows * p.group; i += kGroups) {
+      const int row = i / p.group, h = i - row * p.group;
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(q + row * p.ldq + h * p.hsq));
+      float f[8] = {};
+      add8<T>(f, v);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) sum[x] += f[x];
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) part[from][piece * 8 + x] = sum[x];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < D; c += kSlThreads) {
+    double sum = part[0][c];
+    for (int i = 1; i < kGroups; ++i) sum += part[i][c];
+    part[0][c] = sum;
+  }
+  __syncthreads();
+  // Scores: 8 lanes to a block.
+  {
+    const int l = lane & 7;
+    double q[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) q[4 * i + x] = part[0][32 * i + 4 * l + x];
+    for (int j0 = warp * 4; j0 < nb; j0 += kSlThreads / 8) {
+      const int j = j0 + (lane >> 3);
+      double sum = 0.0;
+      if (j < nb && base + j < a.blocks) {
+        const float* m = a.means + (static_cast<long long>(base + j) * p.hk + g) * D + 4 * l;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(m + 32 * i));
+          sum = fma(q[4 * i], static_cast<double>(v.x), sum);
+          sum = fma(q[4 * i + 1], static_cast<double>(v.y), sum);
+          sum = fma(q[4 * i + 2], static_cast<double>(v.z), sum);
+          sum = fma(q[4 * i + 3], static_cast<double>(v.w), sum);
+        }
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (l == 0 && j < nb) order[j] = sure(j) ? 0 : score_order(sum);
+    }
+  }
+  __syncthreads();
+  if (nb <= kSlCounted) {
+    for (int w = warp; w < a.words; w += kSlThreads / 32) {
+      const int j = 32 * w + lane;
+      bool take = false;
+      if (j < nb) {
+        const unsigned long long mine = order[j];
+        int above = 0;
+        for (int i = 0; i < nb; ++i) above += order[i] > mine || (order[i] == mine && i < j);
+        take = mine == 0 || above < a.top;
+      }
+      const uint32_t bits = __ballot_sync(0xffffffffu, take);
+      if (lane == 0) out[w] = bits;
+    }
+    return;
+  }
+  // The largest threshold that `top` scores reach, bit by bit from above (fewer scores: 1, all of them).
+  unsigned long long least = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long next = least | (1ull << bit);
+    if (threadIdx.x == 0) counts[bit & 1] = 0;
+    __syncthreads();
+    int n = 0;
+    for (int j = threadIdx.x; j < nb; j += kSlThreads) n += order[j] >= next;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) atomicAdd(&counts[bit & 1], n);
+    __syncthreads();
+    if (counts[bit & 1] >= a.top) least = next;
+  }
+  if (least == 0) least = 1;
+  if (warp != 0) return;
+  int over = 0;  // scores above it; of those that equal it the first fill the rest
+  for (int j = lane; j < nb; j += 32) over += order[j] > least;
+  int room = a.top - __reduce_add_sync(0xffffffffu, over);
+  for (int w = 0; w < a.words; ++w) {
+    const int j = 32 * w + lane;
+    const unsigned long long mine = j < nb ? order[j] : 0;
+    const uint32_t equal = __ballot_sync(0xffffffffu, j < nb && mine == least);
+    const bool take = j < nb && (mine == 0 || mine > least ||
+                                 (mine == least && __popc(equal & ((1u << lane) - 1u)) < room));
+    const uint32_t bits = __ballot_sync(0xffffffffu, take);
+    room -= __popc(equal);
+    if (lane == 0) out[w] = bits;
+  }
+}
+
+// ---------------------------------------------------------------------------- few rows over chosen blocks
+//
+// The query rows of one key head (lq tokens x group heads) in tiles of 16, each taken by a cluster, whose CTAs
+// share out the chunks of 16 keys of the chosen blocks evenly; in a CTA 4 warps take chunks in turn.  The
+// products, the lanes' layout and the copies are those of packed_rows_kernel (attention_packed.cu).  The warps'
+// sums meet in shared memory, the CTAs' through distributed shared memory: one launch.
+constexpr int kCrWarps = 4;
+constexpr int kCrRows = 16;
+constexpr int kCrKeys = 16;
+constexpr int kCrBlocksPerSm = 2;
+constexpr int kCrListed = 256;  // chosen blocks that are listed at a time
+template <int D>
+constexpr int kCrPieces = D / 8;
+template <int D>
+constexpr int kCrStages = D == 128 ? 3 : 6;
+template <int D>
+constexpr uint32_t kCrSmem = kCrWarps * kCrStages<D> * kCrPieces<D> * 512u;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_kernel(const PkParams p, const int S) {
+  constexpr int KC = D / 32, VC = D / 64, NS = kCrStages<D>;
+  constexpr uint32_t kStage = kCrPieces<D> * 512u;
+  extern __shared__ __align__(16) uint8_t smem_rows[];
+  __shared__ float2 sml[kCrWarps][kCrRows];
+  __shared__ __align__(16) float2 cta_ml[kCrRows];
+  __shared__ int list[kCrListed];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem_rows) + warp * NS * kStage + lane * 16;
+  auto so = [&](int w) { return reinterpret_cast<float*>(smem_rows + w * NS * kStage); };
+  static_assert(kCrRows * (D + 4) * 4 <= NS * kStage, "sums fit a ring");
+  griddep_wait();
+  griddep_launch_dependents();
+  const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int item = static_cast<int>(blockIdx.x) / S, at_tile = item / p.hk, head = item - at_tile * p.hk;
+  int before = 0;
+  const int b = find_seq(p.batch, at_tile, lane, [&](int i) {
+    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+    return static_cast<int>((static_cast<long long>(clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo) * p.group + kCrRows - 1) / kCrRows);
+  }, &before);
+  if (b < 0) return;  // (the whole cluster)
+  const Seq s = load_seq(p, b);
+  const int rows = s.lq * p.group, row0 = (at_tile - before) * kCrRows;
+  const int first_token = row0 / p.group, last_token = (min(row0 + kCrRows, rows) - 1) / p.group;
+  const int tile_sees = p.causal ? clampi(last_token + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
+  int tile = 0;  // of `chosen`: 128 / 16 * group tiles of rows have one
+  for (int i = lane; i < b; i += 32) {
+    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+    tile += (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+  }
+  tile = __reduce_add_sync(0xffffffffu, tile) + first_token / kPtRows;
+  const uint32_t* words = p.chosen + (static_cast<long long>(tile) * p.hk + head) * p.chosen_words;
+  const int nb = tile < p.chosen_tiles ? min((tile_sees + kPtKeys - 1) / kPtKeys, 32 * p.chosen_words) : 0;
+  auto word = [&](int w) {
+    if (32 * w >= nb) return 0u;
+    const uint32_t bits = __ldg(words + w);
+    return nb - 32 * w >= 32 ? bits : bits & ((1u << (nb - 32 * w)) - 1u);
+  };
+  int count = 0;
+  for (int w = lane; 32 * w < nb; w += 32) count += __popc(word(w));
+  count = __reduce_add_sync(0xffffffffu, count);
+  // This CTA's chunks: a block has 8; of the last one in sight only those with keys.
+  const bool ends_short = nb > 0 && (word((nb - 1) >> 5) >> ((nb - 1) & 31) & 1u) != 0;
+  const int chunks = 8 * count - (ends_short ? 8 - (min(tile_sees - (nb - 1) * kPtKeys, kPtKeys) + kCrKeys - 1) / kCrKeys : 0);
+  const int c_from = static_cast<int>(static_cast<long long>(chunks) * rank / S);
+  const int c_to = static_cast<int>(static_cast<long long>(chunks) * (rank + 1) / S);
+
+  const T* kbase = static_cast<const T*>(p.k) + s.k0 * p.ldk + head * p.hsk + 8 * t;
+  const T* vbase = static_cast<const T*>(p.v) + s.k0 * p.ldv + head * p.hsv + 8 * g;
+  // Q: rows g and g + 8 of the tile (row r is token r / group, head r % group of the group).
+  uint4 q[2][KC];
+  int sees[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = min(row0 + g + 8 * i, rows - 1);
+    const int token = r / p.group, h = r - token * p.group;
+    sees[i] = p.causal ? min(s.lk, token + 1 + s.lk - s.lq) : s.lk;
+    const T* src = static_cast<const T*>(p.q) + (s.q0 + token) * p.ldq +
+                   (static_cast<long long>(head) * p.group + h) * p.hsq + 8 * t;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) q[i][c] = __ldg(reinterpret_cast<const uint4*>(src + 32 * c));
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  for (int block0 = c_from / 8; block0 * 8 < c_to; block0 += kCrListed) {
+    // The chosen blocks block0 to block0 + kCrListed, in order.
+    __syncthreads();
+    if (warp == 0) {
+      int seen = 0;
+      for (int w0 = 0; 32 * w0 < nb && seen < block0 + kCrListed; w0 += 32) {
+        uint32_t bits = word(w0 + lane);
+        int sum = __popc(bits);
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, sum, x);
+          if (lane >= x) sum += up;
+        }
+        int at = seen + sum - __popc(bits) - block0;
+        for (; bits; bits &= bits - 1, ++at)
+          if (at >= 0 && at < kCrListed) list[at] = (w0 + lane) * 32 + __ffs(bits) - 1;
+        seen += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    __syncthreads();
+    const int c0 = max(c_from, block0 * 8), c1 = min(c_to, (block0 + kCrListed) * 8);
+    auto first_key = [&](int c) { return list[(c >> 3) - block0] * kPtKeys + (c & 7) * kCrKeys; };
+    // Copies chunk c into stage st: keys that no row of the tile sees are zeros.
+    auto fetch = [&](int c, int st) {
+      const uint32_t dst = ring + st * kStage;
+      const int key0 = first_key(c);
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const int key = key0 + nt * 8 + g;
+        const bool live = key < tile_sees;
+        const T* src = live ? kbase + key * p.ldk : kbase;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) copy16(dst + (nt * KC + i) * 512, src + 32 * i, live);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
+        const bool live = key < tile_sees;
+        const T* src = live ? vbase + key * p.ldv : vbase;
+#pragma unroll
+        for (int k = 0; k < VC; ++k) copy16(dst + (2 * KC + i * VC + k) * 512, src + 64 * k, live);
+      }
+    };
+    int ahead = c0 + warp;
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i, ahead += kCrWarps) {
+      if (ahead < c1) fetch(ahead, i);
+      copy_commit();
+    }
+    int st = 0;
+    for (int c = c0 + warp; c < c1; c += kCrWarps) {
+      copy_wait<NS - 2>();
+      if (ahead < c1) fetch(ahead, st == 0 ? NS - 1 : st - 1);  // (the stage used up in the last round)
+      copy_commit();
+      ahead += kCrWarps;
+      const uint32_t src = ring + st * kStage;
+      st = st + 1 == NS ? 0 : st + 1;
+      float sc[2][4] = {};
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint4 kr = lds16(src + (nt * KC + i) * 512);
+          mma_16816<T>(sc[nt], q[0][i].x, q[1][i].x, q[0][i].y, q[1][i].y, kr.x, kr.y);
+          mma_16816<T>(sc[nt], q[0][i].z, q[1][i].z, q[0][i].w, q[1][i].w, kr.z, kr.w);
+        }
+      // Scores in log2 units; sc[nt][2i + e] is row g + 8i, key 8nt + 2t + e of the chunk.
+      const int key0 = first_key(c);
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = key0 + nt * 8 + 2 * t + (j & 1);
+          sc[nt][j] = key < sees[j >> 1] ? sc[nt][j] * p.scale_log2 : -INFINITY;
+          mx[j >> 1] = fmaxf(mx[j >> 1], sc[nt][j]);
+        }
+      float alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        const float top = fmaxf(m[i], mx[i]);
+        alpha[i] = top == m[i] ? 1.f : fast_exp2(m[i] - top);
+        m[i] = top;
+        l[i] *= alpha[i];
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          o[i][0] *= alpha[0];
+          o[i][1] *= alpha[0];
+          o[i][2] *= alpha[1];
+          o[i][3] *= alpha[1];
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float shift = m[i] == -INFINITY ? 0.f : m[i];
+          const float e0 = fast_exp2(sc[nt][2 * i] - shift), e1 = fast_exp2(sc[nt][2 * i + 1] - shift);
+          l[i] += e0 + e1;
+          pa[2 * nt + i] = pack2<T>(e0, e1);
+        }
+#pragma unroll
+      for (int k = 0; k < VC; ++k) {
+        uint4 vr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[i] = lds16(src + (2 * KC + i * VC + k) * 512);
+        const uint32_t v0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, v1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+        const uint32_t v2[4] = {vr[2].x, vr[2].y, vr[2].z, vr[2].w}, v3[4] = {vr[3].x, vr[3].y, vr[3].z, vr[3].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
+          mma_16816<T>(o[8 * k + i], pa[0], pa[1], pa[2], pa[3], __byte_perm(v0[i >> 1], v1[i >> 1], pick),
+                       __byte_perm(v2[i >> 1], v3[i >> 1], pick));
+        }
+      }
+    }
+    copy_wait<0>();
+  }
+  // The warps' statistics and sums.
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (t == 0) sml[warp][g + 8 * i] = make_float2(m[i], l[i]);
+  }
+  __syncwarp();  // (the ring's slots belong to lanes, the sums do not)
+#pragma unroll
+  for (int k = 0; k < VC; ++k)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {  // column 2t + e of product i is d = 64 k + 8 (2t + e) + i
+        float* dst = so(warp) + g * (D + 4) + 64 * k + 16 * t + 8 * e + i;
+        const float(*x)[4] = o + 8 * k + i;
+        *reinterpret_cast<float4*>(dst) = make_float4(x[0][e], x[1][e], x[2][e], x[3][e]);
+        *reinterpret_cast<float4*>(dst + 8 * (D + 4)) = make_float4(x[0][2 + e], x[1][2 + e], x[2][2 + e], x[3][2 + e]);
+      }
+  __syncthreads();
+  // With part i holding (m_i, l_i) and O_i: O = sum 2^(m_i - M) O_i, l = sum 2^(m_i - M) l_i.  (A part without a key has
+  // the sums 0; a NaN maximum does not occur, a NaN sum stays one.)
+  auto weight = [](float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top); };
+  auto add = [](float4& acc, float w, float4 x) {
+    acc.x += w * x.x;
+    acc.y += w * x.y;
+    acc.z += w * x.z;
+    acc.w += w * x.w;
+  };
+  auto store = [&](int r, int d, float sum, float4 acc) {
+    const int token = (row0 + r) / p.group, h = (row0 + r) - token * p.group;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  };
+  const int live_rows = min(kCrRows, rows - row0);
+  for (int at = threadIdx.x; at < live_rows * (D / 4); at += 32 * kCrWarps) {
+    const int r = at / (D / 4), d = (at - r * (D / 4)) * 4;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kCrWarps; ++w) top = fmaxf(top, sml[w][r].x);
+#pragma unroll
+    for (int w = 0; w < kCrWarps; ++w) {
+      const float wgt = weight(sml[w][r], top);
+      sum += wgt * sml[w][r].y;
+      add(acc, wgt, *reinterpret_cast<const float4*>(so(w) + r * (D + 4) + d));
+    }
+    if (S == 1) store(r, d, sum, acc);
+    else {
+      *reinterpret_cast<float4*>(so(0) + r * (D + 4) + d) = acc;  // (read by this thread alone until here)
+      if (d == 0) cta_ml[r] = make_float2(top, sum);
+    }
+  }
+  if (S == 1) return;
+  cluster_sync_all();  // every CTA's sums are in its shared memory
+  const uint32_t my_o = smem_u32(so(0)), my_ml = smem_u32(cta_ml);
+  for (int at = rank * 32 * kCrWarps + threadIdx.x; at < live_rows * (D / 4); at += S * 32 * kCrWarps) {
+    const int r = at / (D / 4), d = (at - r * (D / 4)) * 4;
+    float2 ml[8];
+    float4 x[8];
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ml[i] = make_float2(-INFINITY, 0.f);
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i >= S) continue;
+      ml[i] = ld_cluster_f2(map_to_cta(my_ml + r * 8, i));
+      x[i] = ld_cluster_f4(map_to_cta(my_o + (r * (D + 4) + d) * 4, i));
+      top = fmaxf(top, ml[i].x);
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float wgt = weight(ml[i], top);
+      sum += wgt * ml[i].y;
+      add(acc, wgt, x[i]);
+    }
+    store(r, d, sum, acc);
+  }
+  cluster_sync_all();  // nobody leaves while its sums are still read
+}
+
+// ---------------------------------------------------------------------------- host side
+
+// Average queries per sequence up to which chosen_rows takes a call, as in attention_packed.cu.
+constexpr int64_t kCrQueries = 16;
+
+template <typename T, int D>
+b2g_status launch_chosen_rows(const PkParams& p, int sms, cudaStream_t st) {
+  const int64_t items = (static_cast<int64_t>(p.total_q) * p.group / kCrRows + p.batch) * p.hk;
+  // As many CTAs as run at the same time, up to 8 to an item.
+  int64_t S = static_cast<int64_t>(kCrBlocksPerSm) * sms / items;
+  S = S < 1 ? 1 : S > 8 ? 8 : S;
+  if (items * S > (1ll << 31) - 1) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_blocks: size");
+  auto kern = chosen_rows_kernel<T, D>;
+  b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCrSmem<D>)),
+                            "cudaFuncSetAttribute(chosen_rows)");
+  if (s != B2G_OK) return s;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * S));
+  cfg.blockDim = dim3(32 * kCrWarps);
+  cfg.dynamicSmemBytes = kCrSmem<D>;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(S);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = S > 1 ? 2 : 1;
+  s = check_cuda(cudaLaunchKernelEx(&cfg, kern, p, static_cast<int>(S)), "chosen_rows launch");
+  if (s == B2G_OK) note_launch();
+  return s;
+}
+
+template <typename T, int D>
+b2g_status run_chosen(const b2g_attention_packed_desc* d, PkParams p, int sms, cudaStream_t st) {
+  if (d->total_q <= kCrQueries * d->batch || d->total_k == 0) return launch_chosen_rows<T, D>(p, sms, st);
+  CUtensorMap tq, tk, tv;
+  b2g_status s;
+  if ((s = make_operand_map(&tq, p.q, d->dtype, D, p.total_q, p.ldq, p.hq, p.hsq, kPtRows)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tk, p.k, d->dtype, D, p.total_k, p.ldk, p.hk, p.hsk, kPtKeys)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tv, p.v, d->dtype, D, p.total_k, p.ldv, p.hk, p.hsv, kPtKeys)) != B2G_OK) return s;
+  p.item_heads = 2;
+  if ((static_cast<int64_t>(p.total_q) / kPtRows + p.batch) * p.hq <= sms) {  // (every tile finds an SM of its own)
+    p.item_heads = 1;
+    return launch_tiles<T, D, kHeadsApart, true>(p, tq, tk, tv, sms, st);
+  }
+  // Two heads of a group have the same blocks and share their stages; others have their own.
+  if (p.group % 2 == 0) return launch_tiles<T, D, kHeadsOfGroup, true>(p, tq, tk, tv, sms, st);
+  return launch_tiles<T, D, kHeadsApart, true>(p, tq, tk, tv, sms, st);
+}
+
+// The checks that the three operators have in common, and the parameters; uses_q: q and cu_q, uses_v: v and out.
+b2g_status blocks_params(const b2g_attention_packed_desc* d, const char* who, bool uses_q, bool uses_v, PkParams* p) {
+  auto fail = [&](b2g_status st, const char* why) { return set_error(st, std::string(who) + ": " + why); };
+  if (!d) return fail(B2G_ERR_INVALID, "null descriptor");
+  if (d->batch < 0 || d->total_q < 0 || d->total_k < 0 || d->n_head < 0 || d->n_kv_head < 0)
+    return fail(B2G_ERR_INVALID, "negative size");
+  if (d->dtype != B2G_BF16 && d->dtype != B2G_F16) return fail(B2G_ERR_UNSUPPORTED, "BF16 or F16 operands");
+  if (d->d_head != 64 && d->d_head != 128) return fail(B2G_ERR_UNSUPPORTED, "head dim must be 64 or 128");
+  if (uses_q && d->n_head > 0 && (d->n_kv_head < 1 || d->n_head % d->n_kv_head != 0))
+    return fail(B2G_ERR_INVALID, "n_head must be a multiple of n_kv_head");
+  if (uses_v && (!(d->scale > 0.f) || !std::isfinite(d->scale))) return fail(B2G_ERR_INVALID, "scale must be positive");
+  if (d->batch > 65536 || d->total_q > (1ll << 30) || d->total_k > (1ll << 30) || d->n_head > 65535 || d->n_kv_head > 65535)
+    return fail(B2G_ERR_UNSUPPORTED, "size");
+  const int64_t D = d->d_head;
+  p->ldq = used(d->ldq, d->total_q, d->n_head * D); p->hsq = used(d->hsq, d->n_head, D);
+  p->ldk = used(d->ldk, d->total_k, d->n_kv_head * D); p->hsk = used(d->hsk, d->n_kv_head, D);
+  p->ldv = used(d->ldv, d->total_k, d->n_kv_head * D); p->hsv = used(d->hsv, d->n_kv_head, D);
+  p->ldo = used(d->ldo, d->total_q, d->n_head * D); p->hso = used(d->hso, d->n_head, D);
+  const bool uses_k = uses_v || !uses_q;
+  struct { bool in_use; const void* at; int64_t ld, hs, rows; } ops[4] = {{uses_q, d->q, p->ldq, p->hsq, d->total_q * d->n_head},
+                                                                       {uses_k, d->k, p->ldk, p->hsk, d->total_k * d->n_kv_head},
+                                                                       {uses_v, d->v, p->ldv, p->hsv, d->total_k * d->n_kv_head},
+                                                                       {uses_v, d->out, p->ldo, p->hso, d->total_q * d->n_head}};
+  for (const auto& o : ops) {
+    if (!o.in_use || o.rows == 0) continue;
+    if (!o.at) return fail(B2G_ERR_INVALID, "null operand");
+    if (o.ld < D || o.hs < D) return fail(B2G_ERR_INVALID, "a token or head stride is below the head dim");
+    if (o.ld % 8 != 0 || o.hs % 8 != 0 || o.ld >= (1ll << 38) || o.hs >= (1ll << 38))
+      return fail(B2G_ERR_UNSUPPORTED, "strides must be multiples of 8 elements");
+    if (reinterpret_cast<uintptr_t>(o.at) & 15u) return fail(B2G_ERR_UNSUPPORTED, "16-byte aligned operands required");
+  }
+  if (d->batch > 0 && (!d->cu_k || (uses_q && !d->cu_q))) return fail(B2G_ERR_INVALID, "null operand");
+  p->cu_q = d->cu_q; p->cu_k = d->cu_k; p->k_lens = d->k_lens;
+  p->batch = static_cast<int>(d->batch);
+  p->total_q = static_cast<int>(d->total_q); p->total_k = static_cast<int>(d->total_k);
+  p->hq = d->n_head; p->hk = d->n_kv_head; p->group = uses_q && d->n_kv_head > 0 ? d->n_head / d->n_kv_head : 1;
+  p->causal = d->causal ? 1 : 0;
+  p->scale_log2 = d->scale * 1.4426950408889634f;
+  p->q = d->q; p->k = d->k; p->v = d->v; p->out = d->out;
+  return B2G_OK;
+}
+
+}  // namespace
+
+b2g_status block_means(const b2g_attention_packed_desc* d, const int32_t* since, float* means, int64_t blocks,
+                       cudaStream_t st) {
+  MnParams a{};
+  b2g_status s = blocks_params(d, "b2g_block_means", false, false, &a.p);
+  if (s != B2G_OK) return s;
+  if (blocks < 0) return set_error(B2G_ERR_INVALID, "b2g_block_means: negative size");
+  if (blocks == 0 || d->n_kv_head == 0) return B2G_OK;
+  if (!means) return set_error(B2G_ERR_INVALID, "b2g_block_means: null operand");
+  if (reinterpret_cast<uintptr_t>(means) & 15u)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_block_means: 16-byte aligned operands required");
+  if (blocks > (1ll << 30)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_block_means: size");
+  if (since && d->batch == 0) return B2G_OK;
+  DeviceInfo* dev = nullptr;
+  if ((s = device_info(&dev)) != B2G_OK) return s;
+  a.since = since;
+  a.means = means;
+  a.blocks = static_cast<int>(blocks);
+  a.D = d->d_head;
+  const int64_t parts = (static_cast<int64_t>(d->n_kv_head) * d->d_head + kMnCols - 1) / kMnCols;
+  if (parts > 65535) return set_error(B2G_ERR_UNSUPPORTED, "b2g_block_means: size");
+  int64_t z = 1;
+  if (since) {  // as many blocks of a sequence side by side as the SMs have room for
+    z = 8ll * dev->num_sms / (d->batch * parts);
+    z = z < 1 ? 1 : z > blocks ? blocks : z;
+    if (z > 65535) z = 65535;
+  }
+  const dim3 grid(static_cast<unsigned>(since ? d->batch : blocks), static_cast<unsigned>(parts), static_cast<unsigned>(z));
+  const dim3 block(32 * kMnWarps);
+  if (d->dtype == B2G_F16) return launch_pdl(block_means_kernel<__half>, grid, block, 0, st, "block_means launch", a);
+  return launch_pdl(block_means_kernel<__nv_bfloat16>, grid, block, 0, st, "block_means launch", a);
+}
+
+b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means, int64_t blocks, int64_t top, int64_t first,
+                         int64_t last, int32_t* chosen, int64_t tiles, int64_t words, cudaStream_t st) {
+  SlParams a{};
+  b2g_status s = blocks_params(d, "b2g_select_blocks", true, false, &a.p);
+  if (s != B2G_OK) return s;
+  if (blocks < 0 || tiles < 0 || words < 0 || top < 0 || first < 0 || last < 0)
+    return set_error(B2G_ERR_INVALID, "b2g_select_blocks: negative size");
+  if (tiles == 0 || words == 0 || d->n_kv_head == 0) return B2G_OK;
+  if (!chosen || (blocks > 0 && !means)) return set_error(B2G_ERR_INVALID, "b2g_select_blocks: null operand");
+  if (words > kSlMostWords) return set_error(B2G_ERR_UNSUPPORTED, "b2g_select_blocks: at most 2^20 keys a sequence");
+  if ((reinterpret_cast<uintptr_t>(means) & 15u) || (reinterpret_cast<uintptr_t>(chosen) & 3u))
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_select_blocks: 16-byte aligned means required");
+  if (blocks > (1ll << 30) || tiles * d->n_kv_head > (1ll << 31) - 1)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_select_blocks: size");
+  DeviceInfo* dev = nullptr;
+  if ((s = device_info(&dev)) != B2G_OK) return s;
+  const int64_t most = 32 * words;  // (more of them take every block just the same)
+  a.means = means;
+  a.blocks = static_cast<int>(blocks);
+  a.top = static_cast<int>(top < most ? top : most);
+  a.first = static_cast<int>(first < most ? first : most);
+  a.last = static_cast<int>(last < most ? last : most);
+  a.chosen = reinterpret_cast<uint32_t*>(chosen);
+  a.tiles = static_cast<int>(tiles);
+  a.words = static_cast<int>(words);
+  const dim3 grid(static_cast<unsigned>(tiles * d->n_kv_head)), block(kSlThreads);
+  const size_t smem = static_cast<size_t>(words) * 32 * 8;
+  auto run = [&](auto kern) {
+    b2g_status st2 = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlMostWords * 32 * 8),
+                                "cudaFuncSetAttribute(select_blocks)");
+    return st2 != B2G_OK ? st2 : launch_pdl(kern, grid, block, smem, st, "select_blocks launch", a);
+  };
+  if (d->dtype == B2G_F16) return d->d_head == 128 ? run(select_blocks_kernel<__half, 128>) : run(select_blocks_kernel<__half, 64>);
+  return d->d_head == 128 ? run(select_blocks_kernel<__nv_bfloat16, 128>) : run(select_blocks_kernel<__nv_bfloat16, 64>);
+}
+
+b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* chosen, int64_t tiles, int64_t words,
+                            cudaStream_t st) {
+  PkParams p{};
+  b2g_status s = blocks_params(d, "b2g_attention_blocks", true, true, &p);
+  if (s != B2G_OK) return s;
+  if (tiles < 0 || words < 0) return set_error(B2G_ERR_INVALID, "b2g_attention_blocks: negative size");
+  if (d->batch == 0 || d->total_q == 0 || d->n_head == 0) return B2G_OK;
+  if (tiles > 0 && words > 0 && !chosen) return set_error(B2G_ERR_INVALID, "b2g_attention_blocks: null operand");
+  if (reinterpret_cast<uintptr_t>(chosen) & 3u)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_blocks: 4-byte aligned words required");
+  if (tiles > (1ll << 30) || words > (1ll << 20)) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_blocks: size");
+  DeviceInfo* dev = nullptr;
+  if ((s = device_info(&dev)) != B2G_OK) return s;
+  p.chosen = reinterpret_cast<const uint32_t*>(chosen);
+  p.chosen_tiles = words > 0 ? static_cast<int>(tiles) : 0;
+  p.chosen_words = static_cast<int>(words);
+  p.err = dev->err_word;
+  if (d->dtype == B2G_F16)
+    return d->d_head == 128 ? run_chosen<__half, 128>(d, p, dev->num_sms, st) : run_chosen<__half, 64>(d, p, dev->num_sms, st);
+  return d->d_head == 128 ? run_chosen<__nv_bfloat16, 128>(d, p, dev->num_sms, st)
+                          : run_chosen<__nv_bfloat16, 64>(d, p, dev->num_sms, st);
+}
+
+}  // namespace b2g

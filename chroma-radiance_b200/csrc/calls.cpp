@@ -30,6 +30,11 @@ decltype(&b2g_gemm_s8_workspace) call_gemm_s8_workspace = nullptr;
 decltype(&b2g_qk_norm_rope) call_qk_norm_rope = nullptr;
 decltype(&b2g_attention_packed) call_attention_packed = nullptr;
 decltype(&b2g_attention_packed_workspace) call_attention_packed_workspace = nullptr;
+decltype(&b2g_block_means) call_block_means = nullptr;
+decltype(&b2g_select_blocks) call_select_blocks = nullptr;
+decltype(&b2g_attention_blocks) call_attention_blocks = nullptr;
+decltype(&b2g_lora_down) call_lora_down = nullptr;
+decltype(&b2g_lora_up) call_lora_up = nullptr;
 decltype(&b2g_last_error) call_last_error = nullptr;
 PyObject* error_type = nullptr;
 
@@ -301,6 +306,262 @@ PyObject* attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+int64_t whole(PyObject* o, const char* what) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw PythonError{};
+  if (v < 0) refuse(std::string(what) + " must not be negative");
+  return v;
+}
+
+// The keys' side of a descriptor: offsets, lengths, sizes.
+void key_side(b2g_attention_packed_desc& d, const Tensor& cu_k, const Tensor* lens, int64_t B, const std::string& who) {
+  d.cu_k = static_cast<const int32_t*>(vector(cu_k, ScalarType::Int, B + 1, (who + ": cu_k").c_str()));
+  if (lens) d.k_lens = static_cast<const int32_t*>(vector(*lens, ScalarType::Int, B, (who + ": k_lens").c_str()));
+  d.batch = B;
+}
+bool is_half(ScalarType t) { return t == ScalarType::BFloat16 || t == ScalarType::Half; }
+
+// (k, cu_k, k_lens, since, out) -> means
+PyObject* block_means(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 5);
+    const Tensor &k = tensor(a[0], "block_means: k"), &cu_k = tensor(a[1], "block_means: cu_k");
+    const Tensor *lens = maybe(a[2], "block_means: k_lens"), *since = maybe(a[3], "block_means: since"),
+                 *given = maybe(a[4], "block_means: out");
+    const Heads hk = heads(k, "block_means: k");
+    if (!is_half(k.scalar_type())) refuse("block_means: k must be BF16 or F16");
+    const int64_t B = cu_k.numel() - 1, D = k.size(2);
+    if (B < 0) refuse("block_means: cu_k must hold batch + 1 offsets");
+    if (since && !given) refuse("block_means: since needs `out` (the means kept so far)");
+    if (given && (given->dim() != 3 || given->size(1) != k.size(1) || given->size(2) != D || !given->is_contiguous() ||
+                  given->scalar_type() != ScalarType::Float))
+      refuse("block_means: out must be contiguous F32 [blocks, n_kv_head, d]");
+    b2g_attention_packed_desc d{};
+    key_side(d, cu_k, lens, B, "block_means");
+    const int32_t* from = since ? static_cast<const int32_t*>(vector(*since, ScalarType::Int, B, "block_means: since")) : nullptr;
+    void* stream = stream_of({&k, &cu_k, lens, since, given});
+    const Tensor out = given ? *given : make({k.size(0) / 128 + B, k.size(1), D}, ScalarType::Float, k);
+    d.k = k.data_ptr();
+    d.dtype = static_cast<b2g_dtype>(dtype_of(k.scalar_type()));
+    d.ldk = hk.ld; d.hsk = hk.hs;
+    d.total_k = k.size(0);
+    d.n_kv_head = static_cast<int>(k.size(1)); d.d_head = static_cast<int>(D);
+    check(call_block_means(&d, from, static_cast<float*>(out.data_ptr()), out.size(0), stream));
+    return result(a[4], out);
+  });
+}
+
+// (q, means, cu_q, top, cu_k, k_lens, first, last, causal, max_k, out) -> chosen
+PyObject* select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 11);
+    const Tensor &q = tensor(a[0], "select_blocks: q"), &means = tensor(a[1], "select_blocks: means"),
+                 &cu_q = tensor(a[2], "select_blocks: cu_q");
+    const Tensor *cu_k = maybe(a[4], "select_blocks: cu_k"), *lens = maybe(a[5], "select_blocks: k_lens"),
+                 *given = maybe(a[10], "select_blocks: out");
+    const Heads hq = heads(q, "select_blocks: q");
+    const int64_t D = q.size(2);
+    if (!is_half(q.scalar_type())) refuse("select_blocks: q must be BF16 or F16");
+    if (means.dim() != 3 || means.size(2) != D || means.scalar_type() != ScalarType::Float || !means.is_contiguous())
+      refuse("select_blocks: means must be contiguous F32 [blocks, n_kv_head, d]");
+    if (!cu_k) cu_k = &cu_q;
+    const int64_t B = cu_q.numel() - 1, blocks = means.size(0);
+    if (B < 0) refuse("select_blocks: cu_q must hold batch + 1 offsets");
+    b2g_attention_packed_desc d{};
+    d.cu_q = static_cast<const int32_t*>(vector(cu_q, ScalarType::Int, B + 1, "select_blocks: cu_q"));
+    key_side(d, *cu_k, lens, B, "select_blocks");
+    const int64_t top = whole(a[3], "select_blocks: top"), first = whole(a[6], "select_blocks: first"),
+                  last = whole(a[7], "select_blocks: last");
+    int64_t most = blocks;  // blocks of a sequence
+    if (a[9] != Py_None) {
+      const int64_t keys = whole(a[9], "select_blocks: max_k");
+      most = keys / 128 + (keys % 128 != 0);
+    }
+    if (given && (given->dim() != 3 || given->size(1) != means.size(1) || !given->is_contiguous() ||
+                  given->scalar_type() != ScalarType::Int))
+      refuse("select_blocks: out must be contiguous int32 [tiles, n_kv_head, words]");
+    void* stream = stream_of({&q, &means, &cu_q, cu_k, lens, given});
+    const Tensor out = given ? *given : make({q.size(0) / 128 + B, means.size(1), (most + 31) / 32}, ScalarType::Int, q);
+    d.q = q.data_ptr();
+    d.dtype = static_cast<b2g_dtype>(dtype_of(q.scalar_type()));
+    d.ldq = hq.ld; d.hsq = hq.hs;
+    d.total_q = q.size(0);
+    d.total_k = blocks < (1 << 23) ? 128 * blocks : 1 << 30;  // (no key is read: a bound for the offsets)
+    d.n_head = static_cast<int>(q.size(1)); d.n_kv_head = static_cast<int>(means.size(1)); d.d_head = static_cast<int>(D);
+    d.causal = PyObject_IsTrue(a[8]);
+    if (PyErr_Occurred()) throw PythonError{};
+    check(call_select_blocks(&d, static_cast<const float*>(means.data_ptr()), blocks, top, first, last,
+                             static_cast<int32_t*>(out.data_ptr()), out.size(0), out.size(2), stream));
+    return result(a[10], out);
+  });
+}
+
+// (q, k, v, chosen, cu_q, cu_k, k_lens, causal, scale, out) -> out
+PyObject* attention_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 10);
+    const Tensor &q = tensor(a[0], "attention_blocks: q"), &k = tensor(a[1], "attention_blocks: k"),
+                 &v = tensor(a[2], "attention_blocks: v"), &chosen = tensor(a[3], "attention_blocks: chosen"),
+                 &cu_q = tensor(a[4], "attention_blocks: cu_q");
+    const Tensor *cu_k = maybe(a[5], "attention_blocks: cu_k"), *lens = maybe(a[6], "attention_blocks: k_lens"),
+                 *given = maybe(a[9], "attention_blocks: out");
+    const Heads hq = heads(q, "attention_blocks: q"), hk = heads(k, "attention_blocks: k"), hv = heads(v, "attention_blocks: v");
+    const int64_t D = q.size(2);
+    const ScalarType type = q.scalar_type();
+    if (v.sizes() != k.sizes() || k.size(2) != D || k.scalar_type() != type || v.scalar_type() != type || !is_half(type))
+      refuse("attention_blocks: q, k, v must be BF16 or F16 of one head width, k and v of one shape");
+    if (chosen.dim() != 3 || chosen.size(1) != k.size(1) || chosen.scalar_type() != ScalarType::Int || !chosen.is_contiguous())
+      refuse("attention_blocks: chosen must be contiguous int32 [tiles, n_kv_head, words]");
+    if (!cu_k) cu_k = &cu_q;
+    const int64_t B = cu_q.numel() - 1;
+    if (B < 0) refuse("attention_blocks: cu_q must hold batch + 1 offsets");
+    b2g_attention_packed_desc d{};
+    d.cu_q = static_cast<const int32_t*>(vector(cu_q, ScalarType::Int, B + 1, "attention_blocks: cu_q"));
+    key_side(d, *cu_k, lens, B, "attention_blocks");
+    void* stream = stream_of({&q, &k, &v, &chosen, &cu_q, cu_k, lens, given});
+    const Tensor out = output_like(q, given, type, "attention_blocks: out");
+    const Heads ho = heads(out, "attention_blocks: out");
+    d.q = q.data_ptr(); d.k = k.data_ptr(); d.v = v.data_ptr(); d.out = out.data_ptr();
+    d.dtype = static_cast<b2g_dtype>(dtype_of(type));
+    d.ldq = hq.ld; d.hsq = hq.hs; d.ldk = hk.ld; d.hsk = hk.hs;
+    d.ldv = hv.ld; d.hsv = hv.hs; d.ldo = ho.ld; d.hso = ho.hs;
+    d.total_q = q.size(0); d.total_k = k.size(0);
+    d.n_head = static_cast<int>(q.size(1)); d.n_kv_head = static_cast<int>(k.size(1)); d.d_head = static_cast<int>(D);
+    d.causal = PyObject_IsTrue(a[7]);
+    d.scale = a[8] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)))
+                              : static_cast<float>(PyFloat_AsDouble(a[8]));
+    if (PyErr_Occurred()) throw PythonError{};
+    check(call_attention_blocks(&d, static_cast<const int32_t*>(chosen.data_ptr()), chosen.size(0), chosen.size(2), stream));
+    return result(a[9], out);
+  });
+}
+
+// The parts of lora's descriptor: requests; x and A; t; B, y and what is done with them.
+void lora_requests(b2g_lora_desc& d, const Tensor& cu, const Tensor* ids, const std::string& who) {
+  d.batch = cu.numel() - 1;
+  if (d.batch < 0) refuse(who + ": cu must hold batch + 1 offsets");
+  d.cu = static_cast<const int32_t*>(vector(cu, ScalarType::Int, d.batch + 1, (who + ": cu").c_str()));
+  if (ids) d.ids = static_cast<const int32_t*>(vector(*ids, ScalarType::Int, d.batch, (who + ": ids").c_str()));
+}
+void lora_first(b2g_lora_desc& d, const Tensor& x, const Tensor& a, const std::string& who) {
+  if (x.dim() != 2 || a.dim() != 3 || !is_half(x.scalar_type()) || a.scalar_type() != x.scalar_type())
+    refuse(who + ": x [rows, K] and a [adapters, R, K] must be BF16 or F16, of one type");
+  if (x.size(1) != a.size(2))
+    refuse(who + ": K mismatch (" + std::to_string(x.size(1)) + " and " + std::to_string(a.size(2)) + ")");
+  if (x.size(1) > 1 && (x.stride(1) != 1 || a.stride(2) != 1)) refuse(who + ": x and a need unit stride along K");
+  d.rows = x.size(0); d.K = x.size(1); d.R = a.size(1); d.adapters = a.size(0);
+  d.x = x.data_ptr(); d.a = a.data_ptr();
+  d.dtype = static_cast<b2g_dtype>(dtype_of(x.scalar_type()));
+  d.ldx = x.stride(0); d.lda = a.stride(1); d.a_stride = a.stride(0);
+}
+void lora_second(b2g_lora_desc& d, const Tensor& b, const Tensor& y, const Tensor* scale, PyObject* epilogue, const Tensor* gate,
+                 const Tensor* given, const std::string& who) {
+  if (b.dim() != 3 || !is_half(b.scalar_type()) || b.size(2) != d.R || (b.size(2) > 1 && b.stride(2) != 1))
+    refuse(who + ": b must be BF16 or F16 [adapters, N, R] with unit stride along R");
+  d.N = b.size(1);
+  if (y.dim() != 2 || y.size(0) != d.rows || y.size(1) != d.N || (d.N > 1 && y.stride(1) != 1))
+    refuse(who + ": y must be [rows, N] with unit column stride");
+  if (given && (given->sizes() != y.sizes() || given->scalar_type() != y.scalar_type() || (d.N > 1 && given->stride(1) != 1)))
+    refuse(who + ": out must be of y's shape and type with unit column stride");
+  if (y.scalar_type() != ScalarType::Float && y.scalar_type() != b.scalar_type()) refuse(who + ": y must be F32 or of b's type");
+  int epi = -1;
+  static const struct { const char* name; int value; } kEpilogues[] = {
+      {"none", B2G_EPI_NONE}, {"gelu", B2G_EPI_GELU}, {"gated_residual", B2G_EPI_GATED_RESIDUAL}, {"silu", B2G_EPI_SILU}};
+  if (PyUnicode_Check(epilogue))
+    for (const auto& e : kEpilogues)
+      if (PyUnicode_CompareWithASCIIString(epilogue, e.name) == 0) epi = e.value;
+  if (epi < 0) refuse(who + ": unknown epilogue");
+  d.epilogue = static_cast<b2g_epilogue>(epi);
+  if (epi == B2G_EPI_GATED_RESIDUAL) {
+    if (!gate) refuse(who + ": gated_residual needs a gate");
+    d.gate = static_cast<const float*>(vector(*gate, ScalarType::Float, d.N, (who + ": gate").c_str()));
+  }
+  if (scale) d.scale = static_cast<const float*>(vector(*scale, ScalarType::Float, b.size(0), (who + ": scale").c_str()));
+  d.dtype = static_cast<b2g_dtype>(dtype_of(b.scalar_type()));
+  d.adapters = b.size(0);
+  d.b = b.data_ptr();
+  d.ldb = b.stride(1); d.b_stride = b.stride(0);
+  d.y = y.data_ptr();
+  d.y_dtype = static_cast<b2g_dtype>(dtype_of(y.scalar_type()));
+  d.ldy = y.stride(0);
+}
+void lora_out(b2g_lora_desc& d, const Tensor& out) {
+  d.out = out.data_ptr();
+  d.ldo = out.stride(0);
+}
+void lora_t(b2g_lora_desc& d, const Tensor& t, const std::string& who) {
+  if (t.dim() != 2 || t.scalar_type() != ScalarType::Float || (t.size(1) > 1 && t.stride(1) != 1))
+    refuse(who + ": t must be F32 [rows, R] with unit column stride");
+  d.rows = t.size(0); d.R = t.size(1);
+  d.t = static_cast<float*>(t.data_ptr());
+  d.ldt = t.size(0) > 1 ? t.stride(0) : t.size(1);
+}
+
+// (x, a, cu, ids, out) -> t
+PyObject* lora_down(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 5);
+    const Tensor &x = tensor(a[0], "lora_down: x"), &w = tensor(a[1], "lora_down: a"), &cu = tensor(a[2], "lora_down: cu");
+    const Tensor *ids = maybe(a[3], "lora_down: ids"), *given = maybe(a[4], "lora_down: out");
+    b2g_lora_desc d{};
+    lora_first(d, x, w, "lora_down");
+    if (given && (given->dim() != 2 || given->size(0) != d.rows || given->size(1) != d.R)) refuse("lora_down: out must be F32 [rows, R]");
+    lora_requests(d, cu, ids, "lora_down");
+    void* stream = stream_of({&x, &w, &cu, ids, given});
+    const Tensor out = given ? *given : make({d.rows, d.R}, ScalarType::Float, x);
+    lora_t(d, out, "lora_down");
+    check(call_lora_down(&d, stream));
+    return result(a[4], out);
+  });
+}
+
+// (t, b, y, cu, ids, scale, epilogue, gate, out) -> out
+PyObject* lora_up(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 9);
+    const Tensor &t = tensor(a[0], "lora_up: t"), &w = tensor(a[1], "lora_up: b"), &y = tensor(a[2], "lora_up: y"),
+                 &cu = tensor(a[3], "lora_up: cu");
+    const Tensor *ids = maybe(a[4], "lora_up: ids"), *scale = maybe(a[5], "lora_up: scale"), *gate = maybe(a[7], "lora_up: gate"),
+                 *given = maybe(a[8], "lora_up: out");
+    b2g_lora_desc d{};
+    lora_t(d, t, "lora_up");
+    lora_second(d, w, y, scale, a[6], gate, given, "lora_up");
+    if (!d.gate) gate = nullptr;
+    lora_requests(d, cu, ids, "lora_up");
+    void* stream = stream_of({&t, &w, &y, &cu, ids, scale, gate, given});
+    const Tensor out = given ? *given : make(y.sizes(), y.scalar_type(), y);
+    lora_out(d, out);
+    check(call_lora_up(&d, stream));
+    return result(a[8], out);
+  });
+}
+
+// (x, a, b, y, cu, ids, scale, epilogue, gate, out) -> out
+PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    expect(n_args, 10);
+    const Tensor &x = tensor(a[0], "lora: x"), &down = tensor(a[1], "lora: a"), &up = tensor(a[2], "lora: b"),
+                 &y = tensor(a[3], "lora: y"), &cu = tensor(a[4], "lora: cu");
+    const Tensor *ids = maybe(a[5], "lora: ids"), *scale = maybe(a[6], "lora: scale"), *gate = maybe(a[8], "lora: gate"),
+                 *given = maybe(a[9], "lora: out");
+    b2g_lora_desc d{};
+    lora_first(d, x, down, "lora");
+    if (up.dim() != 3 || up.size(0) != down.size(0) || up.scalar_type() != down.scalar_type())
+      refuse("lora: a and b must hold as many adapters, of one type");
+    lora_second(d, up, y, scale, a[7], gate, given, "lora");
+    if (!d.gate) gate = nullptr;
+    lora_requests(d, cu, ids, "lora");
+    void* stream = stream_of({&x, &down, &up, &y, &cu, ids, scale, gate, given});
+    const Tensor t = make({d.rows, d.R}, ScalarType::Float, x);
+    lora_t(d, t, "lora");
+    const Tensor out = given ? *given : make(y.sizes(), y.scalar_type(), y);
+    lora_out(d, out);
+    check(call_lora_down(&d, stream));
+    check(call_lora_up(&d, stream));
+    return result(a[9], out);
+  });
+}
+
 // (library: a ctypes-like callable that gives a symbol's address, error type)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
@@ -321,6 +582,11 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     call_attention_packed = reinterpret_cast<decltype(call_attention_packed)>(address("b2g_attention_packed"));
     call_attention_packed_workspace =
         reinterpret_cast<decltype(call_attention_packed_workspace)>(address("b2g_attention_packed_workspace"));
+    call_block_means = reinterpret_cast<decltype(call_block_means)>(address("b2g_block_means"));
+    call_select_blocks = reinterpret_cast<decltype(call_select_blocks)>(address("b2g_select_blocks"));
+    call_attention_blocks = reinterpret_cast<decltype(call_attention_blocks)>(address("b2g_attention_blocks"));
+    call_lora_down = reinterpret_cast<decltype(call_lora_down)>(address("b2g_lora_down"));
+    call_lora_up = reinterpret_cast<decltype(call_lora_up)>(address("b2g_lora_up"));
     call_last_error = reinterpret_cast<decltype(call_last_error)>(address("b2g_last_error"));
     Py_INCREF(a[1]);
     Py_XDECREF(error_type);
@@ -330,7 +596,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 #define B2G_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {B2G_METHOD(gemm_s8), B2G_METHOD(qk_norm_rope), B2G_METHOD(attention_packed), B2G_METHOD(bind),
+PyMethodDef methods[] = {B2G_METHOD(gemm_s8), B2G_METHOD(qk_norm_rope), B2G_METHOD(attention_packed), B2G_METHOD(block_means),
+                         B2G_METHOD(select_blocks), B2G_METHOD(attention_blocks), B2G_METHOD(lora_down), B2G_METHOD(lora_up),
+                         B2G_METHOD(lora), B2G_METHOD(bind),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b2g_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -495,6 +495,27 @@ b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* wor
   return attention_packed(desc, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
+b2g_status b2g_block_means(const b2g_attention_packed_desc* desc, const int32_t* since, float* means, int64_t blocks,
+                           void* stream) {
+  return block_means(desc, since, means, blocks, static_cast<cudaStream_t>(stream));
+}
+
+b2g_status b2g_select_blocks(const b2g_attention_packed_desc* desc, const float* means, int64_t blocks, int64_t top,
+                             int64_t first, int64_t last, int32_t* chosen, int64_t tiles, int64_t words, void* stream) {
+  return select_blocks(desc, means, blocks, top, first, last, chosen, tiles, words, static_cast<cudaStream_t>(stream));
+}
+
+b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int32_t* chosen, int64_t tiles, int64_t words,
+                                void* stream) {
+  return attention_blocks(desc, chosen, tiles, words, static_cast<cudaStream_t>(stream));
+}
+
+b2g_status b2g_lora_down(const b2g_lora_desc* desc, void* stream) {
+  return lora_down(desc, static_cast<cudaStream_t>(stream));
+}
+
+b2g_status b2g_lora_up(const b2g_lora_desc* desc, void* stream) { return lora_up(desc, static_cast<cudaStream_t>(stream)); }
+
 b2g_status b2g_gemm_fp8_group(const b2g_gemm_desc* descs, const float* const* a_scales,
                               const float* const* b_scales, int count, void* stream) {
   if (count < 0 || (count > 0 && (!descs || !a_scales || !b_scales)))

@@ -147,6 +147,18 @@ size_t attention_packed_workspace(const b2g_attention_packed_desc* d);
 b2g_status attention_packed(const b2g_attention_packed_desc* d, void* workspace, size_t workspace_bytes,
                             cudaStream_t st);
 
+// Attention over chosen key blocks (attention_blocks.cu); see b2g_block_means, b2g_select_blocks, b2g_attention_blocks.
+b2g_status block_means(const b2g_attention_packed_desc* d, const int32_t* since, float* means, int64_t blocks,
+                       cudaStream_t st);
+b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means, int64_t blocks, int64_t top, int64_t first,
+                         int64_t last, int32_t* chosen, int64_t tiles, int64_t words, cudaStream_t st);
+b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* chosen, int64_t tiles, int64_t words,
+                            cudaStream_t st);
+
+// Low-rank adapters (lora.cu); see b2g_lora_down and b2g_lora_up.
+b2g_status lora_down(const b2g_lora_desc* d, cudaStream_t st);
+b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st);
+
 // residual[m, n] += gate[n] * (y[m, n] + bias[n]) after a tensor-parallel all-reduce
 // (elementwise.cu); y BF16 or F32, bias may be NULL.
 b2g_status bias_gated_residual(const void* y, b2g_dtype y_dtype, int64_t ldy, const float* bias, const float* gate,

@@ -544,6 +544,63 @@ size_t b2g_attention_packed_workspace(const b2g_attention_packed_desc* desc);
 b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* workspace, size_t workspace_bytes,
                                 void* stream);
 
+/* Attention of a packed batch over key blocks that a cheap score chooses.  A sequence's keys lie in blocks
+ * of 128 from its first key on, its queries in tiles of 128 (a single query is a tile).  The three calls share
+ * b2g_attention_packed_desc: cu_k, k_lens, batch, n_kv_head, d_head (64 or 128), total_k and
+ *   b2g_block_means       k
+ *   b2g_select_blocks     q, cu_q, total_q, n_head, causal
+ *   b2g_attention_blocks  all of it
+ * with the meaning, the clamping and the alignment that they have there; other fields are not looked at.
+ *
+ * b2g_block_means: means[i] (F32 [blocks, n_kv_head, d_head], 16-byte aligned) is the mean of the keys of a block, the
+ * last one's of those it has; a sequence has a row for every block that [cu_k[b], cu_k[b+1]) has room for, sequence
+ * after sequence.  Rows of blocks without a key, and rows past the last block, are 0.  With since (device, [batch]): only
+ * the blocks that hold a key from since[b] on are written (what a step that added those keys has changed).
+ * total_k / 128 + batch rows always suffice; blocks past `blocks` are left out.
+ *
+ * b2g_select_blocks: chosen (32-bit words [tiles, n_kv_head, words]) gets bit j % 32 of word j / 32 set if the tile is
+ * to see key block j of its sequence: the `first` first and the `last` last of the blocks in its sight (up to the last key
+ * that its last query sees), every block that some of its queries see in part only (causal), and of the others the
+ * `top` with the largest (sum of the tile's queries, of all heads that share the key head) . means[block], of equal
+ * ones the first.  The scores are summed in 64 bits; NaN counts as -inf.  Sequences' tiles follow one another; rows past the
+ * last tile are 0 (total_q / 128 + batch rows always suffice).  words <= 256; blocks past 32 * words are never chosen.
+ *
+ * b2g_attention_blocks: b2g_attention_packed over the keys of the chosen blocks.  Bits of blocks out of a tile's
+ * sight are not looked at; a tile without a bit, or past `tiles`, sees nothing, and its rows are 0.  No workspace. */
+b2g_status b2g_block_means(const b2g_attention_packed_desc* desc, const int32_t* since, float* means, int64_t blocks,
+                           void* stream);
+b2g_status b2g_select_blocks(const b2g_attention_packed_desc* desc, const float* means, int64_t blocks, int64_t top,
+                             int64_t first, int64_t last, int32_t* chosen, int64_t tiles, int64_t words, void* stream);
+b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int32_t* chosen, int64_t tiles, int64_t words,
+                                void* stream);
+
+/* Low-rank adapters of the requests of a packed batch beside a projection that they share:
+ *   b2g_lora_down  t[m]   = x[m] . a[r]^T                            F32 [rows, R]
+ *   b2g_lora_up    out[m] = act(y[m] + scale[r] * t[m] . b[r]^T)     B2G_EPI_NONE, _GELU, _SILU
+ *                  out[m] = y[m] + gate * (scale[r] * t[m] . b[r]^T) B2G_EPI_GATED_RESIDUAL
+ * for the rows m of [cu[i], cu[i+1]) of request i, r = ids[i] (NULL: i).  A request whose r is not in [0, adapters) has no
+ * adapter: t = 0, out = act(y).  Rows of no request are not written.  cu and ids are device memory, read when the
+ * kernels run; offsets are clamped to the rows.  x, a [adapters, R, K] and b [adapters, N, R] are BF16 or F16, of one type, with
+ * 16-byte aligned bases and strides; y and out F32 or of that type, any N, strides and alignment (16-byte rows are
+ * faster); out may be y (same pointer and stride), and must not overlap it otherwise.  R a multiple of 8 up to 128 (an
+ * adapter of a lower rank is padded with zeros), K a multiple of 8.  One t serves several b (parts of a fused
+ * projection).  No workspace. */
+typedef struct {
+  const void* x; const void* a; const void* b; b2g_dtype dtype;
+  int64_t ldx, lda, a_stride, ldb, b_stride;          /* row strides, strides between adapters (elements) */
+  float* t; int64_t ldt;
+  const void* y; void* out; b2g_dtype y_dtype;        /* y_dtype: of both */
+  int64_t ldy, ldo;
+  int64_t rows, K, N, R, adapters, batch;
+  const int32_t* cu;                                  /* [batch + 1] */
+  const int32_t* ids;                                 /* [batch] or NULL */
+  const float* scale;                                 /* [adapters] or NULL (1) */
+  const float* gate;                                  /* [N] */
+  b2g_epilogue epilogue;
+} b2g_lora_desc;
+b2g_status b2g_lora_down(const b2g_lora_desc* desc, void* stream);
+b2g_status b2g_lora_up(const b2g_lora_desc* desc, void* stream);
+
 /* Reads and clears the device-side error word that the tensor-core kernels set when a
  * pipeline wait exceeds its time limit (they then drain and return instead of hanging).
  * Synchronises the device.  Returns B2G_OK or B2G_ERR_DEVICE_TIMEOUT; *code gets the
