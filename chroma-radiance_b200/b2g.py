@@ -217,6 +217,7 @@ _SIGNATURES = {
     "b2g_attention_blocks": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                               ctypes.c_void_p], ctypes.c_int),
     "b2g_lora_down": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
+    "b2g_lora": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
     "b2g_lora_up": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
     "b2g_check_device_error": ([ctypes.POINTER(ctypes.c_int)], ctypes.c_int),
     "b2g_launch_count": ([], ctypes.c_uint64),

@@ -35,6 +35,7 @@ decltype(&b2g_select_blocks) call_select_blocks = nullptr;
 decltype(&b2g_attention_blocks) call_attention_blocks = nullptr;
 decltype(&b2g_lora_down) call_lora_down = nullptr;
 decltype(&b2g_lora_up) call_lora_up = nullptr;
+decltype(&b2g_lora) call_lora = nullptr;
 decltype(&b2g_last_error) call_last_error = nullptr;
 PyObject* error_type = nullptr;
 
@@ -556,8 +557,7 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     lora_t(d, t, "lora");
     const Tensor out = given ? *given : make(y.sizes(), y.scalar_type(), y);
     lora_out(d, out);
-    check(call_lora_down(&d, stream));
-    check(call_lora_up(&d, stream));
+    check(call_lora(&d, stream));
     return result(a[9], out);
   });
 }
@@ -586,6 +586,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     call_select_blocks = reinterpret_cast<decltype(call_select_blocks)>(address("b2g_select_blocks"));
     call_attention_blocks = reinterpret_cast<decltype(call_attention_blocks)>(address("b2g_attention_blocks"));
     call_lora_down = reinterpret_cast<decltype(call_lora_down)>(address("b2g_lora_down"));
+    call_lora = reinterpret_cast<decltype(call_lora)>(address("b2g_lora"));
     call_lora_up = reinterpret_cast<decltype(call_lora_up)>(address("b2g_lora_up"));
     call_last_error = reinterpret_cast<decltype(call_last_error)>(address("b2g_last_error"));
     Py_INCREF(a[1]);

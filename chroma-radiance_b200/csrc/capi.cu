@@ -514,6 +514,8 @@ b2g_status b2g_lora_down(const b2g_lora_desc* desc, void* stream) {
   return lora_down(desc, static_cast<cudaStream_t>(stream));
 }
 
+b2g_status b2g_lora(const b2g_lora_desc* desc, void* stream) { return lora(desc, static_cast<cudaStream_t>(stream)); }
+
 b2g_status b2g_lora_up(const b2g_lora_desc* desc, void* stream) { return lora_up(desc, static_cast<cudaStream_t>(stream)); }
 
 b2g_status b2g_gemm_fp8_group(const b2g_gemm_desc* descs, const float* const* a_scales,

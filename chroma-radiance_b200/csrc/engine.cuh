@@ -155,9 +155,11 @@ b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means,
 b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* chosen, int64_t tiles, int64_t words,
                             cudaStream_t st);
 
-// Low-rank adapters (lora.cu); see b2g_lora_down and b2g_lora_up.
+// Low-rank adapters (lora.cu); see b2g_lora_down, b2g_lora_up and b2g_lora.  early: launched right behind
+// lora_down, before which all but t was ready.
 b2g_status lora_down(const b2g_lora_desc* d, cudaStream_t st);
-b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st);
+b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st, bool early = false);
+b2g_status lora(const b2g_lora_desc* d, cudaStream_t st);
 
 // residual[m, n] += gate[n] * (y[m, n] + bias[n]) after a tensor-parallel all-reduce
 // (elementwise.cu); y BF16 or F32, bias may be NULL.

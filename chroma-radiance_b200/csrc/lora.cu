@@ -12,7 +12,11 @@
 //
 //   lora_down_tiles  128 rows of a request: tcgen05, x and A by TMA, K shared out over a cluster
 //   lora_down_rows   few rows a request: m16n8k16 products from registers, K shared out over warps and a cluster
-//   lora_up          m16n8k16 products; t is two 16-bit numbers a value, so that its rounding is 2^-16 or less
+//   lora_up_tiles    128 rows of a request: tcgen05, y, B and out by TMA
+//   lora_up          few rows a request, and y or out that TMA cannot take: m16n8k16 products
+//
+// In the second product s t is the sum of two numbers of the operands' 16-bit type: bf16 keeps 2^-17 of a value, fp16, whose
+// range is small, 2^-22 of its row's largest, as the row is brought to [1, 2) by a power of two.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
@@ -42,6 +46,7 @@ struct LoraParams {
   int splits;              // CTAs of a cluster (lora_down)
   int stages;              // lora_down_tiles
   int slices;              // lora_up: parts of N
+  int early;               // lora_up: all but t was ready before the launch in front of it
   int in_place;            // lora_up: out is y
   int* err;
 };
@@ -214,22 +219,24 @@ __global__ void __launch_bounds__(kLdThreads)
 
 // ---------------------------------------------------------------------------- down, few rows
 //
-// 16 rows of a request, of which often one is there: what has to be read is the adapter.  A warp takes 32 values
-// of K in turn: lane (g, t) holds 16 bytes of row g (of x, of A) at k = 32 c + 8 t, words (0, 1) and (2, 3) of which are
-// the operands of two products.  kAhead chunks are loaded together.  The warps' sums meet in shared memory, a cluster's
-// in distributed shared memory, in a fixed order.
+// 16 rows of a request, of which often one is there: what has to be read is the adapter.  A CTA takes 8 NT rows of A,
+// a warp 32 values of K in turn: lane (g, t) holds 16 bytes of row g (of x, of A) at k = 32 c + 8 t, words (0, 1) and
+// (2, 3) of which are the operands of two products.  kLrAhead neighbouring chunks, 256 bytes of a row, are loaded
+// together.  The warps' sums meet in shared memory, a cluster's in distributed shared memory, in a fixed order.
 constexpr int kLrWarps = 4;
+constexpr int kLrAhead = 4;
 
-template <typename T, int NT>  // NT * 8 >= R
+template <typename T, int NT>
 __global__ void __launch_bounds__(32 * kLrWarps) lora_down_rows_kernel(const LoraParams p) {
-  constexpr int kAhead = NT <= 2 ? 4 : NT == 4 ? 2 : 1;
   constexpr int kCols = 8 * NT;
   __shared__ float sums[kLrWarps][16][kCols + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   griddep_wait();
   griddep_launch_dependents();
   const int S = p.splits, rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const LoraTile tile = lora_tile(p, static_cast<int>(blockIdx.x) / S, 16, lane);
+  const int item = static_cast<int>(blockIdx.x) / S, parts = (p.R + kCols - 1) / kCols;
+  const int r0 = item % parts * kCols, width = min(kCols, p.R - r0);  // this CTA's rows of A
+  const LoraTile tile = lora_tile(p, item / parts, 16, lane);
   if (tile.first < 0) return;  // (the whole cluster)
   const int rows = min(16, tile.end - tile.first);
   float acc[NT][4] = {};
@@ -238,22 +245,22 @@ __global__ void __launch_bounds__(32 * kLrWarps) lora_down_rows_kernel(const Lor
     const int c0 = static_cast<int>(static_cast<long long>(chunks) * rank / S);
     const int c1 = static_cast<int>(static_cast<long long>(chunks) * (rank + 1) / S);
     const T* x = static_cast<const T*>(p.x) + static_cast<long long>(tile.first + g) * p.ldx + 8 * t;
-    const T* a = static_cast<const T*>(p.a) + tile.adapter * p.as + g * p.lda + 8 * t;
+    const T* a = static_cast<const T*>(p.a) + tile.adapter * p.as + (r0 + g) * p.lda + 8 * t;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int c = c0 + warp * kAhead; c < c1; c += kLrWarps * kAhead) {
-      uint4 xr[kAhead][2], ar[kAhead][NT];
+    for (int c = c0 + warp * kLrAhead; c < c1; c += kLrWarps * kLrAhead) {
+      uint4 xr[kLrAhead][2], ar[kLrAhead][NT];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
+      for (int u = 0; u < kLrAhead; ++u) {
         const bool in = c + u < c1 && 32 * (c + u) + 8 * t < p.K;
         const int k = 32 * (c + u);
-        xr[u][0] = in && g < rows ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
-        xr[u][1] = in && g + 8 < rows ? __ldg(reinterpret_cast<const uint4*>(x + 8 * p.ldx + k)) : zero;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-          ar[u][i] = in && 8 * i < p.R ? __ldg(reinterpret_cast<const uint4*>(a + 8 * i * p.lda + k)) : zero;
+          ar[u][i] = in && 8 * i < width ? __ldg(reinterpret_cast<const uint4*>(a + 8 * i * p.lda + k)) : zero;
+        xr[u][0] = in && g < rows ? __ldg(reinterpret_cast<const uint4*>(x + k)) : zero;
+        xr[u][1] = in && g + 8 < rows ? __ldg(reinterpret_cast<const uint4*>(x + 8 * p.ldx + k)) : zero;
       }
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
+      for (int u = 0; u < kLrAhead; ++u)
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           mma_16816<T>(acc[i], xr[u][0].x, xr[u][1].x, xr[u][0].y, xr[u][1].y, ar[u][i].x, ar[u][i].y);
@@ -266,199 +273,574 @@ __global__ void __launch_bounds__(32 * kLrWarps) lora_down_rows_kernel(const Lor
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[warp][g + 8 * (j >> 1)][8 * i + 2 * t + (j & 1)] = acc[i][j];
   __syncthreads();
-  const int count = rows * p.R;
+  const int count = rows * width;
+  float* to = p.t + r0;
   for (int i = threadIdx.x; i < count; i += 32 * kLrWarps) {
-    const int m = i / p.R, c = i - m * p.R;
+    const int m = i / width, c = i - m * width;
     const float sum = (sums[0][m][c] + sums[1][m][c]) + (sums[2][m][c] + sums[3][m][c]);
-    if (S == 1) p.t[static_cast<long long>(tile.first + m) * p.ldt + c] = sum;
+    if (S == 1) to[static_cast<long long>(tile.first + m) * p.ldt + c] = sum;
     else sums[0][m][c] = sum;  // (read by this thread alone until here)
   }
   if (S == 1) return;
   cluster_sync_all();
   const uint32_t from = smem_u32(&sums[0][0][0]);
   for (int i = rank * 32 * kLrWarps + threadIdx.x; i < count; i += S * 32 * kLrWarps) {
-    const int m = i / p.R, c = i - m * p.R;
+    const int m = i / width, c = i - m * width;
     float v[8];
 #pragma unroll
     for (int s = 0; s < 8; ++s) v[s] = s < S ? ld_cluster_f1(map_to_cta(from + (m * (kCols + 1) + c) * 4, s)) : 0.f;
-    p.t[static_cast<long long>(tile.first + m) * p.ldt + c] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    to[static_cast<long long>(tile.first + m) * p.ldt + c] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
   }
   cluster_sync_all();
 }
 
-// ---------------------------------------------------------------------------- up
-//
-// A CTA of 8 warps, WM of them along rows (16 each) and 8 / WM along columns, takes one tile of rows and one part of N.
-// A lane's 8 neighbouring columns are two columns of each of four products (column 8 (c / 2) + 2 i + c % 2 of the
-// group of 32 is column c of product i), so y is read and written 16 or 32 bytes a lane; k is taken in the order in
-// which a lane's 4 values are neighbours.  s t = hi + lo in the operands' type: bf16 keeps 2^-17 of a value, fp16, whose
-// range is small, 2^-22 of the row's largest, as the row is brought to [1, 2) by a power of two.
-constexpr int kLuThreads = 256;
-constexpr int kLuCols = 256;  // columns of a part
+// ---------------------------------------------------------------------------- up: values
 
-// N values of type T at p, or where !live of any memory 0; VEC: aligned.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// 8 values of type TY, as they lie in memory.
+template <typename TY>
+struct Eight {
+  uint4 w[sizeof(TY) / 2];
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+    if constexpr (sizeof(TY) == 4) {
+      const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
     } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(p);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float2 f;
-        if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        if constexpr (std::is_same<TY, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
         else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[i]));
         v[2 * i] = f.x;
         v[2 * i + 1] = f.y;
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? static_cast<float>(p[i]) : 0.f;
   }
-}
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    if constexpr (sizeof(TY) == 4) {
+      w[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      w[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
     } else {
-      *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      w[0] = make_uint4(pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3]), pack2<TY>(v[4], v[5]), pack2<TY>(v[6], v[7]));
     }
-  } else {
+  }
+};
+
+// fp16: the power of two 2^e <= top < 2^(e + 1), e in [-126, 126], and its inverse.
+__device__ __forceinline__ float row_unit(float top, float* down) {
+  const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
+  *down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+// Two values as sums of two of type T: hi + lo.
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  const float ha = static_cast<float>(static_cast<T>(a)), hb = static_cast<float>(static_cast<T>(b));
+  *hi = pack2<T>(a, b);
+  *lo = pack2<T>(isfinite(ha) ? a - ha : 0.f, isfinite(hb) ? b - hb : 0.f);
+}
+// out of y and delta.
+template <int EPI>
+__device__ __forceinline__ float lora_out(float y, float delta, float gate) {
+  if constexpr (EPI == B2G_EPI_GATED_RESIDUAL) return fmaf(gate, delta, y);
+  y += delta;
+  if constexpr (EPI == B2G_EPI_GELU) return gelu_tanh<true>(y);
+  if constexpr (EPI == B2G_EPI_SILU) return silu_fast<true>(y);
+  return y;
+}
+// The same of 8 values, the epilogue chosen once.
+__device__ __forceinline__ void lora_out8(int epilogue, float (&v)[8], const float (&delta)[8], const float (&gate)[8]) {
+  auto all = [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = static_cast<T>(v[i]);
+    for (int x = 0; x < 8; ++x) v[x] = f(v[x], delta[x], gate[x]);
+  };
+  if (epilogue == B2G_EPI_GATED_RESIDUAL) all(lora_out<B2G_EPI_GATED_RESIDUAL>);
+  else if (epilogue == B2G_EPI_GELU) all(lora_out<B2G_EPI_GELU>);
+  else if (epilogue == B2G_EPI_SILU) all(lora_out<B2G_EPI_SILU>);
+  else all(lora_out<B2G_EPI_NONE>);
+}
+// Whether a tile's rows are left as they are: no adapter, in place, and nothing else to do.
+__device__ __forceinline__ bool lora_nothing(const LoraParams& p, const LoraTile& tile) {
+  return tile.adapter < 0 && p.in_place && (p.epilogue == B2G_EPI_NONE || p.epilogue == B2G_EPI_GATED_RESIDUAL);
+}
+
+// ---------------------------------------------------------------------------- up, many rows
+//
+// A CTA takes 128 rows and a part of N, 128 bytes of y's rows (kCols columns) at a time: y and the columns' rows of B
+// come by TMA into a ring, one thread issues the products into one of four accumulators in TMEM, and the
+// epilogue warps, a row per thread, add y in place in the ring's stage, which leaves by TMA.  Rows move in groups
+// of 32: groups past the request's end are not loaded, and one that it ends in is stored row by row.
+// A operand: hi and lo of s t, in one 128-byte row where they fit (R <= 32), else in tiles of 64 values of k.
+constexpr int kUtThreads = 192;
+constexpr int kUtRows = 128;
+constexpr int kUtAcc = 4;
+constexpr int kUtMostStages = 6;
+struct UtLayout {
+  int r16, atoms;            // k of one product, tiles of 64 values of it
+  uint32_t a_bytes, stage;   // A operand; y and B of a stage
+};
+__host__ __device__ inline UtLayout ut_layout(int R, int cols) {
+  UtLayout l;
+  l.r16 = (R + 15) / 16 * 16;
+  l.atoms = (R + 63) / 64;
+  l.a_bytes = (l.r16 <= 32 ? 1 : 2 * l.atoms) * kUtRows * 128;
+  l.stage = kUtRows * 128 + l.atoms * cols * 128;
+  return l;
+}
+
+template <typename T, typename TY, int EPI>
+__global__ void __launch_bounds__(kUtThreads)
+    lora_up_tiles_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmO,
+                         const __grid_constant__ CUtensorMap tmB, const LoraParams p) {
+  constexpr int kCols = 128 / sizeof(TY);
+  constexpr uint32_t kFmt = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kUtMostStages], empty[kUtMostStages], acc_full[kUtAcc], acc_empty[kUtAcc], a_ready, drain;
+  __shared__ uint32_t tmem_slot;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const UtLayout ly = ut_layout(p.R, kCols);
+  uint8_t* ring = smem + ly.a_bytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int at_tile = static_cast<int>(blockIdx.x) / p.slices, slice = static_cast<int>(blockIdx.x) - at_tile * p.slices;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    for (int i = 0; i < kUtAcc; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    mbar_init(&a_ready, 4);
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmY);
+    tma_prefetch_desc(&tmO);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 5) {
+    tmem_alloc(&tmem_slot, kUtAcc * kCols);
+    tmem_relinquish();
+  }
+  if (!p.early) griddep_wait();
+  griddep_launch_dependents();
+  const LoraTile tile = lora_tile(p, at_tile, kUtRows, lane);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const bool has = tile.adapter >= 0;
+  const int rows = tile.first < 0 || lora_nothing(p, tile) ? 0 : min(kUtRows, tile.end - tile.first);
+  const int groups = (rows + 31) / 32;
+  const int chunks = (p.N + kCols - 1) / kCols;
+  const int c0 = static_cast<int>(static_cast<long long>(chunks) * slice / p.slices);
+  const int n = rows > 0 ? static_cast<int>(static_cast<long long>(chunks) * (slice + 1) / p.slices) - c0 : 0;
+  if (warp == 4) {
+    if (lane == 0) {
+      const uint64_t once = policy_evict_first(), shared = policy_evict_last();
+      const uint32_t bytes = groups * 4096u + (has ? ly.atoms * kCols * 128u : 0u);
+      int stage = 0, used = 0;
+      uint32_t parity = 0;
+      for (int i = 0; i < n; ++i) {
+        if (!mbar_wait_short(&empty[stage], parity ^ 1u, p.err, kErrWaitProducer)) break;
+        uint8_t* at = ring + stage * ly.stage;
+        const int col = (c0 + i) * kCols;
+        mbar_arrive_expect_tx(&full[stage], bytes);
+        for (int w = 0; w < groups; ++w) tma_load_3d(at + w * 4096, &tmY, &full[stage], col, tile.first + 32 * w, 0, once);
+        if (has)
+          for (int a = 0; a < ly.atoms; ++a)
+            tma_load_3d(at + kUtRows * 128 + a * kCols * 128, &tmB, &full[stage], a * 64, col, tile.adapter, shared);
+        ++used;
+        if (++stage == p.stages) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+      // This thread's copies land before the shared memory goes away.
+      for (int i = min(used, p.stages); i > 0; --i) {
+        if (stage-- == 0) {
+          stage = p.stages - 1;
+          parity ^= 1u;
+        }
+        mbar_wait_drain(&full[stage], parity);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0 && has && n > 0) {
+      const uint32_t idesc = idesc_make(kFmt, kUtRows, kCols);
+      const uint32_t a_hi = smem_u32(smem);
+      bool ok = mbar_wait_short(&a_ready, 0, p.err, kErrWaitMma);
+      int stage = 0, acc = 0;
+      uint32_t parity = 0, acc_parity = 0;
+      for (int i = 0; i < n && ok; ++i) {
+        ok = mbar_wait_short(&acc_empty[acc], acc_parity ^ 1u, p.err, kErrWaitMma) &&
+             mbar_wait_short(&full[stage], parity, p.err, kErrWaitMma);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t b0 = smem_u32(ring + stage * ly.stage) + kUtRows * 128;
+        for (int k = 0; k < ly.r16; k += 16) {
+          const uint32_t at = (k >> 6) * (kUtRows * 128) + (k & 63) * 2;
+          const uint64_t b = smem_desc_k_sw128(b0 + (k >> 6) * (kCols * 128) + (k & 63) * 2);
+          const uint32_t lo = ly.r16 <= 32 ? (ly.r16 + k) * 2 : at + ly.atoms * (kUtRows * 128);
+          umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + at), b, idesc, k != 0 ? 1u : 0u);
+          umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + lo), b, idesc, 1u);
+        }
+        umma_commit(&acc_full[acc]);
+        if (++acc == kUtAcc) {
+          acc = 0;
+          acc_parity ^= 1u;
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          parity ^= 1u;
+        }
+      }
+      if (!ok) {  // products already issued are complete before TMEM and the ring go away
+        umma_commit(&drain);
+        mbar_wait_drain(&drain, 0);
+      }
+    }
+  } else if (n > 0) {
+    if (p.early) griddep_wait();  // t
+    const int row = warp * 32 + lane, live = min(max(rows - warp * 32, 0), 32);  // rows of this warp
+    float unit = 1.f;
+    if (has) {
+      const float* t = p.t + static_cast<long long>(tile.first + row) * p.ldt;
+      float s = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
+      if constexpr (std::is_same<T, __half>::value) {
+        float top = 0.f;
+        if (row < rows)
+          for (int k = 0; k < p.R; k += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(t + k);
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(f.x * s), fabsf(f.y * s))), fmaxf(fabsf(f.z * s), fabsf(f.w * s)));
+          }
+        float down;
+        unit = row_unit(top, &down);
+        s *= down;
+      }
+#pragma unroll 2
+      for (int k = 0; k < ly.r16; k += 8) {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
+        if (row < rows && k < p.R) {
+          f = *reinterpret_cast<const float4*>(t + k);
+          g = *reinterpret_cast<const float4*>(t + k + 4);
+        }
+        uint32_t hi[4], lo[4];
+        split2<T>(f.x * s, f.y * s, &hi[0], &lo[0]);
+        split2<T>(f.z * s, f.w * s, &hi[1], &lo[1]);
+        split2<T>(g.x * s, g.y * s, &hi[2], &lo[2]);
+        split2<T>(g.z * s, g.w * s, &hi[3], &lo[3]);
+        // 16-byte pieces of a 128-byte row are swizzled by the row.
+        auto put = [&](uint32_t tile_at, int kk, const uint32_t(&v)[4]) {
+          *reinterpret_cast<uint4*>(smem + tile_at + row * 128 + (((kk >> 3) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        };
+        const uint32_t atom = (k >> 6) * (kUtRows * 128);
+        put(atom, k & 63, hi);
+        if (ly.r16 <= 32) put(0, ly.r16 + k, lo);
+        else put(atom + ly.atoms * (kUtRows * 128), k & 63, lo);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_ready);
+    }
+    int stage = 0, acc = 0, last = -1;
+    uint32_t parity = 0, acc_parity = 0;
+    for (int i = 0; i < n; ++i) {
+      bool ok = mbar_wait_short(&full[stage], parity, p.err, kErrWaitEpilogue);
+      if (has) ok = ok && mbar_wait_short(&acc_full[acc], acc_parity, p.err, kErrWaitEpilogue);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const int col = (c0 + i) * kCols;
+      uint8_t* mine = ring + stage * ly.stage + row * 128;
+#pragma unroll
+      for (int h = 0; h < kCols / 32; ++h) {
+        uint32_t d[32];
+        if (has) {
+          tmem_ld_32x32b_x32(tmem + acc * kCols + (static_cast<uint32_t>(warp * 32) << 16) + h * 32, d);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) d[x] = 0u;
+        }
+        if (live > 0) {
+#pragma unroll
+          for (int x0 = 0; x0 < 32; x0 += 8) {  // 8 columns: 16 or 32 bytes of y
+            constexpr int kWords = sizeof(TY) / 2;
+            Eight<TY> y;
+            uint4* at[kWords];
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              at[w] = reinterpret_cast<uint4*>(mine + ((((h * 32 + x0) * static_cast<int>(sizeof(TY)) / 16 + w) ^ (row & 7)) << 4));
+              y.w[w] = *at[w];
+            }
+            float v[8];
+            y.values(v);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              float delta = __uint_as_float(d[x0 + x]), gate = 0.f;
+              if constexpr (std::is_same<T, __half>::value) delta *= unit;
+              const int c = col + h * 32 + x0 + x;
+              if (EPI == B2G_EPI_GATED_RESIDUAL && has) gate = c < p.N ? __ldg(p.gate + c) : 0.f;
+              v[x] = lora_out<EPI>(v[x], delta, gate);
+            }
+            y.set(v);
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) *at[w] = y.w[w];
+          }
+        }
+      }
+      tc_fence_before();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && has) mbar_arrive(&acc_empty[acc]);
+      if (live == 32) {
+        if (lane == 0) tma_store_3d(&tmO, ring + stage * ly.stage + warp * 4096, col, tile.first + warp * 32, 0);
+      } else if (live > 0) {  // the request's last rows, 16 bytes a lane
+        constexpr int kPiece = 16 / sizeof(TY);
+        const int c = col + (lane & 7) * kPiece;
+        for (int r = lane >> 3; r < live; r += 4) {
+          const uint8_t* from = ring + stage * ly.stage + (warp * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4);
+          TY* to = static_cast<TY*>(p.out) + static_cast<long long>(tile.first + warp * 32 + r) * p.ldo + c;
+          if (c + kPiece <= p.N) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+          else
+            for (int x = 0; x < kPiece && c + x < p.N; ++x) to[x] = reinterpret_cast<const TY*>(from)[x];
+        }
+        __syncwarp();
+      }
+      if (lane == 0) {
+        // The stage before this one goes back once its store has read it.
+        bulk_commit_group();
+        bulk_wait_group_read<1>();
+        if (last >= 0) mbar_arrive(&empty[last]);
+      }
+      last = stage;
+      if (++acc == kUtAcc) {
+        acc = 0;
+        acc_parity ^= 1u;
+      }
+      if (++stage == p.stages) {
+        stage = 0;
+        parity ^= 1u;
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();
+  }
+  __syncwarp();
+  if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kUtAcc * kCols);
   }
 }
 
-template <typename T, typename TY, int KC, int WM, bool VEC>
+// ---------------------------------------------------------------------------- up, few rows, any alignment
+//
+// A CTA of 8 warps, WM of them along rows (16 each) and 8 / WM along columns, takes one tile of rows and a part of N.
+// k is taken as in lora_down_rows: lane (g, t) holds 8 neighbouring values of a row, 16 bytes of B.  Of y a lane has 8
+// neighbouring columns, two of each of four products (column 8 (c / 2) + 2 i + c % 2 of the group of 32 is column c of
+// product i).  Where rows are 16-byte aligned (VEC) it reads and writes them itself; else a warp's 16 rows x 64
+// columns pass through shared memory, so that a warp's loads and stores are of neighbouring values of one row.
+// Several warps along rows share B in shared memory; one warp loads its own, kBatch groups of 32 columns at a time.
+constexpr int kLuThreads = 256;
+// Steps of 32 columns that a warp takes together; columns of a CTA's part.
+template <int KK, bool VEC>
+constexpr int kLuBatch = !VEC ? 2 : KK >= 4 ? 1 : 2;
+template <int KK, int WM, bool VEC>
+constexpr int kLuCols = WM == 1 ? 8 * 32 * kLuBatch<KK, VEC> : 256;
+template <typename TY>
+constexpr int kLuPitch = 64 + 16 / sizeof(TY);  // values from row to row in shared memory
+template <typename TY, int KK, int WM, bool VEC>
+constexpr size_t kLuSmem = (WM > 1 ? kLuCols<KK, WM, VEC> / 8 * KK * 32 * sizeof(uint4) : 0) + (VEC ? 0 : 8 * 16 * kLuPitch<TY> * sizeof(TY));
+
+template <typename T, typename TY, int KK, int WM, bool VEC>  // 32 KK >= R
 __global__ void __launch_bounds__(kLuThreads) lora_up_kernel(const LoraParams p) {
   constexpr int WN = 8 / WM;
-  constexpr bool kStaged = WM > 1;  // B passes through shared memory where several warps use it
-  extern __shared__ uint2 sb[];     // [column group of 8][KC][lane]
+  constexpr bool kStaged = WM > 1;
+  constexpr int kBatch = kLuBatch<KK, VEC>, kCols = kLuCols<KK, WM, VEC>;
+  static_assert(kCols / 32 % (WN * kBatch) == 0, "whole steps");
+  extern __shared__ __align__(16) uint8_t smem_up[];
+  uint4* sb = reinterpret_cast<uint4*>(smem_up);  // [column group of 8][KK][lane]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  TY* sy = reinterpret_cast<TY*>(smem_up + (kStaged ? kCols / 8 * KK * 32 * sizeof(uint4) : 0)) + warp * 16 * kLuPitch<TY>;
   const int wm = warp % WM, wn = warp / WM;
   const int at_tile = static_cast<int>(blockIdx.x / p.slices), slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(at_tile) * p.slices);
-  griddep_wait();
+  if (!p.early) griddep_wait();
   griddep_launch_dependents();
   const LoraTile tile = lora_tile(p, at_tile, 16 * WM, lane);
-  if (tile.first < 0) return;
+  if (tile.first < 0 || lora_nothing(p, tile)) {
+    if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
+    return;
+  }
   const bool has = tile.adapter >= 0;
-  if (!has && p.in_place && (p.epilogue == B2G_EPI_NONE || p.epilogue == B2G_EPI_GATED_RESIDUAL)) return;
-  const int n0 = slice * kLuCols, n1 = min(p.N, n0 + kLuCols);
+  const int n0 = slice * kCols, n1 = min(p.N, n0 + kCols);
   const T* b = static_cast<const T*>(p.b) + (has ? tile.adapter : 0) * p.bs;
-  // Operand B of product i of column group j: 4 values of k at 16 kc + 4 t of the column that lane g stands for.
-  auto load_b = [&](int group, int kc, int ln) {
-    const int gg = ln >> 2, col = n0 + (group >> 2) * 32 + 8 * (gg >> 1) + 2 * (group & 3) + (gg & 1), k = 16 * kc + 4 * (ln & 3);
-    if (col >= n1 || k >= p.R) return make_uint2(0, 0);
-    return __ldg(reinterpret_cast<const uint2*>(b + col * p.ldb + k));
+  // 8 values of k of the column that lane ln stands for in product `group`.
+  auto load_b = [&](int group, int kk, int ln) {
+    const int gg = ln >> 2, col = n0 + (group >> 2) * 32 + 8 * (gg >> 1) + 2 * (group & 3) + (gg & 1), k = 32 * kk + 8 * (ln & 3);
+    if (!has || col >= n1 || k >= p.R) return make_uint4(0, 0, 0, 0);
+    return __ldg(reinterpret_cast<const uint4*>(b + col * p.ldb + k));
   };
   if (kStaged && has)
-    for (int i = threadIdx.x; i < kLuCols / 8 * KC * 32; i += kLuThreads) sb[i] = load_b(i / (32 * KC), i / 32 % KC, i & 31);
-  const int row[2] = {tile.first + 16 * wm + g, tile.first + 16 * wm + g + 8};
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kCols / 8 * KK * 32; i += kLuThreads) sb[i] = load_b(i / (32 * KK), i / 32 % KK, i & 31);
+  const int first = tile.first + 16 * wm, row[2] = {first + g, first + g + 8};
   const bool in[2] = {row[0] < tile.end, row[1] < tile.end};
-  uint32_t hi[KC][4], lo[KC][4];
+  const int rows = min(16, tile.end - first);
+  uint32_t hi[KK][2][4], lo[KK][2][4];  // [k / 32][row][pair of k]
   float unit[2] = {1.f, 1.f};
-  {
+  auto load_t = [&]() {
+    if (p.early) griddep_wait();
     const float s = has ? (p.scale ? __ldg(p.scale + tile.adapter) : 1.f) : 0.f;
-    float v[2][KC][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float top = 0.f;
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        const int k = 16 * kc + 4 * t;
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (has && in[i] && k < p.R) f = *reinterpret_cast<const float4*>(p.t + row[i] * p.ldt + k);
-        v[i][kc][0] = f.x * s;
-        v[i][kc][1] = f.y * s;
-        v[i][kc][2] = f.z * s;
-        v[i][kc][3] = f.w * s;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[i][kc][e]));
-      }
-      if constexpr (std::is_same<T, __half>::value) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^e <= top < 2^(e + 1), e in [-126, 126]
-        const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        unit[i] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) v[i][kc][x] *= down;
-      }
-#pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        float rest[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float f = v[i][kc][x];
-          const float h = static_cast<float>(static_cast<T>(f));
-          rest[x] = isfinite(h) ? f - h : 0.f;
-        }
-        hi[kc][i] = pack2<T>(v[i][kc][0], v[i][kc][1]);
-        hi[kc][2 + i] = pack2<T>(v[i][kc][2], v[i][kc][3]);
-        lo[kc][i] = pack2<T>(rest[0], rest[1]);
-        lo[kc][2 + i] = pack2<T>(rest[2], rest[3]);
-      }
-    }
-  }
-  if (kStaged) __syncthreads();
-  for (int j = wn; j < kLuCols / 32; j += WN) {
-    const int col = n0 + 32 * j + 8 * t, left = n1 - col;
-    if (n0 + 32 * j >= n1) break;
-    float v[2][8];
+    float v[2][KK][8];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (in[i] && left > 0) load8<TY, VEC>(v[i], static_cast<const TY*>(p.y) + row[i] * p.ldy + col, left);
-    float acc[4][4] = {};
-    if (has) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int k = 32 * kk + 8 * t;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f), h = f;
+        if (has && in[i] && k < p.R) {
+          f = *reinterpret_cast<const float4*>(p.t + row[i] * p.ldt + k);
+          h = *reinterpret_cast<const float4*>(p.t + row[i] * p.ldt + k + 4);
+        }
+        v[i][kk][0] = f.x * s; v[i][kk][1] = f.y * s; v[i][kk][2] = f.z * s; v[i][kk][3] = f.w * s;
+        v[i][kk][4] = h.x * s; v[i][kk][5] = h.y * s; v[i][kk][6] = h.z * s; v[i][kk][7] = h.w * s;
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float down = 1.f;
+      if constexpr (std::is_same<T, __half>::value) {
+        float top = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+          for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(v[i][kk][x]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        unit[i] = row_unit(top, &down);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) split2<T>(v[i][kk][2 * x] * down, v[i][kk][2 * x + 1] * down, &hi[kk][i][x], &lo[kk][i][x]);
+    }
+  };
+  bool loaded = false;
+  for (int j0 = wn * kBatch; j0 < kCols / 32; j0 += WN * kBatch) {
+    if (n0 + 32 * j0 >= n1) break;
+    Eight<TY> y[kBatch][2];
+    uint4 w[kStaged ? 1 : kBatch][4][KK];
+    if (!kStaged) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) w[j][i][kk] = load_b(4 * (j0 + j) + i, kk, lane);
+    }
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int col = n0 + 32 * (j0 + j) + 8 * t;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
+            if (in[i] && col < n1) y[j][i].w[x] = *(reinterpret_cast<const uint4*>(static_cast<const TY*>(p.y) + row[i] * p.ldy + col) + x);
+      }
+    } else {
+      const int col = n0 + 32 * j0 + lane;
+      const TY* from = static_cast<const TY*>(p.y) + first * p.ldy + col;
+      TY raw[16][2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (r < rows && col + 32 * x < n1) raw[r][x] = from[r * p.ldy + 32 * x];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (r < rows && col + 32 * x < n1) sy[r * kLuPitch<TY> + lane + 32 * x] = raw[r][x];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
+            y[j][i].w[x] = *(reinterpret_cast<const uint4*>(sy + (g + 8 * i) * kLuPitch<TY> + 32 * j + 8 * t) + x);
+    }
+    if (!loaded) {
+      load_t();
+      if (kStaged) __syncthreads();
+      loaded = true;
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      float acc[4][4] = {};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          const uint2 w = kStaged ? sb[((4 * j + i) * KC + kc) * 32 + lane] : load_b(4 * j + i, kc, lane);
-          mma_16816<T>(acc[i], hi[kc][0], hi[kc][1], hi[kc][2], hi[kc][3], w.x, w.y);
-          mma_16816<T>(acc[i], lo[kc][0], lo[kc][1], lo[kc][2], lo[kc][3], w.x, w.y);
+        for (int kk = 0; kk < KK; ++kk) {
+          const uint4 u = kStaged ? sb[((4 * (j0 + j) + i) * KK + kk) * 32 + lane] : w[kStaged ? 0 : j][i][kk];
+          const uint32_t(&h)[2][4] = hi[kk];
+          const uint32_t(&l)[2][4] = lo[kk];
+          mma_16816<T>(acc[i], h[0][0], h[1][0], h[0][1], h[1][1], u.x, u.y);
+          mma_16816<T>(acc[i], h[0][2], h[1][2], h[0][3], h[1][3], u.z, u.w);
+          mma_16816<T>(acc[i], l[0][0], l[1][0], l[0][1], l[1][1], u.x, u.y);
+          mma_16816<T>(acc[i], l[0][2], l[1][2], l[0][3], l[1][3], u.z, u.w);
         }
-    }
-    if (left <= 0) continue;
-    float gate[8];
-    if (p.epilogue == B2G_EPI_GATED_RESIDUAL) {
+      const int col = n0 + 32 * (j0 + j) + 8 * t;
+      float gate[8];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) gate[x] = x < left ? __ldg(p.gate + col + x) : 0.f;
-    }
+      for (int x = 0; x < 8; ++x)
+        gate[x] = p.epilogue == B2G_EPI_GATED_RESIDUAL && has && col + x < n1 ? __ldg(p.gate + col + x) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (!in[i]) continue;
+      for (int i = 0; i < 2; ++i) {
+        float v[8], delta[8];
+        y[j][i].values(v);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {  // column 2 t + e of product x / 2
-        float delta = acc[x >> 1][2 * i + (x & 1)];
-        if constexpr (std::is_same<T, __half>::value) delta *= unit[i];
-        if (p.epilogue == B2G_EPI_GATED_RESIDUAL) v[i][x] = has ? fmaf(gate[x], delta, v[i][x]) : v[i][x];
-        else {
-          v[i][x] += delta;
-          if (p.epilogue == B2G_EPI_GELU) v[i][x] = gelu_tanh<true>(v[i][x]);
-          else if (p.epilogue == B2G_EPI_SILU) v[i][x] = silu_fast<true>(v[i][x]);
+        for (int x = 0; x < 8; ++x) {  // column 2 t + e of product x / 2
+          delta[x] = has ? acc[x >> 1][2 * i + (x & 1)] : 0.f;
+          if constexpr (std::is_same<T, __half>::value) delta[x] *= unit[i];
+        }
+        lora_out8(p.epilogue, v, delta, gate);
+        y[j][i].set(v);
+        if constexpr (VEC) {
+#pragma unroll
+          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
+            if (in[i] && col < n1) *(reinterpret_cast<uint4*>(static_cast<TY*>(p.out) + row[i] * p.ldo + col) + x) = y[j][i].w[x];
+        } else {
+#pragma unroll
+          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
+            *(reinterpret_cast<uint4*>(sy + (g + 8 * i) * kLuPitch<TY> + 32 * j + 8 * t) + x) = y[j][i].w[x];
         }
       }
-      store8<TY, VEC>(static_cast<TY*>(p.out) + row[i] * p.ldo + col, v[i], left);
     }
+    if constexpr (!VEC) {
+      __syncwarp();
+      const int col = n0 + 32 * j0 + lane;
+      TY* to = static_cast<TY*>(p.out) + first * p.ldo + col;
+      for (int r = 0; r < rows; ++r)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (col + 32 * x < n1) to[r * p.ldo + 32 * x] = sy[r * kLuPitch<TY> + lane + 32 * x];
+      __syncwarp();
+    }
+  }
+  if (!loaded) {  // (a warp without columns)
+    if (p.early) griddep_wait();
+    if (kStaged) __syncthreads();
   }
 }
 
 // ---------------------------------------------------------------------------- host side
 
-// Average rows of a request up to which the few-rows forms take a call; up's middle form, of 32-row tiles.
-constexpr int64_t kLoraFewRows = 16, kLoraMiddleRows = 64;
+// Average rows of a request up to which the few-rows forms take a call.
+constexpr int64_t kLoraFewRows = 16;
 
 b2g_status lora_launch_cluster(const void* kern, int64_t tiles, int64_t S, int threads, size_t smem, cudaStream_t st,
                                const char* what, void** args) {
@@ -483,19 +865,17 @@ b2g_status lora_launch_cluster(const void* kern, int64_t tiles, int64_t S, int t
 template <typename T>
 b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t st) {
   if (d->rows <= kLoraFewRows * d->batch || d->adapters == 0) {  // (without adapters there is nothing to load)
-    const int64_t tiles = d->rows / 16 + d->batch;
-    // Two CTAs an SM; a warp's part of K is at least one step of its loads.
-    int64_t S = 4ll * sms / tiles;
-    const int64_t most = (d->K + 32 * kLrWarps - 1) / (32 * kLrWarps);
+    const int NT = p.R <= 8 ? 1 : 2;
+    const int64_t items = (d->rows / 16 + d->batch) * ((p.R + 8 * NT - 1) / (8 * NT));
+    // Four CTAs an SM; a warp's part of K is at least one step of its loads.
+    int64_t S = 4ll * sms / items;
+    const int64_t most = (d->K + 32 * kLrAhead * kLrWarps - 1) / (32 * kLrAhead * kLrWarps);
     S = S > most ? most : S;
     p.splits = static_cast<int>(S < 1 ? 1 : S > 8 ? 8 : S);
-    const void* kern = p.R <= 8 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 1>)
-                       : p.R <= 16 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 2>)
-                       : p.R <= 32 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 4>)
-                       : p.R <= 64 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 8>)
-                                   : reinterpret_cast<const void*>(lora_down_rows_kernel<T, 16>);
+    const void* kern = NT == 1 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 1>)
+                               : reinterpret_cast<const void*>(lora_down_rows_kernel<T, 2>);
     void* args[] = {&p};
-    return lora_launch_cluster(kern, tiles, p.splits, 32 * kLrWarps, 0, st, "lora_down_rows launch", args);
+    return lora_launch_cluster(kern, items, p.splits, 32 * kLrWarps, 0, st, "lora_down_rows launch", args);
   }
   const int Rp = (p.R + 15) & ~15;
   CUtensorMap tx, ta;
@@ -517,34 +897,59 @@ b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t
   return lora_launch_cluster(reinterpret_cast<const void*>(kern), tiles, p.splits, kLdThreads, smem, st, "lora_down_tiles launch", args);
 }
 
-template <typename T, typename TY, int KC, int WM, bool VEC>
-b2g_status launch_up(const LoraParams& p, int64_t tiles, cudaStream_t st) {
-  constexpr size_t smem = WM > 1 ? kLuCols / 8 * KC * 32 * sizeof(uint2) : 0;
-  auto kern = lora_up_kernel<T, TY, KC, WM, VEC>;
+template <typename T, typename TY, int KK, int WM, bool VEC>
+b2g_status launch_up(LoraParams& p, cudaStream_t st) {
+  constexpr size_t smem = kLuSmem<TY, KK, WM, VEC>;
+  auto kern = lora_up_kernel<T, TY, KK, WM, VEC>;
   if constexpr (smem > 48 * 1024) {
     b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                               "cudaFuncSetAttribute(lora_up)");
     if (s != B2G_OK) return s;
   }
+  p.slices = (p.N + kLuCols<KK, WM, VEC> - 1) / kLuCols<KK, WM, VEC>;
+  const int64_t tiles = static_cast<int64_t>(p.rows) / (16 * WM) + p.batch;
   return launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.slices)), dim3(kLuThreads), smem, st, "lora_up launch", p);
 }
-template <typename T, typename TY, int KC, int WM>
-b2g_status launch_up(const LoraParams& p, bool vec, int64_t tiles, cudaStream_t st) {
-  return vec ? launch_up<T, TY, KC, WM, true>(p, tiles, st) : launch_up<T, TY, KC, WM, false>(p, tiles, st);
-}
-template <typename T, typename TY, int KC>
-b2g_status launch_up(const LoraParams& p, bool vec, cudaStream_t st) {
-  const int64_t batch = p.batch, rows = p.rows;
-  if (rows <= kLoraFewRows * batch) return launch_up<T, TY, KC, 1>(p, vec, rows / 16 + batch, st);
-  if (rows <= kLoraMiddleRows * batch) return launch_up<T, TY, KC, 2>(p, vec, rows / 32 + batch, st);
-  return launch_up<T, TY, KC, 8>(p, vec, rows / 128 + batch, st);
+template <typename T, typename TY, int WM, bool VEC>
+b2g_status launch_up(LoraParams& p, cudaStream_t st) {
+  if (p.R <= 32) return launch_up<T, TY, 1, WM, VEC>(p, st);
+  if (p.R <= 64) return launch_up<T, TY, 2, WM, VEC>(p, st);
+  return launch_up<T, TY, 4, WM, VEC>(p, st);
 }
 template <typename T, typename TY>
-b2g_status launch_up(const LoraParams& p, bool vec, cudaStream_t st) {
-  if (p.R <= 16) return launch_up<T, TY, 1>(p, vec, st);
-  if (p.R <= 32) return launch_up<T, TY, 2>(p, vec, st);
-  if (p.R <= 64) return launch_up<T, TY, 4>(p, vec, st);
-  return launch_up<T, TY, 8>(p, vec, st);
+b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cudaStream_t st) {
+  const bool few = d->rows <= kLoraFewRows * d->batch;
+  if (few) return vec ? launch_up<T, TY, 1, true>(p, st) : launch_up<T, TY, 1, false>(p, st);
+  // TMA: 16-byte aligned rows, whatever their width.
+  const int64_t esz = sizeof(TY);
+  const bool tma = (p.ldy * esz) % 16 == 0 && (p.ldo * esz) % 16 == 0 && p.adapters > 0 &&
+                   ((reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0;
+  if (!tma) return launch_up<T, TY, 8, false>(p, st);
+  constexpr int kCols = 128 / sizeof(TY);
+  CUtensorMap ty, to, tb;
+  b2g_status s;
+  if ((s = make_operand_map(&ty, p.y, d->y_dtype, p.N, p.rows, p.ldy, 1, p.ldy * p.rows, 32)) != B2G_OK) return s;
+  if ((s = make_operand_map(&to, p.out, d->y_dtype, p.N, p.rows, p.ldo, 1, p.ldo * p.rows, 32)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tb, p.b, d->dtype, p.R, p.N, p.ldb, p.adapters, p.bs, kCols)) != B2G_OK) return s;
+  const UtLayout ly = ut_layout(p.R, kCols);
+  // Two CTAs an SM where four stages fit beside the A operand, else one.
+  const int two = static_cast<int>((111 * 1024 - ly.a_bytes) / ly.stage), one = static_cast<int>((225 * 1024 - ly.a_bytes) / ly.stage);
+  p.stages = two >= 3 ? two : one;
+  if (p.stages > kUtMostStages) p.stages = kUtMostStages;
+  const int64_t tiles = static_cast<int64_t>(p.rows) / kUtRows + p.batch, chunks = (p.N + kCols - 1) / kCols;
+  // Some four rounds of CTAs, of four steps or more each.
+  int64_t slices = (8ll * sms + tiles - 1) / tiles;
+  if (slices > chunks / 4) slices = chunks / 4;
+  p.slices = static_cast<int>(slices < 1 ? 1 : slices);
+  auto kern = p.epilogue == B2G_EPI_GATED_RESIDUAL ? lora_up_tiles_kernel<T, TY, B2G_EPI_GATED_RESIDUAL>
+              : p.epilogue == B2G_EPI_GELU           ? lora_up_tiles_kernel<T, TY, B2G_EPI_GELU>
+              : p.epilogue == B2G_EPI_SILU           ? lora_up_tiles_kernel<T, TY, B2G_EPI_SILU>
+                                                     : lora_up_tiles_kernel<T, TY, B2G_EPI_NONE>;
+  if ((s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024),
+                      "cudaFuncSetAttribute(lora_up_tiles)")) != B2G_OK)
+    return s;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.slices)), dim3(kUtThreads), 1024 + ly.a_bytes + p.stages * ly.stage, st,
+                    "lora_up_tiles launch", ty, to, tb, p);
 }
 
 // The checks of both halves, and the parameters.
@@ -614,21 +1019,32 @@ b2g_status lora_down(const b2g_lora_desc* d, cudaStream_t st) {
   return run_down<__nv_bfloat16>(d, p, dev->num_sms, st);
 }
 
-b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st) {
+b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st, bool early) {
   LoraParams p{};
   b2g_status s = lora_params(d, "b2g_lora_up", false, &p);
   if (s != B2G_OK || p.rows == 0) return s;
-  p.slices = (p.N + kLuCols - 1) / kLuCols;
-  if ((static_cast<int64_t>(p.rows) / 16 + p.batch) * p.slices > (1ll << 31) - 1) return set_error(B2G_ERR_UNSUPPORTED, "b2g_lora_up: size");
+  if ((static_cast<int64_t>(p.rows) / 16 + p.batch) * ((p.N + 31) / 32) > (1ll << 31) - 1)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_lora_up: size");
   DeviceInfo* dev = nullptr;
   if ((s = device_info(&dev)) != B2G_OK) return s;
+  p.err = dev->err_word;
+  p.early = early ? 1 : 0;
   const int64_t esz = d->y_dtype == B2G_F32 ? 4 : 2;
   const bool vec = p.N % 8 == 0 && (p.ldy * esz) % 16 == 0 && (p.ldo * esz) % 16 == 0 &&
                    ((reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0;
   p.in_place = p.y == p.out && p.ldy == p.ldo;
+  const int sms = dev->num_sms;
   if (d->dtype == B2G_F16)
-    return d->y_dtype == B2G_F32 ? launch_up<__half, float>(p, vec, st) : launch_up<__half, __half>(p, vec, st);
-  return d->y_dtype == B2G_F32 ? launch_up<__nv_bfloat16, float>(p, vec, st) : launch_up<__nv_bfloat16, __nv_bfloat16>(p, vec, st);
+    return d->y_dtype == B2G_F32 ? run_up<__half, float>(d, p, vec, sms, st) : run_up<__half, __half>(d, p, vec, sms, st);
+  return d->y_dtype == B2G_F32 ? run_up<__nv_bfloat16, float>(d, p, vec, sms, st)
+                               : run_up<__nv_bfloat16, __nv_bfloat16>(d, p, vec, sms, st);
+}
+
+b2g_status lora(const b2g_lora_desc* d, cudaStream_t st) {
+  LoraParams p{};
+  b2g_status s = lora_params(d, "b2g_lora", false, &p);  // (both halves are checked before one runs)
+  if (s != B2G_OK || (s = lora_down(d, st)) != B2G_OK) return s;
+  return lora_up(d, st, true);
 }
 
 }  // namespace b2g

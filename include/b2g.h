@@ -600,6 +600,8 @@ typedef struct {
 } b2g_lora_desc;
 b2g_status b2g_lora_down(const b2g_lora_desc* desc, void* stream);
 b2g_status b2g_lora_up(const b2g_lora_desc* desc, void* stream);
+/* Both, t being room for the result between them. */
+b2g_status b2g_lora(const b2g_lora_desc* desc, void* stream);
 
 /* Reads and clears the device-side error word that the tensor-core kernels set when a
  * pipeline wait exceeds its time limit (they then drain and return instead of hanging).
