@@ -372,10 +372,11 @@ __device__ __forceinline__ bool lora_nothing(const LoraParams& p, const LoraTile
 // epilogue warps, a row per thread, add y in place in the ring's stage, which leaves by TMA.  Rows move in groups
 // of 32: groups past the request's end are not loaded, and one that it ends in is stored row by row.
 // A operand: hi and lo of s t, in one 128-byte row where they fit (R <= 32), else in tiles of 64 values of k.
-constexpr int kUtThreads = 192;
+constexpr int kUtThreads = 320;  // two sets of four epilogue warps, loads, products
 constexpr int kUtRows = 128;
 constexpr int kUtAcc = 4;
 constexpr int kUtMostStages = 6;
+constexpr int kUtOnce = 4;
 struct UtLayout {
   int r16, atoms;            // k of one product, tiles of 64 values of it
   uint32_t a_bytes, stage;   // A operand; y and B of a stage
@@ -412,14 +413,14 @@ __global__ void __launch_bounds__(kUtThreads)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 4);
     }
-    mbar_init(&a_ready, 4);
+    mbar_init(&a_ready, 8);
     mbar_init(&drain, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmY);
     tma_prefetch_desc(&tmO);
     tma_prefetch_desc(&tmB);
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tmem_alloc(&tmem_slot, kUtAcc * kCols);
     tmem_relinquish();
   }
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kUtThreads)
   const int chunks = (p.N + kCols - 1) / kCols;
   const int c0 = static_cast<int>(static_cast<long long>(chunks) * slice / p.slices);
   const int n = rows > 0 ? static_cast<int>(static_cast<long long>(chunks) * (slice + 1) / p.slices) - c0 : 0;
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0) {
       const uint64_t once = policy_evict_first(), shared = policy_evict_last();
       const uint32_t bytes = groups * 4096u + (has ? ly.atoms * kCols * 128u : 0u);
@@ -466,11 +467,11 @@ __global__ void __launch_bounds__(kUtThreads)
         mbar_wait_drain(&full[stage], parity);
       }
     }
-  } else if (warp == 5) {
-    if (lane == 0 && has && n > 0) {
+  } else if (warp == 9) {
+    if (lane == 0 && n > 0) {
       const uint32_t idesc = idesc_make(kFmt, kUtRows, kCols);
       const uint32_t a_hi = smem_u32(smem);
-      bool ok = mbar_wait_short(&a_ready, 0, p.err, kErrWaitMma);
+      bool ok = !has || mbar_wait_short(&a_ready, 0, p.err, kErrWaitMma);
       int stage = 0, acc = 0;
       uint32_t parity = 0, acc_parity = 0;
       for (int i = 0; i < n && ok; ++i) {
@@ -479,14 +480,15 @@ __global__ void __launch_bounds__(kUtThreads)
         if (!ok) break;
         tc_fence_after();
         const uint32_t b0 = smem_u32(ring + stage * ly.stage) + kUtRows * 128;
-        for (int k = 0; k < ly.r16; k += 16) {
+        for (int k = 0; has && k < ly.r16; k += 16) {
           const uint32_t at = (k >> 6) * (kUtRows * 128) + (k & 63) * 2;
           const uint64_t b = smem_desc_k_sw128(b0 + (k >> 6) * (kCols * 128) + (k & 63) * 2);
           const uint32_t lo = ly.r16 <= 32 ? (ly.r16 + k) * 2 : at + ly.atoms * (kUtRows * 128);
           umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + at), b, idesc, k != 0 ? 1u : 0u);
           umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + lo), b, idesc, 1u);
         }
-        umma_commit(&acc_full[acc]);
+        if (has) umma_commit(&acc_full[acc]);
+        else mbar_arrive(&acc_full[acc]);
         if (++acc == kUtAcc) {
           acc = 0;
           acc_parity ^= 1u;
@@ -503,7 +505,9 @@ __global__ void __launch_bounds__(kUtThreads)
     }
   } else if (n > 0) {
     if (p.early) griddep_wait();  // t
-    const int row = warp * 32 + lane, live = min(max(rows - warp * 32, 0), 32);  // rows of this warp
+    // Warps 0-3 and 4-7 take steps in turn, each a row per thread.
+    const int set = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane, live = min(max(rows - quarter * 32, 0), 32);  // rows of this warp
     float unit = 1.f;
     if (has) {
       const float* t = p.t + static_cast<long long>(tile.first + row) * p.ldt;
@@ -511,6 +515,7 @@ __global__ void __launch_bounds__(kUtThreads)
       if constexpr (std::is_same<T, __half>::value) {
         float top = 0.f;
         if (row < rows)
+#pragma unroll 8
           for (int k = 0; k < p.R; k += 4) {
             const float4 f = *reinterpret_cast<const float4*>(t + k);
             top = fmaxf(fmaxf(top, fmaxf(fabsf(f.x * s), fabsf(f.y * s))), fmaxf(fabsf(f.z * s), fabsf(f.w * s)));
@@ -519,8 +524,8 @@ __global__ void __launch_bounds__(kUtThreads)
         unit = row_unit(top, &down);
         s *= down;
       }
-#pragma unroll 2
-      for (int k = 0; k < ly.r16; k += 8) {
+#pragma unroll 4
+      for (int k = set * 8; k < ly.r16; k += 16) {
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
         if (row < rows && k < p.R) {
           f = *reinterpret_cast<const float4*>(t + k);
@@ -544,11 +549,13 @@ __global__ void __launch_bounds__(kUtThreads)
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_ready);
     }
-    int stage = 0, acc = 0, last = -1;
+    int stage = set, acc = set;  // (three stages or more, and an even number of accumulators)
     uint32_t parity = 0, acc_parity = 0;
-    for (int i = 0; i < n; ++i) {
-      bool ok = mbar_wait_short(&full[stage], parity, p.err, kErrWaitEpilogue);
-      if (has) ok = ok && mbar_wait_short(&acc_full[acc], acc_parity, p.err, kErrWaitEpilogue);
+    for (int i = set; i < n; i += 2) {
+      // The accumulator first: it is of this step or an earlier one, where the stage may still be on its way to the step
+      // before, the other set's, with the same parity as this one behind it.
+      const bool ok = mbar_wait_short(&acc_full[acc], acc_parity, p.err, kErrWaitEpilogue) &&
+                      mbar_wait_short(&full[stage], parity, p.err, kErrWaitEpilogue);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       const int col = (c0 + i) * kCols;
@@ -556,24 +563,25 @@ __global__ void __launch_bounds__(kUtThreads)
 #pragma unroll
       for (int h = 0; h < kCols / 32; ++h) {
         uint32_t d[32];
-        if (has) {
-          tmem_ld_32x32b_x32(tmem + acc * kCols + (static_cast<uint32_t>(warp * 32) << 16) + h * 32, d);
-          tmem_wait_ld();
-        } else {
+        if (has) tmem_ld_32x32b_x32(tmem + acc * kCols + (static_cast<uint32_t>(quarter * 32) << 16) + h * 32, d);
+        else {
 #pragma unroll
           for (int x = 0; x < 32; ++x) d[x] = 0u;
         }
+        constexpr int kWords = sizeof(TY) / 2;  // 16-byte pieces of 8 columns
+        auto piece = [&](int x0, int w) {
+          return reinterpret_cast<uint4*>(mine + ((((h * 32 + x0) * static_cast<int>(sizeof(TY)) / 16 + w) ^ (row & 7)) << 4));
+        };
+        Eight<TY> ys[4];
+#pragma unroll
+        for (int x0 = 0; x0 < 32; x0 += 8)
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) ys[x0 / 8].w[w] = *piece(x0, w);
+        if (has) tmem_wait_ld();
         if (live > 0) {
 #pragma unroll
-          for (int x0 = 0; x0 < 32; x0 += 8) {  // 8 columns: 16 or 32 bytes of y
-            constexpr int kWords = sizeof(TY) / 2;
-            Eight<TY> y;
-            uint4* at[kWords];
-#pragma unroll
-            for (int w = 0; w < kWords; ++w) {
-              at[w] = reinterpret_cast<uint4*>(mine + ((((h * 32 + x0) * static_cast<int>(sizeof(TY)) / 16 + w) ^ (row & 7)) << 4));
-              y.w[w] = *at[w];
-            }
+          for (int x0 = 0; x0 < 32; x0 += 8) {
+            Eight<TY>& y = ys[x0 / 8];
             float v[8];
             y.values(v);
 #pragma unroll
@@ -586,22 +594,22 @@ __global__ void __launch_bounds__(kUtThreads)
             }
             y.set(v);
 #pragma unroll
-            for (int w = 0; w < kWords; ++w) *at[w] = y.w[w];
+            for (int w = 0; w < kWords; ++w) *piece(x0, w) = y.w[w];
           }
         }
       }
       tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && has) mbar_arrive(&acc_empty[acc]);
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
       if (live == 32) {
-        if (lane == 0) tma_store_3d(&tmO, ring + stage * ly.stage + warp * 4096, col, tile.first + warp * 32, 0);
+        if (lane == 0) tma_store_3d(&tmO, ring + stage * ly.stage + quarter * 4096, col, tile.first + quarter * 32, 0);
       } else if (live > 0) {  // the request's last rows, 16 bytes a lane
         constexpr int kPiece = 16 / sizeof(TY);
         const int c = col + (lane & 7) * kPiece;
         for (int r = lane >> 3; r < live; r += 4) {
-          const uint8_t* from = ring + stage * ly.stage + (warp * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4);
-          TY* to = static_cast<TY*>(p.out) + static_cast<long long>(tile.first + warp * 32 + r) * p.ldo + c;
+          const uint8_t* from = ring + stage * ly.stage + (quarter * 32 + r) * 128 + (((lane & 7) ^ (r & 7)) << 4);
+          TY* to = static_cast<TY*>(p.out) + static_cast<long long>(tile.first + quarter * 32 + r) * p.ldo + c;
           if (c + kPiece <= p.N) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
           else
             for (int x = 0; x < kPiece && c + x < p.N; ++x) to[x] = reinterpret_cast<const TY*>(from)[x];
@@ -609,18 +617,16 @@ __global__ void __launch_bounds__(kUtThreads)
         __syncwarp();
       }
       if (lane == 0) {
-        // The stage before this one goes back once its store has read it.
         bulk_commit_group();
-        bulk_wait_group_read<1>();
-        if (last >= 0) mbar_arrive(&empty[last]);
+        bulk_wait_group_read<0>();  // (the other warps of this quarter's scheduler are at work meanwhile)
+        mbar_arrive(&empty[stage]);
       }
-      last = stage;
-      if (++acc == kUtAcc) {
-        acc = 0;
+      if ((acc += 2) >= kUtAcc) {
+        acc -= kUtAcc;
         acc_parity ^= 1u;
       }
-      if (++stage == p.stages) {
-        stage = 0;
+      if ((stage += 2) >= p.stages) {
+        stage -= p.stages;
         parity ^= 1u;
       }
     }
@@ -937,10 +943,16 @@ b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cuda
   p.stages = two >= 3 ? two : one;
   if (p.stages > kUtMostStages) p.stages = kUtMostStages;
   const int64_t tiles = static_cast<int64_t>(p.rows) / kUtRows + p.batch, chunks = (p.N + kCols - 1) / kCols;
-  // Some four rounds of CTAs, of four steps or more each.
-  int64_t slices = (8ll * sms + tiles - 1) / tiles;
-  if (slices > chunks / 4) slices = chunks / 4;
-  p.slices = static_cast<int>(slices < 1 ? 1 : slices);
+  // Parts of N: what a CTA costs once is as much as some four of its steps; CTAs run in rounds.
+  const int64_t at_once = (p.stages == two ? 2ll : 1ll) * sms;
+  int64_t best = 0;
+  for (int64_t s2 = 1; s2 <= 64 && s2 <= chunks; ++s2) {
+    const int64_t cost = (tiles * s2 + at_once - 1) / at_once * ((chunks + s2 - 1) / s2 + kUtOnce);
+    if (best == 0 || cost < best) {
+      best = cost;
+      p.slices = static_cast<int>(s2);
+    }
+  }
   auto kern = p.epilogue == B2G_EPI_GATED_RESIDUAL ? lora_up_tiles_kernel<T, TY, B2G_EPI_GATED_RESIDUAL>
               : p.epilogue == B2G_EPI_GELU           ? lora_up_tiles_kernel<T, TY, B2G_EPI_GELU>
               : p.epilogue == B2G_EPI_SILU           ? lora_up_tiles_kernel<T, TY, B2G_EPI_SILU>

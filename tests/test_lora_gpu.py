@@ -122,6 +122,17 @@ def test_lora_odd_sizes(engine, lens, K, N, y_dtype):
     check(engine, lens, K, N, 40, y_dtype=y_dtype, seed=K + N)
 
 
+@pytest.mark.parametrize("lens", [[700, 130, 90], [40, 3, 60]])
+@pytest.mark.parametrize("y_dtype", [BF16, F32])
+@pytest.mark.parametrize("R", [16, 64, 128])
+@pytest.mark.parametrize("epilogue", ["none", "silu"])
+def test_lora_wide_layers_with_and_without_adapters(engine, lens, y_dtype, R, epilogue):
+    """Many steps along N; a request without an adapter, whose rows are copied, between two with one."""
+    for _ in range(3):
+        check(engine, lens, 64, 9000, R, y_dtype=y_dtype, epilogue=epilogue, seed=R, ids=[0, -1, 2])
+        check(engine, lens, 64, 9000, R, y_dtype=y_dtype, epilogue=epilogue, seed=R, ids=[-1, 1, 9])
+
+
 @pytest.mark.parametrize("lens", [[1, 2, 1, 0], [30, 60, 3], [260, 129]])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("R", [8, 64, 128])
