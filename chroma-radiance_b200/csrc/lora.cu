@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kUtThreads)
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kUtMostStages], empty[kUtMostStages], acc_full[kUtAcc], acc_empty[kUtAcc], a_ready, drain;
   __shared__ uint32_t tmem_slot;
+  __shared__ float units[kUtRows];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const UtLayout ly = ut_layout(p.R, kCols);
   uint8_t* ring = smem + ly.a_bytes;
@@ -508,47 +509,42 @@ __global__ void __launch_bounds__(kUtThreads)
     // Warps 0-3 and 4-7 take steps in turn, each a row per thread.
     const int set = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane, live = min(max(rows - quarter * 32, 0), 32);  // rows of this warp
-    float unit = 1.f;
     if (has) {
-      const float* t = p.t + static_cast<long long>(tile.first + row) * p.ldt;
-      float s = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
-      if constexpr (std::is_same<T, __half>::value) {
-        float top = 0.f;
-        if (row < rows)
-#pragma unroll 8
-          for (int k = 0; k < p.R; k += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(t + k);
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(f.x * s), fabsf(f.y * s))), fmaxf(fabsf(f.z * s), fabsf(f.w * s)));
-          }
-        float down;
-        unit = row_unit(top, &down);
-        s *= down;
-      }
+      // 16 rows a warp: `lanes` lanes to a row, 4 values of k each.
+      const float s = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
+      const int lanes = ly.r16 <= 16 ? 4 : ly.r16 <= 32 ? 8 : ly.r16 <= 64 ? 16 : 32, k = lane % lanes * 4;
 #pragma unroll 4
-      for (int k = set * 8; k < ly.r16; k += 16) {
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f), g = f;
-        if (row < rows && k < p.R) {
-          f = *reinterpret_cast<const float4*>(t + k);
-          g = *reinterpret_cast<const float4*>(t + k + 4);
+      for (int at = lane / lanes; at < 16; at += 32 / lanes) {
+        const int r = warp * 16 + at;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && k < p.R) f = *reinterpret_cast<const float4*>(p.t + static_cast<long long>(tile.first + r) * p.ldt + k);
+        float down = s;
+        if constexpr (std::is_same<T, __half>::value) {
+          float top = fmaxf(fmaxf(fabsf(f.x * s), fabsf(f.y * s)), fmaxf(fabsf(f.z * s), fabsf(f.w * s)));
+          for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float unit = row_unit(top, &down);
+          if (k == 0) units[r] = unit;
+          down *= s;
         }
-        uint32_t hi[4], lo[4];
-        split2<T>(f.x * s, f.y * s, &hi[0], &lo[0]);
-        split2<T>(f.z * s, f.w * s, &hi[1], &lo[1]);
-        split2<T>(g.x * s, g.y * s, &hi[2], &lo[2]);
-        split2<T>(g.z * s, g.w * s, &hi[3], &lo[3]);
+        uint2 hi, lo;
+        split2<T>(f.x * down, f.y * down, &hi.x, &lo.x);
+        split2<T>(f.z * down, f.w * down, &hi.y, &lo.y);
         // 16-byte pieces of a 128-byte row are swizzled by the row.
-        auto put = [&](uint32_t tile_at, int kk, const uint32_t(&v)[4]) {
-          *reinterpret_cast<uint4*>(smem + tile_at + row * 128 + (((kk >> 3) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        auto put = [&](uint32_t tile_at, int kk, uint2 v) {
+          *reinterpret_cast<uint2*>(smem + tile_at + r * 128 + (((kk >> 3) ^ (r & 7)) << 4) + (kk & 4) * 2) = v;
         };
         const uint32_t atom = (k >> 6) * (kUtRows * 128);
-        put(atom, k & 63, hi);
-        if (ly.r16 <= 32) put(0, ly.r16 + k, lo);
-        else put(atom + ly.atoms * (kUtRows * 128), k & 63, lo);
+        if (k < ly.r16) {
+          put(atom, k & 63, hi);
+          if (ly.r16 <= 32) put(0, ly.r16 + k, lo);
+          else put(atom + ly.atoms * (kUtRows * 128), k & 63, lo);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_ready);
     }
+    float unit = 1.f;
     int stage = set, acc = set;  // (three stages or more, and an even number of accumulators)
     uint32_t parity = 0, acc_parity = 0;
     for (int i = set; i < n; i += 2) {
@@ -558,6 +554,7 @@ __global__ void __launch_bounds__(kUtThreads)
                       mbar_wait_short(&full[stage], parity, p.err, kErrWaitEpilogue);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
+      if (std::is_same<T, __half>::value && has) unit = units[row];  // (written before a_ready, on which the products waited)
       const int col = (c0 + i) * kCols;
       uint8_t* mine = ring + stage * ly.stage + row * 128;
 #pragma unroll
