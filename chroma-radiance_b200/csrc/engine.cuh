@@ -122,10 +122,10 @@ void workspace_release();
 
 // True if the tensor-core path can run this problem (dtypes, strides, alignment).
 // 3-D TMA map over a K-major bf16/fp16/fp32 operand: dims {K, rows, batch}, row stride ld,
-// batch stride bstride (elements); box = 128 bytes of K x box_rows, 128-byte swizzle, zero
+// batch stride bstride (elements); box = row_bytes (32, 64 or 128) of K x box_rows, swizzled over them, zero
 // fill outside the tensor.  (CUtensorMap from <cuda.h>.)
 b2g_status make_operand_map(CUtensorMap* map, const void* base, b2g_dtype dt, int64_t K, int64_t rows, int64_t ld,
-                            int64_t batch, int64_t bstride, uint32_t box_rows);
+                            int64_t batch, int64_t bstride, uint32_t box_rows, uint32_t row_bytes = 128);
 
 // Per-row E4M3 quantisation (fp8.cu): scales[r] = absmax_r / 448 (1 for a zero row),
 // dst[r, c] = E4M3(src[r, c] * 448 / absmax_r), round to nearest even, saturating.

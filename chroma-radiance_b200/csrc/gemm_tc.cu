@@ -1374,22 +1374,24 @@ b2g_status get_encode() {
 // 3-D K-major operand map: dims {K, rows, batch}, box {128 bytes of K, box_rows, 1}, 128-byte
 // swizzle, out-of-bounds elements read as zero (so ragged M, N and K tiles need no special case).
 b2g_status make_operand_map(CUtensorMap* map, const void* base, b2g_dtype dt, int64_t K, int64_t rows,
-                            int64_t ld, int64_t batch, int64_t bstride, uint32_t box_rows) {
+                            int64_t ld, int64_t batch, int64_t bstride, uint32_t box_rows, uint32_t row_bytes) {
   b2g_status s = get_encode();
   if (s != B2G_OK) return s;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(batch)};
   const cuuint64_t esz = dt == B2G_F32 ? 4u : (dt == B2G_E4M3 || dt == B2G_S8 ? 1u : 2u);
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * esz, static_cast<cuuint64_t>(bstride) * esz};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / esz), box_rows, 1u};  // 128-byte rows
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(row_bytes / esz), box_rows, 1u};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
   const CUtensorMapDataType t = dt == B2G_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : dt == B2G_F16  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                 : dt == B2G_E4M3 || dt == B2G_S8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = g_encode(map, t, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        row_bytes == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                        : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                          : CU_TENSOR_MAP_SWIZZLE_32B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(B2G_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
   return B2G_OK;
 }

@@ -376,17 +376,18 @@ constexpr int kUtThreads = 320;  // two sets of four epilogue warps, loads, prod
 constexpr int kUtRows = 128;
 constexpr int kUtAcc = 4;
 constexpr int kUtMostStages = 6;
-constexpr int kUtOnce = 4;
 struct UtLayout {
   int r16, atoms;            // k of one product, tiles of 64 values of it
   uint32_t a_bytes, stage;   // A operand; y and B of a stage
+  uint32_t b_row;            // bytes of B's rows in shared memory
 };
 __host__ __device__ inline UtLayout ut_layout(int R, int cols) {
   UtLayout l;
   l.r16 = (R + 15) / 16 * 16;
   l.atoms = (R + 63) / 64;
   l.a_bytes = (l.r16 <= 32 ? 1 : 2 * l.atoms) * kUtRows * 128;
-  l.stage = kUtRows * 128 + l.atoms * cols * 128;
+  l.b_row = l.r16 <= 16 ? 32 : l.r16 <= 32 ? 64 : 128;
+  l.stage = kUtRows * 128 + l.atoms * cols * l.b_row;
   return l;
 }
 
@@ -436,18 +437,18 @@ __global__ void __launch_bounds__(kUtThreads)
   const int rows = tile.first < 0 || lora_nothing(p, tile) ? 0 : min(kUtRows, tile.end - tile.first);
   const int groups = (rows + 31) / 32;
   const int chunks = (p.N + kCols - 1) / kCols;
-  const int c0 = static_cast<int>(static_cast<long long>(chunks) * slice / p.slices);
-  const int n = rows > 0 ? static_cast<int>(static_cast<long long>(chunks) * (slice + 1) / p.slices) - c0 : 0;
+  // Its steps are slice, slice + slices, ..: CTAs side by side are at neighbouring columns.
+  const int n = rows > 0 ? (chunks - slice + p.slices - 1) / p.slices : 0;
   if (warp == 8) {
     if (lane == 0) {
       const uint64_t once = policy_evict_first(), shared = policy_evict_last();
-      const uint32_t bytes = groups * 4096u + (has ? ly.atoms * kCols * 128u : 0u);
+      const uint32_t bytes = groups * 4096u + (has ? ly.atoms * kCols * ly.b_row : 0u);
       int stage = 0, used = 0;
       uint32_t parity = 0;
       for (int i = 0; i < n; ++i) {
         if (!mbar_wait_short(&empty[stage], parity ^ 1u, p.err, kErrWaitProducer)) break;
         uint8_t* at = ring + stage * ly.stage;
-        const int col = (c0 + i) * kCols;
+        const int col = (slice + i * p.slices) * kCols;
         mbar_arrive_expect_tx(&full[stage], bytes);
         for (int w = 0; w < groups; ++w) tma_load_3d(at + w * 4096, &tmY, &full[stage], col, tile.first + 32 * w, 0, once);
         if (has)
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(kUtThreads)
         const uint32_t b0 = smem_u32(ring + stage * ly.stage) + kUtRows * 128;
         for (int k = 0; has && k < ly.r16; k += 16) {
           const uint32_t at = (k >> 6) * (kUtRows * 128) + (k & 63) * 2;
-          const uint64_t b = smem_desc_k_sw128(b0 + (k >> 6) * (kCols * 128) + (k & 63) * 2);
+          const uint64_t b = smem_desc_k_rows(b0 + (k >> 6) * (kCols * 128) + (k & 63) * 2, ly.b_row);
           const uint32_t lo = ly.r16 <= 32 ? (ly.r16 + k) * 2 : at + ly.atoms * (kUtRows * 128);
           umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + at), b, idesc, k != 0 ? 1u : 0u);
           umma_f16(tmem + acc * kCols, smem_desc_k_sw128(a_hi + lo), b, idesc, 1u);
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kUtThreads)
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       if (std::is_same<T, __half>::value && has) unit = units[row];  // (written before a_ready, on which the products waited)
-      const int col = (c0 + i) * kCols;
+      const int col = (slice + i * p.slices) * kCols;
       uint8_t* mine = ring + stage * ly.stage + row * 128;
 #pragma unroll
       for (int h = 0; h < kCols / 32; ++h) {
@@ -933,18 +934,21 @@ b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cuda
   b2g_status s;
   if ((s = make_operand_map(&ty, p.y, d->y_dtype, p.N, p.rows, p.ldy, 1, p.ldy * p.rows, 32)) != B2G_OK) return s;
   if ((s = make_operand_map(&to, p.out, d->y_dtype, p.N, p.rows, p.ldo, 1, p.ldo * p.rows, 32)) != B2G_OK) return s;
-  if ((s = make_operand_map(&tb, p.b, d->dtype, p.R, p.N, p.ldb, p.adapters, p.bs, kCols)) != B2G_OK) return s;
   const UtLayout ly = ut_layout(p.R, kCols);
-  // Two CTAs an SM where four stages fit beside the A operand, else one.
+  if ((s = make_operand_map(&tb, p.b, d->dtype, p.R, p.N, p.ldb, p.adapters, p.bs, kCols, ly.b_row)) != B2G_OK) return s;
+  // Two CTAs an SM where three stages fit beside the A operand, else one.
   const int two = static_cast<int>((111 * 1024 - ly.a_bytes) / ly.stage), one = static_cast<int>((225 * 1024 - ly.a_bytes) / ly.stage);
   p.stages = two >= 3 ? two : one;
   if (p.stages > kUtMostStages) p.stages = kUtMostStages;
   const int64_t tiles = static_cast<int64_t>(p.rows) / kUtRows + p.batch, chunks = (p.N + kCols - 1) / kCols;
-  // Parts of N: what a CTA costs once is as much as some four of its steps; CTAs run in rounds.
-  const int64_t at_once = (p.stages == two ? 2ll : 1ll) * sms;
-  int64_t best = 0;
+  // Parts of N: rounds of CTAs times what one takes, its steps and what it costs once (in steps; little where another
+  // CTA of the SM is at work meanwhile and A is small).  More of them side by side read and write longer runs of a row
+  // (13938 rows of 9216, rank 16: 5 parts 108 us, 16 parts 93 us).
+  const int64_t at_once = (p.stages == one ? 1ll : 2ll) * sms, once = p.stages == one ? 8 : ly.a_bytes <= 16 * 1024 ? 1 : 4;
+  double best = 0;
   for (int64_t s2 = 1; s2 <= 64 && s2 <= chunks; ++s2) {
-    const int64_t cost = (tiles * s2 + at_once - 1) / at_once * ((chunks + s2 - 1) / s2 + kUtOnce);
+    const double cost = static_cast<double>((tiles * s2 + at_once - 1) / at_once) *
+                        static_cast<double>((chunks + s2 - 1) / s2 + once) * (1.0 + 1.0 / static_cast<double>(s2));
     if (best == 0 || cost < best) {
       best = cost;
       p.slices = static_cast<int>(s2);

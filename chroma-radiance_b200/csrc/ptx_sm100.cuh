@@ -503,6 +503,17 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(uint32_t saddr) {
   return d;
 }
 
+// The same for rows of 32, 64 or 128 bytes, swizzled over their own width (layout 6, 4, 2): 8-row groups are 8 rows apart.
+__device__ __forceinline__ uint64_t smem_desc_k_rows(uint32_t saddr, uint32_t row_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>(row_bytes >> 1) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(row_bytes == 128 ? 2u : row_bytes == 64 ? 4u : 6u) << 61;
+  return d;
+}
+
 // Packed fp32 pairs (sm_100): one instruction does the same fp32 operation, correctly rounded,
 // on both halves of a 64-bit register pair.
 __device__ __forceinline__ uint64_t f2_pack(uint32_t lo_bits, uint32_t hi_bits) {
