@@ -214,8 +214,9 @@ _SIGNATURES = {
                         ctypes.c_int),
     "b2g_select_blocks": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p] + [ctypes.c_int64] * 4 +
                           [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p], ctypes.c_int),
+    "b2g_attention_blocks_workspace": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_int64], ctypes.c_size_t),
     "b2g_attention_blocks": ([ctypes.POINTER(AttentionPackedDesc), ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
-                              ctypes.c_void_p], ctypes.c_int),
+                              ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
     "b2g_lora_down": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
     "b2g_lora": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),
     "b2g_lora_up": ([ctypes.POINTER(LoraDesc), ctypes.c_void_p], ctypes.c_int),

@@ -12,7 +12,7 @@
 // Offsets are read on the device and clamped to the buffers, as in attention_packed.cu.
 //
 //   packed_tiles (attention_packed.cuh)  long queries: tensor cores through TMEM, K and V by chosen block
-//   chosen_rows                          few query rows per key head: a cluster shares out the chosen blocks
+//   chosen_rows, chosen_combine          few query rows per key head: equal shares of all that is chosen
 #include "attention_packed.cuh"
 
 namespace b2g {
@@ -267,15 +267,22 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
 
 // ---------------------------------------------------------------------------- few rows over chosen blocks
 //
-// The query rows of one key head (lq tokens x group heads) in tiles of 16, each taken by a cluster, whose CTAs
-// share out the chunks of 16 keys of the chosen blocks evenly; in a CTA 4 warps take chunks in turn.  The
-// products, the lanes' layout and the copies are those of packed_rows_kernel (attention_packed.cu).  The warps'
-// sums meet in shared memory, the CTAs' through distributed shared memory: one launch.
+// The query rows of one key head (lq tokens x group heads) in tiles of 16.  The products, the lanes' layout and the
+// copies are those of packed_rows_kernel (attention_packed.cu): in a CTA the warps take 16 keys of the chosen blocks in turn.
+//
+// Pairs of a sequence and a key head choose different numbers of blocks (an empty cache none, a long one all that it
+// may).  Their tiles lie end to end on a line, each as long as its chunks of 16 chosen keys and kCrTileCost more; the line
+// is cut into equal shares, one a CTA, and a tile that lies in several is joined by chosen_combine.  A CTA finds its
+// share in sums over the pairs that it takes itself, from the words of `chosen`: up to kCrPairs pairs; with more of
+// them a CTA takes a tile.
 constexpr int kCrWarps = 4;
 constexpr int kCrRows = 16;
 constexpr int kCrKeys = 16;
 constexpr int kCrBlocksPerSm = 2;
 constexpr int kCrListed = 256;  // chosen blocks that are listed at a time
+constexpr int kCrPairs = 1024;
+constexpr int kCrTileCost = 6;   // what a tile costs beside its chunks, in chunks
+constexpr int kCrMinShare = 16;  // a share is at least so long
 template <int D>
 constexpr int kCrPieces = D / 8;
 template <int D>
@@ -283,54 +290,152 @@ constexpr int kCrStages = D == 128 ? 3 : 6;
 template <int D>
 constexpr uint32_t kCrSmem = kCrWarps * kCrStages<D> * kCrPieces<D> * 512u;
 
+// A tile of 16 rows of a sequence and key head, and its row of `chosen`.
+struct CrTile {
+  Seq s;
+  int head, rows, row0, sees;  // rows of the sequence; the keys that any of the tile's rows sees
+  const uint32_t* words;
+  int nb;                      // blocks in sight
+  __device__ __forceinline__ uint32_t word(int w) const {
+    if (32 * w >= nb) return 0u;
+    const uint32_t bits = __ldg(words + w);
+    return nb - 32 * w >= 32 ? bits : bits & ((1u << (nb - 32 * w)) - 1u);
+  }
+  // Chunks: a block has 8; of the last one in sight, where it is chosen, only those with keys.
+  __device__ __forceinline__ int less() const {
+    const bool last = nb > 0 && (word((nb - 1) >> 5) >> ((nb - 1) & 31) & 1u) != 0;
+    return last ? 8 - (min(sees - (nb - 1) * kPtKeys, kPtKeys) + kCrKeys - 1) / kCrKeys : 0;
+  }
+};
+// mask_tiles: rows of `chosen` before sequence b's.
+__device__ __forceinline__ CrTile chosen_tile(const PkParams& p, const Seq& s, int head, int tile, int mask_tiles) {
+  CrTile r;
+  r.s = s;
+  r.head = head;
+  r.rows = s.lq * p.group;
+  r.row0 = tile * kCrRows;
+  const int first_token = r.row0 / p.group, last_token = (min(r.row0 + kCrRows, r.rows) - 1) / p.group;
+  r.sees = p.causal ? clampi(last_token + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
+  const int at = mask_tiles + first_token / kPtRows;  // (128 / 16 * group tiles of rows share one)
+  r.words = p.chosen + (static_cast<long long>(at) * p.hk + head) * p.chosen_words;
+  r.nb = at < p.chosen_tiles ? min((r.sees + kPtKeys - 1) / kPtKeys, 32 * p.chosen_words) : 0;
+  return r;
+}
+__device__ __forceinline__ int chosen_tiles_of(const PkParams& p, int lq) {
+  return static_cast<int>((static_cast<long long>(lq) * p.group + kCrRows - 1) / kCrRows);
+}
+// One thread's count of a tile's length on the line.
+__device__ __forceinline__ int chosen_length(const CrTile& c) {
+  int count = 0;
+  for (int w = 0; 32 * w < c.nb; ++w) count += __popc(c.word(w));
+  return 8 * count - c.less() + kCrTileCost;
+}
+
+// The line: sums over the pairs (sequence b, key head g) at b * hk + g, taken by all threads of the CTA.
+struct CrLine {
+  const long long* ends;  // shared memory [pairs]: the line's length up to the pair's end
+  const int* mask_tiles;  // shared memory [batch]: rows of `chosen` up to the sequence's end
+  long long total;
+  int shares;
+};
+// Inclusive sums of n values given by value(i), to ends.
+template <int kThreads, typename I, typename Value>
+__device__ __forceinline__ void sums_of(int n, I* ends, long long* carry, Value value) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < n; i += kThreads) ends[i] = value(i);
+  __syncthreads();
+  I base = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    I sum = i < n ? ends[i] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const I up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) carry[warp] = sum;
+    __syncthreads();
+    I before = base;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      before += w < warp ? static_cast<I>(carry[w]) : 0;
+      base += static_cast<I>(carry[w]);
+    }
+    if (i < n) ends[i] = before + sum;
+    __syncthreads();
+  }
+}
+template <int kThreads>
+__device__ __forceinline__ CrLine chosen_line(const PkParams& p, long long* ends, int* mask_tiles, long long* carry) {
+  sums_of<kThreads>(p.batch, mask_tiles, carry, [&](int b) {
+    const int lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
+    return (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+  });
+  const int pairs = p.batch * p.hk;
+  sums_of<kThreads>(pairs, ends, carry, [&](int i) {
+    const int b = i / p.hk;
+    const Seq s = load_seq(p, b);
+    const int tiles = chosen_tiles_of(p, s.lq), before = mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows;
+    long long sum = 0;
+    for (int t = 0; t < tiles; ++t) sum += chosen_length(chosen_tile(p, s, i - b * p.hk, t, before));
+    return sum;
+  });
+  const long long total = ends[pairs - 1], most = (total + kCrMinShare - 1) / kCrMinShare;
+  return {ends, mask_tiles, total, static_cast<int>(min(static_cast<long long>(p.shares), most))};
+}
+// Where share i begins.
+__device__ __forceinline__ long long cut_at(const CrLine& line, int i) { return line.total * i / line.shares; }
+// The tile that holds place `at` of the line: the tile, its start and length.
+__device__ __forceinline__ CrTile chosen_at(const PkParams& p, const CrLine& line, long long at, long long* start, int* length) {
+  int lo = 0, hi = p.batch * p.hk - 1;  // the first pair that ends past `at`
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (line.ends[mid] > at) hi = mid;
+    else lo = mid + 1;
+  }
+  const int b = lo / p.hk;
+  const Seq s = load_seq(p, b);
+  const int before = line.mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows, tiles = chosen_tiles_of(p, s.lq);
+  *start = lo > 0 ? line.ends[lo - 1] : 0;
+  for (int t = 0;; ++t) {
+    const CrTile c = chosen_tile(p, s, lo - b * p.hk, t, before);
+    *length = tiles == 1 ? static_cast<int>(line.ends[lo] - *start) : chosen_length(c);
+    if (t + 1 >= tiles || at < *start + *length) return c;
+    *start += *length;
+  }
+}
+
+// With part i holding (m_i, l_i) and O_i: O = sum 2^(m_i - M) O_i, l = sum 2^(m_i - M) l_i.  (A part without a key has
+// the sums 0; a NaN maximum does not occur, a NaN sum stays one.)
+__device__ __forceinline__ float part_weight(float2 ml, float top) {
+  return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
+}
+__device__ __forceinline__ void add_part(float4& acc, float w, float4 x) {
+  acc.x += w * x.x;
+  acc.y += w * x.y;
+  acc.z += w * x.z;
+  acc.w += w * x.w;
+}
+template <typename T>
+__device__ __forceinline__ void store_row(const PkParams& p, const CrTile& c, int r, int d, float sum, float4 acc) {
+  const int token = (c.row0 + r) / p.group, h = (c.row0 + r) - token * p.group;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.out) + (c.s.q0 + token) * p.ldo + (static_cast<long long>(c.head) * p.group + h) * p.hso + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+}
+
+// Chunks [c_from, c_to) of a tile: its rows of `out` if slot < 0, else a part there.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_kernel(const PkParams p, const int S) {
+__device__ __forceinline__ void chosen_part(const PkParams& p, const CrTile& tile, int c_from, int c_to, int slot, uint8_t* smem_rows,
+                                            float2 (*sml)[kCrRows], int* list) {
   constexpr int KC = D / 32, VC = D / 64, NS = kCrStages<D>;
   constexpr uint32_t kStage = kCrPieces<D> * 512u;
-  extern __shared__ __align__(16) uint8_t smem_rows[];
-  __shared__ float2 sml[kCrWarps][kCrRows];
-  __shared__ __align__(16) float2 cta_ml[kCrRows];
-  __shared__ int list[kCrListed];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem_rows) + warp * NS * kStage + lane * 16;
   auto so = [&](int w) { return reinterpret_cast<float*>(smem_rows + w * NS * kStage); };
   static_assert(kCrRows * (D + 4) * 4 <= NS * kStage, "sums fit a ring");
-  griddep_wait();
-  griddep_launch_dependents();
-  const int rank = S > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int item = static_cast<int>(blockIdx.x) / S, at_tile = item / p.hk, head = item - at_tile * p.hk;
-  int before = 0;
-  const int b = find_seq(p.batch, at_tile, lane, [&](int i) {
-    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
-    return static_cast<int>((static_cast<long long>(clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo) * p.group + kCrRows - 1) / kCrRows);
-  }, &before);
-  if (b < 0) return;  // (the whole cluster)
-  const Seq s = load_seq(p, b);
-  const int rows = s.lq * p.group, row0 = (at_tile - before) * kCrRows;
-  const int first_token = row0 / p.group, last_token = (min(row0 + kCrRows, rows) - 1) / p.group;
-  const int tile_sees = p.causal ? clampi(last_token + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
-  int tile = 0;  // of `chosen`: 128 / 16 * group tiles of rows have one
-  for (int i = lane; i < b; i += 32) {
-    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
-    tile += (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
-  }
-  tile = __reduce_add_sync(0xffffffffu, tile) + first_token / kPtRows;
-  const uint32_t* words = p.chosen + (static_cast<long long>(tile) * p.hk + head) * p.chosen_words;
-  const int nb = tile < p.chosen_tiles ? min((tile_sees + kPtKeys - 1) / kPtKeys, 32 * p.chosen_words) : 0;
-  auto word = [&](int w) {
-    if (32 * w >= nb) return 0u;
-    const uint32_t bits = __ldg(words + w);
-    return nb - 32 * w >= 32 ? bits : bits & ((1u << (nb - 32 * w)) - 1u);
-  };
-  int count = 0;
-  for (int w = lane; 32 * w < nb; w += 32) count += __popc(word(w));
-  count = __reduce_add_sync(0xffffffffu, count);
-  // This CTA's chunks: a block has 8; of the last one in sight only those with keys.
-  const bool ends_short = nb > 0 && (word((nb - 1) >> 5) >> ((nb - 1) & 31) & 1u) != 0;
-  const int chunks = 8 * count - (ends_short ? 8 - (min(tile_sees - (nb - 1) * kPtKeys, kPtKeys) + kCrKeys - 1) / kCrKeys : 0);
-  const int c_from = static_cast<int>(static_cast<long long>(chunks) * rank / S);
-  const int c_to = static_cast<int>(static_cast<long long>(chunks) * (rank + 1) / S);
-
+  const Seq& s = tile.s;
+  const int head = tile.head, rows = tile.rows, row0 = tile.row0, tile_sees = tile.sees, nb = tile.nb;
   const T* kbase = static_cast<const T*>(p.k) + s.k0 * p.ldk + head * p.hsk + 8 * t;
   const T* vbase = static_cast<const T*>(p.v) + s.k0 * p.ldv + head * p.hsv + 8 * g;
   // Q: rows g and g + 8 of the tile (row r is token r / group, head r % group of the group).
@@ -357,7 +462,7 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
     if (warp == 0) {
       int seen = 0;
       for (int w0 = 0; 32 * w0 < nb && seen < block0 + kCrListed; w0 += 32) {
-        uint32_t bits = word(w0 + lane);
+        uint32_t bits = tile.word(w0 + lane);
         int sum = __popc(bits);
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -494,21 +599,6 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
         *reinterpret_cast<float4*>(dst + 8 * (D + 4)) = make_float4(x[0][2 + e], x[1][2 + e], x[2][2 + e], x[3][2 + e]);
       }
   __syncthreads();
-  // With part i holding (m_i, l_i) and O_i: O = sum 2^(m_i - M) O_i, l = sum 2^(m_i - M) l_i.  (A part without a key has
-  // the sums 0; a NaN maximum does not occur, a NaN sum stays one.)
-  auto weight = [](float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top); };
-  auto add = [](float4& acc, float w, float4 x) {
-    acc.x += w * x.x;
-    acc.y += w * x.y;
-    acc.z += w * x.z;
-    acc.w += w * x.w;
-  };
-  auto store = [&](int r, int d, float sum, float4 acc) {
-    const int token = (row0 + r) / p.group, h = (row0 + r) - token * p.group;
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    T* dst = static_cast<T*>(p.out) + (s.q0 + token) * p.ldo + (static_cast<long long>(head) * p.group + h) * p.hso + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-  };
   const int live_rows = min(kCrRows, rows - row0);
   for (int at = threadIdx.x; at < live_rows * (D / 4); at += 32 * kCrWarps) {
     const int r = at / (D / 4), d = (at - r * (D / 4)) * 4;
@@ -518,43 +608,117 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
     for (int w = 0; w < kCrWarps; ++w) top = fmaxf(top, sml[w][r].x);
 #pragma unroll
     for (int w = 0; w < kCrWarps; ++w) {
-      const float wgt = weight(sml[w][r], top);
+      const float wgt = part_weight(sml[w][r], top);
       sum += wgt * sml[w][r].y;
-      add(acc, wgt, *reinterpret_cast<const float4*>(so(w) + r * (D + 4) + d));
+      add_part(acc, wgt, *reinterpret_cast<const float4*>(so(w) + r * (D + 4) + d));
     }
-    if (S == 1) store(r, d, sum, acc);
+    if (slot < 0) store_row<T>(p, tile, r, d, sum, acc);
     else {
-      *reinterpret_cast<float4*>(so(0) + r * (D + 4) + d) = acc;  // (read by this thread alone until here)
-      if (d == 0) cta_ml[r] = make_float2(top, sum);
+      const long long to = static_cast<long long>(slot) * kCrRows + r;
+      *reinterpret_cast<float4*>(p.part_o + to * D + d) = acc;
+      if (d == 0) p.part_ml[to] = make_float2(top, sum);
     }
   }
-  if (S == 1) return;
-  cluster_sync_all();  // every CTA's sums are in its shared memory
-  const uint32_t my_o = smem_u32(so(0)), my_ml = smem_u32(cta_ml);
-  for (int at = rank * 32 * kCrWarps + threadIdx.x; at < live_rows * (D / 4); at += S * 32 * kCrWarps) {
-    const int r = at / (D / 4), d = (at - r * (D / 4)) * 4;
-    float2 ml[8];
-    float4 x[8];
+  __syncthreads();  // the shared buffers are used again
+}
+
+template <typename T, int D, bool kLine>
+__global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_kernel(const PkParams p) {
+  extern __shared__ __align__(16) uint8_t smem_rows[];
+  __shared__ float2 sml[kCrWarps][kCrRows];
+  __shared__ int list[kCrListed];
+  griddep_wait();
+  griddep_launch_dependents();
+  if constexpr (kLine) {
+    __shared__ int mask_tiles[kCrPairs];
+    __shared__ long long ends[kCrPairs], carry[kCrWarps];
+    const CrLine line = chosen_line<32 * kCrWarps>(p, ends, mask_tiles, carry);
+    const int share = blockIdx.x;
+    if (share >= line.shares) return;
+    const long long end = cut_at(line, share + 1);
+    for (long long at = cut_at(line, share); at < end;) {
+      long long start;
+      int length;
+      const CrTile tile = chosen_at(p, line, at, &start, &length);
+      const int from = static_cast<int>(at - start), to = static_cast<int>(min(static_cast<long long>(length), end - start));
+      at = max(start + to, at + 1);  // (further on also where the words change under the kernel)
+      const int slot = to - from < length ? 2 * share + (from == 0 ? 1 : 0) : -1;
+      chosen_part<T, D>(p, tile, max(0, from - kCrTileCost), max(0, to - kCrTileCost), slot, smem_rows, sml, list);
+    }
+  } else {
+    const int lane = threadIdx.x & 31;
+    const int at_tile = static_cast<int>(blockIdx.x) / p.hk, head = static_cast<int>(blockIdx.x) - at_tile * p.hk;
+    int before = 0;
+    const int b = find_seq(p.batch, at_tile, lane, [&](int i) {
+      const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+      return chosen_tiles_of(p, clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo);
+    }, &before);
+    if (b < 0) return;
+    int mask_tiles = 0;
+    for (int i = lane; i < b; i += 32) {
+      const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+      mask_tiles += (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+    }
+    const CrTile tile = chosen_tile(p, load_seq(p, b), head, at_tile - before, __reduce_add_sync(0xffffffffu, mask_tiles));
+    chosen_part<T, D>(p, tile, 0, chosen_length(tile) - kCrTileCost, -1, smem_rows, sml, list);
+  }
+}
+
+// Joins the parts of every tile that lies in several shares.  A CTA looks at the cut between two shares and takes the
+// tile there if it is the tile's first cut; a thread joins 4 values of a row, kCcAhead parts' loads at a time.  All but the
+// parts is read before the wait for chosen_rows, which lets this kernel start after its own wait.
+constexpr int kCcAhead = 8;
+constexpr int kCcThreads = 128;
+template <typename T, int D>
+__global__ void __launch_bounds__(kCcThreads) chosen_combine_kernel(const PkParams p) {
+  __shared__ int mask_tiles[kCrPairs];
+  __shared__ long long ends[kCrPairs], carry[kCcThreads / 32];
+  const CrLine line = chosen_line<kCcThreads>(p, ends, mask_tiles, carry);
+  const int cut = static_cast<int>(blockIdx.x) + 1;
+  CrTile tile{};
+  int parts = 0;
+  if (cut < line.shares) {
+    long long start;
+    int length;
+    tile = chosen_at(p, line, cut_at(line, cut), &start, &length);
+    // (a share may be longer than the tile: then the cut before this one is outside it)
+    if (start != cut_at(line, cut) && cut_at(line, cut - 1) <= start)
+      for (parts = 2; cut + parts - 1 < line.shares && cut_at(line, cut + parts - 1) < start + length;) ++parts;
+  }
+  griddep_wait();  // (this kernel's end stands for chosen_rows' end too)
+  if (parts == 0) return;
+  const int live_rows = min(kCrRows, tile.rows - tile.row0);
+  const long long first = static_cast<long long>(2 * (cut - 1) + 1) * kCrRows, second = 2ll * cut * kCrRows, step = 2ll * kCrRows;
+  for (int at4 = threadIdx.x; at4 < live_rows * (D / 4); at4 += kCcThreads) {
+    const int r = at4 / (D / 4), d = (at4 - r * (D / 4)) * 4;
     float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ml[i] = make_float2(-INFINITY, 0.f);
-      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i >= S) continue;
-      ml[i] = ld_cluster_f2(map_to_cta(my_ml + r * 8, i));
-      x[i] = ld_cluster_f4(map_to_cta(my_o + (r * (D + 4) + d) * 4, i));
-      top = fmaxf(top, ml[i].x);
-    }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < parts; i0 += kCcAhead) {
+      float2 ml[kCcAhead];
+      float4 x[kCcAhead];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float wgt = weight(ml[i], top);
-      sum += wgt * ml[i].y;
-      add(acc, wgt, x[i]);
+      for (int i = 0; i < kCcAhead; ++i) {
+        const bool in = i0 + i < parts;
+        const long long slot = (i0 + i == 0 ? first : second + (i0 + i - 1) * step) + r;
+        ml[i] = in ? __ldcg(p.part_ml + slot) : make_float2(-INFINITY, 0.f);
+        x[i] = in ? __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float next = top;
+#pragma unroll
+      for (int i = 0; i < kCcAhead; ++i) next = fmaxf(next, ml[i].x);
+      const float alpha = top == next ? 1.f : fast_exp2(top - next);
+      top = next;
+      sum *= alpha;
+      acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
+#pragma unroll
+      for (int i = 0; i < kCcAhead; ++i) {
+        const float wgt = part_weight(ml[i], top);
+        sum += wgt * ml[i].y;
+        add_part(acc, wgt, x[i]);
+      }
     }
-    store(r, d, sum, acc);
+    store_row<T>(p, tile, r, d, sum, acc);
   }
-  cluster_sync_all();  // nobody leaves while its sums are still read
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -562,38 +726,45 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
 // Average queries per sequence up to which chosen_rows takes a call, as in attention_packed.cu.
 constexpr int64_t kCrQueries = 16;
 
-template <typename T, int D>
-b2g_status launch_chosen_rows(const PkParams& p, int sms, cudaStream_t st) {
-  const int64_t items = (static_cast<int64_t>(p.total_q) * p.group / kCrRows + p.batch) * p.hk;
-  // As many CTAs as run at the same time, up to 8 to an item.
-  int64_t S = static_cast<int64_t>(kCrBlocksPerSm) * sms / items;
-  S = S < 1 ? 1 : S > 8 ? 8 : S;
-  if (items * S > (1ll << 31) - 1) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_blocks: size");
-  auto kern = chosen_rows_kernel<T, D>;
-  b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCrSmem<D>)),
-                            "cudaFuncSetAttribute(chosen_rows)");
-  if (s != B2G_OK) return s;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * S));
-  cfg.blockDim = dim3(32 * kCrWarps);
-  cfg.dynamicSmemBytes = kCrSmem<D>;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(S);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = S > 1 ? 2 : 1;
-  s = check_cuda(cudaLaunchKernelEx(&cfg, kern, p, static_cast<int>(S)), "chosen_rows launch");
-  if (s == B2G_OK) note_launch();
-  return s;
+// What a call runs, from its sizes alone.
+struct CrPlan {
+  bool rows = false;  // chosen_rows (+ chosen_combine), else packed_tiles
+  int shares = 0;     // 0: a CTA a tile
+  size_t o_bytes = 0, bytes = 0;
+};
+CrPlan chosen_plan(const b2g_attention_packed_desc* d, int64_t words, int sms) {
+  CrPlan r;
+  r.rows = d->total_q <= kCrQueries * d->batch || d->total_k == 0;
+  if (!r.rows || d->batch * d->n_kv_head > kCrPairs) return r;
+  // A share a CTA, as many as run at the same time; no more than the longest line possible has pieces of kCrMinShare.
+  const int64_t tiles = (d->total_q * (d->n_head / d->n_kv_head) / kCrRows + d->batch) * d->n_kv_head;
+  const int64_t blocks = d->total_k / kPtKeys + 1, length = 8 * (blocks < 32 * words ? blocks : 32 * words) + kCrTileCost;
+  const int64_t most = tiles < (1ll << 30) / length ? (tiles * length + kCrMinShare - 1) / kCrMinShare : 1ll << 30;
+  int64_t shares = static_cast<int64_t>(kCrBlocksPerSm) * sms;
+  r.shares = static_cast<int>(shares < most ? shares : most);
+  r.o_bytes = static_cast<size_t>(round_up(2 * static_cast<int64_t>(r.shares) * kCrRows * d->d_head * 4, 256));
+  r.bytes = r.o_bytes + 2 * static_cast<size_t>(r.shares) * kCrRows * sizeof(float2);
+  return r;
 }
 
 template <typename T, int D>
-b2g_status run_chosen(const b2g_attention_packed_desc* d, PkParams p, int sms, cudaStream_t st) {
-  if (d->total_q <= kCrQueries * d->batch || d->total_k == 0) return launch_chosen_rows<T, D>(p, sms, st);
+b2g_status launch_chosen_rows(const PkParams& p, cudaStream_t st) {
+  const int64_t items = (static_cast<int64_t>(p.total_q) * p.group / kCrRows + p.batch) * p.hk;
+  if (p.shares == 0 && items > (1ll << 31) - 1) return set_error(B2G_ERR_UNSUPPORTED, "b2g_attention_blocks: size");
+  auto kern = p.shares ? chosen_rows_kernel<T, D, true> : chosen_rows_kernel<T, D, false>;
+  b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kCrSmem<D>)),
+                            "cudaFuncSetAttribute(chosen_rows)");
+  if (s != B2G_OK) return s;
+  s = launch_pdl(kern, dim3(static_cast<unsigned>(p.shares ? p.shares : items)), dim3(32 * kCrWarps), kCrSmem<D>, st,
+                 "chosen_rows launch", p);
+  if (s != B2G_OK || p.shares <= 1) return s;
+  return launch_pdl(chosen_combine_kernel<T, D>, dim3(static_cast<unsigned>(p.shares - 1)), dim3(kCcThreads), 0, st,
+                    "chosen_combine launch", p);
+}
+
+template <typename T, int D>
+b2g_status run_chosen(const b2g_attention_packed_desc* d, PkParams p, const CrPlan& pl, int sms, cudaStream_t st) {
+  if (pl.rows) return launch_chosen_rows<T, D>(p, st);
   CUtensorMap tq, tk, tv;
   b2g_status s;
   if ((s = make_operand_map(&tq, p.q, d->dtype, D, p.total_q, p.ldq, p.hq, p.hsq, kPtRows)) != B2G_OK) return s;
@@ -721,8 +892,17 @@ b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means,
   return d->d_head == 128 ? run(select_blocks_kernel<__nv_bfloat16, 128>) : run(select_blocks_kernel<__nv_bfloat16, 64>);
 }
 
+size_t attention_blocks_workspace(const b2g_attention_packed_desc* d, int64_t words) {
+  PkParams p{};
+  DeviceInfo* dev = nullptr;
+  if (blocks_params(d, "b2g_attention_blocks_workspace", true, true, &p) != B2G_OK || words < 0 || words > (1ll << 20) ||
+      d->batch == 0 || d->total_q == 0 || d->n_head == 0 || device_info(&dev) != B2G_OK)
+    return 0;
+  return chosen_plan(d, words, dev->num_sms).bytes;
+}
+
 b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* chosen, int64_t tiles, int64_t words,
-                            cudaStream_t st) {
+                            void* workspace, size_t workspace_bytes, cudaStream_t st) {
   PkParams p{};
   b2g_status s = blocks_params(d, "b2g_attention_blocks", true, true, &p);
   if (s != B2G_OK) return s;
@@ -738,10 +918,21 @@ b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* c
   p.chosen_tiles = words > 0 ? static_cast<int>(tiles) : 0;
   p.chosen_words = static_cast<int>(words);
   p.err = dev->err_word;
+  const CrPlan pl = chosen_plan(d, words, dev->num_sms);
+  void* ws = workspace;
+  if (pl.bytes > 0) {
+    if (!ws && (s = workspace_get(pl.bytes, &ws, kWsAttnSplit)) != B2G_OK) return s;
+    if (workspace && (workspace_bytes < pl.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+      return set_error(B2G_ERR_INVALID, "b2g_attention_blocks: the workspace is too small or not 256-byte aligned");
+  }
+  p.shares = pl.shares;
+  p.part_o = static_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + pl.o_bytes);
+  const int sms = dev->num_sms;
   if (d->dtype == B2G_F16)
-    return d->d_head == 128 ? run_chosen<__half, 128>(d, p, dev->num_sms, st) : run_chosen<__half, 64>(d, p, dev->num_sms, st);
-  return d->d_head == 128 ? run_chosen<__nv_bfloat16, 128>(d, p, dev->num_sms, st)
-                          : run_chosen<__nv_bfloat16, 64>(d, p, dev->num_sms, st);
+    return d->d_head == 128 ? run_chosen<__half, 128>(d, p, pl, sms, st) : run_chosen<__half, 64>(d, p, pl, sms, st);
+  return d->d_head == 128 ? run_chosen<__nv_bfloat16, 128>(d, p, pl, sms, st)
+                          : run_chosen<__nv_bfloat16, 64>(d, p, pl, sms, st);
 }
 
 }  // namespace b2g

@@ -33,6 +33,7 @@ decltype(&b2g_attention_packed_workspace) call_attention_packed_workspace = null
 decltype(&b2g_block_means) call_block_means = nullptr;
 decltype(&b2g_select_blocks) call_select_blocks = nullptr;
 decltype(&b2g_attention_blocks) call_attention_blocks = nullptr;
+decltype(&b2g_attention_blocks_workspace) call_attention_blocks_workspace = nullptr;
 decltype(&b2g_lora_down) call_lora_down = nullptr;
 decltype(&b2g_lora_up) call_lora_up = nullptr;
 decltype(&b2g_lora) call_lora = nullptr;
@@ -432,7 +433,11 @@ PyObject* attention_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     d.scale = a[8] == Py_None ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)))
                               : static_cast<float>(PyFloat_AsDouble(a[8]));
     if (PyErr_Occurred()) throw PythonError{};
-    check(call_attention_blocks(&d, static_cast<const int32_t*>(chosen.data_ptr()), chosen.size(0), chosen.size(2), stream));
+    Tensor space;
+    const size_t n = call_attention_blocks_workspace(&d, chosen.size(2));
+    if (n) space = make({static_cast<int64_t>(n)}, ScalarType::Char, q);
+    check(call_attention_blocks(&d, static_cast<const int32_t*>(chosen.data_ptr()), chosen.size(0), chosen.size(2),
+                                n ? space.data_ptr() : nullptr, n, stream));
     return result(a[9], out);
   });
 }
@@ -585,6 +590,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     call_block_means = reinterpret_cast<decltype(call_block_means)>(address("b2g_block_means"));
     call_select_blocks = reinterpret_cast<decltype(call_select_blocks)>(address("b2g_select_blocks"));
     call_attention_blocks = reinterpret_cast<decltype(call_attention_blocks)>(address("b2g_attention_blocks"));
+    call_attention_blocks_workspace =
+        reinterpret_cast<decltype(call_attention_blocks_workspace)>(address("b2g_attention_blocks_workspace"));
     call_lora_down = reinterpret_cast<decltype(call_lora_down)>(address("b2g_lora_down"));
     call_lora = reinterpret_cast<decltype(call_lora)>(address("b2g_lora"));
     call_lora_up = reinterpret_cast<decltype(call_lora_up)>(address("b2g_lora_up"));

@@ -505,9 +505,13 @@ b2g_status b2g_select_blocks(const b2g_attention_packed_desc* desc, const float*
   return select_blocks(desc, means, blocks, top, first, last, chosen, tiles, words, static_cast<cudaStream_t>(stream));
 }
 
+size_t b2g_attention_blocks_workspace(const b2g_attention_packed_desc* desc, int64_t words) {
+  return attention_blocks_workspace(desc, words);
+}
+
 b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int32_t* chosen, int64_t tiles, int64_t words,
-                                void* stream) {
-  return attention_blocks(desc, chosen, tiles, words, static_cast<cudaStream_t>(stream));
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return attention_blocks(desc, chosen, tiles, words, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 b2g_status b2g_lora_down(const b2g_lora_desc* desc, void* stream) {

@@ -152,8 +152,9 @@ b2g_status block_means(const b2g_attention_packed_desc* d, const int32_t* since,
                        cudaStream_t st);
 b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means, int64_t blocks, int64_t top, int64_t first,
                          int64_t last, int32_t* chosen, int64_t tiles, int64_t words, cudaStream_t st);
+size_t attention_blocks_workspace(const b2g_attention_packed_desc* d, int64_t words);
 b2g_status attention_blocks(const b2g_attention_packed_desc* d, const int32_t* chosen, int64_t tiles, int64_t words,
-                            cudaStream_t st);
+                            void* workspace, size_t workspace_bytes, cudaStream_t st);
 
 // Low-rank adapters (lora.cu); see b2g_lora_down, b2g_lora_up and b2g_lora.  early: launched right behind
 // lora_down, before which all but t was ready.

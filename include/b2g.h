@@ -566,13 +566,15 @@ b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* wor
  * last tile are 0 (total_q / 128 + batch rows always suffice).  words <= 256; blocks past 32 * words are never chosen.
  *
  * b2g_attention_blocks: b2g_attention_packed over the keys of the chosen blocks.  Bits of blocks out of a tile's
- * sight are not looked at; a tile without a bit, or past `tiles`, sees nothing, and its rows are 0.  No workspace. */
+ * sight are not looked at; a tile without a bit, or past `tiles`, sees nothing, and its rows are 0.
+ * workspace: as for b2g_gemm_s8. */
 b2g_status b2g_block_means(const b2g_attention_packed_desc* desc, const int32_t* since, float* means, int64_t blocks,
                            void* stream);
 b2g_status b2g_select_blocks(const b2g_attention_packed_desc* desc, const float* means, int64_t blocks, int64_t top,
                              int64_t first, int64_t last, int32_t* chosen, int64_t tiles, int64_t words, void* stream);
+size_t b2g_attention_blocks_workspace(const b2g_attention_packed_desc* desc, int64_t words);
 b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int32_t* chosen, int64_t tiles, int64_t words,
-                                void* stream);
+                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* Low-rank adapters of the requests of a packed batch beside a projection that they share:
  *   b2g_lora_down  t[m]   = x[m] . a[r]^T                            F32 [rows, R]

@@ -125,16 +125,16 @@ def test_attention_blocks_refusals():
 
     lib = b2g.load()
     f = lib.b2g_attention_blocks
-    refused(lib, f(None, 256, 2, 1, None), 1, "b2g_attention_blocks: null")
+    refused(lib, f(None, 256, 2, 1, None, 0, None), 1, "b2g_attention_blocks: null")
     for kw, code, word in ((dict(batch=-1), 1, "negative"), (dict(dtype=b2g.F32), 2, "BF16 or F16"), (dict(d_head=96), 2, "head dim"),
                            (dict(n_head=3), 1, "multiple"), (dict(scale=0.0), 1, "scale"), (dict(scale=float("nan")), 1, "scale"),
                            (dict(q=None), 1, "null"), (dict(v=None), 1, "null"), (dict(cu_k=None), 1, "null"),
                            (dict(ldv=260), 2, "strides"), (dict(out=264), 2, "aligned")):
-        refused(lib, f(packed(**kw), 256, 2, 1, None), code, word)
-    refused(lib, f(packed(), 256, -2, 1, None), 1, "negative")
-    refused(lib, f(packed(), None, 2, 1, None), 1, "null")
-    refused(lib, f(packed(), 258, 2, 1, None), 2, "aligned")
-    assert f(packed(batch=0), 256, 2, 1, None) == 0 and f(packed(total_q=0), None, 0, 0, None) == 0
+        refused(lib, f(packed(**kw), 256, 2, 1, None, 0, None), code, word)
+    refused(lib, f(packed(), 256, -2, 1, None, 0, None), 1, "negative")
+    refused(lib, f(packed(), None, 2, 1, None, 0, None), 1, "null")
+    refused(lib, f(packed(), 258, 2, 1, None, 0, None), 2, "aligned")
+    assert f(packed(batch=0), 256, 2, 1, None, 0, None) == 0 and f(packed(total_q=0), None, 0, 0, None, 0, None) == 0
 
 
 def test_python_refusals():
