@@ -281,7 +281,7 @@ constexpr int kCrKeys = 16;
 constexpr int kCrBlocksPerSm = 2;
 constexpr int kCrListed = 256;  // chosen blocks that are listed at a time
 constexpr int kCrPairs = 1024;
-constexpr int kCrTileCost = 6;   // what a tile costs beside its chunks, in chunks
+constexpr int kCrTileCost = 12;  // what a tile costs beside its chunks, in chunks
 constexpr int kCrMinShare = 16;  // a share is at least so long
 template <int D>
 constexpr int kCrPieces = D / 8;
