@@ -118,7 +118,6 @@ __global__ void __launch_bounds__(32 * kMnWarps) block_means_kernel(const MnPara
 // Scores are sums of 64 bits: a choice compares neighbours, and any rounding of theirs in 32 bits would decide
 // the choice where two are close; in 64 bits the order of a sum moves one in some 10^12.
 constexpr int kSlThreads = 256;
-constexpr int kSlCounted = 256;  // up to so many blocks a block's rank is counted, else the threshold is searched
 constexpr int kSlMostWords = 256;
 
 struct SlParams {
@@ -137,128 +136,214 @@ __device__ __forceinline__ unsigned long long score_order(double s) {
   return u >> 63 ? ~u : u | (1ull << 63);
 }
 
-template <typename T, int D>
+// hi + lo += x exactly, up to lo's own rounding (2^-48 of the sum), for two values at a time.
+__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_fma(b, f2_splat(-1.f), a); }
+__device__ __forceinline__ void add_pair(uint64_t& hi, uint64_t& lo, uint64_t x) {
+  const uint64_t sum = f2_add(hi, x), part = f2_sub(sum, hi);
+  lo = f2_add(lo, f2_add(f2_sub(hi, f2_sub(sum, part)), f2_sub(x, part)));
+  hi = sum;
+}
+
+// c += a b, 8 x 8 x 4 in 64 bits.
+__device__ __forceinline__ void mma_884(double (&c)[2], double a, double b) {
+  asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));
+}
+
+template <typename T, int D, int NT>  // NT neighbouring tiles a CTA
 __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParams a) {
   constexpr int kPieces = D / 8, kGroups = kSlThreads / kPieces;  // 16-byte pieces of a row, rows at a time
-  extern __shared__ unsigned long long order[];  // [32 words] the blocks' scores
-  __shared__ double part[kGroups][D];
-  __shared__ int counts[2];
+  constexpr int kWarps = kSlThreads / 32, kPitch = D + 4;         // (values from sum to sum, for the banks)
+  static_assert(NT <= 8 && NT <= kWarps, "tiles");
+  extern __shared__ __align__(16) unsigned char smem_sl[];
+  double* part = reinterpret_cast<double*>(smem_sl);                                                    // [warp][NT][kPitch]
+  unsigned long long* order = reinterpret_cast<unsigned long long*>(part + NT * kWarps * kPitch);             // [NT][32 words]: scores
   const PkParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / p.hk, g = blockIdx.x - tile * p.hk;
+  const int g = blockIdx.x % p.hk, tile0 = static_cast<int>(blockIdx.x / p.hk) * NT;
+  const int most = 32 * a.words;
   griddep_wait();
   griddep_launch_dependents();
-  uint32_t* out = a.chosen + (static_cast<long long>(tile) * p.hk + g) * a.words;
-  int before = 0;
-  const int b = find_seq(p.batch, tile, lane, [&](int i) {
-    const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
-    return (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
-  }, &before);
-  if (b < 0) {
-    for (int i = threadIdx.x; i < a.words; i += kSlThreads) out[i] = 0;
-    return;
-  }
-  const Seq s = load_seq(p, b);
-  const int base = blocks_before(p, b, lane);
-  const int row0 = (tile - before) * kPtRows, rows = min(kPtRows, s.lq - row0);
-  const int sees_first = p.causal ? clampi(row0 + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
-  const int sees_last = p.causal ? clampi(row0 + rows + s.lk - s.lq, 0, s.lk) : s.lk;
-  const int nb = min((sees_last + kPtKeys - 1) / kPtKeys, 32 * a.words);
-  auto sure = [&](int j) {
-    return j < a.first || j >= nb - a.last || min((j + 1) * kPtKeys, sees_last) > sees_first;
+  // The tiles: rows, blocks in sight, the first and the last query's keys, where the sequence's means begin.
+  struct Tile {
+    int rows, q0, sees_first, sees_last, nb, base;
   };
-
-  // The tile's queries, summed.
-  {
-    const int piece = threadIdx.x % kPieces, from = threadIdx.x / kPieces;
-    double sum[8] = {};
-    const T* q = static_cast<const T*>(p.q) + static_cast<long long>(s.q0 + row0) * p.ldq +
-                 static_cast<long long>(g) * p.group * p.hsq + piece * 8;
-    for (int i = from; i < rows * p.group; i += kGroups) {
-      const int row = i / p.group, h = i - row * p.group;
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(q + row * p.ldq + h * p.hsq));
-      float f[8] = {};
-      add8<T>(f, v);
+  __shared__ Tile tiles[NT];
+  if (warp < NT) {
+    Tile t{};
+    int before = 0;
+    const int tile = tile0 + warp;
+    const int b = tile < a.tiles ? find_seq(p.batch, tile, lane, [&](int i) {
+      const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
+      return (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+    }, &before) : -1;
+    if (b >= 0) {
+      const Seq s = load_seq(p, b);
+      const int row0 = (tile - before) * kPtRows;
+      t.base = blocks_before(p, b, lane);
+      t.rows = min(kPtRows, s.lq - row0);
+      t.q0 = s.q0 + row0;
+      t.sees_first = p.causal ? clampi(row0 + 1 + s.lk - s.lq, 0, s.lk) : s.lk;
+      t.sees_last = p.causal ? clampi(row0 + t.rows + s.lk - s.lq, 0, s.lk) : s.lk;
+      t.nb = min((t.sees_last + kPtKeys - 1) / kPtKeys, most);
+    }
+    if (lane == 0) tiles[warp] = t;
+  }
+  __syncthreads();
+  // The tiles' queries, summed: in pairs of fp32 by a thread, in 64 bits after that.
+  const int piece = threadIdx.x % kPieces, from = threadIdx.x / kPieces;
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    const Tile t = tiles[n];
+    const T* q = static_cast<const T*>(p.q) + static_cast<long long>(t.q0) * p.ldq + static_cast<long long>(g) * p.group * p.hsq + piece * 8;
+    uint64_t hi[4], lo[4];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) sum[x] += f[x];
+    for (int x = 0; x < 4; ++x) hi[x] = lo[x] = 0;
+    const int items = t.nb > 0 ? t.rows * p.group : 0;
+    constexpr int kAheadQ = 8;
+    for (int i0 = from; i0 < items; i0 += kAheadQ * kGroups) {
+      uint4 v[kAheadQ];
+#pragma unroll
+      for (int u = 0; u < kAheadQ; ++u) {
+        const int i = i0 + u * kGroups, row = p.group == 1 ? i : i / p.group, h = i - row * p.group;
+        v[u] = i < items ? __ldg(reinterpret_cast<const uint4*>(q + row * p.ldq + h * p.hsq)) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < kAheadQ; ++u) {
+        float f[8] = {};
+        add8<T>(f, v[u]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) add_pair(hi[x], lo[x], f2_pack(__float_as_uint(f[2 * x]), __float_as_uint(f[2 * x + 1])));
+      }
+    }
+    double sum[8];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float2 h = f2_unpack(hi[x]), l = f2_unpack(lo[x]);
+      // (the second is no number where the first is infinite)
+      sum[2 * x] = isfinite(h.x) ? static_cast<double>(h.x) + static_cast<double>(l.x) : static_cast<double>(h.x);
+      sum[2 * x + 1] = isfinite(h.y) ? static_cast<double>(h.y) + static_cast<double>(l.y) : static_cast<double>(h.y);
     }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) part[from][piece * 8 + x] = sum[x];
+    for (int o = 16; o >= kPieces; o >>= 1)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], o);
+    if (lane < kPieces)
+#pragma unroll
+      for (int x = 0; x < 8; ++x) part[(warp * NT + n) * kPitch + piece * 8 + x] = sum[x];
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < D; c += kSlThreads) {
-    double sum = part[0][c];
-    for (int i = 1; i < kGroups; ++i) sum += part[i][c];
-    part[0][c] = sum;
+  for (int c = threadIdx.x; c < NT * D; c += kSlThreads) {
+    double* at = part + c / D * kPitch + c % D;
+    double sum = at[0];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) sum += at[i * NT * kPitch];
+    at[0] = sum;
   }
   __syncthreads();
-  // Scores: 8 lanes to a block.
-  {
-    const int l = lane & 7;
-    double q[D / 8];
+  // Scores, by products of 8 tiles x 8 blocks x 4 values in 64 bits: lane (r, t) holds the values 16 c + 4 t + e of tile r and
+  // of block r for the products e of the 16 values c, and gets the scores of tile r for blocks 2 t and 2 t + 1.
+  int nb_most = 0, base = 0;
+  bool one = true;  // one sequence (the others see nothing), whose means are read once for all tiles
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+  for (int n = 0; n < NT; ++n)
+    if (tiles[n].nb > 0) {
+      one = one && (nb_most == 0 || base == tiles[n].base);
+      base = tiles[n].base;
+      nb_most = max(nb_most, tiles[n].nb);
+    }
+  const int r = lane >> 2, t4 = lane & 3;
+  auto scores = [&](int nb, int mean0, int n0, int n1) {  // blocks below nb of tiles n0 to n1
+    for (int j0 = warp * 8; j0 < nb; j0 += kWarps * 8) {
+      float4 m[D / 16];
+      const int at = mean0 + j0 + r;
+      const bool in = j0 + r < nb && at < a.blocks;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) q[4 * i + x] = part[0][32 * i + 4 * l + x];
-    for (int j0 = warp * 4; j0 < nb; j0 += kSlThreads / 8) {
-      const int j = j0 + (lane >> 3);
-      double sum = 0.0;
-      if (j < nb && base + j < a.blocks) {
-        const float* m = a.means + (static_cast<long long>(base + j) * p.hk + g) * D + 4 * l;
+      for (int c = 0; c < D / 16; ++c)
+        m[c] = in ? __ldg(reinterpret_cast<const float4*>(a.means + (static_cast<long long>(at) * p.hk + g) * D + 16 * c + 4 * t4))
+                  : make_float4(0.f, 0.f, 0.f, 0.f);
+      double s[2][2] = {};  // (two sums side by side)
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(m + 32 * i));
-          sum = fma(q[4 * i], static_cast<double>(v.x), sum);
-          sum = fma(q[4 * i + 1], static_cast<double>(v.y), sum);
-          sum = fma(q[4 * i + 2], static_cast<double>(v.z), sum);
-          sum = fma(q[4 * i + 3], static_cast<double>(v.w), sum);
+      for (int c = 0; c < D / 16; ++c) {
+        double2 q01 = make_double2(0.0, 0.0), q23 = q01;
+        if (NT == 8 || r < NT) {
+          const double* q = part + r * kPitch + 16 * c + 4 * t4;
+          q01 = *reinterpret_cast<const double2*>(q);
+          q23 = *reinterpret_cast<const double2*>(q + 2);
         }
+        mma_884(s[0], q01.x, m[c].x);
+        mma_884(s[1], q01.y, m[c].y);
+        mma_884(s[0], q23.x, m[c].z);
+        mma_884(s[1], q23.y, m[c].w);
       }
+      if (r < n0 || r >= n1) continue;
+      const Tile& tile = tiles[r];
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (l == 0 && j < nb) order[j] = sure(j) ? 0 : score_order(sum);
-    }
-  }
-  __syncthreads();
-  if (nb <= kSlCounted) {
-    for (int w = warp; w < a.words; w += kSlThreads / 32) {
-      const int j = 32 * w + lane;
-      bool take = false;
-      if (j < nb) {
-        const unsigned long long mine = order[j];
-        int above = 0;
-        for (int i = 0; i < nb; ++i) above += order[i] > mine || (order[i] == mine && i < j);
-        take = mine == 0 || above < a.top;
+      for (int e = 0; e < 2; ++e) {
+        const int j = j0 + 2 * t4 + e;
+        const bool sure = j < a.first || j >= tile.nb - a.last || min((j + 1) * kPtKeys, tile.sees_last) > tile.sees_first;
+        if (j < tile.nb) order[r * most + j] = sure ? 0 : score_order(s[0][e] + s[1][e]);
       }
-      const uint32_t bits = __ballot_sync(0xffffffffu, take);
-      if (lane == 0) out[w] = bits;
     }
-    return;
-  }
-  // The largest threshold that `top` scores reach, bit by bit from above (fewer scores: 1, all of them).
-  unsigned long long least = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const unsigned long long next = least | (1ull << bit);
-    if (threadIdx.x == 0) counts[bit & 1] = 0;
-    __syncthreads();
+  };
+  if (one) scores(nb_most, base, 0, NT);
+  else
+    for (int n = 0; n < NT; ++n) scores(tiles[n].nb, tiles[n].base, n, n + 1);
+  __syncthreads();
+  // A warp takes a tile: the largest threshold that `top` scores reach, bit by bit from above (fewer scores: 1, all of
+  // them), looked for until it parts them; then the words.
+  if (warp >= NT || tile0 + warp >= a.tiles) return;
+  const unsigned long long* mine = order + warp * most;
+  const int nb = tiles[warp].nb;
+  uint32_t* out = a.chosen + (static_cast<long long>(tile0 + warp) * p.hk + g) * a.words;
+  constexpr int kHeld = 8;  // scores in a lane's registers, as they come first
+  unsigned long long held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < nb ? mine[32 * i + lane] : 0;
+  auto reach = [&](unsigned long long least) {
     int n = 0;
-    for (int j = threadIdx.x; j < nb; j += kSlThreads) n += order[j] >= next;
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) atomicAdd(&counts[bit & 1], n);
-    __syncthreads();
-    if (counts[bit & 1] >= a.top) least = next;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) n += held[i] >= least;
+    for (int j = 32 * kHeld + lane; j < nb; j += 32) n += mine[j] >= least;
+    return __reduce_add_sync(0xffffffffu, n);
+  };
+  unsigned long long least = 0;
+  int reached = reach(1), bit = -1;  // (no more than are to be taken: all of them)
+  if (reached > a.top) {
+    // The upper words' common bits need no search.
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+    auto extend = [&](unsigned long long x) {
+      const uint32_t word = static_cast<uint32_t>(x >> 32);
+      if (x) {
+        low = min(low, word);
+        high = max(high, word);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) extend(held[i]);
+    for (int j = 32 * kHeld + lane; j < nb; j += 32) extend(mine[j]);
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    const int same = __clz(low ^ high);
+    bit = 63 - same;
+    if (same > 0) least = static_cast<unsigned long long>(high & ~(same >= 32 ? 0u : 0xFFFFFFFFu >> same)) << 32;
+  }
+  for (; bit >= 0 && reached > a.top; --bit) {
+    const unsigned long long next = least | (1ull << bit);
+    const int n = reach(next);
+    if (n >= a.top) {
+      least = next;
+      reached = n;
+    }
   }
   if (least == 0) least = 1;
-  if (warp != 0) return;
-  int over = 0;  // scores above it; of those that equal it the first fill the rest
-  for (int j = lane; j < nb; j += 32) over += order[j] > least;
-  int room = a.top - __reduce_add_sync(0xffffffffu, over);
+  int room = 0;  // of the scores that equal the threshold, as many as are still to be taken
+  if (reached > a.top) room = a.top - (least == ~0ull ? 0 : reach(least + 1));
+  else room = nb;
   for (int w = 0; w < a.words; ++w) {
     const int j = 32 * w + lane;
-    const unsigned long long mine = j < nb ? order[j] : 0;
-    const uint32_t equal = __ballot_sync(0xffffffffu, j < nb && mine == least);
-    const bool take = j < nb && (mine == 0 || mine > least ||
-                                 (mine == least && __popc(equal & ((1u << lane) - 1u)) < room));
+    const unsigned long long x = j < nb ? mine[j] : 0;
+    const uint32_t equal = __ballot_sync(0xffffffffu, j < nb && x == least);
+    const bool take = j < nb && (x == 0 || x > least || (x == least && __popc(equal & ((1u << lane) - 1u)) < room));
     const uint32_t bits = __ballot_sync(0xffffffffu, take);
     room -= __popc(equal);
     if (lane == 0) out[w] = bits;
@@ -881,15 +966,22 @@ b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means,
   a.chosen = reinterpret_cast<uint32_t*>(chosen);
   a.tiles = static_cast<int>(tiles);
   a.words = static_cast<int>(words);
-  const dim3 grid(static_cast<unsigned>(tiles * d->n_kv_head)), block(kSlThreads);
-  const size_t smem = static_cast<size_t>(words) * 32 * 8;
-  auto run = [&](auto kern) {
-    b2g_status st2 = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlMostWords * 32 * 8),
+  // Four tiles a CTA, which share the means, where that leaves CTAs for all SMs and their scores fit.
+  const bool four = tiles / 4 * d->n_kv_head >= dev->num_sms && d->total_q > 64 * d->batch && words <= kSlMostWords / 4;
+  auto run = [&](auto kern, int nt) {
+    const size_t sums = static_cast<size_t>(nt) * kSlThreads / 32 * (d->d_head + 4) * 8, smem = sums + static_cast<size_t>(nt) * words * 32 * 8;
+    b2g_status st2 = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024),
                                 "cudaFuncSetAttribute(select_blocks)");
-    return st2 != B2G_OK ? st2 : launch_pdl(kern, grid, block, smem, st, "select_blocks launch", a);
+    return st2 != B2G_OK ? st2
+                         : launch_pdl(kern, dim3(static_cast<unsigned>((tiles + nt - 1) / nt * d->n_kv_head)), dim3(kSlThreads), smem, st,
+                                      "select_blocks launch", a);
   };
-  if (d->dtype == B2G_F16) return d->d_head == 128 ? run(select_blocks_kernel<__half, 128>) : run(select_blocks_kernel<__half, 64>);
-  return d->d_head == 128 ? run(select_blocks_kernel<__nv_bfloat16, 128>) : run(select_blocks_kernel<__nv_bfloat16, 64>);
+  auto pick = [&](auto type) {
+    using T = decltype(type);
+    if (d->d_head == 128) return four ? run(select_blocks_kernel<T, 128, 4>, 4) : run(select_blocks_kernel<T, 128, 1>, 1);
+    return four ? run(select_blocks_kernel<T, 64, 4>, 4) : run(select_blocks_kernel<T, 64, 1>, 1);
+  };
+  return d->dtype == B2G_F16 ? pick(__half()) : pick(__nv_bfloat16());
 }
 
 size_t attention_blocks_workspace(const b2g_attention_packed_desc* d, int64_t words) {
