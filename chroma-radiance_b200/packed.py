@@ -19,6 +19,17 @@ and qkv is held once; q and k are thus rounded before the norm and again after t
 bf16 block's projection rounds them once, at the end.  In F32 they would be written and read as 4 bytes a value: for
 1536 rows 38 MB more of traffic.  The rounding is at most 2^-8 of a value; the operands' 8 bits leave an rms of 1.3 % (two
 roundings with a step of 4 sigma / 127).
+
+Requests may bring adapters of their own (`AdaptersS8`): low-rank products beside both layers, in 16 bits, as the weights that
+they stand beside have 8.
+
+    t1       = lora_down(x_mod, A1)                          once, for both halves of linear1
+    q, k, v += scale t1 B1[0:9216]                           on the projection's bf16 result
+    cat[mlp] = gelu(cat[mlp] + scale t1 B1[9216:])           the GELU here instead of in the product's epilogue
+    x       += gate * scale (cat A2) B2
+
+Long sequences need not attend to all of their keys (`Choice`): block_means and select_blocks on the rotated q and k,
+attention_blocks over what they chose.
 """
 from __future__ import annotations
 
@@ -68,6 +79,25 @@ def pack(requests: list[tuple[int, int, int]], dev) -> Packed:
     return Packed(torch.tensor(offsets, dtype=torch.int32, device=dev), torch.cat(positions).to(dev))
 
 
+@dataclass
+class AdaptersS8:
+    """Low-rank adapters of a block's layers, bf16 or fp16, as x_mod; every adapter is padded to one rank with zeros."""
+    linear1_a: torch.Tensor  # [adapters, rank, 3072]
+    linear1_b: torch.Tensor  # [adapters, 21504, rank]
+    linear2_a: torch.Tensor  # [adapters, rank, 15360], bf16 (the concat buffer's type)
+    linear2_b: torch.Tensor  # [adapters, 3072, rank], bf16
+    scale: torch.Tensor | None = None  # f32 [adapters]
+
+
+@dataclass
+class Choice:
+    """Which key blocks a tile of 128 queries attends to: the first few (the prompt's), the last few, the best others."""
+    top: int
+    first: int = 0
+    last: int = 0
+    max_k: int | None = None  # rows of the longest sequence, or more
+
+
 class Scratch:
     """Activations of a block over up to `rows` packed rows, allocated once."""
 
@@ -79,17 +109,34 @@ class Scratch:
 
 
 def single_block(w: SingleWeightsS8, x_mod: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, batch: Packed,
-                 s: Scratch) -> None:
+                 s: Scratch, adapters: AdaptersS8 | None = None, ids: torch.Tensor | None = None,
+                 choice: Choice | None = None) -> None:
     """Updates x [rows, 3072] (F32 residual stream of all sequences) in place from the modulated x_mod
-    (bf16, fp16 or F32)."""
+    (bf16, fp16 or F32; with adapters bf16).  ids: each sequence's adapter (int32, device; negative: none; None: the
+    sequences' own numbers).  choice: attention over chosen key blocks."""
     n = x.shape[0]
     codes, scales = b2g.quantize_s8(x_mod, out=s.codes[:n], scales=s.scales[:n])
     qkv, cat = s.qkv[:n], s.cat[:n]
     b2g.gemm_s8(codes, w.linear1_q[:3 * HIDDEN], w.linear1_s[:3 * HIDDEN], w.linear1_b[:3 * HIDDEN],
                 out=qkv.view(n, 3 * HIDDEN), x_scale=scales)
     b2g.gemm_s8(codes, w.linear1_q[3 * HIDDEN:], w.linear1_s[3 * HIDDEN:], w.linear1_b[3 * HIDDEN:],
-                out=cat[:, HIDDEN:], epilogue="gelu", x_scale=scales)
+                out=cat[:, HIDDEN:], epilogue="none" if adapters else "gelu", x_scale=scales)
+    if adapters:
+        flat, mlp = qkv.view(n, 3 * HIDDEN), cat[:, HIDDEN:]
+        t = b2g.lora_down(x_mod, adapters.linear1_a, batch.offsets, ids=ids)
+        b2g.lora_up(t, adapters.linear1_b[:, :3 * HIDDEN], flat, batch.offsets, ids=ids, scale=adapters.scale, out=flat)
+        b2g.lora_up(t, adapters.linear1_b[:, 3 * HIDDEN:], mlp, batch.offsets, ids=ids, scale=adapters.scale,
+                    epilogue="gelu", out=mlp)
     q, k, v = qkv.unbind(1)
     b2g.qk_norm_rope(q, k, batch.positions, AXES, q_norm=w.q_norm, k_norm=w.k_norm, q_out=q, k_out=k)
-    b2g.attention_packed(q, k, v, batch.offsets, out=cat[:, :HIDDEN].unflatten(1, (HEADS, DHEAD)))
+    attn = cat[:, :HIDDEN].unflatten(1, (HEADS, DHEAD))
+    if choice:
+        means = b2g.block_means(k, batch.offsets)
+        chosen = b2g.select_blocks(q, means, batch.offsets, choice.top, first=choice.first, last=choice.last, max_k=choice.max_k)
+        b2g.attention_blocks(q, k, v, chosen, batch.offsets, out=attn)
+    else:
+        b2g.attention_packed(q, k, v, batch.offsets, out=attn)
     b2g.gemm_s8(cat, w.linear2_q, w.linear2_s, w.linear2_b, out=x, epilogue="gated_residual", gate=gate)
+    if adapters:
+        b2g.lora(cat, adapters.linear2_a, adapters.linear2_b, x, batch.offsets, ids=ids, scale=adapters.scale,
+                 epilogue="gated_residual", gate=gate, out=x)
