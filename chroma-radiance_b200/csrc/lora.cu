@@ -13,7 +13,8 @@
 //   lora_down_tiles  128 rows of a request: tcgen05, x and A by TMA, K shared out over a cluster
 //   lora_down_rows   few rows a request: m16n8k16 products from registers, K shared out over warps and a cluster
 //   lora_up_tiles    128 rows of a request: tcgen05, y, B and out by TMA
-//   lora_up          few rows a request, and y or out that TMA cannot take: m16n8k16 products
+//   lora_up_rows     few rows a request: m16n8k16 products, B through rings in shared memory
+//   lora_up_any      many rows where TMA cannot take y or out: m16n8k16 products
 //
 // In the second product s t is the sum of two numbers of the operands' 16-bit type: bf16 keeps 2^-17 of a value, fp16, whose
 // range is small, 2^-22 of its row's largest, as the row is brought to [1, 2) by a power of two.
@@ -55,20 +56,39 @@ struct LoraParams {
 struct LoraTile {
   int first, end, adapter;
 };
+// A whole warp looks, 32 requests at a time, whose offsets and adapters are loaded together: one round trip of memory.
 __device__ __forceinline__ LoraTile lora_tile(const LoraParams& p, int tile, int span, int lane) {
-  int before = 0;
-  const int b = find_seq(p.batch, tile, lane, [&](int i) {
-    const int lo = clampi(__ldg(p.cu + i), 0, p.rows);
-    return (clampi(__ldg(p.cu + i + 1), lo, p.rows) - lo + span - 1) / span;
-  }, &before);
-  if (b < 0) return {-1, 0, -1};
-  const int lo = clampi(__ldg(p.cu + b), 0, p.rows);
-  LoraTile t;
-  t.first = lo + (tile - before) * span;
-  t.end = clampi(__ldg(p.cu + b + 1), lo, p.rows);
-  t.adapter = p.ids ? __ldg(p.ids + b) : b;
-  if (t.adapter < 0 || t.adapter >= p.adapters) t.adapter = -1;
-  return t;
+  int base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane;
+    int lo = 0, end = 0, adapter = -1;
+    if (b < p.batch) {
+      lo = __ldg(p.cu + b);
+      end = __ldg(p.cu + b + 1);
+      adapter = p.ids ? __ldg(p.ids + b) : b;
+    }
+    lo = clampi(lo, 0, p.rows);
+    end = clampi(end, lo, p.rows);
+    const int n = (end - lo + span - 1) / span;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, base + sum > tile);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      LoraTile t;
+      t.first = __shfl_sync(0xffffffffu, lo + (tile - base - sum + n) * span, at);
+      t.end = __shfl_sync(0xffffffffu, end, at);
+      t.adapter = __shfl_sync(0xffffffffu, adapter, at);
+      if (t.adapter < 0 || t.adapter >= p.adapters) t.adapter = -1;
+      return t;
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {-1, 0, -1};
 }
 
 // ---------------------------------------------------------------------------- down, many rows
@@ -219,12 +239,13 @@ __global__ void __launch_bounds__(kLdThreads)
 
 // ---------------------------------------------------------------------------- down, few rows
 //
-// 16 rows of a request, of which often one is there: what has to be read is the adapter.  A CTA takes 8 NT rows of A,
-// a warp 32 values of K in turn: lane (g, t) holds 16 bytes of row g (of x, of A) at k = 32 c + 8 t, words (0, 1) and
-// (2, 3) of which are the operands of two products.  kLrAhead neighbouring chunks, 256 bytes of a row, are loaded
-// together.  The warps' sums meet in shared memory, a cluster's in distributed shared memory, in a fixed order.
-constexpr int kLrWarps = 4;
-constexpr int kLrAhead = 4;
+// 16 rows of a request, of which often one is there: what has to be read is the adapter.  A CTA takes 8 rows of A,
+// its 16 warps 32 values of K in turn: lane (g, t) holds 16 bytes of row g (of x, of A) at k = 32 c + 8 t, words (0, 1) and
+// (2, 3) of which are the operands of two products.  kLrAhead neighbouring chunks, 128 bytes of a row, are loaded
+// together.  The warps' sums meet in shared memory in a fixed order; where there are few CTAs, those of a cluster
+// share out K and meet in distributed shared memory.
+constexpr int kLrWarps = 16;
+constexpr int kLrAhead = 2;
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(32 * kLrWarps) lora_down_rows_kernel(const LoraParams p) {
@@ -277,7 +298,14 @@ __global__ void __launch_bounds__(32 * kLrWarps) lora_down_rows_kernel(const Lor
   float* to = p.t + r0;
   for (int i = threadIdx.x; i < count; i += 32 * kLrWarps) {
     const int m = i / width, c = i - m * width;
-    const float sum = (sums[0][m][c] + sums[1][m][c]) + (sums[2][m][c] + sums[3][m][c]);
+    float v[kLrWarps];
+#pragma unroll
+    for (int w = 0; w < kLrWarps; ++w) v[w] = sums[w][m][c];
+#pragma unroll
+    for (int o = 1; o < kLrWarps; o *= 2)
+#pragma unroll
+      for (int w = 0; w < kLrWarps; w += 2 * o) v[w] += v[w + o];
+    const float sum = v[0];
     if (S == 1) to[static_cast<long long>(tile.first + m) * p.ldt + c] = sum;
     else sums[0][m][c] = sum;  // (read by this thread alone until here)
   }
@@ -640,63 +668,15 @@ __global__ void __launch_bounds__(kUtThreads)
   }
 }
 
-// ---------------------------------------------------------------------------- up, few rows, any alignment
-//
-// A CTA of 8 warps, WM of them along rows (16 each) and 8 / WM along columns, takes one tile of rows and a part of N.
-// k is taken as in lora_down_rows: lane (g, t) holds 8 neighbouring values of a row, 16 bytes of B.  Of y a lane has 8
-// neighbouring columns, two of each of four products (column 8 (c / 2) + 2 i + c % 2 of the group of 32 is column c of
-// product i).  Where rows are 16-byte aligned (VEC) it reads and writes them itself; else a warp's 16 rows x 64
-// columns pass through shared memory, so that a warp's loads and stores are of neighbouring values of one row.
-// Several warps along rows share B in shared memory; one warp loads its own, kBatch groups of 32 columns at a time.
-constexpr int kLuThreads = 256;
-// Steps of 32 columns that a warp takes together; columns of a CTA's part.
-template <int KK, bool VEC>
-constexpr int kLuBatch = !VEC ? 2 : KK >= 4 ? 1 : 2;
-template <int KK, int WM, bool VEC>
-constexpr int kLuCols = WM == 1 ? 8 * 32 * kLuBatch<KK, VEC> : 256;
-template <typename TY>
-constexpr int kLuPitch = 64 + 16 / sizeof(TY);  // values from row to row in shared memory
-template <typename TY, int KK, int WM, bool VEC>
-constexpr size_t kLuSmem = (WM > 1 ? kLuCols<KK, WM, VEC> / 8 * KK * 32 * sizeof(uint4) : 0) + (VEC ? 0 : 8 * 16 * kLuPitch<TY> * sizeof(TY));
+// ---------------------------------------------------------------------------- up, values in registers
 
-template <typename T, typename TY, int KK, int WM, bool VEC>  // 32 KK >= R
-__global__ void __launch_bounds__(kLuThreads) lora_up_kernel(const LoraParams p) {
-  constexpr int WN = 8 / WM;
-  constexpr bool kStaged = WM > 1;
-  constexpr int kBatch = kLuBatch<KK, VEC>, kCols = kLuCols<KK, WM, VEC>;
-  static_assert(kCols / 32 % (WN * kBatch) == 0, "whole steps");
-  extern __shared__ __align__(16) uint8_t smem_up[];
-  uint4* sb = reinterpret_cast<uint4*>(smem_up);  // [column group of 8][KK][lane]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  TY* sy = reinterpret_cast<TY*>(smem_up + (kStaged ? kCols / 8 * KK * 32 * sizeof(uint4) : 0)) + warp * 16 * kLuPitch<TY>;
-  const int wm = warp % WM, wn = warp / WM;
-  const int at_tile = static_cast<int>(blockIdx.x / p.slices), slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(at_tile) * p.slices);
-  if (!p.early) griddep_wait();
-  griddep_launch_dependents();
-  const LoraTile tile = lora_tile(p, at_tile, 16 * WM, lane);
-  if (tile.first < 0 || lora_nothing(p, tile)) {
-    if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
-    return;
-  }
-  const bool has = tile.adapter >= 0;
-  const int n0 = slice * kCols, n1 = min(p.N, n0 + kCols);
-  const T* b = static_cast<const T*>(p.b) + (has ? tile.adapter : 0) * p.bs;
-  // 8 values of k of the column that lane ln stands for in product `group`.
-  auto load_b = [&](int group, int kk, int ln) {
-    const int gg = ln >> 2, col = n0 + (group >> 2) * 32 + 8 * (gg >> 1) + 2 * (group & 3) + (gg & 1), k = 32 * kk + 8 * (ln & 3);
-    if (!has || col >= n1 || k >= p.R) return make_uint4(0, 0, 0, 0);
-    return __ldg(reinterpret_cast<const uint4*>(b + col * p.ldb + k));
-  };
-  if (kStaged && has)
-#pragma unroll 4
-    for (int i = threadIdx.x; i < kCols / 8 * KK * 32; i += kLuThreads) sb[i] = load_b(i / (32 * KK), i / 32 % KK, i & 31);
-  const int first = tile.first + 16 * wm, row[2] = {first + g, first + g + 8};
-  const bool in[2] = {row[0] < tile.end, row[1] < tile.end};
-  const int rows = min(16, tile.end - first);
+// s t of a lane's rows g and g + 8 of 16 (k = 32 c + 8 t + ..), as hi + lo in the layout of the products' A operands.
+template <typename T, int KK>
+struct LoraRows {
   uint32_t hi[KK][2][4], lo[KK][2][4];  // [k / 32][row][pair of k]
-  float unit[2] = {1.f, 1.f};
-  auto load_t = [&]() {
-    if (p.early) griddep_wait();
+  float unit[2];
+  __device__ __forceinline__ void load(const LoraParams& p, const LoraTile& tile, const int (&row)[2], int t) {
+    const bool has = tile.adapter >= 0;
     const float s = has ? (p.scale ? __ldg(p.scale + tile.adapter) : 1.f) : 0.f;
     float v[2][KK][8];
 #pragma unroll
@@ -705,7 +685,7 @@ __global__ void __launch_bounds__(kLuThreads) lora_up_kernel(const LoraParams p)
       for (int kk = 0; kk < KK; ++kk) {
         const int k = 32 * kk + 8 * t;
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f), h = f;
-        if (has && in[i] && k < p.R) {
+        if (has && row[i] < tile.end && k < p.R) {
           f = *reinterpret_cast<const float4*>(p.t + row[i] * p.ldt + k);
           h = *reinterpret_cast<const float4*>(p.t + row[i] * p.ldt + k + 4);
         }
@@ -715,6 +695,7 @@ __global__ void __launch_bounds__(kLuThreads) lora_up_kernel(const LoraParams p)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float down = 1.f;
+      unit[i] = 1.f;
       if constexpr (std::is_same<T, __half>::value) {
         float top = 0.f;
 #pragma unroll
@@ -730,115 +711,270 @@ __global__ void __launch_bounds__(kLuThreads) lora_up_kernel(const LoraParams p)
 #pragma unroll
         for (int x = 0; x < 4; ++x) split2<T>(v[i][kk][2 * x] * down, v[i][kk][2 * x + 1] * down, &hi[kk][i][x], &lo[kk][i][x]);
     }
-  };
-  bool loaded = false;
-  for (int j0 = wn * kBatch; j0 < kCols / 32; j0 += WN * kBatch) {
-    if (n0 + 32 * j0 >= n1) break;
-    Eight<TY> y[kBatch][2];
-    uint4 w[kStaged ? 1 : kBatch][4][KK];
-    if (!kStaged) {
+  }
+  __device__ __forceinline__ void multiply(float (&acc)[4], int kk, uint4 b) const {
+    const uint32_t(&h)[2][4] = hi[kk];
+    const uint32_t(&l)[2][4] = lo[kk];
+    mma_16816<T>(acc, h[0][0], h[1][0], h[0][1], h[1][1], b.x, b.y);
+    mma_16816<T>(acc, h[0][2], h[1][2], h[0][3], h[1][3], b.z, b.w);
+    mma_16816<T>(acc, l[0][0], l[1][0], l[0][1], l[1][1], b.x, b.y);
+    mma_16816<T>(acc, l[0][2], l[1][2], l[0][3], l[1][3], b.z, b.w);
+  }
+};
+// Lane (g, t) has 8 neighbouring columns of y, two of each of four products: column 8 (c / 2) + 2 i + c % 2 of a group of 32 is
+// column c of product i.  The column of B that lane ln loads for product i:
+__device__ __forceinline__ int b_column(int i, int ln) { return 8 * (ln >> 3) + 2 * i + ((ln >> 2) & 1); }
+// A lane's 8 values of row i of the 16, from y to out.
+template <typename T, int KK>
+__device__ __forceinline__ void lora_finish(const LoraParams& p, const LoraRows<T, KK>& rows, bool has, int i, const float (&acc)[4][4],
+                                            const float (&gate)[8], float (&v)[8]) {
+  float delta[8];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j)
+  for (int x = 0; x < 8; ++x) {  // column 2 t + e of product x / 2
+    delta[x] = has ? acc[x >> 1][2 * i + (x & 1)] : 0.f;
+    if constexpr (std::is_same<T, __half>::value) delta[x] *= rows.unit[i];
+  }
+  lora_out8(p.epilogue, v, delta, gate);
+}
+__device__ __forceinline__ void load_gate(const LoraParams& p, bool has, int col, int end, float (&gate)[8]) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) gate[x] = p.epilogue == B2G_EPI_GATED_RESIDUAL && has && col + x < end ? __ldg(p.gate + col + x) : 0.f;
+}
+
+// ---------------------------------------------------------------------------- up, few rows
+//
+// 16 rows of a request, of which often one is there: what has to be read is B.  A warp takes 32 columns at a time, whose
+// rows of B it copies ahead into its own ring: every lane the 16-byte pieces that it will use (k as in lora_down_rows).
+constexpr int kUrWarps = 4;
+template <int KK>
+constexpr int kUrStages = KK == 4 ? 3 : 4;
+template <int KK>
+constexpr size_t kUrSmem = static_cast<size_t>(kUrWarps) * kUrStages<KK> * KK * 2048;
+
+template <typename T, typename TY, int KK, bool VEC>  // 32 KK >= R
+__global__ void __launch_bounds__(32 * kUrWarps) lora_up_rows_kernel(const LoraParams p) {
+  constexpr int NS = kUrStages<KK>;
+  constexpr uint32_t kStage = KK * 2048;
+  extern __shared__ __align__(16) uint8_t smem_up[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = smem_u32(smem_up) + warp * NS * kStage + lane * 16;
+  const int at_tile = static_cast<int>(blockIdx.x / p.slices), slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(at_tile) * p.slices);
+  if (!p.early) griddep_wait();
+  griddep_launch_dependents();
+  const LoraTile tile = lora_tile(p, at_tile, 16, lane);
+  if (tile.first < 0 || lora_nothing(p, tile)) {
+    if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
+    return;
+  }
+  const bool has = tile.adapter >= 0;
+  // Groups of 32 columns: this CTA's from g0 on, its warps in turn.
+  const int groups = (p.N + 31) / 32;
+  const int g0 = static_cast<int>(static_cast<long long>(groups) * slice / p.slices), g1 = static_cast<int>(static_cast<long long>(groups) * (slice + 1) / p.slices);
+  const T* b = static_cast<const T*>(p.b) + (has ? tile.adapter : 0) * p.bs;
+  auto fetch = [&](int group, int st) {
+    const uint32_t dst = ring + st * kStage;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = 32 * group + b_column(i, lane);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const int k = 32 * kk + 8 * t;
+        const bool live = has && col < p.N && k < p.R;
+        copy16(dst + (i * KK + kk) * 512, live ? b + col * p.ldb + k : p.b, live);
+      }
+    }
+  };
+  int ahead = g0 + warp;
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i, ahead += kUrWarps) {
+    if (ahead < g1) fetch(ahead, i);
+    copy_commit();
+  }
+  const int row[2] = {tile.first + g, tile.first + g + 8};
+  const bool in[2] = {row[0] < tile.end, row[1] < tile.end};
+  auto load_y = [&](int group, Eight<TY> (&y)[2]) {
+    const int col = 32 * group + 8 * t;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const TY* from = static_cast<const TY*>(p.y) + row[i] * p.ldy + col;
+      if constexpr (VEC) {
+#pragma unroll
+        for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
+          if (in[i] && col < p.N) y[i].w[x] = *(reinterpret_cast<const uint4*>(from) + x);
+      } else {
+        float v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) v[x] = in[i] && col + x < p.N ? static_cast<float>(from[x]) : 0.f;
+        y[i].set(v);
+      }
+    }
+  };
+  Eight<TY> y[2], y_next[2];
+  if (g0 + warp < g1) load_y(g0 + warp, y);
+  if (p.early) griddep_wait();
+  LoraRows<T, KK> rows;
+  rows.load(p, tile, row, t);
+  int st = 0;
+#pragma unroll 1
+  for (int group = g0 + warp; group < g1; group += kUrWarps) {
+    copy_wait<NS - 2>();
+    if (ahead < g1) fetch(ahead, st == 0 ? NS - 1 : st - 1);  // (the stage used up in the last round)
+    copy_commit();
+    ahead += kUrWarps;
+    if (group + kUrWarps < g1) load_y(group + kUrWarps, y_next);
+    const uint32_t src = ring + st * kStage;
+    st = st + 1 == NS ? 0 : st + 1;
+    float acc[4][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) rows.multiply(acc[i], kk, lds16(src + (i * KK + kk) * 512));
+    const int col = 32 * group + 8 * t;
+    float gate[8];
+    load_gate(p, has, col, p.N, gate);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float v[8];
+      y[i].values(v);
+      lora_finish(p, rows, has, i, acc, gate, v);
+      TY* to = static_cast<TY*>(p.out) + row[i] * p.ldo + col;
+      if (!in[i] || col >= p.N) continue;
+      if constexpr (VEC) {
+        y[i].set(v);
+#pragma unroll
+        for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x) *(reinterpret_cast<uint4*>(to) + x) = y[i].w[x];
+      } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (col + x < p.N) to[x] = static_cast<TY>(v[x]);
+      }
+    }
+    y[0] = y_next[0];
+    y[1] = y_next[1];
+  }
+  copy_wait<0>();
+}
+
+// ---------------------------------------------------------------------------- up, many rows, any alignment
+//
+// Where TMA cannot take y or out: 128 rows and 256 columns a CTA, 16 rows a warp, 64 columns at a time.  B's part is laid out
+// in shared memory as the products take it.  y is copied ahead in whole 16-byte pieces of memory, a piece at either
+// end with values of its neighbours (no piece is read that holds no value of y), so that a row lies in shared memory
+// as far from a 16-byte boundary as in memory; out is made up the same way and leaves in whole pieces, but for the ends.
+constexpr int kLuWarps = 8;
+constexpr int kLuCols = 256;
+constexpr int kLuStages = 3;
+template <typename TY>
+constexpr int kLuPieces = 64 * sizeof(TY) / 16 + 1;           // of a row's 64 values
+template <typename TY>
+constexpr int kLuPitch = (kLuPieces<TY> + 1) * 16;             // bytes from row to row in shared memory
+template <typename TY, int KK>
+constexpr size_t kLuSmem = kLuCols / 8 * KK * 32 * sizeof(uint4) + static_cast<size_t>(kLuWarps) * (kLuStages + 1) * 16 * kLuPitch<TY>;
+
+template <typename T, typename TY, int KK>  // 32 KK >= R
+__global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraParams p) {
+  constexpr int kPieces = kLuPieces<TY>, kPitch = kLuPitch<TY>, kEsz = sizeof(TY);
+  extern __shared__ __align__(16) uint8_t smem_up[];
+  uint4* sb = reinterpret_cast<uint4*>(smem_up);  // [column group of 8][KK][lane]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* sy = smem_up + kLuCols / 8 * KK * 32 * sizeof(uint4) + warp * (kLuStages + 1) * 16 * kPitch;  // y's stages, then out's
+  uint8_t* so = sy + kLuStages * 16 * kPitch;
+  const int at_tile = static_cast<int>(blockIdx.x / p.slices), slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(at_tile) * p.slices);
+  if (!p.early) griddep_wait();
+  griddep_launch_dependents();
+  const LoraTile tile = lora_tile(p, at_tile, 16 * kLuWarps, lane);
+  if (tile.first < 0 || lora_nothing(p, tile)) {
+    if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
+    return;
+  }
+  const bool has = tile.adapter >= 0;
+  const int n0 = slice * kLuCols, n1 = min(p.N, n0 + kLuCols), steps = (n1 - n0 + 63) / 64;
+  const int first = tile.first + 16 * warp, live = min(16, tile.end - first);
+  // A row's 64 values from column c0 on: their address, and how far it is past a 16-byte boundary.
+  auto y_at = [&](int r, int c0) { return static_cast<const uint8_t*>(p.y) + ((first + r) * p.ldy + c0) * kEsz; };
+  auto out_at = [&](int r, int c0) { return static_cast<uint8_t*>(p.out) + ((first + r) * p.ldo + c0) * kEsz; };
+  auto past = [](const uint8_t* at) { return static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15u); };
+  auto fetch = [&](int step) {
+    const int c0 = n0 + 64 * step, bytes = min(64, n1 - c0) * kEsz;
+    const uint32_t dst = smem_u32(sy + step % kLuStages * 16 * kPitch);
+#pragma unroll
+    for (int i0 = 0; i0 < (16 * kPieces + 31) / 32; ++i0) {
+      const int i = 32 * i0 + lane, r = i / kPieces, piece = i - r * kPieces;
+      if (r >= live) continue;
+      const uint8_t* at = y_at(r, c0);
+      const int off = past(at);
+      if (piece * 16 < off + bytes) copy16(dst + r * kPitch + piece * 16, at - off + piece * 16, true);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kLuStages - 1; ++i) {
+    if (i < steps) fetch(i);
+    copy_commit();
+  }
+  const T* b = static_cast<const T*>(p.b) + (has ? tile.adapter : 0) * p.bs;
+  if (has)
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kLuCols / 8 * KK * 32; i += 32 * kLuWarps) {
+      const int product = i / (32 * KK), col = n0 + (product >> 2) * 32 + b_column(product & 3, i & 31), k = 32 * (i / 32 % KK) + 8 * (i & 3);
+      sb[i] = col < n1 && k < p.R ? __ldg(reinterpret_cast<const uint4*>(b + col * p.ldb + k)) : make_uint4(0, 0, 0, 0);
+    }
+  const int row[2] = {first + g, first + g + 8};
+  if (p.early) griddep_wait();
+  LoraRows<T, KK> rows;
+  rows.load(p, tile, row, t);
+  __syncthreads();
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    copy_wait<kLuStages - 2>();
+    __syncwarp();  // (all lanes' copies of this step; nobody is at the stage that is filled next)
+    if (step + kLuStages - 1 < steps) fetch(step + kLuStages - 1);
+    copy_commit();
+    const int c0 = n0 + 64 * step, width = min(64, n1 - c0);
+    const uint8_t* from = sy + step % kLuStages * 16 * kPitch;
+    const int y_off[2] = {past(y_at(g, c0)), past(y_at(g + 8, c0))}, o_off[2] = {past(out_at(g, c0)), past(out_at(g + 8, c0))};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (32 * j >= width) break;
+      float acc[4][4] = {};
+      if (has) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk) w[j][i][kk] = load_b(4 * (j0 + j) + i, kk, lane);
-    }
-    if constexpr (VEC) {
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int col = n0 + 32 * (j0 + j) + 8 * t;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
-            if (in[i] && col < n1) y[j][i].w[x] = *(reinterpret_cast<const uint4*>(static_cast<const TY*>(p.y) + row[i] * p.ldy + col) + x);
+          for (int kk = 0; kk < KK; ++kk) rows.multiply(acc[i], kk, sb[(((c0 - n0) / 8 + 4 * j + i) * KK + kk) * 32 + lane]);
       }
-    } else {
-      const int col = n0 + 32 * j0 + lane;
-      const TY* from = static_cast<const TY*>(p.y) + first * p.ldy + col;
-      TY raw[16][2];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (r < rows && col + 32 * x < n1) raw[r][x] = from[r * p.ldy + 32 * x];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (r < rows && col + 32 * x < n1) sy[r * kLuPitch<TY> + lane + 32 * x] = raw[r][x];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
-            y[j][i].w[x] = *(reinterpret_cast<const uint4*>(sy + (g + 8 * i) * kLuPitch<TY> + 32 * j + 8 * t) + x);
-    }
-    if (!loaded) {
-      load_t();
-      if (kStaged) __syncthreads();
-      loaded = true;
-    }
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      float acc[4][4] = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          const uint4 u = kStaged ? sb[((4 * (j0 + j) + i) * KK + kk) * 32 + lane] : w[kStaged ? 0 : j][i][kk];
-          const uint32_t(&h)[2][4] = hi[kk];
-          const uint32_t(&l)[2][4] = lo[kk];
-          mma_16816<T>(acc[i], h[0][0], h[1][0], h[0][1], h[1][1], u.x, u.y);
-          mma_16816<T>(acc[i], h[0][2], h[1][2], h[0][3], h[1][3], u.z, u.w);
-          mma_16816<T>(acc[i], l[0][0], l[1][0], l[0][1], l[1][1], u.x, u.y);
-          mma_16816<T>(acc[i], l[0][2], l[1][2], l[0][3], l[1][3], u.z, u.w);
-        }
-      const int col = n0 + 32 * (j0 + j) + 8 * t;
       float gate[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        gate[x] = p.epilogue == B2G_EPI_GATED_RESIDUAL && has && col + x < n1 ? __ldg(p.gate + col + x) : 0.f;
+      load_gate(p, has, c0 + 32 * j + 8 * t, n1, gate);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float v[8], delta[8];
-        y[j][i].values(v);
+        const int at = (g + 8 * i) * kPitch + (32 * j + 8 * t) * kEsz;
+        const TY* y = reinterpret_cast<const TY*>(from + at + y_off[i]);
+        TY* o = reinterpret_cast<TY*>(so + at + o_off[i]);
+        float v[8];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {  // column 2 t + e of product x / 2
-          delta[x] = has ? acc[x >> 1][2 * i + (x & 1)] : 0.f;
-          if constexpr (std::is_same<T, __half>::value) delta[x] *= unit[i];
-        }
-        lora_out8(p.epilogue, v, delta, gate);
-        y[j][i].set(v);
-        if constexpr (VEC) {
+        for (int x = 0; x < 8; ++x) v[x] = static_cast<float>(y[x]);
+        lora_finish(p, rows, has, i, acc, gate, v);
 #pragma unroll
-          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
-            if (in[i] && col < n1) *(reinterpret_cast<uint4*>(static_cast<TY*>(p.out) + row[i] * p.ldo + col) + x) = y[j][i].w[x];
-        } else {
-#pragma unroll
-          for (int x = 0; x < static_cast<int>(sizeof(TY)) / 2; ++x)
-            *(reinterpret_cast<uint4*>(sy + (g + 8 * i) * kLuPitch<TY> + 32 * j + 8 * t) + x) = y[j][i].w[x];
-        }
+        for (int x = 0; x < 8; ++x) o[x] = static_cast<TY>(v[x]);
       }
     }
-    if constexpr (!VEC) {
-      __syncwarp();
-      const int col = n0 + 32 * j0 + lane;
-      TY* to = static_cast<TY*>(p.out) + first * p.ldo + col;
-      for (int r = 0; r < rows; ++r)
+    __syncwarp();
+    const int bytes = width * kEsz;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (col + 32 * x < n1) to[r * p.ldo + 32 * x] = sy[r * kLuPitch<TY> + lane + 32 * x];
-      __syncwarp();
+    for (int i0 = 0; i0 < (16 * kPieces + 31) / 32; ++i0) {
+      const int i = 32 * i0 + lane, r = i / kPieces, piece = i - r * kPieces;
+      if (r >= live) continue;
+      uint8_t* at = out_at(r, c0);
+      const int off = past(at), lo = max(off - piece * 16, 0), hi = min(off + bytes - piece * 16, 16);
+      if (lo >= hi) continue;
+      uint8_t* to = at - off + piece * 16;
+      const uint8_t* src = so + r * kPitch + piece * 16;
+      if (lo == 0 && hi == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(src);
+      else
+        for (int x = lo; x < hi; x += kEsz) *reinterpret_cast<TY*>(to + x) = *reinterpret_cast<const TY*>(src + x);
     }
+    __syncwarp();
   }
-  if (!loaded) {  // (a warp without columns)
-    if (p.early) griddep_wait();
-    if (kStaged) __syncthreads();
-  }
+  copy_wait<0>();
 }
 
 // ---------------------------------------------------------------------------- host side
@@ -869,15 +1005,17 @@ b2g_status lora_launch_cluster(const void* kern, int64_t tiles, int64_t S, int t
 template <typename T>
 b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t st) {
   if (d->rows <= kLoraFewRows * d->batch || d->adapters == 0) {  // (without adapters there is nothing to load)
-    const int NT = p.R <= 8 ? 1 : 2;
-    const int64_t items = (d->rows / 16 + d->batch) * ((p.R + 8 * NT - 1) / (8 * NT));
-    // Four CTAs an SM; a warp's part of K is at least one step of its loads.
-    int64_t S = 4ll * sms / items;
+    // 8 rows of A a CTA; 16 where that still leaves every SM two.
+    const int64_t tiles = d->rows / 16 + d->batch;
+    const int NT = p.R > 8 && tiles * ((p.R + 15) / 16) >= 2 * sms ? 2 : 1;
+    const int64_t items = tiles * ((p.R + 8 * NT - 1) / (8 * NT));
+    // Clusters where half of the SMs would have no CTA; a warp's part of K is at least one step of its loads.
+    int64_t S = sms / items;
     const int64_t most = (d->K + 32 * kLrAhead * kLrWarps - 1) / (32 * kLrAhead * kLrWarps);
     S = S > most ? most : S;
     p.splits = static_cast<int>(S < 1 ? 1 : S > 8 ? 8 : S);
-    const void* kern = NT == 1 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 1>)
-                               : reinterpret_cast<const void*>(lora_down_rows_kernel<T, 2>);
+    const void* kern = NT == 2 ? reinterpret_cast<const void*>(lora_down_rows_kernel<T, 2>)
+                               : reinterpret_cast<const void*>(lora_down_rows_kernel<T, 1>);
     void* args[] = {&p};
     return lora_launch_cluster(kern, items, p.splits, 32 * kLrWarps, 0, st, "lora_down_rows launch", args);
   }
@@ -901,34 +1039,43 @@ b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t
   return lora_launch_cluster(reinterpret_cast<const void*>(kern), tiles, p.splits, kLdThreads, smem, st, "lora_down_tiles launch", args);
 }
 
-template <typename T, typename TY, int KK, int WM, bool VEC>
-b2g_status launch_up(LoraParams& p, cudaStream_t st) {
-  constexpr size_t smem = kLuSmem<TY, KK, WM, VEC>;
-  auto kern = lora_up_kernel<T, TY, KK, WM, VEC>;
-  if constexpr (smem > 48 * 1024) {
+b2g_status lora_launch_up(void (*kern)(LoraParams), const LoraParams& p, int64_t tiles, int threads, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
     b2g_status s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
                               "cudaFuncSetAttribute(lora_up)");
     if (s != B2G_OK) return s;
   }
-  p.slices = (p.N + kLuCols<KK, WM, VEC> - 1) / kLuCols<KK, WM, VEC>;
-  const int64_t tiles = static_cast<int64_t>(p.rows) / (16 * WM) + p.batch;
-  return launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.slices)), dim3(kLuThreads), smem, st, "lora_up launch", p);
+  return launch_pdl(kern, dim3(static_cast<unsigned>(tiles * p.slices)), dim3(static_cast<unsigned>(threads)), smem, st, "lora_up launch", p);
 }
-template <typename T, typename TY, int WM, bool VEC>
-b2g_status launch_up(LoraParams& p, cudaStream_t st) {
-  if (p.R <= 32) return launch_up<T, TY, 1, WM, VEC>(p, st);
-  if (p.R <= 64) return launch_up<T, TY, 2, WM, VEC>(p, st);
-  return launch_up<T, TY, 4, WM, VEC>(p, st);
+template <typename T, typename TY, int KK>
+b2g_status launch_up(LoraParams& p, bool few, bool vec, int sms, cudaStream_t st) {
+  if (few) {
+    // As many CTAs as run at the same time, or, with few requests, a step a warp.
+    const int64_t tiles = static_cast<int64_t>(p.rows) / 16 + p.batch, steps = (p.N + 32 * kUrWarps - 1) / (32 * kUrWarps);
+    const int64_t per_sm = KK == 4 ? 2 : KK == 2 ? 3 : 4, slices = per_sm * sms / tiles;
+    p.slices = static_cast<int>(slices < 1 ? 1 : slices < steps ? slices : steps);
+    return lora_launch_up(vec ? lora_up_rows_kernel<T, TY, KK, true> : lora_up_rows_kernel<T, TY, KK, false>, p, tiles, 32 * kUrWarps,
+                          kUrSmem<KK>, st);
+  }
+  p.slices = (p.N + kLuCols - 1) / kLuCols;
+  return lora_launch_up(lora_up_any_kernel<T, TY, KK>, p, static_cast<int64_t>(p.rows) / (16 * kLuWarps) + p.batch, 32 * kLuWarps,
+                        kLuSmem<TY, KK>, st);
+}
+template <typename T, typename TY>
+b2g_status launch_up(LoraParams& p, bool few, bool vec, int sms, cudaStream_t st) {
+  if (p.R <= 32) return launch_up<T, TY, 1>(p, few, vec, sms, st);
+  if (p.R <= 64) return launch_up<T, TY, 2>(p, few, vec, sms, st);
+  return launch_up<T, TY, 4>(p, few, vec, sms, st);
 }
 template <typename T, typename TY>
 b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cudaStream_t st) {
   const bool few = d->rows <= kLoraFewRows * d->batch;
-  if (few) return vec ? launch_up<T, TY, 1, true>(p, st) : launch_up<T, TY, 1, false>(p, st);
+  if (few) return launch_up<T, TY>(p, true, vec, sms, st);
   // TMA: 16-byte aligned rows, whatever their width.
   const int64_t esz = sizeof(TY);
   const bool tma = (p.ldy * esz) % 16 == 0 && (p.ldo * esz) % 16 == 0 && p.adapters > 0 &&
                    ((reinterpret_cast<uintptr_t>(p.y) | reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0;
-  if (!tma) return launch_up<T, TY, 8, false>(p, st);
+  if (!tma) return launch_up<T, TY>(p, false, false, sms, st);
   constexpr int kCols = 128 / sizeof(TY);
   CUtensorMap ty, to, tb;
   b2g_status s;
