@@ -857,28 +857,27 @@ __global__ void __launch_bounds__(32 * kUrWarps) lora_up_rows_kernel(const LoraP
 
 // ---------------------------------------------------------------------------- up, many rows, any alignment
 //
-// Where TMA cannot take y or out: 128 rows and 256 columns a CTA, 16 rows a warp, 64 columns at a time.  B's part is laid out
-// in shared memory as the products take it.  y is copied ahead in whole 16-byte pieces of memory, a piece at either
-// end with values of its neighbours (no piece is read that holds no value of y), so that a row lies in shared memory
-// as far from a 16-byte boundary as in memory; out is made up the same way and leaves in whole pieces, but for the ends.
+// Where TMA cannot take y or out: 128 rows and 256 columns a CTA, 16 rows a warp, 256 bytes of each at a time.  B's part is
+// laid out in shared memory as the products take it.  The products' sums pass through shared memory, so that a lane can
+// take 16 aligned bytes of y's memory, wherever in a row they begin: of a row's values, those in whole pieces of 16
+// bytes first, eight pieces a lane; then the 32 ends of the 16 rows, one a lane, value by value.  (Value by value
+// throughout, through shared memory, the instructions bound it: 79 us for 1536 rows of 21503.)
 constexpr int kLuWarps = 8;
 constexpr int kLuCols = 256;
-constexpr int kLuStages = 3;
 template <typename TY>
-constexpr int kLuPieces = 64 * sizeof(TY) / 16 + 1;           // of a row's 64 values
+constexpr int kLuStep = 256 / sizeof(TY);                  // columns of a step
 template <typename TY>
-constexpr int kLuPitch = (kLuPieces<TY> + 1) * 16;             // bytes from row to row in shared memory
+constexpr int kLuPitch = kLuStep<TY> / 8 * 9 + 1;          // words of a row of sums: 9 to 8 columns, for the banks
 template <typename TY, int KK>
-constexpr size_t kLuSmem = kLuCols / 8 * KK * 32 * sizeof(uint4) + static_cast<size_t>(kLuWarps) * (kLuStages + 1) * 16 * kLuPitch<TY>;
+constexpr size_t kLuSmem = kLuCols / 8 * KK * 32 * sizeof(uint4) + static_cast<size_t>(kLuWarps) * 16 * kLuPitch<TY> * 4;
 
 template <typename T, typename TY, int KK>  // 32 KK >= R
 __global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraParams p) {
-  constexpr int kPieces = kLuPieces<TY>, kPitch = kLuPitch<TY>, kEsz = sizeof(TY);
+  constexpr int kEsz = sizeof(TY), kPiece = 16 / kEsz, kStep = kLuStep<TY>, kPitch = kLuPitch<TY>;
   extern __shared__ __align__(16) uint8_t smem_up[];
-  uint4* sb = reinterpret_cast<uint4*>(smem_up);  // [column group of 8][KK][lane]
+  uint4* sb = reinterpret_cast<uint4*>(smem_up);  // [product][KK][lane]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* sy = smem_up + kLuCols / 8 * KK * 32 * sizeof(uint4) + warp * (kLuStages + 1) * 16 * kPitch;  // y's stages, then out's
-  uint8_t* so = sy + kLuStages * 16 * kPitch;
+  float* sums = reinterpret_cast<float*>(smem_up + kLuCols / 8 * KK * 32 * sizeof(uint4)) + warp * 16 * kPitch;
   const int at_tile = static_cast<int>(blockIdx.x / p.slices), slice = static_cast<int>(blockIdx.x - static_cast<unsigned>(at_tile) * p.slices);
   if (!p.early) griddep_wait();
   griddep_launch_dependents();
@@ -887,35 +886,32 @@ __global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraPa
     if (p.early) griddep_wait();  // (this kernel's end stands for the end of the one in front of it too)
     return;
   }
-  const bool has = tile.adapter >= 0;
-  const int n0 = slice * kLuCols, n1 = min(p.N, n0 + kLuCols), steps = (n1 - n0 + 63) / 64;
+  const bool has = tile.adapter >= 0, gated = p.epilogue == B2G_EPI_GATED_RESIDUAL;
+  const int n0 = slice * kLuCols, n1 = min(p.N, n0 + kLuCols);
   const int first = tile.first + 16 * warp, live = min(16, tile.end - first);
-  // A row's 64 values from column c0 on: their address, and how far it is past a 16-byte boundary.
-  auto y_at = [&](int r, int c0) { return static_cast<const uint8_t*>(p.y) + ((first + r) * p.ldy + c0) * kEsz; };
-  auto out_at = [&](int r, int c0) { return static_cast<uint8_t*>(p.out) + ((first + r) * p.ldo + c0) * kEsz; };
-  auto past = [](const uint8_t* at) { return static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15u); };
-  auto fetch = [&](int step) {
-    const int c0 = n0 + 64 * step, bytes = min(64, n1 - c0) * kEsz;
-    const uint32_t dst = smem_u32(sy + step % kLuStages * 16 * kPitch);
+  // Of row r's columns [c0, c1): its values before the first whole piece of y's memory, and its whole pieces.
+  auto head = [&](int r, int c0, int c1) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(static_cast<const TY*>(p.y) + (first + r) * p.ldy + c0);
+    return min(static_cast<int>((16 - (at & 15u)) & 15u) / kEsz, c1 - c0);
+  };
+  // (pieces of y are pieces of out where the two are as far from a boundary; else all values go one by one)
+  const bool alike = ((reinterpret_cast<uintptr_t>(p.y) - reinterpret_cast<uintptr_t>(p.out)) & 15u) == 0 && ((p.ldy - p.ldo) * kEsz) % 16 == 0;
+  // Whole pieces: 16 lanes to a row, two rows at a time.
+  uint4 y[8];
+  auto load_y = [&](int c0) {
+    const int c1 = min(c0 + kStep, n1);
 #pragma unroll
-    for (int i0 = 0; i0 < (16 * kPieces + 31) / 32; ++i0) {
-      const int i = 32 * i0 + lane, r = i / kPieces, piece = i - r * kPieces;
-      if (r >= live) continue;
-      const uint8_t* at = y_at(r, c0);
-      const int off = past(at);
-      if (piece * 16 < off + bytes) copy16(dst + r * kPitch + piece * 16, at - off + piece * 16, true);
+    for (int i = 0; i < 8; ++i) {
+      const int r = 2 * i + (lane >> 4), c = c0 + head(r, c0, c1) + (lane & 15) * kPiece;
+      if (r < live && c + kPiece <= c1) y[i] = *reinterpret_cast<const uint4*>(static_cast<const TY*>(p.y) + (first + r) * p.ldy + c);
     }
   };
-#pragma unroll
-  for (int i = 0; i < kLuStages - 1; ++i) {
-    if (i < steps) fetch(i);
-    copy_commit();
-  }
+  if (alike) load_y(n0);
   const T* b = static_cast<const T*>(p.b) + (has ? tile.adapter : 0) * p.bs;
   if (has)
 #pragma unroll 4
     for (int i = threadIdx.x; i < kLuCols / 8 * KK * 32; i += 32 * kLuWarps) {
-      const int product = i / (32 * KK), col = n0 + (product >> 2) * 32 + b_column(product & 3, i & 31), k = 32 * (i / 32 % KK) + 8 * (i & 3);
+      const int col = n0 + i / (32 * KK) * 8 + ((i >> 2) & 7), k = 32 * (i / 32 % KK) + 8 * (i & 3);
       sb[i] = col < n1 && k < p.R ? __ldg(reinterpret_cast<const uint4*>(b + col * p.ldb + k)) : make_uint4(0, 0, 0, 0);
     }
   const int row[2] = {first + g, first + g + 8};
@@ -923,58 +919,81 @@ __global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraPa
   LoraRows<T, KK> rows;
   rows.load(p, tile, row, t);
   __syncthreads();
+  auto sum_at = [&](int r, int c) -> float& { return sums[r * kPitch + c + (c >> 3)]; };
 #pragma unroll 1
-  for (int step = 0; step < steps; ++step) {
-    copy_wait<kLuStages - 2>();
-    __syncwarp();  // (all lanes' copies of this step; nobody is at the stage that is filled next)
-    if (step + kLuStages - 1 < steps) fetch(step + kLuStages - 1);
-    copy_commit();
-    const int c0 = n0 + 64 * step, width = min(64, n1 - c0);
-    const uint8_t* from = sy + step % kLuStages * 16 * kPitch;
-    const int y_off[2] = {past(y_at(g, c0)), past(y_at(g + 8, c0))}, o_off[2] = {past(out_at(g, c0)), past(out_at(g + 8, c0))};
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (32 * j >= width) break;
-      float acc[4][4] = {};
+  for (int c0 = n0; c0 < n1; c0 += kStep) {
+    const int c1 = min(c0 + kStep, n1);
+    __syncwarp();
+#pragma unroll 2
+    for (int j = 0; j < kStep / 8; ++j) {
+      if (c0 + 8 * j >= c1) break;
+      float acc[4] = {};
       if (has) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) rows.multiply(acc[i], kk, sb[(((c0 - n0) / 8 + 4 * j + i) * KK + kk) * 32 + lane]);
+        for (int kk = 0; kk < KK; ++kk) rows.multiply(acc, kk, sb[(((c0 - n0) / 8 + j) * KK + kk) * 32 + lane]);
       }
-      float gate[8];
-      load_gate(p, has, c0 + 32 * j + 8 * t, n1, gate);
+      const int c = 8 * j + 2 * t;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int at = (g + 8 * i) * kPitch + (32 * j + 8 * t) * kEsz;
-        const TY* y = reinterpret_cast<const TY*>(from + at + y_off[i]);
-        TY* o = reinterpret_cast<TY*>(so + at + o_off[i]);
-        float v[8];
+      for (int e = 0; e < 2; ++e) {
+        const float by = gated ? (c0 + c + e < c1 ? __ldg(p.gate + c0 + c + e) : 0.f) : 1.f;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = static_cast<float>(y[x]);
-        lora_finish(p, rows, has, i, acc, gate, v);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) o[x] = static_cast<TY>(v[x]);
+        for (int i = 0; i < 2; ++i) {
+          float delta = acc[2 * i + e];
+          if constexpr (std::is_same<T, __half>::value) delta *= rows.unit[i];
+          sum_at(g + 8 * i, c + e) = gated ? (has ? by * delta : 0.f) : delta;
+        }
       }
     }
     __syncwarp();
-    const int bytes = width * kEsz;
+    const float ones[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+    if (alike) {
 #pragma unroll
-    for (int i0 = 0; i0 < (16 * kPieces + 31) / 32; ++i0) {
-      const int i = 32 * i0 + lane, r = i / kPieces, piece = i - r * kPieces;
-      if (r >= live) continue;
-      uint8_t* at = out_at(r, c0);
-      const int off = past(at), lo = max(off - piece * 16, 0), hi = min(off + bytes - piece * 16, 16);
-      if (lo >= hi) continue;
-      uint8_t* to = at - off + piece * 16;
-      const uint8_t* src = so + r * kPitch + piece * 16;
-      if (lo == 0 && hi == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(src);
-      else
-        for (int x = lo; x < hi; x += kEsz) *reinterpret_cast<TY*>(to + x) = *reinterpret_cast<const TY*>(src + x);
+      for (int i = 0; i < 8; ++i) {
+        const int r = 2 * i + (lane >> 4), c = c0 + head(r, c0, c1) + (lane & 15) * kPiece;
+        if (r >= live || c + kPiece > c1) continue;
+        float v[8] = {}, delta[8] = {};
+        const uint32_t w[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+        for (int x = 0; x < kPiece; ++x) {
+          if constexpr (kEsz == 4) v[x] = __uint_as_float(w[x]);
+          else v[x] = static_cast<float>(reinterpret_cast<const TY*>(w)[x]);
+          delta[x] = sum_at(r, c - c0 + x);
+        }
+        lora_out8(gated ? B2G_EPI_NONE : p.epilogue, v, delta, ones);
+        uint4 o;
+        if constexpr (kEsz == 4) o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else o = make_uint4(pack2<TY>(v[0], v[1]), pack2<TY>(v[2], v[3]), pack2<TY>(v[4], v[5]), pack2<TY>(v[6], v[7]));
+        *reinterpret_cast<uint4*>(static_cast<TY*>(p.out) + (first + r) * p.ldo + c) = o;
+      }
+      if (c0 + kStep < n1) load_y(c0 + kStep);
     }
-    __syncwarp();
+    // The ends, a lane each: before the first whole piece, and behind the last.  (not alike: half a row a lane)
+    const int r = lane >> 1;
+    if (r < live) {
+      const int h = head(r, c0, c1);
+      int from = c0, to = c0 + h;
+      if (!alike) to = c0 + kStep / 2;
+      if (lane & 1) {
+        from = alike ? c0 + h + (c1 - c0 - h) / kPiece * kPiece : c0 + kStep / 2;
+        to = c1;
+      }
+      to = min(to, c1);
+      const TY* yr = static_cast<const TY*>(p.y) + (first + r) * p.ldy;
+      TY* o = static_cast<TY*>(p.out) + (first + r) * p.ldo;
+      for (; from < to; from += 8) {
+        float v[8], delta[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          v[x] = from + x < to ? static_cast<float>(yr[from + x]) : 0.f;
+          delta[x] = from + x < to ? sum_at(r, from + x - c0) : 0.f;
+        }
+        lora_out8(gated ? B2G_EPI_NONE : p.epilogue, v, delta, ones);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (from + x < to) o[from + x] = static_cast<TY>(v[x]);
+      }
+    }
   }
-  copy_wait<0>();
 }
 
 // ---------------------------------------------------------------------------- host side
