@@ -998,8 +998,17 @@ __global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraPa
 
 // ---------------------------------------------------------------------------- host side
 
-// Average rows of a request up to which the few-rows forms take a call.
-constexpr int64_t kLoraFewRows = 16;
+// Which form takes a call.  Few rows cost by tiles of 16 rows, each of which reads its adapter, many by tiles of 128, of
+// which a request of 30 rows fills a quarter.  us, few and many, K 4096, N 8192, bf16:
+//   requests x rows   1 x 700      1 x 1536     16 x 64      64 x 32      64 x 64      9 x 75 (rank 64)
+//   down, rank 16     6.7, 7.9     7.2, 8.8     6.4, 8.9     7.7, 13.2    11.1, 13.5   10.4, 9.7
+//   down, rank 128    16.5, 11.5   23.5, 12.5   16.0, 11.8   32.1, 17.2   58.9, 18.8
+//   up, rank 16       10.5, 10.5   19.9, 13.2   15.7, 11.8   30.3, 32.3   72.6, 37.1   13.3, 15.0
+//   up, rank 128      17.8, 21.5   32.4, 31.0   30.8, 41.2   76.0, 103    82.9, 131
+bool few_down(int64_t rows, int64_t batch, int64_t R) {
+  return rows <= (R > 32 ? 16 : 32) * batch || (rows / 16 + batch) * R <= 2600;
+}
+bool few_up(int64_t rows, int64_t batch, int64_t R) { return rows <= (R > 64 ? 64 : 32) * batch || rows <= 768; }
 
 b2g_status lora_launch_cluster(const void* kern, int64_t tiles, int64_t S, int threads, size_t smem, cudaStream_t st,
                                const char* what, void** args) {
@@ -1023,7 +1032,7 @@ b2g_status lora_launch_cluster(const void* kern, int64_t tiles, int64_t S, int t
 
 template <typename T>
 b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t st) {
-  if (d->rows <= kLoraFewRows * d->batch || d->adapters == 0) {  // (without adapters there is nothing to load)
+  if (few_down(d->rows, d->batch, d->R) || d->adapters == 0) {  // (without adapters there is nothing to load)
     // 8 rows of A a CTA; 16 where that still leaves every SM two.
     const int64_t tiles = d->rows / 16 + d->batch;
     const int NT = p.R > 8 && tiles * ((p.R + 15) / 16) >= 2 * sms ? 2 : 1;
@@ -1088,7 +1097,7 @@ b2g_status launch_up(LoraParams& p, bool few, bool vec, int sms, cudaStream_t st
 }
 template <typename T, typename TY>
 b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cudaStream_t st) {
-  const bool few = d->rows <= kLoraFewRows * d->batch;
+  const bool few = few_up(d->rows, d->batch, d->R);
   if (few) return launch_up<T, TY>(p, true, vec, sms, st);
   // TMA: 16-byte aligned rows, whatever their width.
   const int64_t esz = sizeof(TY);

@@ -97,7 +97,7 @@ def check(engine, lens, K, N, R, adapters=3, dtype=BF16, y_dtype=BF16, epilogue=
     assert_within(got, want, bound, (lens, ids))
 
 
-LENGTHS = [[1], [1] * 9, [5, 0, 17, 1], [33, 64, 1, 40], [127, 128, 129], [300, 0, 700, 20], [0, 0, 3, 0]]
+LENGTHS = [[1], [1] * 9, [5, 0, 17, 1], [33, 64, 1, 40], [127, 128, 129], [300, 0, 700, 20], [900, 50], [0, 0, 3, 0]]
 
 
 @pytest.mark.parametrize("lens", LENGTHS)
