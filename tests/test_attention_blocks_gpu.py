@@ -170,6 +170,15 @@ def test_select_blocks_long_caches(engine, lk, top):
     check_choice(engine, [1, 130], [lk, 40000], [lk, 40000], 4, 2, 64, torch.bfloat16, top, 1, 1, True)
 
 
+@pytest.mark.parametrize("lens", [[4100, 300, 129], [500] * 9, [3000, 0, 1700]])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("hq,hk,d,dtype", [(24, 24, 128, torch.bfloat16), (48, 24, 64, torch.float16)])
+def test_select_blocks_many_tiles(engine, lens, causal, hq, hk, d, dtype):
+    """Four tiles a CTA, of one sequence and of two, the last ones of none."""
+    check_choice(engine, lens, lens, lens, hq, hk, d, dtype, 5, 1, 1, causal, sum(lens))
+    check_choice(engine, lens, [max(0, n - 150) for n in lens], lens, hq, hk, d, dtype, 2, 0, 0, causal, sum(lens))
+
+
 @pytest.mark.parametrize("blocks", [20, 600])
 @pytest.mark.parametrize("top", [1, 6, 19, 64])
 def test_select_blocks_ties_and_odd_scores(engine, blocks, top):
