@@ -41,6 +41,7 @@ __device__ __forceinline__ int key_blocks(const PkParams& p, int b) {  // with r
 // Blocks before sequence b's first (the whole warp).
 __device__ __forceinline__ int blocks_before(const PkParams& p, int b, int lane) {
   int sum = 0;
+#pragma unroll 4
   for (int i = lane; i < b; i += 32) sum += key_blocks(p, i);
   return __reduce_add_sync(0xffffffffu, sum);
 }
@@ -70,9 +71,10 @@ __global__ void __launch_bounds__(32 * kMnWarps) block_means_kernel(const MnPara
   const int step = a.since ? static_cast<int>(gridDim.z) : 1;
   if (a.since) {  // sequence blockIdx.x, its blocks from the one of key since[b] on
     b = blockIdx.x;
-    base = blocks_before(p, b, lane);
+    const int since = __ldg(a.since + b);
     const Seq s = load_seq(p, b);
-    j = clampi(__ldg(a.since + b), 0, s.lk) / kPtKeys + static_cast<int>(blockIdx.z);
+    base = blocks_before(p, b, lane);
+    j = clampi(since, 0, s.lk) / kPtKeys + static_cast<int>(blockIdx.z);
     stop = (s.lk + kPtKeys - 1) / kPtKeys;
   } else {        // row blockIdx.x of the means
     base = 0;
@@ -209,6 +211,7 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
       }
 #pragma unroll
       for (int u = 0; u < kAheadQ; ++u) {
+        if (i0 - from + u * kGroups >= items) break;  // (for the whole CTA)
         float f[8] = {};
         add8<T>(f, v[u]);
 #pragma unroll
@@ -423,11 +426,10 @@ struct CrLine {
   long long total;
   int shares;
 };
-// Inclusive sums of n values given by value(i), to ends.
-template <int kThreads, typename I, typename Value>
-__device__ __forceinline__ void sums_of(int n, I* ends, long long* carry, Value value) {
+// Inclusive sums of the n values in `ends`.
+template <int kThreads, typename I>
+__device__ __forceinline__ void sums_of(int n, I* ends, long long* carry) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < n; i += kThreads) ends[i] = value(i);
   __syncthreads();
   I base = 0;
   for (int i0 = 0; i0 < n; i0 += kThreads) {
@@ -452,19 +454,61 @@ __device__ __forceinline__ void sums_of(int n, I* ends, long long* carry, Value 
 }
 template <int kThreads>
 __device__ __forceinline__ CrLine chosen_line(const PkParams& p, long long* ends, int* mask_tiles, long long* carry) {
-  sums_of<kThreads>(p.batch, mask_tiles, carry, [&](int b) {
+  for (int b = threadIdx.x; b < p.batch; b += kThreads) {
     const int lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
-    return (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
-  });
-  const int pairs = p.batch * p.hk;
-  sums_of<kThreads>(pairs, ends, carry, [&](int i) {
-    const int b = i / p.hk;
-    const Seq s = load_seq(p, b);
-    const int tiles = chosen_tiles_of(p, s.lq), before = mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows;
-    long long sum = 0;
-    for (int t = 0; t < tiles; ++t) sum += chosen_length(chosen_tile(p, s, i - b * p.hk, t, before));
-    return sum;
-  });
+    mask_tiles[b] = (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+  }
+  sums_of<kThreads>(p.batch, mask_tiles, carry);
+  // A thread takes kAhead pairs, whose loads go out together: of sequences with one tile of rows (most of them) four
+  // words at a time; others' tiles one after the other.
+  constexpr int kAhead = 4;
+  const int pairs = p.batch * p.hk, words = p.chosen_words;
+  for (int i0 = threadIdx.x; i0 < pairs; i0 += kAhead * kThreads) {
+    const uint32_t* from[kAhead];
+    int tiles[kAhead], nb[kAhead], keys[kAhead], count[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = min(i0 + u * kThreads, pairs - 1), b = i / p.hk;
+      const Seq s = load_seq(p, b);
+      const int before = mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows;
+      tiles[u] = chosen_tiles_of(p, s.lq);
+      keys[u] = s.lk;  // (a sequence's last query sees every key)
+      nb[u] = tiles[u] == 1 && before < p.chosen_tiles ? min((s.lk + kPtKeys - 1) / kPtKeys, 32 * words) : 0;
+      from[u] = p.chosen + (static_cast<long long>(before) * p.hk + i - b * p.hk) * words;
+      count[u] = 0;
+    }
+    for (int w0 = 0; w0 < words; w0 += 4) {
+      uint32_t bits[kAhead][4];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bits[u][w] = 32 * (w0 + w) < nb[u] ? __ldg(from[u] + w0 + w) : 0u;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int left = nb[u] - 32 * (w0 + w);  // of the word's blocks in sight
+          const uint32_t in = left >= 32 ? bits[u][w] : left > 0 ? bits[u][w] & ((1u << left) - 1u) : 0u;
+          count[u] += 8 * __popc(in);
+          if (left > 0 && left <= 32 && (in >> (left - 1) & 1u))  // the last block, of which only chunks with keys count
+            count[u] -= 8 - (min(keys[u] - (nb[u] - 1) * kPtKeys, kPtKeys) + kCrKeys - 1) / kCrKeys;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i >= pairs) continue;
+      long long sum = tiles[u] == 1 ? count[u] + kCrTileCost : 0;
+      if (tiles[u] > 1) {
+        const int b = i / p.hk;
+        const Seq s = load_seq(p, b);
+        for (int tile = 0; tile < tiles[u]; ++tile)
+          sum += chosen_length(chosen_tile(p, s, i - b * p.hk, tile, mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows));
+      }
+      ends[i] = sum;
+    }
+  }
+  sums_of<kThreads>(pairs, ends, carry);
   const long long total = ends[pairs - 1], most = (total + kCrMinShare - 1) / kCrMinShare;
   return {ends, mask_tiles, total, static_cast<int>(min(static_cast<long long>(p.shares), most))};
 }
@@ -584,18 +628,16 @@ __device__ __forceinline__ void chosen_part(const PkParams& p, const CrTile& til
         for (int k = 0; k < VC; ++k) copy16(dst + (2 * KC + i * VC + k) * 512, src + 64 * k, live);
       }
     };
-    int ahead = c0 + warp;
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i, ahead += kCrWarps) {
-      if (ahead < c1) fetch(ahead, i);
-      copy_commit();
-    }
-    int st = 0;
-    for (int c = c0 + warp; c < c1; c += kCrWarps) {
-      copy_wait<NS - 2>();
-      if (ahead < c1) fetch(ahead, st == 0 ? NS - 1 : st - 1);  // (the stage used up in the last round)
+    // The first NS - 1 rounds only copy.  (One place in the code for all copies: a kernel begins with its instructions far away.)
+    int ahead = c0 + warp, ahead_st = 0, st = 0;
+#pragma unroll 1
+    for (int c = c0 + warp - (NS - 1) * kCrWarps; c < c1; c += kCrWarps) {
+      if (ahead < c1) fetch(ahead, ahead_st);  // (the stage used up in the last round)
       copy_commit();
       ahead += kCrWarps;
+      ahead_st = ahead_st + 1 == NS ? 0 : ahead_st + 1;
+      if (c < c0) continue;
+      copy_wait<NS - 1>();
       const uint32_t src = ring + st * kStage;
       st = st + 1 == NS ? 0 : st + 1;
       float sc[2][4] = {};
@@ -931,7 +973,7 @@ b2g_status block_means(const b2g_attention_packed_desc* d, const int32_t* since,
   if (parts > 65535) return set_error(B2G_ERR_UNSUPPORTED, "b2g_block_means: size");
   int64_t z = 1;
   if (since) {  // as many blocks of a sequence side by side as the SMs have room for
-    z = 8ll * dev->num_sms / (d->batch * parts);
+    z = 2ll * dev->num_sms / (d->batch * parts);
     z = z < 1 ? 1 : z > blocks ? blocks : z;
     if (z > 65535) z = 65535;
   }
