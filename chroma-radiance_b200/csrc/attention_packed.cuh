@@ -292,8 +292,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   }
   griddep_wait();  // the set-up above overlapped the previous kernel's tail
   griddep_launch_dependents();
-  // (a tile's row of `chosen` counts the tiles in front of its sequence; chosen blocks even out the tiles' work)
-  const bool sorted = !kChosen && p.batch <= kPtSorted;
+  const bool sorted = p.batch <= kPtSorted;
   if (sorted) {
     // Rank of each sequence by its keys (the counts pass through Q's space, still unused).
     int* count = reinterpret_cast<int*>(sQ);
@@ -327,6 +326,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int head_units = (p.hq + item_heads - 1) / item_heads;
       const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
       int units_before = 0, i = 0;
+      [[maybe_unused]] int tiles_of = -1, tiles_before = 0;  // kChosen: tiles in front of sequence tiles_of
       Turn<kPtItems> at;
       for (int round = 0; i >= 0; ++round) {
         const long long index = static_cast<long long>(round) * grid + (round & 1 ? grid - 1 - cta : cta);
@@ -341,6 +341,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         w.head = -1;
         if (i >= 0) {
           const Seq s = load_seq(p, seq_of(i));
+          if constexpr (kChosen) {
+            if (tiles_of != seq_of(i)) {
+              tiles_of = seq_of(i);
+              int sum = 0;
+              for (int b = lane; b < tiles_of; b += 32) {
+                const int lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
+                sum += (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+              }
+              tiles_before = __reduce_add_sync(0xffffffffu, sum);
+            }
+          }
           w.q0 = s.q0;
           w.lq = s.lq;
           w.k0 = s.k0;
@@ -354,7 +365,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (p.causal) n = clampi(min(row + kPtRows, s.lq) + s.lk - s.lq, 0, n);
             w.blocks[t] = (n + kPtKeys - 1) / kPtKeys;
             if constexpr (kChosen) {
-              w.tile = units_before + w.row0 / kPtRows;
+              w.tile = tiles_before + w.row0 / kPtRows;
               const int nb = w.tile < p.chosen_tiles ? min(w.blocks[t], 32 * p.chosen_words) : 0;
               const uint32_t* words =
                   p.chosen + (static_cast<long long>(w.tile) * p.hk + min((w.head + t) / p.group, p.hk - 1)) * p.chosen_words;
