@@ -46,14 +46,18 @@ __device__ __forceinline__ int blocks_before(const PkParams& p, int b, int lane)
   return __reduce_add_sync(0xffffffffu, sum);
 }
 
+// Two values of a word.
+template <typename T>
+__device__ __forceinline__ float2 two(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
 template <typename T>
 __device__ __forceinline__ void add8(float (&sum)[8], uint4 v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 f;
-    if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    else f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    const float2 f = two<T>(w[i]);
     sum[2 * i] += f.x;
     sum[2 * i + 1] += f.y;
   }
@@ -212,10 +216,12 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
 #pragma unroll
       for (int u = 0; u < kAheadQ; ++u) {
         if (i0 - from + u * kGroups >= items) break;  // (for the whole CTA)
-        float f[8] = {};
-        add8<T>(f, v[u]);
+        const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) add_pair(hi[x], lo[x], f2_pack(__float_as_uint(f[2 * x]), __float_as_uint(f[2 * x + 1])));
+        for (int x = 0; x < 4; ++x) {
+          const float2 f = two<T>(w[x]);
+          add_pair(hi[x], lo[x], f2_pack(__float_as_uint(f.x), __float_as_uint(f.y)));
+        }
       }
     }
     double sum[8];

@@ -1060,6 +1060,8 @@ b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t
   p.stages = static_cast<int>(100 * 1024 / ld_stage_bytes(Rp));
   if (p.stages > kLdMostStages) p.stages = kLdMostStages;
   const size_t smem = 1024 + static_cast<size_t>(p.stages) * ld_stage_bytes(Rp);
+  if (static_cast<size_t>(p.stages) * ld_stage_bytes(Rp) < sizeof(float) * kLdRows * (Rp + 4))  // (the sums take the ring's place)
+    return set_error(B2G_ERR_UNSUPPORTED, "b2g_lora_down: shared memory");
   auto kern = lora_down_tiles_kernel<T>;
   s = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 110 * 1024), "cudaFuncSetAttribute(lora_down)");
   if (s != B2G_OK) return s;
