@@ -547,13 +547,13 @@ __global__ void __launch_bounds__(kUtThreads)
         const int r = warp * 16 + at;
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < rows && k < p.R) f = *reinterpret_cast<const float4*>(p.t + static_cast<long long>(tile.first + r) * p.ldt + k);
-        float down = s;
+        f.x *= s; f.y *= s; f.z *= s; f.w *= s;
+        float down = 1.f;  // (times s might be infinite, and a row of zeros then no number)
         if constexpr (std::is_same<T, __half>::value) {
-          float top = fmaxf(fmaxf(fabsf(f.x * s), fabsf(f.y * s)), fmaxf(fabsf(f.z * s), fabsf(f.w * s)));
+          float top = fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w)));
           for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const float unit = row_unit(top, &down);
           if (k == 0) units[r] = unit;
-          down *= s;
         }
         uint2 hi, lo;
         split2<T>(f.x * down, f.y * down, &hi.x, &lo.x);

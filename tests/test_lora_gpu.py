@@ -270,3 +270,16 @@ def test_lora_past_32_bits_of_elements(engine):
         part = slice(lo, lo + 2)
         want, bound = plain(x[part], a, b, torch.zeros((2, N), dtype=BF16, device=DEV), [2], [i], None, "none", None)
         assert_within(y[part], want, bound)
+
+
+@pytest.mark.parametrize("lens", [[3, 1, 6], [40, 70, 9], [500, 40, 390]])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("R", [16, 64, 128])
+def test_lora_rows_of_zeros_with_large_scales(engine, lens, dtype, R):
+    x, a, b, y = inputs(lens, 128, 264, R, 3, dtype, F32, R)
+    x[::2] = 0
+    scale = torch.tensor([1.0, 8.0, 4096.0], device=DEV)
+    got = engine.lora(x, a, b, y, offsets(lens), scale=scale)
+    assert torch.equal(got[::2], y[::2])
+    want, bound = plain(x, a, b, y, lens, [0, 1, 2], scale, "none", None)
+    assert_within(got, want, bound)
