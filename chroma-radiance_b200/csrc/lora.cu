@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kLdThreads)
       uint8_t* at = ring + stage * stage_bytes;
       mbar_arrive_expect_tx(&full[stage], stage_bytes);
       tma_load_3d(at, &tmX, &full[stage], (k0 + i) * 64, tile.first, 0, once);
-      tma_load_3d(at + kLdRows * 128, &tmA, &full[stage], (k0 + i) * 64, 0, tile.adapter, shared);
+      tma_load_3d(at + kLdRows * 128, &tmA, &full[stage], (k0 + i) * 64, 0, p.as != 0 ? tile.adapter : 0, shared);
       ++used;
       if (++stage == p.stages) {
         stage = 0;
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kUtThreads)
         for (int w = 0; w < groups; ++w) tma_load_3d(at + w * 4096, &tmY, &full[stage], col, tile.first + 32 * w, 0, once);
         if (has)
           for (int a = 0; a < ly.atoms; ++a)
-            tma_load_3d(at + kUtRows * 128 + a * kCols * 128, &tmB, &full[stage], a * 64, col, tile.adapter, shared);
+            tma_load_3d(at + kUtRows * 128 + a * kCols * 128, &tmB, &full[stage], a * 64, col, p.bs != 0 ? tile.adapter : 0, shared);
         ++used;
         if (++stage == p.stages) {
           stage = 0;
@@ -1051,7 +1051,9 @@ b2g_status run_down(const b2g_lora_desc* d, LoraParams& p, int sms, cudaStream_t
   CUtensorMap tx, ta;
   b2g_status s;
   if ((s = make_operand_map(&tx, p.x, d->dtype, p.K, p.rows, p.ldx, 1, p.ldx * p.rows, kLdRows)) != B2G_OK) return s;
-  if ((s = make_operand_map(&ta, p.a, d->dtype, p.K, p.R, p.lda, p.adapters, p.as, static_cast<uint32_t>(Rp))) != B2G_OK) return s;
+  if ((s = make_operand_map(&ta, p.a, d->dtype, p.K, p.R, p.lda, p.as != 0 ? p.adapters : 1, p.as != 0 ? p.as : p.lda * p.R,
+                            static_cast<uint32_t>(Rp))) != B2G_OK)  // (a stride of 0: one matrix for all)
+    return s;
   const int64_t tiles = d->rows / kLdRows + d->batch;
   int64_t S = 2ll * sms / tiles;
   const int64_t most = (d->K + 255) / 256;
@@ -1112,7 +1114,9 @@ b2g_status run_up(const b2g_lora_desc* d, LoraParams& p, bool vec, int sms, cuda
   if ((s = make_operand_map(&ty, p.y, d->y_dtype, p.N, p.rows, p.ldy, 1, p.ldy * p.rows, 32)) != B2G_OK) return s;
   if ((s = make_operand_map(&to, p.out, d->y_dtype, p.N, p.rows, p.ldo, 1, p.ldo * p.rows, 32)) != B2G_OK) return s;
   const UtLayout ly = ut_layout(p.R, kCols);
-  if ((s = make_operand_map(&tb, p.b, d->dtype, p.R, p.N, p.ldb, p.adapters, p.bs, kCols, ly.b_row)) != B2G_OK) return s;
+  if ((s = make_operand_map(&tb, p.b, d->dtype, p.R, p.N, p.ldb, p.bs != 0 ? p.adapters : 1, p.bs != 0 ? p.bs : p.ldb * p.N, kCols,
+                            ly.b_row)) != B2G_OK)
+    return s;
   // Two CTAs an SM where three stages fit beside the A operand, else one.
   const int two = static_cast<int>((111 * 1024 - ly.a_bytes) / ly.stage), one = static_cast<int>((225 * 1024 - ly.a_bytes) / ly.stage);
   p.stages = two >= 3 ? two : one;

@@ -283,3 +283,19 @@ def test_lora_rows_of_zeros_with_large_scales(engine, lens, dtype, R):
     assert torch.equal(got[::2], y[::2])
     want, bound = plain(x, a, b, y, lens, [0, 1, 2], scale, "none", None)
     assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("lens", [[1, 3, 2], [40, 70, 9], [500, 40, 390]])
+@pytest.mark.parametrize("R", [16, 128])
+def test_lora_one_matrix_for_all_adapters(engine, lens, R):
+    """Adapters that share A or B, and differ in their scale: views with a stride of 0; and others apart by part of a row."""
+    x, a, b, y = inputs(lens, 128, 264, R, 3, BF16, BF16, R)
+    scale = torch.tensor([0.5, 1.0, 2.0], device=DEV)
+    one_a, one_b = a[:1].expand(3, R, 128), b[:1].expand(3, 264, R)
+    woven_a = a.transpose(0, 1).contiguous().transpose(0, 1)
+    woven_b = b.transpose(0, 1).contiguous().transpose(0, 1)
+    for va, vb in ((one_a, b), (a, one_b), (one_a, one_b), (woven_a, woven_b)):
+        got = engine.lora(x, va, vb, y, offsets(lens), scale=scale)
+        want, bound = plain(x, va, vb, y, lens, [0, 1, 2], scale, "none", None)
+        assert_within(got, want, bound)
+        assert torch.equal(got, engine.lora(x, va.contiguous(), vb.contiguous(), y, offsets(lens), scale=scale))
