@@ -432,3 +432,65 @@ def test_no_rows_no_keys(engine):
     empty = offsets([])
     assert engine.block_means(k, empty).shape[0] == 0
     assert engine.attention_blocks(q[:0], k, v, chosen[:0], empty).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("hq,hk,d,dtype", [(8, 4, 128, torch.bfloat16), (4, 4, 64, torch.float16)])
+def test_attention_blocks_many_short_sequences(engine, causal, hq, hk, d, dtype):
+    """Hundreds of sequences with few queries: more pairs of sequence and key head than one line holds."""
+    lq = [(1, 2, 0, 1, 17)[i % 5] for i in range(300)]
+    lk = [(40, 1, 300, 0, 130)[i % 5] for i in range(300)]
+    check_attention(engine, *qkv(sum(lq), sum(lk), hq, hk, d, dtype, 31), random_choice(lq, lk, hk, 32, extra=1), lq, lk, causal)
+
+
+@pytest.mark.parametrize("lq", [[1, 1], [150, 90]])
+def test_blocks_past_32_bits_of_elements(engine, lq):
+    """Keys and values whose rows lie far apart in one buffer of more than 2^31 elements."""
+    lk, hq, hk, d, ld = [700, 400], 4, 2, 128, 1 << 21
+    buf = torch.empty(sum(lk) * ld, dtype=torch.bfloat16, device=DEV)
+    k = buf.as_strided((sum(lk), hk, d), (ld, d, 1))
+    v = buf.as_strided((sum(lk), hk, d), (ld, d, 1), hk * d)
+    q, near_k, near_v = qkv(sum(lq), sum(lk), hq, hk, d, torch.bfloat16, 33)
+    k.copy_(near_k)
+    v.copy_(near_v)
+    means = engine.block_means(k, offsets(lk))
+    assert torch.equal(means, engine.block_means(near_k, offsets(lk)))
+    chosen = engine.select_blocks(q, means, offsets(lq), 2, cu_k=offsets(lk), last=1)
+    got = engine.attention_blocks(q, k, v, chosen, offsets(lq), cu_k=offsets(lk))
+    assert torch.equal(got, engine.attention_blocks(q, near_k, near_v, chosen, offsets(lq), cu_k=offsets(lk)))
+
+
+def test_blocks_on_several_streams_at_once(engine):
+    """Calls side by side on four streams, and two captured graphs replayed side by side: workspaces of their own."""
+    lq, lk, hq, hk, d = [1] * 6, [3000, 20, 700, 1500, 0, 4000], 8, 2, 128
+    cu_q, cu_k = offsets(lq), offsets(lk)
+    sets = [qkv(6, sum(lk), hq, hk, d, torch.bfloat16, 40 + i) for i in range(4)]
+
+    def run(i, stream=None):
+        q, k, v = sets[i]
+        means = engine.block_means(k, cu_k, stream=stream)
+        chosen = engine.select_blocks(q, means, cu_q, 4, cu_k=cu_k, first=1, last=1, stream=stream)
+        return engine.attention_blocks(q, k, v, chosen, cu_q, cu_k=cu_k, stream=stream)
+
+    want = [run(i) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(20):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(run(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(i))
+        graphs.append(graph)
+    for _ in range(20):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
