@@ -21,7 +21,7 @@ namespace {
 
 // ---------------------------------------------------------------------------- means of blocks
 //
-// Bound by memory: k is read once.  A warp reads 512 bytes of a key's row (8 values a lane) for 32 of the block's
+// Bound by memory: k is read once (16384 keys of 24 heads of 128: 20.7 to 23.9 us, 4.3 to 4.9 TB/s).  A warp reads 512 bytes of a key's row (8 values a lane) for 32 of the block's
 // keys, kMnAhead loads at a time; the four warps' sums meet in shared memory in a fixed order.
 constexpr int kMnWarps = 4;
 constexpr int kMnAhead = 8;
@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(32 * kMnWarps) block_means_kernel(const MnPara
 
 // ---------------------------------------------------------------------------- choice of blocks
 //
-// Scores are sums of 64 bits: a choice compares neighbours, and any rounding of theirs in 32 bits would decide
+// Bound by instructions, not by q's bytes (16384 queries of 24 heads: 46.9 us, floor 15.6): the summing of the queries and the
+// scores after it do not overlap.  Scores are sums of 64 bits: a choice compares neighbours, and any rounding of theirs in 32 bits would decide
 // the choice where two are close; in 64 bits the order of a sum moves one in some 10^12.
 constexpr int kSlThreads = 256;
 constexpr int kSlMostWords = 256;
@@ -361,7 +362,8 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
 
 // ---------------------------------------------------------------------------- few rows over chosen blocks
 //
-// The query rows of one key head (lq tokens x group heads) in tiles of 16.  The products, the lanes' layout and the
+// Bound by memory where caches are long, by round trips otherwise (48 single queries, 32 heads on 8, 18 blocks: 39.4 us for
+// 97 MB with the join).  The query rows of one key head (lq tokens x group heads) in tiles of 16.  The products, the lanes' layout and the
 // copies are those of packed_rows_kernel (attention_packed.cu): in a CTA the warps take 16 keys of the chosen blocks in turn.
 //
 // Pairs of a sequence and a key head choose different numbers of blocks (an empty cache none, a long one all that it
@@ -375,7 +377,9 @@ constexpr int kCrKeys = 16;
 constexpr int kCrBlocksPerSm = 2;
 constexpr int kCrListed = 256;  // chosen blocks that are listed at a time
 constexpr int kCrPairs = 1024;
-constexpr int kCrTileCost = 12;  // what a tile costs beside its chunks, in chunks
+// What a tile costs beside its chunks, in chunks.  (64 caches of up to 700 keys: 4 50.1 us, 12 43.2, 24 45.8; 48 of up to 16383:
+// 94.1, 92.7, 93.7)
+constexpr int kCrTileCost = 12;
 constexpr int kCrMinShare = 16;  // a share is at least so long
 template <int D>
 constexpr int kCrPieces = D / 8;
@@ -856,8 +860,20 @@ __global__ void __launch_bounds__(kCcThreads) chosen_combine_kernel(const PkPara
 
 // ---------------------------------------------------------------------------- host side
 
-// Average queries per sequence up to which chosen_rows takes a call, as in attention_packed.cu.
-constexpr int64_t kCrQueries = 16;
+// Which form takes a call.  chosen_rows costs by tiles of 16 rows of a key head's group, each of which reads its keys,
+// packed_tiles by heads of q.  us, rows and tiles, d 128, 48 sequences with 18 of 32 blocks or 4 with 26 of 128:
+//   q heads, key heads    1 query      8 queries    16 queries
+//   32, 8    48           -            210, 242     391, 242
+//   16, 8    48           106, 124     115, 127     210, 127
+//   32, 4    4            20.7, 58.1   44.4, 58.2   71.5, 58.3
+//   8, 8     4            26.5, 57.6   28.0, 57.8   31.4, 57.9
+// Heads of their own leave nothing to share, and tiles of many long caches stream faster (8 heads: 128 of 4096 keys
+// 253, 202; 64: 135, 110; 48: 106, 103; 24 heads: 64 of 1500 249, 206, but 64 of 300 69, 72 and of 40 30, 47).
+bool few_queries(const b2g_attention_packed_desc* d, int sms) {
+  const int64_t group = d->n_head / d->n_kv_head;
+  if (d->total_q > 8 * d->batch && d->total_q * group > kCrRows * d->batch) return false;
+  return group > 1 || d->batch * d->n_kv_head < 3ll * sms || d->total_k < 8 * kPtKeys * d->batch;
+}
 
 // What a call runs, from its sizes alone.
 struct CrPlan {
@@ -867,7 +883,7 @@ struct CrPlan {
 };
 CrPlan chosen_plan(const b2g_attention_packed_desc* d, int64_t words, int sms) {
   CrPlan r;
-  r.rows = d->total_q <= kCrQueries * d->batch || d->total_k == 0;
+  r.rows = d->total_k == 0 || few_queries(d, sms);
   if (!r.rows || d->batch * d->n_kv_head > kCrPairs) return r;
   // A share a CTA, as many as run at the same time; no more than the longest line possible has pieces of kCrMinShare.
   const int64_t tiles = (d->total_q * (d->n_head / d->n_kv_head) / kCrRows + d->batch) * d->n_kv_head;
@@ -904,7 +920,9 @@ b2g_status run_chosen(const b2g_attention_packed_desc* d, PkParams p, const CrPl
   if ((s = make_operand_map(&tk, p.k, d->dtype, D, p.total_k, p.ldk, p.hk, p.hsk, kPtKeys)) != B2G_OK) return s;
   if ((s = make_operand_map(&tv, p.v, d->dtype, D, p.total_k, p.ldv, p.hk, p.hsv, kPtKeys)) != B2G_OK) return s;
   p.item_heads = 2;
-  if ((static_cast<int64_t>(p.total_q) / kPtRows + p.batch) * p.hq <= sms) {  // (every tile finds an SM of its own)
+  // A head a CTA where every tile finds an SM of its own (512 tokens of 24 heads 16.1 us against 17.9 with two; twice 512,
+  // where they do not, 26.9 and 19.3).
+  if ((static_cast<int64_t>(p.total_q) / kPtRows + p.batch) * p.hq <= sms) {
     p.item_heads = 1;
     return launch_tiles<T, D, kHeadsApart, true>(p, tq, tk, tv, sms, st);
   }
@@ -1014,8 +1032,9 @@ b2g_status select_blocks(const b2g_attention_packed_desc* d, const float* means,
   a.chosen = reinterpret_cast<uint32_t*>(chosen);
   a.tiles = static_cast<int>(tiles);
   a.words = static_cast<int>(words);
-  // Four tiles a CTA, which share the means, where that leaves CTAs for all SMs and their scores fit.
-  const bool four = tiles / 4 * d->n_kv_head >= dev->num_sms && d->total_q > 64 * d->batch && words <= kSlMostWords / 4;
+  // Four tiles a CTA, which share the means, where that leaves CTAs for all SMs and their scores fit.  (24 heads, us, one and
+  // four: 16384 tokens 62.5, 46.0; 4096 16.1, 16.6; 2048 10.5, 12.5; 16 x 512 22.7, 21.4; 32 x 300 28.8, 30.9)
+  const bool four = tiles / 4 * d->n_kv_head >= dev->num_sms && d->total_q >= 512 * d->batch && words <= kSlMostWords / 4;
   auto run = [&](auto kern, int nt) {
     const size_t sums = static_cast<size_t>(nt) * kSlThreads / 32 * (d->d_head + 4) * 8, smem = sums + static_cast<size_t>(nt) * words * 32 * 8;
     b2g_status st2 = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024),

@@ -494,3 +494,18 @@ def test_blocks_on_several_streams_at_once(engine):
                 graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("n,hq,hk", [(64, 8, 8), (130, 4, 4), (64, 16, 8)])
+def test_attention_blocks_many_long_caches(engine, causal, n, hq, hk):
+    """Single queries to many caches, of which most are in use: heads of their own go to tiles, groups to rows."""
+    lq, lk = [1 + (i == 3) for i in range(n)], [1300 - 11 * (i % 30) for i in range(n)]
+    check_attention(engine, *qkv(sum(lq), sum(lk), hq, hk, 128, torch.bfloat16, n), random_choice(lq, lk, hk, 32), lq, lk, causal)
+
+
+@pytest.mark.parametrize("lq", [8, 9, 16, 17])
+@pytest.mark.parametrize("hq,hk", [(2, 2), (4, 2), (8, 1)])
+def test_attention_blocks_between_the_forms(engine, lq, hq, hk):
+    lens, lk = [lq] * 5, [700, 3, 130, 0, 1024]
+    check_attention(engine, *qkv(5 * lq, sum(lk), hq, hk, 64, torch.float16, lq), random_choice(lens, lk, hk, lq), lens, lk, True)
