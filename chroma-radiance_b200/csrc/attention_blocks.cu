@@ -21,10 +21,11 @@ namespace {
 
 // ---------------------------------------------------------------------------- means of blocks
 //
-// Bound by memory: k is read once (16384 keys of 24 heads of 128: 20.7 to 23.9 us, 4.3 to 4.9 TB/s).  A warp reads 512 bytes of a key's row (8 values a lane) for 32 of the block's
+// Bound by memory: k is read once (16384 keys of 24 heads of 128: 20.1 us, 5.1 TB/s).  A warp reads 512 bytes of a key's row (8 values a lane) for 32 of the block's
 // keys, kMnAhead loads at a time; the four warps' sums meet in shared memory in a fixed order.
 constexpr int kMnWarps = 4;
 constexpr int kMnAhead = 8;
+constexpr int kMnPerSm = 12;  // CTAs an SM (the compiler's own choice is 10: 23.8 us; 16: 20.7)
 constexpr int kMnCols = 256;  // values of a row that a block takes
 
 struct MnParams {
@@ -64,7 +65,7 @@ __device__ __forceinline__ void add8(float (&sum)[8], uint4 v) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kMnWarps) block_means_kernel(const MnParams a) {
+__global__ void __launch_bounds__(32 * kMnWarps, kMnPerSm) block_means_kernel(const MnParams a) {
   __shared__ float4 sums[kMnWarps][2][32];
   const PkParams& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
