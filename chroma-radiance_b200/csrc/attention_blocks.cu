@@ -43,7 +43,7 @@ __device__ __forceinline__ int key_blocks(const PkParams& p, int b) {  // with r
 __device__ __forceinline__ int blocks_before(const PkParams& p, int b, int lane) {
   int sum = 0;
 #pragma unroll 4
-  for (int i = lane; i < b; i += 32) sum += key_blocks(p, i);
+  for (int i = lane; i < b; i += 32) sum = add_count(sum, key_blocks(p, i));
   return __reduce_add_sync(0xffffffffu, sum);
 }
 
@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
     int mask_tiles = 0;
     for (int i = lane; i < b; i += 32) {
       const int lo = clampi(__ldg(p.cu_q + i), 0, p.total_q);
-      mask_tiles += (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+      mask_tiles = add_count(mask_tiles, (clampi(__ldg(p.cu_q + i + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows);
     }
     const CrTile tile = chosen_tile(p, load_seq(p, b), head, at_tile - before, __reduce_add_sync(0xffffffffu, mask_tiles));
     chosen_part<T, D>(p, tile, 0, chosen_length(tile) - kCrTileCost, -1, smem_rows, sml, list);

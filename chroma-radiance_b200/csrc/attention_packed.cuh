@@ -51,6 +51,10 @@ __device__ __forceinline__ Seq load_seq(const PkParams& p, int b) {
   if (p.k_lens) s.lk = clampi(__ldg(p.k_lens + b), 0, s.lk);
   return s;
 }
+// A lane's sum of sequences' tiles or blocks.  Rising offsets give at most 2^30 / 128 + 65536; those that jump back and forth
+// count rows again and again, and their sum stops where 32 lanes' sums and a sequence's blocks still fit 32 bits: what such a sum
+// is compared with (rows of `means`, of `chosen`) then bounds it, as no wrapped one could be.
+__device__ __forceinline__ int add_count(int sum, int n) { return min(sum + n, 1 << 25); }
 
 // The sequence that holds unit `want` when sequence b holds count(b) units, and the number of units
 // before it; -1 if there are not so many.  A whole warp searches, 32 sequences at a time, from
@@ -324,6 +328,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // ---------------------------------------------------------- work items
       const int item_heads = kApart ? p.item_heads : kMode == kTilesOfHead ? 1 : 2;
       const int head_units = (p.hq + item_heads - 1) / item_heads;
+      const int most_units = p.total_q / kSpan + p.batch;  // (offsets that jump back and forth have more: they end here)
       const int grid = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
       int units_before = 0, i = 0;
       [[maybe_unused]] int tiles_of = -1, tiles_before = 0;  // kChosen: tiles in front of sequence tiles_of
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int unit = static_cast<int>(index / head_units);
         const int head_unit = static_cast<int>(index - static_cast<long long>(unit) * head_units);
         auto seq_of = [&](int j) { return sorted ? static_cast<int>(order[j]) : j; };
-        i = find_seq(p.batch, unit, lane, [&](int j) {
+        i = unit >= most_units ? -1 : find_seq(p.batch, unit, lane, [&](int j) {
           const int b = seq_of(j), lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
           return (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kSpan - 1) / kSpan;
         }, &units_before, i);
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               int sum = 0;
               for (int b = lane; b < tiles_of; b += 32) {
                 const int lo = clampi(__ldg(p.cu_q + b), 0, p.total_q);
-                sum += (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows;
+                sum = add_count(sum, (clampi(__ldg(p.cu_q + b + 1), lo, p.total_q) - lo + kPtRows - 1) / kPtRows);
               }
               tiles_before = __reduce_add_sync(0xffffffffu, sum);
             }
