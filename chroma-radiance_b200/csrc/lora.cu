@@ -1187,6 +1187,8 @@ b2g_status lora_params(const b2g_lora_desc* d, const char* who, bool down, LoraP
       return fail(B2G_ERR_UNSUPPORTED, "epilogue");
     if (d->N == 0) return B2G_OK;
     if (!d->y || !d->out) return fail(B2G_ERR_INVALID, "null operand");
+    if ((reinterpret_cast<uintptr_t>(d->y) | reinterpret_cast<uintptr_t>(d->out)) & (d->y_dtype == B2G_F32 ? 3u : 1u))
+      return fail(B2G_ERR_UNSUPPORTED, "y and out must be aligned to their elements");
     if (d->epilogue == B2G_EPI_GATED_RESIDUAL && !d->gate) return fail(B2G_ERR_INVALID, "gated_residual needs a gate");
     p->ldy = used(d->ldy, d->rows, d->N);
     p->ldo = used(d->ldo, d->rows, d->N);

@@ -583,8 +583,8 @@ b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int
  * for the rows m of [cu[i], cu[i+1]) of request i, r = ids[i] (NULL: i).  A request whose r is not in [0, adapters) has no
  * adapter: t = 0, out = act(y).  Rows of no request are not written.  cu and ids are device memory, read when the
  * kernels run; offsets are clamped to the rows.  x, a [adapters, R, K] and b [adapters, N, R] are BF16 or F16, of one type, with
- * 16-byte aligned bases and strides; y and out F32 or of that type, any N, strides and alignment (16-byte rows are
- * faster); out may be y (same pointer and stride), and must not overlap it otherwise.  R a multiple of 8 up to 128 (an
+ * 16-byte aligned bases and strides; y and out F32 or of that type, any N and strides, at multiples of an element's size (16-byte
+ * rows are faster); out may be y (same pointer and stride), and must not overlap it otherwise.  R a multiple of 8 up to 128 (an
  * adapter of a lower rank is padded with zeros), K a multiple of 8.  One t serves several b (parts of a fused
  * projection).  No workspace. */
 typedef struct {
