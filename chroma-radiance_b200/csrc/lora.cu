@@ -1195,6 +1195,7 @@ b2g_status lora_params(const b2g_lora_desc* d, const char* who, bool down, LoraP
     if (p->ldy < d->N || p->ldo < d->N) return fail(B2G_ERR_INVALID, "a row stride is below the width");
     if (p->ldy >= (1ll << 38) || p->ldo >= (1ll << 38)) return fail(B2G_ERR_UNSUPPORTED, "size");
     if (E > 0 && (s = operand(d->b, p->ldb, p->bs, d->N, d->R)) != B2G_OK) return s;
+    if ((d->rows / 16 + d->batch) * ((d->N + 31) / 32) > (1ll << 31) - 1) return fail(B2G_ERR_UNSUPPORTED, "size");
   }
   p->cu = d->cu; p->ids = d->ids; p->scale = d->scale; p->gate = d->gate;
   p->batch = static_cast<int>(d->batch); p->rows = static_cast<int>(d->rows); p->adapters = static_cast<int>(E);
@@ -1223,8 +1224,6 @@ b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st, bool early) {
   LoraParams p{};
   b2g_status s = lora_params(d, "b2g_lora_up", false, &p);
   if (s != B2G_OK || p.rows == 0) return s;
-  if ((static_cast<int64_t>(p.rows) / 16 + p.batch) * ((p.N + 31) / 32) > (1ll << 31) - 1)
-    return set_error(B2G_ERR_UNSUPPORTED, "b2g_lora_up: size");
   DeviceInfo* dev = nullptr;
   if ((s = device_info(&dev)) != B2G_OK) return s;
   p.err = dev->err_word;
@@ -1242,7 +1241,8 @@ b2g_status lora_up(const b2g_lora_desc* d, cudaStream_t st, bool early) {
 
 b2g_status lora(const b2g_lora_desc* d, cudaStream_t st) {
   LoraParams p{};
-  b2g_status s = lora_params(d, "b2g_lora", false, &p);  // (both halves are checked before one runs)
+  // (both halves' arguments are checked before one runs: up's here, down's at its start)
+  b2g_status s = lora_params(d, "b2g_lora", false, &p);
   if (s != B2G_OK || (s = lora_down(d, st)) != B2G_OK) return s;
   return lora_up(d, st, true);
 }
