@@ -81,11 +81,12 @@ def pack(requests: list[tuple[int, int, int]], dev) -> Packed:
 
 @dataclass
 class AdaptersS8:
-    """Low-rank adapters of a block's layers, bf16 or fp16, as x_mod; every adapter is padded to one rank with zeros."""
+    """Low-rank adapters of a block's layers, bf16 as the block's buffers beside which they stand; a layer's adapters are
+    padded to one rank with zeros."""
     linear1_a: torch.Tensor  # [adapters, rank, 3072]
     linear1_b: torch.Tensor  # [adapters, 21504, rank]
-    linear2_a: torch.Tensor  # [adapters, rank, 15360], bf16 (the concat buffer's type)
-    linear2_b: torch.Tensor  # [adapters, 3072, rank], bf16
+    linear2_a: torch.Tensor  # [adapters, rank, 15360]
+    linear2_b: torch.Tensor  # [adapters, 3072, rank]
     scale: torch.Tensor | None = None  # f32 [adapters]
 
 
@@ -108,12 +109,32 @@ class Scratch:
         self.cat = torch.empty((rows, HIDDEN + MLP), dtype=torch.bfloat16, device=dev)
 
 
+def _check(adapters: AdaptersS8, x_mod: torch.Tensor) -> None:
+    """What the adapters' calls would refuse, some of them when x is already updated."""
+    if x_mod.dtype != torch.bfloat16:
+        raise b2g.B2GError(f"single_block: with adapters x_mod must be BF16, not {x_mod.dtype}")
+    for name, a, b, k, n in (("linear1", adapters.linear1_a, adapters.linear1_b, HIDDEN, 3 * HIDDEN + MLP),
+                             ("linear2", adapters.linear2_a, adapters.linear2_b, HIDDEN + MLP, HIDDEN)):
+        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+            raise b2g.B2GError(f"single_block: the adapters of {name} must be BF16, not {a.dtype} and {b.dtype}")
+        if a.dim() != 3 or a.shape[2] != k or b.shape != (a.shape[0], n, a.shape[1]):
+            raise b2g.B2GError(f"single_block: the adapters of {name} must be [adapters, rank, {k}] and [adapters, {n}, rank], "
+                               f"not {list(a.shape)} and {list(b.shape)}")
+        if a.shape[1] % 8 or not 8 <= a.shape[1] <= 128:
+            raise b2g.B2GError(f"single_block: the rank of {name} must be a multiple of 8 up to 128, not {a.shape[1]}")
+        for t in (a, b):
+            if t.data_ptr() % 16 or t.stride(2) != 1 or t.stride(1) < t.shape[2] or t.stride(1) % 8 or (t.shape[0] > 1 and t.stride(0) % 8):
+                raise b2g.B2GError(f"single_block: the adapters of {name} need 16-byte aligned rows, not strides {t.stride()}")
+
+
 def single_block(w: SingleWeightsS8, x_mod: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, batch: Packed,
                  s: Scratch, adapters: AdaptersS8 | None = None, ids: torch.Tensor | None = None,
                  choice: Choice | None = None) -> None:
     """Updates x [rows, 3072] (F32 residual stream of all sequences) in place from the modulated x_mod
     (bf16, fp16 or F32; with adapters bf16).  ids: each sequence's adapter (int32, device; negative: none; None: the
     sequences' own numbers).  choice: attention over chosen key blocks."""
+    if adapters:
+        _check(adapters, x_mod)
     n = x.shape[0]
     codes, scales = b2g.quantize_s8(x_mod, out=s.codes[:n], scales=s.scales[:n])
     qkv, cat = s.qkv[:n], s.cat[:n]
