@@ -1173,8 +1173,8 @@ def select_blocks(q: torch.Tensor, means: torch.Tensor, cu_q: torch.Tensor, top:
     words], bit j % 32 of word j / 32 for block j.  Always the `first` first and `last` last blocks in the tile's sight
     and those that some of its queries see in part; of the others the `top` with the largest product of the summed
     queries (all heads of the key head's group) and the block's mean (block_means), in 64 bits, of equal ones the first.
-    max_k: keys of the longest sequence, or more (None: what `means` has rows for); it sets the number of words, at
-    most 256 of them.  New results have total_q / 128 + batch tiles; rows past the last tile are 0."""
+    max_k: keys of the longest sequence, or more (None: what `means` has rows for, if these are no more than
+    8192); it sets the number of words, at most 256 of them.  New results have total_q / 128 + batch tiles; rows past the last tile are 0."""
     return _call("select_blocks", stream, q, means, cu_q, top, cu_k, k_lens, first, last, causal, max_k, out)
 
 

@@ -378,6 +378,8 @@ PyObject* select_blocks(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (a[9] != Py_None) {
       const int64_t keys = whole(a[9], "select_blocks: max_k");
       most = keys / 128 + (keys % 128 != 0);
+    } else if (!given && blocks > 32 * 256) {  // (no one sequence need have so many)
+      refuse("select_blocks: max_k, the keys of the longest sequence or more, is needed where means has more than 8192 rows");
     }
     if (given && (given->dim() != 3 || given->size(1) != means.size(1) || !given->is_contiguous() ||
                   given->scalar_type() != ScalarType::Int))

@@ -96,7 +96,7 @@ class Choice:
     top: int
     first: int = 0
     last: int = 0
-    max_k: int | None = None  # rows of the longest sequence, or more
+    max_k: int | None = None  # rows of the longest sequence, or more (None: all rows of the batch, for batches below 2^20)
 
 
 class Scratch:
