@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
   const int r = lane >> 2, t4 = lane & 3;
   auto scores = [&](int nb, int mean0, int n0, int n1) {  // blocks below nb of tiles n0 to n1
     for (int j0 = warp * 8; j0 < nb; j0 += kWarps * 8) {
+      __syncwarp();  // (the products are the whole warp's, the end of a round is not)
       float4 m[D / 16];
       const int at = mean0 + j0 + r;
       const bool in = j0 + r < nb && at < a.blocks;
