@@ -472,7 +472,7 @@ __device__ __forceinline__ CrLine chosen_line(const PkParams& p, long long* ends
   }
   sums_of<kThreads>(p.batch, mask_tiles, carry);
   // A thread takes kAhead pairs, whose loads go out together: of sequences with one tile of rows (most of them) four
-  // words at a time; others' tiles one after the other.
+  // words at a time.
   constexpr int kAhead = 4;
   const int pairs = p.batch * p.hk, words = p.chosen_words;
   for (int i0 = threadIdx.x; i0 < pairs; i0 += kAhead * kThreads) {
@@ -509,15 +509,36 @@ __device__ __forceinline__ CrLine chosen_line(const PkParams& p, long long* ends
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * kThreads;
-      if (i >= pairs) continue;
-      long long sum = tiles[u] == 1 ? count[u] + kCrTileCost : 0;
-      if (tiles[u] > 1) {
-        const int b = i / p.hk;
-        const Seq s = load_seq(p, b);
-        for (int tile = 0; tile < tiles[u]; ++tile)
-          sum += chosen_length(chosen_tile(p, s, i - b * p.hk, tile, mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows));
-      }
-      ends[i] = sum;
+      if (i < pairs) ends[i] = tiles[u] == 1 ? count[u] + kCrTileCost : -tiles[u];
+    }
+  }
+  __syncthreads();
+  // Pairs with more tiles of rows (less than 0: as many): each by a lane, or by the whole warp, one pair after the other, where
+  // that takes fewer rounds, as it does for a long sequence among short ones.
+  const int lane = threadIdx.x & 31;
+  for (int i0 = threadIdx.x - lane; i0 < pairs; i0 += kThreads) {
+    const int n = i0 + lane < pairs ? static_cast<int>(max(-ends[i0 + lane], 0ll)) : 0;
+    const uint32_t many = __ballot_sync(0xffffffffu, n > 0);
+    if (!many) continue;
+    const bool shared = 2 * __reduce_add_sync(0xffffffffu, (n + 31) / 32) < __reduce_max_sync(0xffffffffu, n);
+    auto sum_of = [&](int i, int first, int step, int tiles) {
+      const int b = i / p.hk;
+      const Seq s = load_seq(p, b);
+      const int before = mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows;
+      long long sum = 0;
+      for (int tile = first; tile < tiles; tile += step) sum += chosen_length(chosen_tile(p, s, i - b * p.hk, tile, before));
+      return sum;
+    };
+    if (!shared) {
+      if (n > 0) ends[i0 + lane] = sum_of(i0 + lane, 0, 1, n);
+      continue;
+    }
+    for (uint32_t left = many; left; left &= left - 1) {
+      const int at = __ffs(left) - 1;
+      long long sum = sum_of(i0 + at, lane, 32, __shfl_sync(0xffffffffu, n, at));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) ends[i0 + at] = sum;
     }
   }
   sums_of<kThreads>(pairs, ends, carry);
@@ -526,8 +547,15 @@ __device__ __forceinline__ CrLine chosen_line(const PkParams& p, long long* ends
 }
 // Where share i begins.
 __device__ __forceinline__ long long cut_at(const CrLine& line, int i) { return line.total * i / line.shares; }
-// The tile that holds place `at` of the line: the tile, its start and length.
-__device__ __forceinline__ CrTile chosen_at(const PkParams& p, const CrLine& line, long long at, long long* start, int* length) {
+// Where a search left off: tile `tile` of pair `pair` begins at `start`.
+struct CrPlace {
+  int pair, tile;
+  long long start;
+};
+// The tile that holds place `at` of the line: the tile, its start and length.  Whole warps search; of a pair with many tiles 32 at
+// a time, from `from` on where it is in the same pair (a share's tiles follow one another).
+__device__ __forceinline__ CrTile chosen_at(const PkParams& p, const CrLine& line, long long at, long long* start, int* length,
+                                            CrPlace* from) {
   int lo = 0, hi = p.batch * p.hk - 1;  // the first pair that ends past `at`
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -537,13 +565,34 @@ __device__ __forceinline__ CrTile chosen_at(const PkParams& p, const CrLine& lin
   const int b = lo / p.hk;
   const Seq s = load_seq(p, b);
   const int before = line.mask_tiles[b] - (s.lq + kPtRows - 1) / kPtRows, tiles = chosen_tiles_of(p, s.lq);
-  *start = lo > 0 ? line.ends[lo - 1] : 0;
-  for (int t = 0;; ++t) {
-    const CrTile c = chosen_tile(p, s, lo - b * p.hk, t, before);
-    *length = tiles == 1 ? static_cast<int>(line.ends[lo] - *start) : chosen_length(c);
-    if (t + 1 >= tiles || at < *start + *length) return c;
-    *start += *length;
+  if (from->pair != lo) *from = {lo, 0, lo > 0 ? line.ends[lo - 1] : 0};
+  *start = from->start;
+  int tile = from->tile;
+  if (tiles == 1) {
+    *length = static_cast<int>(line.ends[lo] - *start);
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (;; tile += 32) {
+      const int mine = tile + lane < tiles ? chosen_length(chosen_tile(p, s, lo - b * p.hk, tile + lane, before)) : 0;
+      long long sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, *start + sum > at || tile + lane >= tiles - 1);
+      if (past) {
+        const int in = __ffs(past) - 1;
+        *start += __shfl_sync(0xffffffffu, sum - mine, in);
+        *length = __shfl_sync(0xffffffffu, mine, in);
+        tile += in;
+        break;
+      }
+      *start += __shfl_sync(0xffffffffu, sum, 31);
+    }
   }
+  *from = {lo, tile, *start};
+  return chosen_tile(p, s, lo - b * p.hk, tile, before);
 }
 
 // With part i holding (m_i, l_i) and O_i: O = sum 2^(m_i - M) O_i, l = sum 2^(m_i - M) l_i.  (A part without a key has
@@ -775,10 +824,11 @@ __global__ void __launch_bounds__(32 * kCrWarps, kCrBlocksPerSm) chosen_rows_ker
     const int share = blockIdx.x;
     if (share >= line.shares) return;
     const long long end = cut_at(line, share + 1);
+    CrPlace place{-1, 0, 0};
     for (long long at = cut_at(line, share); at < end;) {
       long long start;
       int length;
-      const CrTile tile = chosen_at(p, line, at, &start, &length);
+      const CrTile tile = chosen_at(p, line, at, &start, &length, &place);
       const int from = static_cast<int>(at - start), to = static_cast<int>(min(static_cast<long long>(length), end - start));
       at = max(start + to, at + 1);  // (further on also where the words change under the kernel)
       const int slot = to - from < length ? 2 * share + (from == 0 ? 1 : 0) : -1;
@@ -819,7 +869,8 @@ __global__ void __launch_bounds__(kCcThreads) chosen_combine_kernel(const PkPara
   if (cut < line.shares) {
     long long start;
     int length;
-    tile = chosen_at(p, line, cut_at(line, cut), &start, &length);
+    CrPlace place{-1, 0, 0};
+    tile = chosen_at(p, line, cut_at(line, cut), &start, &length, &place);
     // (a share may be longer than the tile: then the cut before this one is outside it)
     if (start != cut_at(line, cut) && cut_at(line, cut - 1) <= start)
       for (parts = 2; cut + parts - 1 < line.shares && cut_at(line, cut + parts - 1) < start + length;) ++parts;
