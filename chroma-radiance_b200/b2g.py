@@ -1174,7 +1174,8 @@ def select_blocks(q: torch.Tensor, means: torch.Tensor, cu_q: torch.Tensor, top:
     and those that some of its queries see in part; of the others the `top` with the largest product of the summed
     queries (all heads of the key head's group) and the block's mean (block_means), in 64 bits, of equal ones the first.
     max_k: keys of the longest sequence, or more (None: what `means` has rows for, if these are no more than
-    8192); it sets the number of words, at most 256 of them.  New results have total_q / 128 + batch tiles; rows past the last tile are 0."""
+    8192); it sets the number of words, at most 256 of them.  New results have total_q / 128 + batch tiles; rows past
+    the last tile are 0."""
     return _call("select_blocks", stream, q, means, cu_q, top, cu_k, k_lens, first, last, causal, max_k, out)
 
 
@@ -1183,7 +1184,8 @@ def attention_blocks(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, chosen: 
                      scale: float | None = None, out: torch.Tensor | None = None,
                      stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """attention_packed over the keys of chosen blocks: chosen as select_blocks gives it (or set by hand), the other
-    arguments as there.  Blocks out of a tile's sight are not looked at; a row that sees no key is 0."""
+    arguments as there.  Blocks out of a tile's sight are not looked at; a row that sees no key is 0.  One kernel takes
+    the call, by the average number of queries: a prompt among many single tokens is slower than in a call of its own."""
     return _call("attention_blocks", stream, q, k, v, chosen, cu_q, cu_k, k_lens, causal, scale, out)
 
 

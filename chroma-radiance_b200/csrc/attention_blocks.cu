@@ -11,6 +11,10 @@
 //
 // Offsets are read on the device and clamped to the buffers, as in attention_packed.cu.
 //
+// The keys' sums, the statistics (row maximum and sum) and the output's sums are fp32, the blocks' scores 64 bits.  P is rounded
+// to the operands' 16-bit type, as the tensor cores take it, at most 2^-8 (bf16) or 2^-11 (fp16) of a weight; the row's sum
+// is taken before that.
+//
 //   packed_tiles (attention_packed.cuh)  long queries: tensor cores through TMEM, K and V by chosen block
 //   chosen_rows, chosen_combine          few query rows per key head: equal shares of all that is chosen
 #include "attention_packed.cuh"
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(32 * kMnWarps, kMnPerSm) block_means_kernel(co
 
 // ---------------------------------------------------------------------------- choice of blocks
 //
-// Bound by instructions, not by q's bytes (16384 queries of 24 heads: 46.9 us, floor 15.6): the summing of the queries and the
+// Bound by instructions, not by q's bytes (16384 queries of 24 heads: 46.7 us, floor 15.6): the summing of the queries and the
 // scores after it do not overlap.  Scores are sums of 64 bits: a choice compares neighbours, and any rounding of theirs in 32 bits would decide
 // the choice where two are close; in 64 bits the order of a sum moves one in some 10^12.
 constexpr int kSlThreads = 256;
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kSlThreads) select_blocks_kernel(const SlParam
 
 // ---------------------------------------------------------------------------- few rows over chosen blocks
 //
-// Bound by memory where caches are long, by round trips otherwise (48 single queries, 32 heads on 8, 18 blocks: 39.4 us for
+// Bound by memory where caches are long, by round trips otherwise (48 single queries, 32 heads on 8, 18 blocks: 38.3 us for
 // 97 MB with the join).  The query rows of one key head (lq tokens x group heads) in tiles of 16.  The products, the lanes' layout and the
 // copies are those of packed_rows_kernel (attention_packed.cu): in a CTA the warps take 16 keys of the chosen blocks in turn.
 //
@@ -921,7 +925,10 @@ __global__ void __launch_bounds__(kCcThreads) chosen_combine_kernel(const PkPara
 //   32, 4    4            20.7, 58.1   44.4, 58.2   71.5, 58.3
 //   8, 8     4            26.5, 57.6   28.0, 57.8   31.4, 57.9
 // Heads of their own leave nothing to share, and tiles of many long caches stream faster (8 heads: 128 of 4096 keys
-// 253, 202; 64: 135, 110; 48: 106, 103; 24 heads: 64 of 1500 249, 206, but 64 of 300 69, 72 and of 40 30, 47).
+// 253, 202; 64: 135, 110; 48: 106, 103; 24 heads: 64 of 1500 249, 206, but 64 of 300 69, 72 and of 40 30, 47; short keys of more
+// sequences are on the wrong side: 256 of 300 261, 225).
+// One form takes a call, by its average: a prompt among single tokens reads its keys once for every 16 of its rows (95 single
+// queries and a prompt of 512, 32 heads on 8, caches of 4096: 445 us; apart 194 and 51).
 bool few_queries(const b2g_attention_packed_desc* d, int sms) {
   const int64_t group = d->n_head / d->n_kv_head;
   if (d->total_q > 8 * d->batch && d->total_q * group > kCrRows * d->batch) return false;

@@ -17,7 +17,7 @@
 //   lora_up_any      many rows where TMA cannot take y or out: m16n8k16 products
 //
 // In the second product s t is the sum of two numbers of the operands' 16-bit type: bf16 keeps 2^-17 of a value, fp16, whose
-// range is small, 2^-22 of its row's largest, as the row is brought to [1, 2) by a power of two.
+// range is small, 2^-23 of its row's largest, as the row is brought to [1, 2) by a power of two.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cmath>
@@ -1009,6 +1009,7 @@ __global__ void __launch_bounds__(32 * kLuWarps) lora_up_any_kernel(const LoraPa
 //   down, rank 128    16.5, 11.5   23.5, 12.5   16.0, 11.8   32.1, 17.2   58.9, 18.8
 //   up, rank 16       10.5, 10.5   19.9, 13.2   15.7, 11.8   30.3, 32.3   72.6, 37.1   13.3, 15.0
 //   up, rank 128      17.8, 21.5   32.4, 31.0   30.8, 41.2   76.0, 103    82.9, 131
+// (64 x 64 at rank 16 is the one of these whose down is on the wrong side.)
 bool few_down(int64_t rows, int64_t batch, int64_t R) {
   return rows <= (R > 32 ? 16 : 32) * batch || (rows / 16 + batch) * R <= 2600;
 }

@@ -28,6 +28,10 @@ they stand beside have 8.
     cat[mlp] = gelu(cat[mlp] + scale t1 B1[9216:])           the GELU here instead of in the product's epilogue
     x       += gate * scale (cat A2) B2
 
+With adapters the MLP half thus leaves its product in bf16 before the GELU, at most 2^-8 of a value (F32 would be 4 bytes a value more
+each way), and that for all requests of the batch: the update of one without an adapter is not bit for bit that of a batch
+without adapters.
+
 Long sequences need not attend to all of their keys (`Choice`): block_means and select_blocks on the rotated q and k,
 attention_blocks over what they chose.
 """

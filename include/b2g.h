@@ -562,11 +562,14 @@ b2g_status b2g_attention_packed(const b2g_attention_packed_desc* desc, void* wor
  * to see key block j of its sequence: the `first` first and the `last` last of the blocks in its sight (up to the last key
  * that its last query sees), every block that some of its queries see in part only (causal), and of the others the
  * `top` with the largest (sum of the tile's queries, of all heads that share the key head) . means[block], of equal
- * ones the first.  The scores are summed in 64 bits; NaN counts as -inf.  Sequences' tiles follow one another; rows past the
+ * ones the first.  The scores are summed in 64 bits (the queries before that in pairs of fp32, which hold as much, but whose sums
+ * past 3.4e38 are infinite); NaN counts as -inf.  Sequences' tiles follow one another; rows past the
  * last tile are 0 (total_q / 128 + batch rows always suffice).  words <= 256; blocks past 32 * words are never chosen.
  *
  * b2g_attention_blocks: b2g_attention_packed over the keys of the chosen blocks.  Bits of blocks out of a tile's
- * sight are not looked at; a tile without a bit, or past `tiles`, sees nothing, and its rows are 0.
+ * sight are not looked at; a tile without a bit, or past `tiles`, sees nothing, and its rows are 0.  The softmax's weights are
+ * rounded to the operands' type for the second product, at most 2^-8 (BF16) or 2^-11 (F16) of each; their sum is not.  One
+ * kernel takes the call, by the average number of queries: a prompt among many single tokens is slower than in a call of its own.
  * workspace: as for b2g_gemm_s8. */
 b2g_status b2g_block_means(const b2g_attention_packed_desc* desc, const int32_t* since, float* means, int64_t blocks,
                            void* stream);
@@ -585,7 +588,8 @@ b2g_status b2g_attention_blocks(const b2g_attention_packed_desc* desc, const int
  * kernels run; offsets are clamped to the rows.  x, a [adapters, R, K] and b [adapters, N, R] are BF16 or F16, of one type, with
  * 16-byte aligned bases and strides; y and out F32 or of that type, any N and strides, at multiples of an element's size (16-byte
  * rows are faster); out may be y (same pointer and stride), and must not overlap it otherwise.  R a multiple of 8 up to 128 (an
- * adapter of a lower rank is padded with zeros), K a multiple of 8.  One t serves several b (parts of a fused
+ * adapter of a lower rank is padded with zeros), K a multiple of 8.  scale[r] * t enters the second product as the sum of two
+ * numbers of the operands' type: BF16 keeps 2^-17 of a value, F16 2^-23 of its row's largest.  One t serves several b (parts of a fused
  * projection).  No workspace. */
 typedef struct {
   const void* x; const void* a; const void* b; b2g_dtype dtype;
